@@ -33,8 +33,10 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               f"-I{INCLUDE}"]
 
-CU_SOURCES = ["status.cu", "gather.cu", "gather_mma.cu", "window.cu", "window_warp.cu", "window_tc.cu", "rows.cu", "cube.cu", "preprocess.cu", "noalloc.cu", "l2plan.cu", "capi.cu"]
+CU_SOURCES = ["status.cu", "gather.cu", "gather_mma.cu", "window.cu", "window_warp.cu", "window_tc.cu", "rows.cu", "cube.cu", "preprocess.cu", "noalloc.cu", "l2plan.cu", "norm.cu", "grouped.cu", "ortho.cu", "capi_layers.cu", "capi.cu"]
 HEADERS = ["common.cuh", "engine.h"]
+LAYER_SOURCES = ["norm.cu", "grouped.cu", "ortho.cu", "capi_layers.cu"]
+LAYER_HEADERS = ["layer.cuh", "layer.h"]
 
 
 def _newer(target: Path, deps) -> bool:
@@ -57,7 +59,8 @@ def build_lib(force=False, verbose=False) -> Path:
     for src in CU_SOURCES:
         s = CSRC / src
         o = OBJ / (s.stem + ".o")
-        if force or _newer(o, [s, *headers]):
+        extra = [CSRC / h for h in LAYER_HEADERS] if src in LAYER_SOURCES else []
+        if force or _newer(o, [s, *headers, *extra]):
             _run([NVCC, *ARCH, *NVCC_FLAGS, "-c", s, "-o", o], verbose)
         objs.append(o)
     if force or _newer(LIB, objs):

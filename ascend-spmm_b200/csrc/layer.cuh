@@ -1,0 +1,95 @@
+// Device helpers shared by the layer operators (norm.cu, grouped.cu, ortho.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "../../include/spmm_b200.h"
+#include "common.cuh"
+
+namespace spmmb {
+
+template <typename T> __device__ __forceinline__ float elem_f32(T x);
+template <> __device__ __forceinline__ float elem_f32<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float elem_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float elem_f32<float>(float x) { return x; }
+
+template <typename T> __device__ __forceinline__ T elem_of(float x);
+template <> __device__ __forceinline__ __half elem_of<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 elem_of<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ float elem_of<float>(float x) { return x; }
+
+// The rows of a grouped product as segments: segment 0 is the rows before
+// the first group, segment g + 1 is group g, segment groups + 1 the rows
+// after the last group (0 and groups + 1 get zeros).  A malformed group is
+// empty.
+template <typename I>
+__device__ __forceinline__ void segment_rows(const I *ptr, int64_t groups, int64_t rows, int64_t s, int64_t *begin,
+                                             int64_t *end, DevStatus *status)
+{
+    int64_t b = 0, e = 0;
+    if (s == 0) {
+        e = min(max((int64_t)ptr[0], (int64_t)0), rows);
+    } else if (s <= groups) {
+        b = (int64_t)ptr[s - 1];
+        e = (int64_t)ptr[s];
+        if (b < 0 || e < b || e > rows) {
+            raise_status(status, SPMM_DEV_BAD_ROWPTR, s - 1);
+            b = e = 0;
+        }
+    } else if (s == groups + 1) {
+        b = min(max((int64_t)ptr[groups], (int64_t)0), rows);
+        e = rows;
+    }
+    *begin = b;
+    *end = e;
+}
+
+// Walks the row tiles of all segments in order.  Every lane of the warp calls
+// it with the same arguments; `tile` must not decrease from call to call.
+struct TileWalk {
+    int64_t base = 0;    // segments before the current 32
+    int64_t before = 0;  // tiles of the segments before `base`
+    int64_t count = -1;  // this lane's segment: its tiles, rows and the tiles before it
+    int64_t begin = 0, end = 0, first = 0;
+
+    // Finds the segment of `tile`: its index (0 .. groups + 1), its rows and
+    // the tile's number within it; false past the last tile.
+    // `mult` tiles per row tile (column tiles), `height` rows per row tile.
+    template <typename I>
+    __device__ __forceinline__ bool find(const I *ptr, int64_t groups, int64_t rows, int height, int64_t mult,
+                                         int64_t tile, DevStatus *status, int64_t *seg, int64_t *b, int64_t *e,
+                                         int64_t *inner)
+    {
+        const int lane = threadIdx.x & 31;
+        for (;;) {
+            if (count < 0) {
+                const int64_t s = base + lane;
+                segment_rows(ptr, groups, rows, s, &begin, &end, status);
+                count = (end - begin + height - 1) / height * mult;
+                int64_t sum = count;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) sum += v;
+                }
+                first = sum - count;
+            }
+            const int64_t total = __shfl_sync(0xffffffffu, first + count, 31);
+            const unsigned hit = __ballot_sync(0xffffffffu, tile - before >= first && tile - before < first + count);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                *seg = base + l;
+                *b = __shfl_sync(0xffffffffu, begin, l);
+                *e = __shfl_sync(0xffffffffu, end, l);
+                *inner = tile - before - __shfl_sync(0xffffffffu, first, l);
+                return true;
+            }
+            before += total;
+            base += 32;
+            count = -1;
+            if (base >= groups + 2) return false;
+        }
+    }
+};
+
+}  // namespace spmmb

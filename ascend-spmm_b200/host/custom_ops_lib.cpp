@@ -603,6 +603,195 @@ at::Tensor restore_rows(const at::Tensor &packed, const at::Tensor &index)
     return out;
 }
 
+// ---------------------------------------------------------------------------
+// Layer operators (no counterpart in the reference): layer normalisation,
+// products grouped by row ranges, orthogonalised updates.
+// ---------------------------------------------------------------------------
+int layer_dtype(const at::Tensor &t, const char *op)
+{
+    switch (t.scalar_type()) {
+        case at::kHalf: return SPMM_F16;
+        case at::kBFloat16: return SPMM_BF16;
+        case at::kFloat: return SPMM_F32;
+        default: TORCH_CHECK(false, op, " supports only FP16, BF16 and FP32 tensors, but got ", t.scalar_type());
+    }
+    return -1;
+}
+
+// A contiguous, 16-byte aligned form of t (t itself where it is one).
+at::Tensor dense16(const at::Tensor &t) { return aligned16(t.contiguous()); }
+
+// weight or bias of layer_norm: [width], of x's dtype or fp32, on x's device.
+at::Tensor norm_param(const c10::optional<at::Tensor> &p, const at::Tensor &x, int64_t width, const char *name)
+{
+    if (!p.has_value()) return at::Tensor();
+    TORCH_CHECK(p->is_cuda(), "layer_norm: ", name, " must be CUDA tensor");
+    TORCH_CHECK(p->device() == x.device(), "layer_norm: all tensors must be on ", x.device());
+    TORCH_CHECK(p->dim() == 1 && p->size(0) == width, "layer_norm: ", name, " must have shape [", width, "], but got ",
+                p->sizes());
+    TORCH_CHECK(p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat, "layer_norm: ", name,
+                " must have the dtype of x or FP32");
+    return dense16(*p);
+}
+
+const void *ptr_or_null(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+int param_dtype_of(const at::Tensor &w, const at::Tensor &b, int dtype)
+{
+    const at::Tensor &p = w.defined() ? w : b;
+    if (w.defined() && b.defined())
+        TORCH_CHECK(w.scalar_type() == b.scalar_type(), "layer_norm: weight and bias must have the same dtype");
+    return p.defined() ? (p.scalar_type() == at::kFloat ? SPMM_F32 : dtype) : dtype;
+}
+
+// (y, mean, rstd); mean and rstd are undefined without `stats`.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_forward(const at::Tensor &x,
+                                                                  const c10::optional<at::Tensor> &weight,
+                                                                  const c10::optional<at::Tensor> &bias, double eps,
+                                                                  bool stats)
+{
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK(x.dim() >= 1, "layer_norm: x must have at least one dimension");
+    const int dt = layer_dtype(x, "layer_norm");
+    const int64_t width = x.size(-1);
+    TORCH_CHECK(width >= 1, "layer_norm requires a feature width of at least 1");
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor w = norm_param(weight, x, width, "weight"), b = norm_param(bias, x, width, "bias");
+    const int pdt = param_dtype_of(w, b, dt);
+    const at::Tensor xc = dense16(x);
+    const int64_t rows = xc.numel() / width;
+    at::Tensor y = at::empty(xc.sizes(), xc.options()), mean, rstd;
+    if (stats) {
+        mean = at::empty({rows}, xc.options().dtype(at::kFloat));
+        rstd = at::empty({rows}, xc.options().dtype(at::kFloat));
+    }
+    check_rc(spmm_layer_norm_launch(xc.data_ptr(), ptr_or_null(w), ptr_or_null(b), y.data_ptr(),
+                                    stats ? mean.data_ptr<float>() : nullptr,
+                                    stats ? rstd.data_ptr<float>() : nullptr, rows, width, eps, dt, pdt,
+                                    stream_of(xc)));
+    return {y, mean, rstd};
+}
+
+// (dx, dweight, dbias); those not wanted are undefined.  dweight and dbias
+// have the dtype of weight (of x without one).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(const at::Tensor &grad, const at::Tensor &x,
+                                                                   const at::Tensor &mean, const at::Tensor &rstd,
+                                                                   const c10::optional<at::Tensor> &weight,
+                                                                   bool want_x, bool want_weight, bool want_bias,
+                                                                   bool fp32_params)
+{
+    const char *op = "layer_norm_backward";
+    TORCH_CHECK_CUDA(grad);
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK_CUDA(mean);
+    TORCH_CHECK_CUDA(rstd);
+    same_device({&grad, &mean, &rstd}, x, op);
+    TORCH_CHECK(x.dim() >= 1, op, ": x must have at least one dimension");
+    const int dt = layer_dtype(x, op);
+    const int64_t width = x.size(-1);
+    TORCH_CHECK(width >= 1, op, " requires a feature width of at least 1");
+    const int64_t rows = x.numel() / width;
+    TORCH_CHECK(grad.sizes() == x.sizes() && grad.scalar_type() == x.scalar_type(), op,
+                ": grad must have the shape and dtype of x");
+    for (const at::Tensor *s : {&mean, &rstd})
+        TORCH_CHECK(s->scalar_type() == at::kFloat && s->is_contiguous() && s->numel() == rows, op,
+                    ": mean and rstd must be contiguous FP32 with one value per row");
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor w = norm_param(weight, x, width, "weight");
+    const int pdt = w.defined() ? param_dtype_of(w, at::Tensor(), dt) : fp32_params ? SPMM_F32 : dt;
+    const at::Tensor xc = dense16(x), gc = dense16(grad);
+    const auto popt = xc.options().dtype(pdt == SPMM_F32 ? at::kFloat : xc.scalar_type());
+    at::Tensor dx, dw, db;
+    if (want_x) dx = at::empty(xc.sizes(), xc.options());
+    if (want_weight) dw = at::empty({width}, popt);
+    if (want_bias) db = at::empty({width}, popt);
+    const size_t wbytes = want_weight || want_bias ? spmm_layer_norm_backward_workspace_bytes(rows, width) : 0;
+    at::Tensor ws = workspace(wbytes, xc);
+    check_rc(spmm_layer_norm_backward_launch(gc.data_ptr(), xc.data_ptr(), mean.data_ptr<float>(),
+                                             rstd.data_ptr<float>(), ptr_or_null(w),
+                                             const_cast<void *>(ptr_or_null(dx)), const_cast<void *>(ptr_or_null(dw)),
+                                             const_cast<void *>(ptr_or_null(db)), rows, width, dt, pdt, ws.data_ptr(),
+                                             wbytes, stream_of(xc)));
+    return {dx, dw, db};
+}
+
+int check_group_ptr(const at::Tensor &ptr, const at::Tensor &x, int64_t groups, const char *op)
+{
+    TORCH_CHECK(ptr.is_cuda(), op, ": group_ptr must be CUDA tensor");
+    TORCH_CHECK(ptr.device() == x.device(), op, ": all tensors must be on ", x.device());
+    TORCH_CHECK(ptr.dim() == 1, op, ": group_ptr must be one-dimensional");
+    TORCH_CHECK(groups < 0 ? ptr.size(0) >= 1 : ptr.size(0) == groups + 1, op, ": group_ptr must hold groups + 1 entries");
+    return index_code({&ptr}, op);
+}
+
+// x [rows, K] times weight[g] [K, N] (transposed: x [rows, N] times weight[g]^T).
+at::Tensor grouped_matmul(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &group_ptr, bool transposed)
+{
+    const char *op = "grouped_matmul";
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK_CUDA(weight);
+    TORCH_CHECK(x.dim() == 2, op, ": x must be two-dimensional");
+    TORCH_CHECK(weight.dim() == 3, op, ": weight must be three-dimensional");
+    const int dt = layer_dtype(x, op);
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type(), op, ": weight must have the same dtype as x");
+    same_device({&weight}, x, op);
+    const int64_t groups = weight.size(0), K = weight.size(1), N = weight.size(2), rows = x.size(0);
+    TORCH_CHECK(x.size(1) == (transposed ? N : K), op, ": x has ", x.size(1), " features, the weight takes ",
+                transposed ? N : K);
+    const int itype = check_group_ptr(group_ptr, x, groups, op);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = dense16(x), wc = dense16(weight);
+    at::Tensor out = at::empty({rows, transposed ? K : N}, xc.options());
+    const size_t wbytes = spmm_grouped_matmul_workspace_bytes(rows, groups, K, N, transposed, dt);
+    at::Tensor ws = workspace(wbytes, xc);
+    check_rc(spmm_grouped_matmul_launch(xc.data_ptr(), wc.data_ptr(), group_ptr.data_ptr(), out.data_ptr(), rows,
+                                        groups, K, N, transposed, itype, dt, ws.data_ptr(), wbytes, stream_of(xc)));
+    return out;
+}
+
+// dweight [groups, K, N]: x_g^T grad_g over each group's rows.
+at::Tensor grouped_weight_grad(const at::Tensor &x, const at::Tensor &grad, const at::Tensor &group_ptr)
+{
+    const char *op = "grouped_weight_grad";
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK_CUDA(grad);
+    TORCH_CHECK(x.dim() == 2 && grad.dim() == 2, op, ": x and grad must be two-dimensional");
+    const int dt = layer_dtype(x, op);
+    TORCH_CHECK(grad.scalar_type() == x.scalar_type(), op, ": grad must have the same dtype as x");
+    TORCH_CHECK(grad.size(0) == x.size(0), op, ": x and grad must have the same number of rows");
+    same_device({&grad}, x, op);
+    const int itype = check_group_ptr(group_ptr, x, -1, op);
+    const int64_t groups = group_ptr.size(0) - 1, K = x.size(1), N = grad.size(1), rows = x.size(0);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = dense16(x), gc = dense16(grad);
+    at::Tensor dw = at::empty({groups, K, N}, xc.options());
+    const size_t wbytes = spmm_grouped_weight_grad_workspace_bytes(rows, groups, K, N, dt);
+    at::Tensor ws = workspace(wbytes, xc);
+    check_rc(spmm_grouped_weight_grad_launch(xc.data_ptr(), gc.data_ptr(), group_ptr.data_ptr(), dw.data_ptr(), rows,
+                                             groups, K, N, itype, dt, ws.data_ptr(), wbytes, stream_of(xc)));
+    return dw;
+}
+
+at::Tensor orthogonalize(const at::Tensor &update, int64_t steps, double a, double b, double c, double eps)
+{
+    const char *op = "orthogonalize";
+    TORCH_CHECK_CUDA(update);
+    TORCH_CHECK(update.dim() >= 2, op, ": update must have at least two dimensions");
+    const int dt = layer_dtype(update, op);
+    TORCH_CHECK(steps >= 0 && steps <= 100, op, ": steps must be in [0, 100]");
+    c10::cuda::CUDAGuard guard(update.device());
+    const at::Tensor u = dense16(update);
+    at::Tensor out = at::empty(u.sizes(), u.options().dtype(at::kBFloat16));
+    const int64_t m = u.size(-2), n = u.size(-1);
+    if (out.numel() == 0) return out;
+    const int64_t batch = u.numel() / (m * n);
+    const size_t wbytes = spmm_orthogonalize_workspace_bytes(batch, m, n, dt);
+    at::Tensor ws = workspace(wbytes, u);
+    check_rc(spmm_orthogonalize_launch(u.data_ptr(), out.data_ptr(), batch, m, n, (int)steps, a, b, c, eps, dt,
+                                       ws.data_ptr(), wbytes, stream_of(u)));
+    return out;
+}
+
 // Sticky device status (code, detail), optionally cleared.  Synchronises.
 std::tuple<int64_t, int64_t> device_status(bool reset)
 {
@@ -662,6 +851,25 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("a"), pybind11::arg("window_size") = 16);
     m.def("pack_rows", &pack_rows, "dst[index[i]] = src[i]; other rows zero (pack_node_tensor helper)");
     m.def("restore_rows", &restore_rows, "dst[i] = src[index[i]] (restore_node_tensor helper)");
+    m.def("layer_norm_forward", &layer_norm_forward,
+          "Layer normalisation of the last dimension: (y, mean, rstd); mean and rstd only with stats",
+          pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("eps") = 1e-5,
+          pybind11::arg("stats") = true);
+    m.def("layer_norm_backward", &layer_norm_backward,
+          "Gradients of layer_norm_forward: (dx, dweight, dbias), each only where wanted", pybind11::arg("grad"),
+          pybind11::arg("x"), pybind11::arg("mean"), pybind11::arg("rstd"), pybind11::arg("weight"),
+          pybind11::arg("want_x") = true, pybind11::arg("want_weight") = true, pybind11::arg("want_bias") = true,
+          pybind11::arg("fp32_params") = false);
+    m.def("grouped_matmul", &grouped_matmul,
+          "Rows group_ptr[g] .. group_ptr[g + 1] of x times weight[g] (its transpose with transposed); widths "
+          "divisible by 16 for FP16 and BF16, by 8 for FP32",
+          pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("group_ptr"), pybind11::arg("transposed") = false);
+    m.def("grouped_weight_grad", &grouped_weight_grad, "Gradient of grouped_matmul's weight: x_g^T grad_g per group",
+          pybind11::arg("x"), pybind11::arg("grad"), pybind11::arg("group_ptr"));
+    m.def("orthogonalize", &orthogonalize,
+          "Newton-Schulz steps on each matrix of update [..., m, n] divided by its Frobenius norm; BF16 result",
+          pybind11::arg("update"), pybind11::arg("steps"), pybind11::arg("a"), pybind11::arg("b"), pybind11::arg("c"),
+          pybind11::arg("eps"));
     m.def("device_status", &device_status, "Sticky device-side validation status (code, detail)",
           pybind11::arg("reset") = false);
 }

@@ -32,6 +32,13 @@ from custom_ops_lib import (  # noqa: F401  (GPU layout builders)
     preprocess,
 )
 from custom_ops_lib import pack_rows as _pack_rows, restore_rows as _restore_rows
+from custom_ops_lib import (  # noqa: F401  (layer operators)
+    grouped_matmul as _grouped_matmul,
+    grouped_weight_grad,
+    layer_norm_backward,
+    layer_norm_forward,
+    orthogonalize as _orthogonalize,
+)
 
 
 def _index(inv_permutation, device):
@@ -105,11 +112,97 @@ def restore_node_tensor(packed_tensor, inv_permutation):
     return _RestoreRows.apply(packed_tensor, index)
 
 
+# --------------------------------------------------------------------------
+# Layer operators around the SpMM (no counterpart in the reference)
+# --------------------------------------------------------------------------
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.fp32_bias = bias is not None and bias.dtype == torch.float32
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = layer_norm_backward(grad, x, mean, rstd, weight, *ctx.needs_input_grad[:3], ctx.fp32_bias)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension
+    of a CUDA tensor x (fp16, bf16 or fp32, any width), differentiable in x,
+    weight and bias.
+
+    ``weight`` and ``bias`` ([width], or None for ones and zeros) share one
+    dtype, x's or fp32; their gradients have that dtype.  Sums are fp32 and
+    run in a fixed order.  ``layer_norm_forward`` / ``layer_norm_backward`` are
+    the two passes by themselves.
+    """
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return layer_norm_forward(x, weight, bias, eps, False)[0]
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, group_ptr):
+        ctx.save_for_backward(x, weight, group_ptr)
+        return _grouped_matmul(x, weight, group_ptr, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, group_ptr = ctx.saved_tensors
+        dx = _grouped_matmul(grad, weight, group_ptr, True) if ctx.needs_input_grad[0] else None
+        dw = grouped_weight_grad(x, grad, group_ptr) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def grouped_matmul(x, weight, group_ptr, transposed=False):
+    """Row ranges of x times one matrix each: ``y[r] = x[r] @ weight[g]`` for
+    ``group_ptr[g] <= r < group_ptr[g + 1]``; rows outside every group are zero.
+
+    ``x`` [rows, K], ``weight`` [groups, K, N] (fp16, bf16 or fp32; widths
+    divisible by 16, fp32 by 8), ``group_ptr`` [groups + 1] int32 or int64 on
+    the device, like a CSR row pointer (the relations of a typed graph's
+    messages, the experts of routed rows).  ``transposed`` takes x [rows, N] to
+    [rows, K] by ``weight[g].T``.  Differentiable in x and weight (the plain
+    form); ``grouped_weight_grad`` is the weight's gradient by itself.  A
+    malformed range raises the device status instead of a fault.
+    """
+    if not transposed and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _GroupedMatmul.apply(x, weight, group_ptr)
+    return _grouped_matmul(x, weight, group_ptr, transposed)
+
+
+def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """An update's matrices [..., m, n] with their singular values driven
+    towards one: divided by the Frobenius norm + eps, then ``steps`` times
+    ``G = X X^T; X = a X + (b G + c G G) X`` (the step of an optimiser that
+    orthogonalises its momentum before it is applied to a weight matrix).
+
+    ``update`` is fp16, bf16 or fp32; the result is bf16.  The products run on
+    16-bit operands, so fp32 would hold no more of it.
+    """
+    a, b, c = coefficients
+    return _orthogonalize(update, steps, a, b, c, eps)
+
+
 __all__ = [
     "block_level_split",
     "csr_to_ascend_cube",
     "csr_to_bcsr",
     "csr_to_spmm_cube",
+    "grouped_matmul",
+    "grouped_weight_grad",
+    "layer_norm",
+    "layer_norm_backward",
+    "layer_norm_forward",
+    "orthogonalize",
     "pack_node_tensor",
     "preprocess",
     "restore_node_tensor",

@@ -49,7 +49,8 @@ enum spmm_status {
     SPMM_ERR_WORKSPACE = 6     /* workspace smaller than *_workspace_bytes() */
 };
 
-enum spmm_dtype { SPMM_F16 = 0, SPMM_F32 = 1, SPMM_F64 = 2 };
+/* SPMM_BF16: layer operators only (the SpMM operators take fp16 and fp32). */
+enum spmm_dtype { SPMM_F16 = 0, SPMM_F32 = 1, SPMM_F64 = 2, SPMM_BF16 = 3 };
 enum spmm_itype { SPMM_I32 = 0, SPMM_I64 = 1 };
 
 /* Device-status codes raised by kernels (see spmm_device_status). */
@@ -308,6 +309,64 @@ int spmm_pack_rows_launch(const void *src, const int64_t *inv, int64_t n, int64_
  * for i < n; src has src_rows rows. */
 int spmm_restore_rows_launch(const void *src, int64_t src_rows, const int64_t *inv, int64_t n,
                              int64_t row_bytes, void *dst, void *stream);
+
+/* ---------------------------------------------------------------------- */
+/* Layer operators: what a training step runs around its SpMMs.  No        */
+/* counterpart in the reference.  dtype is SPMM_F16, SPMM_BF16 or SPMM_F32; */
+/* sums are fp32, each result is rounded to its type once.                 */
+/* ---------------------------------------------------------------------- */
+
+/* Layer normalisation of the rows of x [rows, width] (any width >= 1):
+ *   y = (x - mean) / sqrt(var + eps) * weight + bias
+ * weight and bias [width] are of type param_dtype (dtype or SPMM_F32); NULL
+ * means ones and zeros.  mean and rstd [rows] receive each row's mean and
+ * 1 / sqrt(var + eps) for the backward pass; both NULL: not written. */
+int spmm_layer_norm_launch(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd,
+                           int64_t rows, int64_t width, double eps, int dtype, int param_dtype, void *stream);
+
+/* Its gradients: with xhat = (x - mean) * rstd and g = grad * weight,
+ *   dx = rstd * (g - E[g] - xhat * E[g * xhat])   (E over the row)
+ *   dweight = sum over rows of grad * xhat,  dbias = sum over rows of grad
+ * Any of the three outputs may be NULL.  The parameter sums run in a fixed
+ * order (no atomics); with rows == 0 they are zero. */
+size_t spmm_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int spmm_layer_norm_backward_launch(const void *grad, const void *x, const float *mean, const float *rstd,
+                                    const void *weight, void *dx, void *dweight, void *dbias, int64_t rows,
+                                    int64_t width, int dtype, int param_dtype, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
+/* Products of row ranges with one matrix each (relations of a typed graph,
+ * routed experts): group g owns rows group_ptr[g] .. group_ptr[g + 1] of x,
+ * like a row of a CSR row pointer; weight is [groups, K, N].
+ *   transposed == 0:  out [rows, N] = x [rows, K] * weight[g]
+ *   transposed != 0:  out [rows, K] = x [rows, N] * weight[g]^T   (the
+ *                     gradient of the first form's x)
+ * Rows before group_ptr[0] and from group_ptr[groups] on are zero.  A group
+ * whose range is decreasing or leaves [0, rows] is skipped (its rows are
+ * then unspecified) and raises SPMM_DEV_BAD_ROWPTR.  K and N are divisible
+ * by 16 (fp16, bf16) or 8 (fp32). */
+size_t spmm_grouped_matmul_workspace_bytes(int64_t rows, int64_t groups, int64_t K, int64_t N, int transposed,
+                                           int dtype);
+int spmm_grouped_matmul_launch(const void *x, const void *weight, const void *group_ptr, void *out, int64_t rows,
+                               int64_t groups, int64_t K, int64_t N, int transposed, int itype, int dtype,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradient of the weight: dweight[g] [K, N] = x_g^T * grad_g over the rows
+ * of group g (zero for a group without rows); x [rows, K], grad [rows, N]. */
+size_t spmm_grouped_weight_grad_workspace_bytes(int64_t rows, int64_t groups, int64_t K, int64_t N, int dtype);
+int spmm_grouped_weight_grad_launch(const void *x, const void *grad, const void *group_ptr, void *dweight,
+                                    int64_t rows, int64_t groups, int64_t K, int64_t N, int itype, int dtype,
+                                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* Orthogonalised updates: each matrix of update [batch, m, n] is divided by
+ * its Frobenius norm + eps and then taken `steps` times through
+ *   G = X X^T,  X <- a X + (b G + c G G) X
+ * (on the smaller side), which drives its singular values towards one.  out
+ * is bf16 [batch, m, n] whatever the input type. */
+size_t spmm_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n, int dtype);
+int spmm_orthogonalize_launch(const void *update, void *out, int64_t batch, int64_t m, int64_t n, int steps, double a,
+                              double b, double c, double eps, int dtype, void *workspace, size_t workspace_bytes,
+                              void *stream);
 
 #ifdef __cplusplus
 }
