@@ -1,0 +1,56 @@
+// Host side of gemm_tc.cuh: tensor maps.
+#include "gemm_tc.cuh"
+
+#include "engine.h"
+
+namespace spmmb {
+namespace tc {
+
+namespace {
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, found through the runtime (no link against libcuda).
+EncodeTiled encoder()
+{
+    static const EncodeTiled f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) !=
+                cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return f;
+}
+
+}  // namespace
+
+bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
+              int64_t batch_stride, int box_rows, bool bf16)
+{
+    const EncodeTiled encode = encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)batch};
+    const cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)((batch > 1 ? batch_stride : ld) * 2)};
+    const cuuint32_t box[3] = {kBK, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const auto type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    for (int attempt = 0; attempt < 2; ++attempt) {
+        const CUresult r = encode(map, type, 3, const_cast<void *>(p), dims, strides, box, step,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r == CUDA_SUCCESS) return true;
+        // a thread that has made no runtime call yet (an autograd worker) has no
+        // current context: setting its device binds the primary one
+        int dev = 0;
+        if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+            return false;
+    }
+    return false;
+}
+
+}  // namespace tc
+}  // namespace spmmb

@@ -1,0 +1,382 @@
+// Dense products on the fifth-generation tensor cores for the layer
+// operators: 16-bit operands brought in by TMA, fp32 accumulators in TMEM.
+//
+// A persistent block per SM walks output tiles of 128 x BN.  One warp issues
+// the TMA loads of 64-deep slices into a ring of stages, one warp the
+// tcgen05.mma of each slice, and four warps read a finished accumulator out
+// of TMEM, round it and store it while the next tile's products run into the
+// other accumulator.  Operands may be stored with the reduction contiguous
+// (K-major) or with the rows or columns contiguous (MN-major): both layouts
+// are read as they lie, so no product needs a transposed copy.
+//
+// What a tile multiplies depends on the mode:
+//   kRows    a row tile of one group times that group's matrix; the group is
+//            found from the row ranges on the device, and rows of a tile
+//            past its group's end are computed and not stored
+//   kRagged  x_g^T dy_g: the reduction runs over a group's rows; of its last
+//            slice the rows past the group's end are set to zero in shared
+//            memory (in both operands: a neighbour's infinity times zero
+//            would be NaN)
+//   kDense   a batch of equal products
+//
+// Every wait is bounded; a wait that runs out raises SPMM_DEV_TIMEOUT, and
+// the block drains its copies and products, frees its TMEM and returns.
+#pragma once
+
+#include <algorithm>
+
+#include "../../include/spmm_b200.h"
+#include "engine.h"
+#include "layer.cuh"
+#include "tc.cuh"
+
+namespace spmmb {
+namespace tc {
+
+enum Mode { kRows, kRagged, kDense };
+// Epilogues of kDense: see ortho.cu.
+enum Epi { kStore, kGram, kPoly, kUpdate };
+enum OutType { kOutF16, kOutBf16, kOutF32 };
+
+struct GemmArgs {
+    Ranges ranges;            // kRows, kRagged
+    int64_t m, n, k;          // kRows: n, k; kRagged: m, n; kDense: all
+    int64_t batch;            // kDense
+    void *out;
+    int64_t ldo, out_batch;   // elements
+    int out_type;
+    bool bf16;                // operand type (else fp16)
+    // The reduction is run `passes` times over planes pa[i], pb[i] of the
+    // operands (plane p of A starts at batch index p * za, of B at p * zb).
+    int passes, za, zb;
+    unsigned char pa[6], pb[6];
+    // kDense epilogues: x = alpha * accumulator + beta * (in + in_lo)
+    float alpha, beta;
+    const __half *in, *in_lo;
+    __half *out_lo;
+    int64_t ldi;
+    DevStatus *status;
+};
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kGemmThreads = 192;   // TMA warp, MMA warp, four epilogue warps
+
+template <int BN> struct GemmShape {
+    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2;
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kChunk = BN < 128 ? 128 : 256;          // bytes of a row staged at a time
+    static constexpr int kPitch = kChunk + 16;                   // odd in 16-byte units: no bank conflicts
+    static constexpr int kStageOff = kStages * (kA + kB);
+    static constexpr int kBarOff = kStageOff + kBM * kPitch;
+    static constexpr int kFull = kBarOff, kEmpty = kFull + 8 * kStages, kAccFull = kEmpty + 8 * kStages;
+    static constexpr int kAccEmpty = kAccFull + 16, kDone = kAccEmpty + 16, kTmem = kDone + 8, kAbort = kTmem + 4;
+    static constexpr int kBytes = kAbort + 4;
+    static constexpr int kCols = 2 * BN;                         // TMEM columns of the two accumulators
+    static_assert(kBytes <= 232448, "shared memory of a block");
+};
+
+// One output tile as each role sees it.
+struct Tile {
+    int64_t batch_a, batch_b, row0, col0;   // operand batch, first row and column
+    int64_t k0, k1;                         // range of the reduction (k0 == k1: zeros)
+    int64_t out;                            // element offset of the tile in `out`
+    int rows, cols;                         // what is stored
+    bool mirror;                            // kGram, kPoly: also the transposed tile
+};
+
+template <int MODE, int BN, int EPI> struct Walk {
+    const GemmArgs &a;
+    TileWalk ranges;
+    int64_t mt, nt;
+    __device__ Walk(const GemmArgs &a) : a(a), mt((a.m + kBM - 1) / kBM), nt((a.n + BN - 1) / BN) {}
+
+    // Warp-wide; `t` must not decrease.  False past the last tile.
+    __device__ __forceinline__ bool at(int64_t t, Tile *o)
+    {
+        if constexpr (MODE == kRows) {
+            int64_t seg, b, e, inner;
+            if (!ranges.find(a.ranges, kBM, nt, t, a.status, &seg, &b, &e, &inner)) return false;
+            o->row0 = b + inner / nt * kBM;
+            o->col0 = inner % nt * BN;
+            o->batch_a = 0;
+            o->batch_b = seg - 1;
+            o->k0 = 0;
+            o->k1 = seg >= 1 && seg <= a.ranges.groups ? a.k : 0;
+            o->rows = (int)min((int64_t)kBM, e - o->row0);
+            o->out = o->row0 * a.ldo + o->col0;
+        } else if constexpr (MODE == kRagged) {
+            if (t >= a.ranges.groups * mt * nt) return false;
+            const int64_t g = t / (mt * nt), i = t % (mt * nt);
+            segment_rows(a.ranges, g + 1, &o->k0, &o->k1, a.status);
+            o->row0 = i / nt * kBM;
+            o->col0 = i % nt * BN;
+            o->batch_a = o->batch_b = 0;
+            o->rows = (int)min((int64_t)kBM, a.m - o->row0);
+            o->out = g * a.out_batch + o->row0 * a.ldo + o->col0;
+        } else {
+            const bool half = EPI == kGram || EPI == kPoly;   // symmetric: the tiles on and below the diagonal
+            const int64_t per = half ? mt * (mt + 1) / 2 : mt * nt;
+            if (t >= a.batch * per) return false;
+            const int64_t q = t / per, r = t % per;
+            int64_t i, j;
+            if (half) {
+                i = (int64_t)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
+                while (i * (i + 1) / 2 > r) --i;
+                while ((i + 1) * (i + 2) / 2 <= r) ++i;
+                j = r - i * (i + 1) / 2;
+            } else {
+                i = r / nt;
+                j = r % nt;
+            }
+            o->batch_a = o->batch_b = q;
+            o->row0 = i * kBM;
+            o->col0 = j * BN;
+            o->k0 = 0;
+            o->k1 = a.k;
+            o->rows = (int)min((int64_t)kBM, a.m - o->row0);
+            o->out = q * a.out_batch + o->row0 * a.ldo + o->col0;
+            o->mirror = half && i != j;
+        }
+        o->cols = (int)min((int64_t)BN, a.n - o->col0);
+        return true;
+    }
+};
+
+template <int BITS> __device__ __forceinline__ uint4 pack8(const float *v, bool bf16)
+{
+    uint4 w;
+    unsigned *u = reinterpret_cast<unsigned *>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (bf16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *reinterpret_cast<const unsigned *>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *reinterpret_cast<const unsigned *>(&h);
+        }
+    }
+    return w;
+}
+
+__device__ __forceinline__ void st_shared16(unsigned at, uint4 v)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+
+template <int MODE, int BN, bool AMN, bool BMN, int EPI>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+            const __grid_constant__ GemmArgs a)
+{
+    using S = GemmShape<BN>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *abort = reinterpret_cast<volatile int *>(smem + S::kAbort);
+    const unsigned full = base + S::kFull, empty = base + S::kEmpty;
+    const unsigned acc_full = base + S::kAccFull, acc_empty = base + S::kAccEmpty, done = base + S::kDone;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            bar_init(full + 8 * i, 1);
+            bar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(acc_full + 8 * i, 1);
+            bar_init(acc_empty + 8 * i, 4);
+        }
+        bar_init(done, 1);
+        // a misaligned stage ring would break the swizzle: give up before any copy
+        *abort = (base & 1023u) ? 1 : 0;
+        if (base & 1023u) raise_status(a.status, SPMM_DEV_TIMEOUT, -1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(base + S::kTmem),
+                     "r"(S::kCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const unsigned tmem = *reinterpret_cast<volatile unsigned *>(smem + S::kTmem);
+
+    Walk<MODE, BN, EPI> walk(a);
+    Tile t;
+    bool ok = *abort == 0;
+    auto give_up = [&](int code) {
+        if (*abort == 0) raise_status(a.status, SPMM_DEV_TIMEOUT, code);
+        *abort = 1;
+        ok = false;
+    };
+
+    if (warp == 0) {
+        // ---- TMA warp: one lane issues
+        unsigned slice = 0;   // slices issued
+        for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
+            for (int pass = 0; pass < a.passes && ok; ++pass) {
+                const int za = (int)t.batch_a + a.pa[pass] * a.za, zb = (int)t.batch_b + a.pb[pass] * a.zb;
+                for (int64_t k = t.k0; k < t.k1; k += kBK, ++slice) {
+                    const unsigned st = slice % S::kStages;
+                    if (!bar_wait(empty + 8 * st, (slice / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
+                    if (lane == 0) {
+                        const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA, bar = full + 8 * st;
+                        bar_expect(bar, S::kA + S::kB);
+                        if constexpr (AMN) {
+#pragma unroll
+                            for (int i = 0; i < kBM / 64; ++i)
+                                tma_load(sa + i * 8192, &map_a, (int)t.row0 + 64 * i, (int)k, za, bar);
+                        } else {
+                            tma_load(sa, &map_a, (int)k, (int)t.row0, za, bar);
+                        }
+                        if constexpr (BMN) {
+#pragma unroll
+                            for (int i = 0; i < BN / 64; ++i)
+                                tma_load(sb + i * 8192, &map_b, (int)t.col0 + 64 * i, (int)k, zb, bar);
+                        } else {
+                            tma_load(sb, &map_b, (int)k, (int)t.col0, zb, bar);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (!ok)   // the copies in flight land before the block leaves (bounded)
+            for (unsigned s = slice > S::kStages ? slice - S::kStages : 0; s < slice; ++s) {
+                volatile int never = 0;
+                bar_wait(full + 8 * (s % S::kStages), s / S::kStages & 1u, &never);
+            }
+    } else if (warp == 1) {
+        // ---- MMA warp
+        const unsigned idesc = idesc16(a.bf16, AMN, BMN, kBM, BN);
+        // byte strides of the operands' layouts: K-major, 8 rows of 128 bytes per
+        // swizzle atom; MN-major, atoms of 64 rows or columns x 8 deep, 8 KB apart
+        const uint64_t da = AMN ? desc128(base, 8192, 1024) : desc128(base, 16, 1024);
+        const uint64_t db = BMN ? desc128(base + S::kA, 8192, 1024) : desc128(base + S::kA, 16, 1024);
+        constexpr unsigned step_a = (AMN ? 2048 : 32) >> 4, step_b = (BMN ? 2048 : 32) >> 4;
+        unsigned slice = 0, used = 0;
+        for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
+            if (t.k0 >= t.k1) continue;
+            const unsigned acc = used & 1u;
+            if (!bar_wait(acc_empty + 8 * acc, (used >> 1 & 1u) ^ 1u, abort)) { give_up(2); break; }
+            fence_after();
+            unsigned first = 1;
+            for (int pass = 0; pass < a.passes && ok; ++pass)
+                for (int64_t k = t.k0; k < t.k1; k += kBK, ++slice) {
+                    const unsigned st = slice % S::kStages;
+                    if (!bar_wait(full + 8 * st, slice / S::kStages & 1u, abort)) { give_up(3); break; }
+                    const int depth = (int)min((int64_t)kBK, t.k1 - k);
+                    if (MODE == kRagged && (depth & 15)) {
+                        // rows [depth, next 16) of both operands: zero
+                        const unsigned at = base + st * (S::kA + S::kB);
+                        const int pad = 16 - (depth & 15), quads = pad * 8;   // 16-byte pieces of a 64-wide column block
+                        for (int i = lane; i < quads * ((S::kA + S::kB) / 8192); i += 32)
+                            st_shared16(at + i / quads * 8192 + depth * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
+                        fence_async();
+                        __syncwarp();
+                    }
+                    fence_after();
+                    if (lane == 0) {
+                        const unsigned off = st * (S::kA + S::kB) >> 4;
+                        for (int i = 0; i * 16 < depth; ++i) {
+                            mma(tmem + acc * BN, da + off + i * step_a, db + off + i * step_b, idesc, first ? 0u : 1u);
+                            first = 0;
+                        }
+                        commit(empty + 8 * st);
+                    }
+                    __syncwarp();
+                }
+            if (!ok) break;
+            if (lane == 0) commit(acc_full + 8 * acc);
+            __syncwarp();
+            ++used;
+        }
+        if (!ok) {   // every product issued is complete before TMEM is freed (bounded)
+            volatile int never = 0;
+            if (lane == 0) commit(done);
+            __syncwarp();
+            bar_wait(done, 0, &never);
+        }
+    } else {
+        // ---- epilogue warps: TMEM lanes 32 (warp % 4) .. + 31 are rows of the tile
+        const int row = (warp & 3) * 32 + lane;
+        const unsigned stage = base + S::kStageOff + row * S::kPitch;
+        const unsigned lanes = tmem + ((unsigned)((warp & 3) * 32) << 16);
+        const int es = a.out_type == kOutF32 ? 4 : 2, chunk = S::kChunk / es;
+        unsigned used = 0;
+        for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
+            const bool zero = t.k0 >= t.k1;
+            const unsigned acc = used & 1u;
+            if (!zero) {
+                if (!bar_wait(acc_full + 8 * acc, used >> 1 & 1u, abort)) { give_up(4); break; }
+                fence_after();
+                ++used;
+            }
+            const bool on = row < t.rows;
+            for (int c0 = 0; c0 < t.cols; c0 += chunk) {
+                bulk_wait_read();
+                for (int c = 0; c < chunk && c0 + c < t.cols; c += 32) {
+                    float v[32];
+                    if (zero) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                    } else {
+                        tmem_ld32(lanes + acc * BN + c0 + c, v);
+                    }
+                    if (es == 4) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            st_shared16(stage + c * 4 + i * 16,
+                                        make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                                                   __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            st_shared16(stage + c * 2 + i * 16, pack8<16>(v + 8 * i, a.out_type == kOutBf16));
+                    }
+                }
+                const int cols = min(chunk, t.cols - c0);
+                if (on) {
+                    fence_async();
+                    bulk_store(static_cast<char *>(a.out) + (t.out + row * a.ldo + c0) * es, stage, cols * es);
+                }
+                bulk_commit();
+            }
+            if (!zero) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+            }
+        }
+        bulk_wait();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::kCols) : "memory");
+}
+
+// Tensor map of a 16-bit operand [batch][rows][inner] (strides in elements),
+// read in boxes of 64 elements x box_rows, 128-byte swizzled, zero outside.
+bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
+              int64_t batch_stride, int box_rows, bool bf16);
+
+template <int MODE, int BN, bool AMN, bool BMN, int EPI>
+cudaError_t launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, const GemmArgs &a, int64_t tiles, cudaStream_t s)
+{
+    auto kernel = gemm_kernel<MODE, BN, AMN, BMN, EPI>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmShape<BN>::kBytes);
+    if (e != cudaSuccess) return e;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count()));
+    kernel<<<grid, kGemmThreads, GemmShape<BN>::kBytes, s>>>(ma, mb, a);
+    return cudaGetLastError();
+}
+
+}  // namespace tc
+}  // namespace spmmb

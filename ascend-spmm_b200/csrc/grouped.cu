@@ -10,6 +10,7 @@
 #include "../../include/spmm_b200.h"
 #include "common.cuh"
 #include "engine.h"
+#include "gemm_tc.cuh"
 #include "layer.cuh"
 #include "layer.h"
 
@@ -18,6 +19,11 @@ namespace spmmb {
 namespace {
 
 constexpr int kTile = 64, kDepth = 16, kThreads = 256;
+
+__host__ __device__ Ranges ranges_of(const GroupedLaunch &a)
+{
+    return Ranges{a.ptr, a.itype == SPMM_I64, a.groups, a.rows};
+}
 
 // acc[4][4] of thread (ty, tx) += A[m, k] B[k, n] over one 64 x 64 tile, operands read by strides.
 template <typename T>
@@ -59,16 +65,14 @@ __device__ __forceinline__ void simt_store(T *C, int64_t ldc, int64_t m, int64_t
             if (ty * 4 + i < m && tx * 4 + j < n) C[(ty * 4 + i) * ldc + tx * 4 + j] = elem_of<T>(acc[i][j]);
 }
 
-template <typename T, typename I>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) grouped_rows_simt_kernel(const GroupedLaunch a)
 {
     __shared__ int64_t where[4];
     if (threadIdx.x < 32) {
         TileWalk walk;
         int64_t seg = -1, b = 0, e = 0, inner = 0;
-        if (!walk.find(static_cast<const I *>(a.ptr), a.groups, a.rows, kTile, 1, blockIdx.x, a.status, &seg, &b, &e,
-                       &inner))
-            seg = -1;
+        if (!walk.find(ranges_of(a), kTile, 1, blockIdx.x, a.status, &seg, &b, &e, &inner)) seg = -1;
         if (threadIdx.x == 0) { where[0] = seg; where[1] = b; where[2] = e; where[3] = inner; }
     }
     __syncthreads();
@@ -86,13 +90,13 @@ __global__ void __launch_bounds__(kThreads) grouped_rows_simt_kernel(const Group
     simt_store<T>(static_cast<T *>(a.out) + r0 * width + c0, width, m, n, acc);
 }
 
-template <typename T, typename I>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) grouped_weight_grad_simt_kernel(const GroupedLaunch a)
 {
     const int64_t tiles = (a.K + kTile - 1) / kTile;
     const int64_t g = blockIdx.x / tiles, i0 = blockIdx.x % tiles * kTile, c0 = (int64_t)blockIdx.y * kTile;
     int64_t b, e;
-    segment_rows(static_cast<const I *>(a.ptr), a.groups, a.rows, g + 1, &b, &e, a.status);
+    segment_rows(ranges_of(a), g + 1, &b, &e, a.status);
     const int64_t m = min((int64_t)kTile, a.K - i0), n = min((int64_t)kTile, a.N - c0);
     float acc[4][4] = {};
     simt_tile<T>(static_cast<const T *>(a.x) + b * a.K + i0, 1, a.K, m, static_cast<const T *>(a.w) + b * a.N + c0, a.N,
@@ -104,17 +108,94 @@ template <typename T> cudaError_t rows_simt(const GroupedLaunch &a, cudaStream_t
 {
     const int64_t width = a.transposed ? a.K : a.N;
     const dim3 grid((unsigned)((a.rows + kTile - 1) / kTile + a.groups + 2), (unsigned)((width + kTile - 1) / kTile));
-    if (a.itype == SPMM_I32) grouped_rows_simt_kernel<T, int><<<grid, kThreads, 0, stream>>>(a);
-    else grouped_rows_simt_kernel<T, int64_t><<<grid, kThreads, 0, stream>>>(a);
+    grouped_rows_simt_kernel<T><<<grid, kThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
 template <typename T> cudaError_t weight_grad_simt(const GroupedLaunch &a, cudaStream_t stream)
 {
     const dim3 grid((unsigned)((a.K + kTile - 1) / kTile * a.groups), (unsigned)((a.N + kTile - 1) / kTile));
-    if (a.itype == SPMM_I32) grouped_weight_grad_simt_kernel<T, int><<<grid, kThreads, 0, stream>>>(a);
-    else grouped_weight_grad_simt_kernel<T, int64_t><<<grid, kThreads, 0, stream>>>(a);
+    grouped_weight_grad_simt_kernel<T><<<grid, kThreads, 0, stream>>>(a);
     return cudaGetLastError();
+}
+
+// ---- 16-bit types: the tensor-core kernels of gemm_tc.cuh ------------------
+
+// Columns per tile: the widest that the output's width fills and that still
+// gives every SM a tile (a narrower tile reads the row operand more often).
+int tile_columns(int64_t row_tiles, int64_t width)
+{
+    const int sms = device_sm_count();
+    if (width > 128 && row_tiles * ((width + 255) / 256) >= sms) return 256;
+    if (width > 64 && row_tiles * ((width + 127) / 128) >= sms) return 128;
+    return 64;
+}
+
+template <int BN> cudaError_t rows_tc(const GroupedLaunch &a, tc::GemmArgs &g, int64_t row_tiles, cudaStream_t stream)
+{
+    CUtensorMap ma, mb;
+    const bool bf = g.bf16;
+    const int64_t tiles = row_tiles * ((g.n + BN - 1) / BN);
+    if (!tc::make_map(&ma, a.x, g.k, a.rows, 1, g.k, 0, tc::kBM, bf)) return cudaErrorInvalidValue;
+    const int64_t groups = std::max<int64_t>(a.groups, 1);
+    const void *w = a.groups > 0 ? a.w : a.x;   // no group: the map is never read
+    if (!tc::make_map(&mb, w, a.N, a.groups > 0 ? a.K : 1, groups, a.N, a.K * a.N, a.transposed ? BN : 64, bf))
+        return cudaErrorInvalidValue;
+    if (a.transposed) return tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(ma, mb, g, tiles, stream);
+    return tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(ma, mb, g, tiles, stream);
+}
+
+cudaError_t launch_rows_tc(const GroupedLaunch &a, cudaStream_t stream)
+{
+    tc::GemmArgs g{};
+    g.ranges = ranges_of(a);
+    g.n = a.transposed ? a.K : a.N;
+    g.k = a.transposed ? a.N : a.K;
+    g.out = a.out;
+    g.ldo = g.n;
+    g.bf16 = a.dtype == SPMM_BF16;
+    g.out_type = g.bf16 ? tc::kOutBf16 : tc::kOutF16;
+    g.passes = 1;
+    g.status = a.status;
+    // every group can end in a partial tile; segments outside the groups too
+    const int64_t row_tiles = std::min(a.rows, (a.rows + tc::kBM - 1) / tc::kBM + a.groups + 1);
+    switch (tile_columns(row_tiles, g.n)) {
+        case 256: return rows_tc<256>(a, g, row_tiles, stream);
+        case 128: return rows_tc<128>(a, g, row_tiles, stream);
+        default: return rows_tc<64>(a, g, row_tiles, stream);
+    }
+}
+
+template <int BN> cudaError_t weight_grad_tc(const GroupedLaunch &a, tc::GemmArgs &g, cudaStream_t stream)
+{
+    CUtensorMap ma, mb;
+    const bool bf = g.bf16;
+    const int64_t rows = std::max<int64_t>(a.rows, 1);
+    const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: the maps are never read
+    if (!tc::make_map(&ma, x, a.K, rows, 1, a.K, 0, 64, bf) || !tc::make_map(&mb, dy, a.N, rows, 1, a.N, 0, 64, bf))
+        return cudaErrorInvalidValue;
+    const int64_t tiles = a.groups * ((a.K + tc::kBM - 1) / tc::kBM) * ((a.N + BN - 1) / BN);
+    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(ma, mb, g, tiles, stream);
+}
+
+cudaError_t launch_weight_grad_tc(const GroupedLaunch &a, cudaStream_t stream)
+{
+    tc::GemmArgs g{};
+    g.ranges = ranges_of(a);
+    g.m = a.K;
+    g.n = a.N;
+    g.out = a.out;
+    g.ldo = a.N;
+    g.out_batch = a.K * a.N;
+    g.bf16 = a.dtype == SPMM_BF16;
+    g.out_type = g.bf16 ? tc::kOutBf16 : tc::kOutF16;
+    g.passes = 1;
+    g.status = a.status;
+    switch (tile_columns(a.groups * ((a.K + tc::kBM - 1) / tc::kBM), a.N)) {
+        case 256: return weight_grad_tc<256>(a, g, stream);
+        case 128: return weight_grad_tc<128>(a, g, stream);
+        default: return weight_grad_tc<64>(a, g, stream);
+    }
 }
 
 }  // namespace
@@ -124,20 +205,12 @@ size_t grouped_weight_grad_workspace(int64_t, int64_t, int64_t, int64_t, int) { 
 
 cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *, cudaStream_t stream)
 {
-    switch (a.dtype) {
-        case SPMM_F16: return rows_simt<__half>(a, stream);
-        case SPMM_BF16: return rows_simt<__nv_bfloat16>(a, stream);
-        default: return rows_simt<float>(a, stream);
-    }
+    return a.dtype == SPMM_F32 ? rows_simt<float>(a, stream) : launch_rows_tc(a, stream);
 }
 
 cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *, cudaStream_t stream)
 {
-    switch (a.dtype) {
-        case SPMM_F16: return weight_grad_simt<__half>(a, stream);
-        case SPMM_BF16: return weight_grad_simt<__nv_bfloat16>(a, stream);
-        default: return weight_grad_simt<float>(a, stream);
-    }
+    return a.dtype == SPMM_F32 ? weight_grad_simt<float>(a, stream) : launch_weight_grad_tc(a, stream);
 }
 
 }  // namespace spmmb

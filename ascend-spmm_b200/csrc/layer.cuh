@@ -22,49 +22,54 @@ template <> __device__ __forceinline__ float elem_of<float>(float x) { return x;
 // the first group, segment g + 1 is group g, segment groups + 1 the rows
 // after the last group (0 and groups + 1 get zeros).  A malformed group is
 // empty.
-template <typename I>
-__device__ __forceinline__ void segment_rows(const I *ptr, int64_t groups, int64_t rows, int64_t s, int64_t *begin,
-                                             int64_t *end, DevStatus *status)
+struct Ranges {
+    const void *ptr;        // [groups + 1], int32 or int64
+    bool wide;              // int64
+    int64_t groups, rows;
+    __device__ __forceinline__ int64_t operator[](int64_t i) const
+    {
+        return wide ? ld_idx(static_cast<const int64_t *>(ptr) + i) : ld_idx(static_cast<const int *>(ptr) + i);
+    }
+};
+
+__device__ __forceinline__ void segment_rows(const Ranges &p, int64_t s, int64_t *begin, int64_t *end, DevStatus *status)
 {
     int64_t b = 0, e = 0;
     if (s == 0) {
-        e = min(max((int64_t)ptr[0], (int64_t)0), rows);
-    } else if (s <= groups) {
-        b = (int64_t)ptr[s - 1];
-        e = (int64_t)ptr[s];
-        if (b < 0 || e < b || e > rows) {
+        e = min(max(p[0], (int64_t)0), p.rows);
+    } else if (s <= p.groups) {
+        b = p[s - 1];
+        e = p[s];
+        if (b < 0 || e < b || e > p.rows) {
             raise_status(status, SPMM_DEV_BAD_ROWPTR, s - 1);
             b = e = 0;
         }
-    } else if (s == groups + 1) {
-        b = min(max((int64_t)ptr[groups], (int64_t)0), rows);
-        e = rows;
+    } else if (s == p.groups + 1) {
+        b = min(max(p[p.groups], (int64_t)0), p.rows);
+        e = p.rows;
     }
     *begin = b;
     *end = e;
 }
 
-// Walks the row tiles of all segments in order.  Every lane of the warp calls
-// it with the same arguments; `tile` must not decrease from call to call.
+// Walks the tiles of all segments in order: `height` rows and `mult` column
+// tiles each.  Every lane of the warp calls it with the same arguments;
+// `tile` must not decrease from call to call.
 struct TileWalk {
     int64_t base = 0;    // segments before the current 32
     int64_t before = 0;  // tiles of the segments before `base`
     int64_t count = -1;  // this lane's segment: its tiles, rows and the tiles before it
     int64_t begin = 0, end = 0, first = 0;
 
-    // Finds the segment of `tile`: its index (0 .. groups + 1), its rows and
-    // the tile's number within it; false past the last tile.
-    // `mult` tiles per row tile (column tiles), `height` rows per row tile.
-    template <typename I>
-    __device__ __forceinline__ bool find(const I *ptr, int64_t groups, int64_t rows, int height, int64_t mult,
-                                         int64_t tile, DevStatus *status, int64_t *seg, int64_t *b, int64_t *e,
-                                         int64_t *inner)
+    // The segment of `tile` (0 .. groups + 1), its rows and the tile's number
+    // within it; false past the last tile.
+    __device__ __forceinline__ bool find(const Ranges &p, int height, int64_t mult, int64_t tile, DevStatus *status,
+                                         int64_t *seg, int64_t *b, int64_t *e, int64_t *inner)
     {
         const int lane = threadIdx.x & 31;
         for (;;) {
             if (count < 0) {
-                const int64_t s = base + lane;
-                segment_rows(ptr, groups, rows, s, &begin, &end, status);
+                segment_rows(p, base + lane, &begin, &end, status);
                 count = (end - begin + height - 1) / height * mult;
                 int64_t sum = count;
 #pragma unroll
@@ -87,7 +92,7 @@ struct TileWalk {
             before += total;
             base += 32;
             count = -1;
-            if (base >= groups + 2) return false;
+            if (base >= p.groups + 2) return false;
         }
     }
 };
