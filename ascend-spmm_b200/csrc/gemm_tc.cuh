@@ -50,11 +50,15 @@ struct GemmArgs {
     // operands (plane p of A starts at batch index p * za, of B at p * zb).
     int passes, za, zb;
     unsigned char pa[6], pb[6];
-    // kDense epilogues: x = alpha * accumulator + beta * (in + in_lo)
+    // kGram: x = alpha * accumulator; kPoly, kUpdate: x = alpha * accumulator
+    // + beta * (in + in_lo), `in` laid out as the output.  kGram and kPoly
+    // are symmetric and also write the transposed tile; kUpdate writes x as
+    // fp16 and, to out_lo, the rest that the rounding left (out_lo null: x
+    // alone, in the output's type).
     float alpha, beta;
     const __half *in, *in_lo;
     __half *out_lo;
-    int64_t ldi;
+    int64_t ldi, in_batch;
     DevStatus *status;
 };
 
@@ -64,7 +68,7 @@ constexpr int kGemmThreads = 192;   // TMA warp, MMA warp, four epilogue warps
 template <int BN> struct GemmShape {
     static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int kChunk = BN < 128 ? 128 : 256;          // bytes of a row staged at a time
+    static constexpr int kChunk = 256;                           // bytes of a row staged at a time
     static constexpr int kPitch = kChunk + 16;                   // odd in 16-byte units: no bank conflicts
     static constexpr int kStageOff = kStages * (kA + kB);
     static constexpr int kBarOff = kStageOff + kBM * kPitch;
@@ -142,7 +146,7 @@ template <int MODE, int BN, int EPI> struct Walk {
     }
 };
 
-template <int BITS> __device__ __forceinline__ uint4 pack8(const float *v, bool bf16)
+__device__ __forceinline__ uint4 pack8(const float *v, bool bf16)
 {
     uint4 w;
     unsigned *u = reinterpret_cast<unsigned *>(&w);
@@ -307,7 +311,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const int row = (warp & 3) * 32 + lane;
         const unsigned stage = base + S::kStageOff + row * S::kPitch;
         const unsigned lanes = tmem + ((unsigned)((warp & 3) * 32) << 16);
-        const int es = a.out_type == kOutF32 ? 4 : 2, chunk = S::kChunk / es;
+        const int es = a.out_type == kOutF32 ? 4 : 2;
+        // kUpdate stages 64 columns of the high and of the low part side by side
+        const int chunk = EPI == kUpdate ? 64 : S::kChunk / es;
+        // rows that do not start on 16 bytes cannot be bulk-copied
+        const bool bulk = (a.ldo * es & 15) == 0 && (a.out_batch * es & 15) == 0;
         unsigned used = 0;
         for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
             const bool zero = t.k0 >= t.k1;
@@ -320,6 +328,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const bool on = row < t.rows;
             for (int c0 = 0; c0 < t.cols; c0 += chunk) {
                 bulk_wait_read();
+                if (EPI == kUpdate && !bulk) __syncwarp();   // the warp reads its rows' staging across lanes below
                 for (int c = 0; c < chunk && c0 + c < t.cols; c += 32) {
                     float v[32];
                     if (zero) {
@@ -327,6 +336,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         for (int i = 0; i < 32; ++i) v[i] = 0.f;
                     } else {
                         tmem_ld32(lanes + acc * BN + c0 + c, v);
+                    }
+                    if constexpr (EPI != kStore) {
+                        const int64_t at = t.batch_a * a.in_batch + (t.row0 + row) * a.ldi + t.col0 + c0 + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                            if (EPI != kGram && on && t.col0 + c0 + c + i < a.ldi) {
+                                hi = *reinterpret_cast<const uint4 *>(a.in + at + i);
+                                if (EPI == kUpdate) lo = *reinterpret_cast<const uint4 *>(a.in_lo + at + i);
+                            }
+                            float h[8], l[8];
+                            unpack16<__half>(hi, h);
+                            unpack16<__half>(lo, l);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                v[i + e] = EPI == kGram ? a.alpha * v[i + e]
+                                                        : fmaf(a.alpha, v[i + e], a.beta * (h[e] + l[e]));
+                        }
                     }
                     if (es == 4) {
 #pragma unroll
@@ -336,16 +363,48 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                                    __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])));
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            st_shared16(stage + c * 2 + i * 16, pack8<16>(v + 8 * i, a.out_type == kOutBf16));
+                        for (int i = 0; i < 4; ++i) {
+                            const uint4 w = pack8(v + 8 * i, a.out_type == kOutBf16);
+                            st_shared16(stage + c * 2 + i * 16, w);
+                            if (EPI == kUpdate && a.out_lo) {   // what the high part's rounding left
+                                float h[8];
+                                unpack16<__half>(w, h);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) h[e] = v[8 * i + e] - h[e];
+                                st_shared16(stage + 128 + c * 2 + i * 16, pack8(h, false));
+                            }
+                        }
+                    }
+                    if ((EPI == kGram || EPI == kPoly) && t.mirror && on) {
+                        // lanes hold consecutive rows: 64 contiguous bytes per column
+                        __half *o = static_cast<__half *>(a.out) + t.batch_a * a.out_batch +
+                                    (t.col0 + c0 + c) * a.ldo + t.row0 + row;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (c0 + c + i < t.cols) o[i * a.ldo] = __float2half_rn(v[i]);
                     }
                 }
                 const int cols = min(chunk, t.cols - c0);
-                if (on) {
-                    fence_async();
-                    bulk_store(static_cast<char *>(a.out) + (t.out + row * a.ldo + c0) * es, stage, cols * es);
+                if (EPI != kUpdate || bulk) {
+                    // a row's last 16-byte piece may end in the padding of its leading dimension
+                    const unsigned bytes = (unsigned)(cols * es + 15) & ~15u;
+                    if (on) {
+                        const int64_t at = t.out + row * a.ldo + c0;
+                        fence_async();
+                        bulk_store(static_cast<char *>(a.out) + at * es, stage, bytes);
+                        if (EPI == kUpdate && a.out_lo) bulk_store(a.out_lo + at, stage + 128, bytes);
+                    }
+                    bulk_commit();
+                } else {
+                    __syncwarp();
+                    for (int r = 0; r < 32 && (warp & 3) * 32 + r < t.rows; ++r) {
+                        const unsigned char *src = smem + S::kStageOff + ((warp & 3) * 32 + r) * S::kPitch;
+                        unsigned short *o = static_cast<unsigned short *>(a.out) + t.out +
+                                            ((warp & 3) * 32 + r) * a.ldo + c0;
+                        for (int c = lane; c < cols; c += 32) o[c] = reinterpret_cast<const unsigned short *>(src)[c];
+                    }
+                    __syncwarp();
                 }
-                bulk_commit();
             }
             if (!zero) {
                 fence_before();

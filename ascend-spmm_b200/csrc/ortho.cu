@@ -1,13 +1,26 @@
 // Orthogonalised updates: X0 = U / (|U|_F + eps), then `steps` times
 //   G = X X^T,  P = b G + c G G,  X <- a X + P X
-// on the smaller side s of the matrix (a tall matrix is worked on as its
-// transpose).  Each step is two symmetric s x s products and one s x s by
-// s x r product.
+// on the smaller side s of the matrix (for a tall one G = X^T X and
+// X <- a X + X P, the same polynomial).  Each step is two symmetric s x s
+// products, of which the tiles on and below the diagonal are computed and
+// written twice, and one s x s by s x r product; all run on the tensor cores
+// (gemm_tc.cuh), which read X, G and P as they lie, so nothing is transposed.
+//
+// Precision.  The operands are fp16, not bf16: every singular value stays of
+// order one (the polynomial maps [0, 1.3] into itself), so the elements need
+// no exponent range, and 11 bits instead of 8 take the result's error from
+// 1e-2 to about 2e-3.  X is kept as a high and a low fp16 part (22 bits): the
+// products take the high part, the term a X both.  Otherwise the rounding of
+// X would be multiplied by a in every step along the directions whose
+// singular values are still small: 5e-3 after five steps on a low-rank update
+// with noise, 2e-4 with the low part.  Powers of two scale the stored values
+// away from fp16's subnormals and leave a factor of 100 below its maximum.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
 #include "common.cuh"
 #include "engine.h"
+#include "gemm_tc.cuh"
 #include "layer.cuh"
 #include "layer.h"
 
@@ -15,19 +28,35 @@ namespace spmmb {
 
 namespace {
 
-constexpr int kTile = 64, kDepth = 16, kThreads = 256;
+constexpr float kScaleX = 512.f, kScaleG = 256.f, kScaleP = 256.f;   // stored = value * scale
+constexpr int kParts = 64;                                           // partial sums of squares per matrix, at most
 
-// 1 / (|U|_F + eps) of each matrix: one block per matrix, squares summed in
-// 64 bits (an fp32 update's squares can pass fp32's range).
+int64_t pad8(int64_t x) { return (x + 7) & ~int64_t(7); }
+
+// Sums of squares, in 64 bits (an fp32 update's squares can leave fp32's range).
 template <typename T>
-__global__ void __launch_bounds__(1024) ortho_norm_kernel(const T *u, int64_t elems, float eps, float *scale)
+__global__ void __launch_bounds__(256) ortho_squares_kernel(const T *u, int64_t elems, double *part)
 {
-    __shared__ double red[32];
-    const T *p = u + (int64_t)blockIdx.x * elems;
+    __shared__ double red[8];
+    constexpr int V = 16 / sizeof(T);
+    const T *p = u + (int64_t)blockIdx.y * elems;
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < elems; i += 1024) {
-        const double v = (double)elem_f32<T>(p[i]);
-        s += v * v;
+    const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (elems % V == 0) {
+        for (int64_t i = first; i < elems / V; i += step) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const double v = (double)elem_f32<T>(e[k]);
+                s += v * v;
+            }
+        }
+    } else {
+        for (int64_t i = first; i < elems; i += step) {
+            const double v = (double)elem_f32<T>(p[i]);
+            s += v * v;
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -35,110 +64,186 @@ __global__ void __launch_bounds__(1024) ortho_norm_kernel(const T *u, int64_t el
     __syncthreads();
     if (threadIdx.x == 0) {
         s = 0.0;
-        for (int w = 0; w < 32; ++w) s += red[w];
-        scale[blockIdx.x] = (float)(1.0 / (sqrt(s) + (double)eps));
+        for (int w = 0; w < 8; ++w) s += red[w];
+        part[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
     }
 }
 
-// X [s, r] in fp32 from the update (transposed when it is tall).
+// X0 as its high and low parts [m][ld] (a thread: 8 columns), or, with no
+// step to follow, the bf16 result.
 template <typename T>
-__global__ void ortho_load_kernel(const T *u, const float *scale, float *x, int64_t m, int64_t n, int64_t batch)
+__global__ void __launch_bounds__(256)
+ortho_split_kernel(const T *u, const double *part, int parts, float eps, int64_t m, int64_t n, int64_t ld, __half *hi,
+                   __half *lo, __nv_bfloat16 *out)
 {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= batch * m * n) return;
-    const int64_t q = i / (m * n), e = i % (m * n), r = e / n, c = e % n;
-    x[q * m * n + (m > n ? c * m + r : e)] = elem_f32<T>(u[i]) * scale[q];
-}
-
-__global__ void ortho_store_kernel(const float *x, __nv_bfloat16 *out, int64_t m, int64_t n, int64_t batch)
-{
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= batch * m * n) return;
-    const int64_t q = i / (m * n), e = i % (m * n), r = e / n, c = e % n;
-    out[i] = __float2bfloat16_rn(x[q * m * n + (m > n ? c * m + r : e)]);
-}
-
-// C = alpha * A B + beta * D, all [.., ..] fp32 row-major of one batch entry; TB: B transposed.
-template <bool TB>
-__global__ void __launch_bounds__(kThreads)
-ortho_product_kernel(const float *A, const float *B, const float *D, float *C, int64_t m, int64_t n, int64_t depth,
-                     float alpha, float beta)
-{
-    __shared__ float As[kDepth][kTile + 4], Bs[kDepth][kTile + 4];
-    const int64_t q = blockIdx.z, i0 = (int64_t)blockIdx.y * kTile, j0 = (int64_t)blockIdx.x * kTile;
-    A += q * m * depth;
-    B += q * n * depth;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < depth; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += kThreads) {
-            const int r = i / kDepth, k = i % kDepth;
-            As[k][r] = i0 + r < m && k0 + k < depth ? A[(i0 + r) * depth + k0 + k] : 0.f;
-            if (TB) {
-                Bs[k][r] = j0 + r < n && k0 + k < depth ? B[(j0 + r) * depth + k0 + k] : 0.f;
-            } else {
-                const int kk = i / kTile, c = i % kTile;
-                Bs[kk][c] = j0 + c < n && k0 + kk < depth ? B[(k0 + kk) * n + j0 + c] : 0.f;
-            }
-        }
-        __syncthreads();
+    __shared__ float scale;
+    if (threadIdx.x < 32) {
+        double s = 0.0;
+        for (int i = threadIdx.x; i < parts; i += 32) s += part[(int64_t)blockIdx.y * parts + i];
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[k][ty * 4 + i], Bs[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (threadIdx.x == 0) scale = (float)(1.0 / (sqrt(s) + (double)eps));
     }
+    __syncthreads();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = ld / 8;
+    if (i >= m * per) return;
+    const int64_t r = i / per, c = i % per * 8;
+    const T *p = u + ((int64_t)blockIdx.y * m + r) * n + c;
+    float v[8];
+    if (n % 8 == 0) {
+        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < 8 / V; ++k) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p) + k);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = i0 + ty * 4 + i, c = j0 + tx * 4 + j;
-            if (r < m && c < n) {
-                const int64_t at = q * m * n + r * n + c;
-                C[at] = alpha * acc[i][j] + (D ? beta * D[at] : 0.f);
-            }
+            for (int e = 0; e < V; ++e) v[k * V + e] = elem_f32<T>(reinterpret_cast<const T *>(&w)[e]);
         }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < n ? elem_f32<T>(p[e]) : 0.f;
+    }
+    if (out) {
+        for (int e = 0; e < 8 && c + e < n; ++e)
+            out[((int64_t)blockIdx.y * m + r) * n + c + e] = __float2bfloat16_rn(v[e] * scale);
+        return;
+    }
+    // one rounding of the normalised value, then scaled by a power of two
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * scale * kScaleX;
+    const uint4 w = tc::pack8(v, false);
+    unpack16<__half>(w, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = v[e] - h[e];
+    const int64_t at = ((int64_t)blockIdx.y * m + r) * ld + c;
+    *reinterpret_cast<uint4 *>(hi + at) = w;
+    *reinterpret_cast<uint4 *>(lo + at) = tc::pack8(h, false);
+}
+
+struct Space {
+    int64_t ldx, lds, x, s;   // leading dimensions; elements of X and of a square matrix, whole batch
+    int parts;
+    __half *hi[2], *lo, *gram, *poly;
+    double *part;
+    Space(int64_t batch, int64_t m, int64_t n, void *ws)
+    {
+        const int64_t side = std::min(m, n);
+        ldx = pad8(n);
+        lds = pad8(side);
+        x = (batch * m * ldx + 127) & ~int64_t(127);
+        s = (batch * side * lds + 127) & ~int64_t(127);
+        parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts, m * n / 8192));
+        hi[0] = static_cast<__half *>(ws);
+        hi[1] = hi[0] + x;
+        lo = hi[1] + x;
+        gram = lo + x;
+        poly = gram + s;
+        part = reinterpret_cast<double *>(poly + s);
+    }
+    size_t bytes(int64_t batch) const { return (size_t)(3 * x + 2 * s) * 2 + (size_t)batch * parts * 8; }
+};
+
+template <typename T> void start(const OrthoLaunch &o, const Space &w, cudaStream_t stream)
+{
+    const T *u = static_cast<const T *>(o.update);
+    ortho_squares_kernel<T><<<dim3(w.parts, (unsigned)o.batch), 256, 0, stream>>>(u, o.m * o.n, w.part);
+    const int64_t items = o.m * (w.ldx / 8);
+    ortho_split_kernel<T><<<dim3((unsigned)((items + 255) / 256), (unsigned)o.batch), 256, 0, stream>>>(
+        u, w.part, w.parts, o.eps, o.m, o.n, w.ldx, w.hi[0], w.lo,
+        o.steps == 0 ? static_cast<__nv_bfloat16 *>(o.out) : nullptr);
+}
+
+template <int BN>
+cudaError_t update(const OrthoLaunch &o, const Space &w, tc::GemmArgs g, const __half *x, cudaStream_t stream)
+{
+    const bool tall = o.m > o.n;
+    const int64_t side = std::min(o.m, o.n);
+    CUtensorMap ma, mb;
+    const int64_t tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM) * ((o.n + BN - 1) / BN);
+    if (tall) {   // X P: P is symmetric, read with the reduction contiguous
+        if (!tc::make_map(&ma, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tc::kBM, false) ||
+            !tc::make_map(&mb, w.poly, side, side, o.batch, w.lds, side * w.lds, BN, false))
+            return cudaErrorInvalidValue;
+        return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate>(ma, mb, g, tiles, stream);
+    }
+    if (!tc::make_map(&ma, w.poly, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false) ||
+        !tc::make_map(&mb, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, 64, false))
+        return cudaErrorInvalidValue;
+    return tc::launch_gemm<tc::kDense, BN, false, true, tc::kUpdate>(ma, mb, g, tiles, stream);
 }
 
 }  // namespace
 
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int)
 {
-    const int64_t s = std::min(m, n);
-    return (size_t)(256 + 4 * batch + 8 * batch * m * n + 8 * batch * s * s);
+    return Space(batch, m, n, nullptr).bytes(batch);
 }
 
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
-    const int64_t s = std::min(o.m, o.n), r = std::max(o.m, o.n), elems = o.m * o.n, all = o.batch * elems;
-    float *x = static_cast<float *>(workspace), *x2 = x + all, *g = x2 + all, *p = g + o.batch * s * s;
-    float *scale = p + o.batch * s * s;
-    const unsigned blocks = (unsigned)((all + 255) / 256);
+    const Space w(o.batch, o.m, o.n, workspace);
     switch (o.dtype) {
-        case SPMM_F16:
-            ortho_norm_kernel<<<(unsigned)o.batch, 1024, 0, stream>>>(static_cast<const __half *>(o.update), elems, o.eps, scale);
-            ortho_load_kernel<<<blocks, 256, 0, stream>>>(static_cast<const __half *>(o.update), scale, x, o.m, o.n, o.batch);
-            break;
-        case SPMM_BF16:
-            ortho_norm_kernel<<<(unsigned)o.batch, 1024, 0, stream>>>(static_cast<const __nv_bfloat16 *>(o.update), elems, o.eps, scale);
-            ortho_load_kernel<<<blocks, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(o.update), scale, x, o.m, o.n, o.batch);
-            break;
-        default:
-            ortho_norm_kernel<<<(unsigned)o.batch, 1024, 0, stream>>>(static_cast<const float *>(o.update), elems, o.eps, scale);
-            ortho_load_kernel<<<blocks, 256, 0, stream>>>(static_cast<const float *>(o.update), scale, x, o.m, o.n, o.batch);
+        case SPMM_F16: start<__half>(o, w, stream); break;
+        case SPMM_BF16: start<__nv_bfloat16>(o, w, stream); break;
+        default: start<float>(o, w, stream);
     }
-    const dim3 square((unsigned)((s + kTile - 1) / kTile), (unsigned)((s + kTile - 1) / kTile), (unsigned)o.batch);
-    const dim3 wide((unsigned)((r + kTile - 1) / kTile), (unsigned)((s + kTile - 1) / kTile), (unsigned)o.batch);
-    for (int i = 0; i < o.steps; ++i) {
-        ortho_product_kernel<true><<<square, kThreads, 0, stream>>>(x, x, nullptr, g, s, s, r, 1.f, 0.f);
-        ortho_product_kernel<true><<<square, kThreads, 0, stream>>>(g, g, g, p, s, s, s, o.c, o.b);   // G is symmetric
-        ortho_product_kernel<false><<<wide, kThreads, 0, stream>>>(p, x, x, x2, s, r, s, 1.f, o.a);
-        std::swap(x, x2);
+    cudaError_t e = cudaGetLastError();
+    const bool tall = o.m > o.n;
+    const int64_t side = std::min(o.m, o.n), long_side = std::max(o.m, o.n);
+    const int64_t mt = (side + tc::kBM - 1) / tc::kBM, half = o.batch * mt * (mt + 1) / 2;
+    for (int i = 0; i < o.steps && e == cudaSuccess; ++i) {
+        const __half *x = w.hi[i & 1];
+        CUtensorMap mx, mg;
+        if (!tc::make_map(&mx, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tall ? 64 : tc::kBM, false) ||
+            !tc::make_map(&mg, w.gram, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false))
+            return cudaErrorInvalidValue;
+        tc::GemmArgs g{};
+        g.batch = o.batch;
+        g.passes = 1;
+        g.status = o.status;
+        g.out_type = tc::kOutF16;
+        // G = X X^T (X^T X)
+        g.m = g.n = side;
+        g.k = long_side;
+        g.out = w.gram;
+        g.ldo = w.lds;
+        g.out_batch = side * w.lds;
+        g.alpha = kScaleG / (kScaleX * kScaleX);
+        e = tall ? tc::launch_gemm<tc::kDense, 128, true, true, tc::kGram>(mx, mx, g, half, stream)
+                 : tc::launch_gemm<tc::kDense, 128, false, false, tc::kGram>(mx, mx, g, half, stream);
+        if (e != cudaSuccess) break;
+        // P = b G + c G G
+        g.k = side;
+        g.in = w.gram;
+        g.ldi = w.lds;
+        g.in_batch = side * w.lds;
+        g.out = w.poly;
+        g.alpha = o.c * (kScaleP / (kScaleG * kScaleG));
+        g.beta = o.b * (kScaleP / kScaleG);
+        e = tc::launch_gemm<tc::kDense, 128, false, false, tc::kPoly>(mg, mg, g, half, stream);
+        if (e != cudaSuccess) break;
+        // X <- a X + P X (X P); the last step writes the result
+        const bool last = i + 1 == o.steps;
+        g.m = o.m;
+        g.n = o.n;
+        g.in = x;
+        g.in_lo = w.lo;
+        g.ldi = w.ldx;
+        g.in_batch = o.m * w.ldx;
+        g.out = last ? o.out : static_cast<void *>(w.hi[i + 1 & 1]);
+        g.out_lo = last ? nullptr : w.lo;
+        g.ldo = last ? o.n : w.ldx;
+        g.out_batch = o.m * g.ldo;
+        g.out_type = last ? tc::kOutBf16 : tc::kOutF16;
+        g.alpha = last ? 1.f / (kScaleP * kScaleX) : 1.f / kScaleP;
+        g.beta = last ? o.a / kScaleX : o.a;
+        const int64_t row_tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM);
+        const int sms = device_sm_count();
+        if (o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms) e = update<256>(o, w, g, x, stream);
+        else if (o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms) e = update<128>(o, w, g, x, stream);
+        else e = update<64>(o, w, g, x, stream);
     }
-    ortho_store_kernel<<<blocks, 256, 0, stream>>>(x, static_cast<__nv_bfloat16 *>(o.out), o.m, o.n, o.batch);
-    return cudaGetLastError();
+    return e;
 }
 
 }  // namespace spmmb
