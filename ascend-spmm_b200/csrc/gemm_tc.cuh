@@ -13,10 +13,11 @@
 //   kRows    a row tile of one group times that group's matrix; the group is
 //            found from the row ranges on the device, and rows of a tile
 //            past its group's end are computed and not stored
-//   kRagged  x_g^T dy_g: the reduction runs over a group's rows; of its last
-//            slice the rows past the group's end are set to zero in shared
-//            memory (in both operands: a neighbour's infinity times zero
-//            would be NaN)
+//   kRagged  x_g^T dy_g: the reduction runs over a group's rows, in parts of
+//            `part_rows` (a longer group's parts are stored in fp32 and added
+//            afterwards); of a group's last slice the rows past its end are
+//            set to zero in shared memory (in both operands: a neighbour's
+//            infinity times zero would be NaN)
 //   kDense   a batch of equal products
 //
 // Every wait is bounded; a wait that runs out raises SPMM_DEV_TIMEOUT, and
@@ -42,6 +43,9 @@ struct GemmArgs {
     Ranges ranges;            // kRows, kRagged
     int64_t m, n, k;          // kRows: n, k; kRagged: m, n; kDense: all
     int64_t batch;            // kDense
+    int64_t part_rows;        // kRagged: a multiple of 64
+    float *parts;             // kRagged: [part_slots][m][n], the parts of groups of several
+    int64_t part_slots;
     void *out;
     int64_t ldo, out_batch;   // elements
     int out_type;
@@ -83,14 +87,15 @@ template <int BN> struct GemmShape {
 struct Tile {
     int64_t batch_a, batch_b, row0, col0;   // operand batch, first row and column
     int64_t k0, k1;                         // range of the reduction (k0 == k1: zeros)
-    int64_t out;                            // element offset of the tile in `out`
+    int64_t out;                            // element offset of the tile in `out` (in `parts`)
+    bool part;                              // kRagged: one part of several
     int rows, cols;                         // what is stored
     bool mirror;                            // kGram, kPoly: also the transposed tile
 };
 
 template <int MODE, int BN, int EPI> struct Walk {
     const GemmArgs &a;
-    TileWalk ranges;
+    TileWalk<MODE == kRagged> ranges;
     int64_t mt, nt;
     __device__ Walk(const GemmArgs &a) : a(a), mt((a.m + kBM - 1) / kBM), nt((a.n + BN - 1) / BN) {}
 
@@ -98,8 +103,8 @@ template <int MODE, int BN, int EPI> struct Walk {
     __device__ __forceinline__ bool at(int64_t t, Tile *o)
     {
         if constexpr (MODE == kRows) {
-            int64_t seg, b, e, inner;
-            if (!ranges.find(a.ranges, kBM, nt, t, a.status, &seg, &b, &e, &inner)) return false;
+            int64_t seg, b, e, inner, slots;
+            if (!ranges.find(a.ranges, kBM, nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
             o->row0 = b + inner / nt * kBM;
             o->col0 = inner % nt * BN;
             o->batch_a = 0;
@@ -109,14 +114,21 @@ template <int MODE, int BN, int EPI> struct Walk {
             o->rows = (int)min((int64_t)kBM, e - o->row0);
             o->out = o->row0 * a.ldo + o->col0;
         } else if constexpr (MODE == kRagged) {
-            if (t >= a.ranges.groups * mt * nt) return false;
-            const int64_t g = t / (mt * nt), i = t % (mt * nt);
-            segment_rows(a.ranges, g + 1, &o->k0, &o->k1, a.status);
+            int64_t seg, b, e, inner, slots;
+            if (!ranges.find(a.ranges, a.part_rows, mt * nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
+            const int64_t p = inner / (mt * nt), i = inner % (mt * nt);
+            o->k0 = b + p * a.part_rows;
+            o->k1 = min(e, o->k0 + a.part_rows);
             o->row0 = i / nt * kBM;
             o->col0 = i % nt * BN;
             o->batch_a = o->batch_b = 0;
             o->rows = (int)min((int64_t)kBM, a.m - o->row0);
-            o->out = g * a.out_batch + o->row0 * a.ldo + o->col0;
+            o->part = slots >= 0;
+            if (o->part && slots + p >= a.part_slots) {   // only overlapping (malformed) ranges can need more
+                o->k1 = o->k0;
+                o->rows = 0;
+            }
+            o->out = (o->part ? (slots + p) * a.m * a.n : (seg - 1) * a.out_batch) + o->row0 * a.n + o->col0;
         } else {
             const bool half = EPI == kGram || EPI == kPoly;   // symmetric: the tiles on and below the diagonal
             const int64_t per = half ? mt * (mt + 1) / 2 : mt * nt;
@@ -311,11 +323,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const int row = (warp & 3) * 32 + lane;
         const unsigned stage = base + S::kStageOff + row * S::kPitch;
         const unsigned lanes = tmem + ((unsigned)((warp & 3) * 32) << 16);
-        const int es = a.out_type == kOutF32 ? 4 : 2;
-        // kUpdate stages 64 columns of the high and of the low part side by side
-        const int chunk = EPI == kUpdate ? 64 : S::kChunk / es;
+        const int out_size = a.out_type == kOutF32 ? 4 : 2;
         // rows that do not start on 16 bytes cannot be bulk-copied
-        const bool bulk = (a.ldo * es & 15) == 0 && (a.out_batch * es & 15) == 0;
+        const bool bulk = (a.ldo * out_size & 15) == 0 && (a.out_batch * out_size & 15) == 0;
         unsigned used = 0;
         for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
             const bool zero = t.k0 >= t.k1;
@@ -325,7 +335,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 fence_after();
                 ++used;
             }
-            const bool on = row < t.rows;
+            const bool on = row < t.rows, part = MODE == kRagged && t.part;
+            const int es = part ? 4 : out_size;
+            // kUpdate stages 64 columns of the high and of the low part side by side
+            const int chunk = EPI == kUpdate ? 64 : S::kChunk / es;
+            char *out = part ? reinterpret_cast<char *>(a.parts) : static_cast<char *>(a.out);
             for (int c0 = 0; c0 < t.cols; c0 += chunk) {
                 bulk_wait_read();
                 if (EPI == kUpdate && !bulk) __syncwarp();   // the warp reads its rows' staging across lanes below
@@ -391,7 +405,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     if (on) {
                         const int64_t at = t.out + row * a.ldo + c0;
                         fence_async();
-                        bulk_store(static_cast<char *>(a.out) + at * es, stage, bytes);
+                        bulk_store(out + at * es, stage, bytes);
                         if (EPI == kUpdate && a.out_lo) bulk_store(a.out_lo + at, stage + 128, bytes);
                     }
                     bulk_commit();

@@ -18,108 +18,70 @@ namespace spmmb {
 
 namespace {
 
-constexpr int kTile = 64, kDepth = 16, kThreads = 256;
-
 __host__ __device__ Ranges ranges_of(const GroupedLaunch &a)
 {
     return Ranges{a.ptr, a.itype == SPMM_I64, a.groups, a.rows};
 }
 
-// acc[4][4] of thread (ty, tx) += A[m, k] B[k, n] over one 64 x 64 tile, operands read by strides.
-template <typename T>
-__device__ __forceinline__ void simt_tile(const T *A, int64_t ars, int64_t acs, int64_t m, const T *B, int64_t brs,
-                                          int64_t bcs, int64_t n, int64_t depth, float (&acc)[4][4])
+// ---- fp32 operands ----------------------------------------------------------
+//
+// The tensor cores take fp32 as tf32 (11 bits).  To keep fp32's 24 bits each
+// operand is written as three bf16 planes x = h + m + l (8 bits each, fp32's
+// exponents) and the product is run as the six plane products above 2^-24 of
+// the result, the smallest first:  h l, l h, m m, h m, m h, h h.  That is six
+// bf16 products, about four times the rate of fp32 FMAs.  An infinite x has
+// zero m and l planes; its products with zero planes are NaN.
+constexpr int kPlanes = 3, kPasses = 6;
+constexpr unsigned char kPassA[kPasses] = {0, 2, 1, 0, 1, 0}, kPassB[kPasses] = {2, 0, 1, 1, 0, 0};
+
+// One thread splits 8 elements.  ranges.ptr set: src is [groups][elems] and
+// groups without rows are skipped.
+__global__ void __launch_bounds__(256) split_planes_kernel(const float *src, __nv_bfloat16 *dst, int64_t elems,
+                                                           int64_t plane, int64_t groups, Ranges ranges,
+                                                           DevStatus *status)
 {
-    __shared__ float As[kDepth][kTile + 4], Bs[kDepth][kTile + 4];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int64_t k0 = 0; k0 < depth; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += kThreads) {
-            const int r = i / kDepth, k = i % kDepth;
-            As[k][r] = r < m && k0 + k < depth ? elem_f32<T>(A[r * ars + (k0 + k) * acs]) : 0.f;
-            const int kk = i / kTile, c = i % kTile;
-            Bs[kk][c] = c < n && k0 + kk < depth ? elem_f32<T>(B[(k0 + kk) * brs + c * bcs]) : 0.f;
+    for (int64_t g = blockIdx.y; g < groups; g += gridDim.y) {
+        if (ranges.ptr) {
+            int64_t b, e;
+            segment_rows(ranges, g + 1, &b, &e, status);
+            if (b == e) continue;
         }
-        __syncthreads();
+        const int64_t at = g * elems;
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < elems; i += (int64_t)gridDim.x * 2048) {
+            const float4 u = __ldg(reinterpret_cast<const float4 *>(src + at + i));
+            const float4 w = __ldg(reinterpret_cast<const float4 *>(src + at + i) + 1);
+            float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k) {
-            float a[4], b[4];
+            for (int p = 0; p < kPlanes; ++p) {
+                __align__(16) __nv_bfloat16 h[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { a[i] = As[k][ty * 4 + i]; b[i] = Bs[k][tx * 4 + i]; }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+                for (int k = 0; k < 8; ++k) {
+                    h[k] = __float2bfloat16_rn(v[k]);
+                    // next to fp32's maximum, rounding up would leave the range
+                    if (isinf(__bfloat162float(h[k])) && !isinf(v[k])) h[k] = __float2bfloat16_rz(v[k]);
+                    v[k] = isfinite(v[k]) ? v[k] - __bfloat162float(h[k]) : 0.f;
+                }
+                *reinterpret_cast<uint4 *>(dst + p * plane + at + i) = *reinterpret_cast<const uint4 *>(h);
+            }
         }
-        __syncthreads();
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void simt_store(T *C, int64_t ldc, int64_t m, int64_t n, const float (&acc)[4][4])
+cudaError_t split_planes(const void *src, void *dst, int64_t batch, int64_t elems, const Ranges &ranges,
+                         DevStatus *status, cudaStream_t stream)
 {
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (ty * 4 + i < m && tx * 4 + j < n) C[(ty * 4 + i) * ldc + tx * 4 + j] = elem_of<T>(acc[i][j]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) grouped_rows_simt_kernel(const GroupedLaunch a)
-{
-    __shared__ int64_t where[4];
-    if (threadIdx.x < 32) {
-        TileWalk walk;
-        int64_t seg = -1, b = 0, e = 0, inner = 0;
-        if (!walk.find(ranges_of(a), kTile, 1, blockIdx.x, a.status, &seg, &b, &e, &inner)) seg = -1;
-        if (threadIdx.x == 0) { where[0] = seg; where[1] = b; where[2] = e; where[3] = inner; }
-    }
-    __syncthreads();
-    const int64_t seg = where[0];
-    if (seg < 0) return;
-    const int64_t depth = a.transposed ? a.N : a.K, width = a.transposed ? a.K : a.N;
-    const int64_t r0 = where[1] + where[3] * kTile, m = min((int64_t)kTile, where[2] - r0);
-    const int64_t c0 = (int64_t)blockIdx.y * kTile, n = min((int64_t)kTile, width - c0);
-    float acc[4][4] = {};
-    if (seg >= 1 && seg <= a.groups) {
-        const T *w = static_cast<const T *>(a.w) + (seg - 1) * a.K * a.N;
-        const int64_t brs = a.transposed ? 1 : a.N, bcs = a.transposed ? a.N : 1;
-        simt_tile<T>(static_cast<const T *>(a.x) + r0 * depth, depth, 1, m, w + c0 * bcs, brs, bcs, n, depth, acc);
-    }
-    simt_store<T>(static_cast<T *>(a.out) + r0 * width + c0, width, m, n, acc);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) grouped_weight_grad_simt_kernel(const GroupedLaunch a)
-{
-    const int64_t tiles = (a.K + kTile - 1) / kTile;
-    const int64_t g = blockIdx.x / tiles, i0 = blockIdx.x % tiles * kTile, c0 = (int64_t)blockIdx.y * kTile;
-    int64_t b, e;
-    segment_rows(ranges_of(a), g + 1, &b, &e, a.status);
-    const int64_t m = min((int64_t)kTile, a.K - i0), n = min((int64_t)kTile, a.N - c0);
-    float acc[4][4] = {};
-    simt_tile<T>(static_cast<const T *>(a.x) + b * a.K + i0, 1, a.K, m, static_cast<const T *>(a.w) + b * a.N + c0, a.N,
-                 1, n, e - b, acc);
-    simt_store<T>(static_cast<T *>(a.out) + (g * a.K + i0) * a.N + c0, a.N, m, n, acc);
-}
-
-template <typename T> cudaError_t rows_simt(const GroupedLaunch &a, cudaStream_t stream)
-{
-    const int64_t width = a.transposed ? a.K : a.N;
-    const dim3 grid((unsigned)((a.rows + kTile - 1) / kTile + a.groups + 2), (unsigned)((width + kTile - 1) / kTile));
-    grouped_rows_simt_kernel<T><<<grid, kThreads, 0, stream>>>(a);
+    if (batch * elems == 0) return cudaSuccess;
+    const int64_t per = std::max<int64_t>(1, 8 * device_sm_count() / batch);
+    const int64_t blocks = std::min((elems + 2047) / 2048, per);
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(batch, 65535));
+    split_planes_kernel<<<grid, 256, 0, stream>>>(static_cast<const float *>(src), static_cast<__nv_bfloat16 *>(dst),
+                                                  elems, batch * elems, batch, ranges, status);
     return cudaGetLastError();
 }
 
-template <typename T> cudaError_t weight_grad_simt(const GroupedLaunch &a, cudaStream_t stream)
-{
-    const dim3 grid((unsigned)((a.K + kTile - 1) / kTile * a.groups), (unsigned)((a.N + kTile - 1) / kTile));
-    grouped_weight_grad_simt_kernel<T><<<grid, kThreads, 0, stream>>>(a);
-    return cudaGetLastError();
-}
+size_t plane_bytes(int64_t elems) { return ((size_t)elems * kPlanes * 2 + 255) & ~size_t(255); }
 
-// ---- 16-bit types: the tensor-core kernels of gemm_tc.cuh ------------------
+// ---- launches --------------------------------------------------------------
 
 // Columns per tile: the widest that the output's width fills and that still
 // gives every SM a tile (a narrower tile reads the row operand more often).
@@ -131,21 +93,130 @@ int tile_columns(int64_t row_tiles, int64_t width)
     return 64;
 }
 
-template <int BN> cudaError_t rows_tc(const GroupedLaunch &a, tc::GemmArgs &g, int64_t row_tiles, cudaStream_t stream)
+void set_types(tc::GemmArgs &g, int dtype)
+{
+    const bool f32 = dtype == SPMM_F32;
+    g.bf16 = f32 || dtype == SPMM_BF16;
+    g.out_type = f32 ? tc::kOutF32 : g.bf16 ? tc::kOutBf16 : tc::kOutF16;
+    g.passes = f32 ? kPasses : 1;
+    if (f32) {
+        std::copy(kPassA, kPassA + kPasses, g.pa);
+        std::copy(kPassB, kPassB + kPasses, g.pb);
+    }
+}
+
+template <int BN>
+cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::GemmArgs &g, int64_t row_tiles,
+                    cudaStream_t stream)
 {
     CUtensorMap ma, mb;
-    const bool bf = g.bf16;
+    const int64_t planes = g.passes > 1 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
     const int64_t tiles = row_tiles * ((g.n + BN - 1) / BN);
-    if (!tc::make_map(&ma, a.x, g.k, a.rows, 1, g.k, 0, tc::kBM, bf)) return cudaErrorInvalidValue;
-    const int64_t groups = std::max<int64_t>(a.groups, 1);
-    const void *w = a.groups > 0 ? a.w : a.x;   // no group: the map is never read
-    if (!tc::make_map(&mb, w, a.N, a.groups > 0 ? a.K : 1, groups, a.N, a.K * a.N, a.transposed ? BN : 64, bf))
+    if (!tc::make_map(&ma, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
+        !tc::make_map(&mb, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? BN : 64, g.bf16))
         return cudaErrorInvalidValue;
     if (a.transposed) return tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(ma, mb, g, tiles, stream);
     return tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(ma, mb, g, tiles, stream);
 }
 
-cudaError_t launch_rows_tc(const GroupedLaunch &a, cudaStream_t stream)
+// Rows of one part of a weight gradient: a group's rows are one reduction
+// unless that leaves SMs idle.  Six units of work per SM bound what an
+// unlucky SM has left at the end; 512 rows are the least that pay for
+// storing and adding a tile in fp32.
+int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn)
+{
+    const int64_t tiles = ((K + tc::kBM - 1) / tc::kBM) * ((N + bn - 1) / bn);
+    const int64_t even = rows * tiles / (6 * device_sm_count());
+    return (std::max<int64_t>(512, even) + 63) & ~int64_t(63);
+}
+
+int weight_grad_columns(int64_t N) { return N > 128 ? 256 : N > 64 ? 128 : 64; }
+
+// A group of n > 1 parts has more than (n - 1) part rows, so n <= 2 rows / part.
+int64_t weight_grad_slots(int64_t rows, int64_t K, int64_t N)
+{
+    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N));
+    return rows <= part ? 0 : 2 * rows / part;
+}
+
+// Adds the parts of each group that has several, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, T *out, int64_t elems, int64_t part_rows,
+                                                        int64_t slots, Ranges ranges, DevStatus *status)
+{
+    __shared__ int64_t range[2];
+    for (int64_t g = blockIdx.y; g < ranges.groups; g += gridDim.y) {
+        if (threadIdx.x < 32) {   // the parts of the groups before g, and its own
+            int64_t before = 0, own = 0;
+            for (int64_t base = 0; base <= g; base += 32) {
+                const int64_t s = base + threadIdx.x;
+                int64_t b = 0, e = 0;
+                if (s <= g) segment_rows(ranges, s + 1, &b, &e, status);
+                int64_t n = (e - b + part_rows - 1) / part_rows;
+                n = n > 1 ? n : 0;
+                if (s == g) own = n;
+                int64_t sum = s < g ? n : 0;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                before += sum;
+            }
+            own = __shfl_sync(0xffffffffu, own, (int)(g & 31));
+            if (threadIdx.x == 0) { range[0] = before; range[1] = own; }
+        }
+        __syncthreads();
+        const int64_t first = range[0], n = range[1];
+        __syncthreads();
+        if (n == 0 || first + n > slots) continue;
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < elems; i += (int64_t)gridDim.x * 1024) {
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int64_t p = 0; p < n; ++p) {
+                const float4 v = __ldcs(reinterpret_cast<const float4 *>(parts + (first + p) * elems + i));
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            T *o = out + g * elems + i;
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>(o) = s;
+            } else {
+                __align__(8) T h[4] = {elem_of<T>(s.x), elem_of<T>(s.y), elem_of<T>(s.z), elem_of<T>(s.w)};
+                *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(h);
+            }
+        }
+    }
+}
+
+template <typename T> cudaError_t add_parts(const GroupedLaunch &a, const tc::GemmArgs &g, cudaStream_t stream)
+{
+    const int64_t elems = a.K * a.N;
+    const int64_t per = std::max<int64_t>(1, 16 * device_sm_count() / a.groups);
+    const unsigned blocks = (unsigned)std::min((elems + 1023) / 1024, per);
+    const dim3 grid(blocks, (unsigned)std::min<int64_t>(a.groups, 65535));
+    add_parts_kernel<T><<<grid, 256, 0, stream>>>(g.parts, static_cast<T *>(a.out), elems, g.part_rows, g.part_slots,
+                                                  g.ranges, a.status);
+    return cudaGetLastError();
+}
+
+template <int BN>
+cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy, tc::GemmArgs &g, cudaStream_t stream)
+{
+    CUtensorMap ma, mb;
+    const int64_t planes = g.passes > 1 ? kPlanes : 1, rows = std::max<int64_t>(a.rows, 1);
+    if (!tc::make_map(&ma, x, a.K, rows, planes, a.K, rows * a.K, 64, g.bf16) ||
+        !tc::make_map(&mb, dy, a.N, rows, planes, a.N, rows * a.N, 64, g.bf16))
+        return cudaErrorInvalidValue;
+    const int64_t tiles = (a.groups + a.rows / g.part_rows) * ((a.K + tc::kBM - 1) / tc::kBM) * ((a.N + BN - 1) / BN);
+    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(ma, mb, g, tiles, stream);
+}
+
+}  // namespace
+
+size_t grouped_rows_workspace(int64_t rows, int64_t groups, int64_t K, int64_t N, bool transposed, int dtype)
+{
+    if (dtype != SPMM_F32) return 0;
+    return plane_bytes(rows * (transposed ? N : K)) + plane_bytes(groups * K * N);
+}
+
+cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStream_t stream)
 {
     tc::GemmArgs g{};
     g.ranges = ranges_of(a);
@@ -153,32 +224,36 @@ cudaError_t launch_rows_tc(const GroupedLaunch &a, cudaStream_t stream)
     g.k = a.transposed ? a.N : a.K;
     g.out = a.out;
     g.ldo = g.n;
-    g.bf16 = a.dtype == SPMM_BF16;
-    g.out_type = g.bf16 ? tc::kOutBf16 : tc::kOutF16;
-    g.passes = 1;
     g.status = a.status;
-    // every group can end in a partial tile; segments outside the groups too
+    set_types(g, a.dtype);
+    const void *x = a.x, *w = a.groups > 0 ? a.w : a.x;   // no group: the weight is never read
+    if (a.dtype == SPMM_F32) {
+        char *px = static_cast<char *>(workspace), *pw = px + plane_bytes(a.rows * g.k);
+        cudaError_t e = split_planes(x, px, 1, a.rows * g.k, Ranges{}, a.status, stream);
+        if (e == cudaSuccess) e = split_planes(a.w, pw, a.groups, a.K * a.N, g.ranges, a.status, stream);
+        if (e != cudaSuccess) return e;
+        x = px;
+        w = a.groups > 0 ? pw : px;
+        g.za = 1;
+        g.zb = (int)a.groups;
+    }
+    // every group can end in a partial tile; the rows outside the groups too
     const int64_t row_tiles = std::min(a.rows, (a.rows + tc::kBM - 1) / tc::kBM + a.groups + 1);
     switch (tile_columns(row_tiles, g.n)) {
-        case 256: return rows_tc<256>(a, g, row_tiles, stream);
-        case 128: return rows_tc<128>(a, g, row_tiles, stream);
-        default: return rows_tc<64>(a, g, row_tiles, stream);
+        case 256: return rows_tc<256>(a, x, w, g, row_tiles, stream);
+        case 128: return rows_tc<128>(a, x, w, g, row_tiles, stream);
+        default: return rows_tc<64>(a, x, w, g, row_tiles, stream);
     }
 }
 
-template <int BN> cudaError_t weight_grad_tc(const GroupedLaunch &a, tc::GemmArgs &g, cudaStream_t stream)
+size_t grouped_weight_grad_workspace(int64_t rows, int64_t groups, int64_t K, int64_t N, int dtype)
 {
-    CUtensorMap ma, mb;
-    const bool bf = g.bf16;
-    const int64_t rows = std::max<int64_t>(a.rows, 1);
-    const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: the maps are never read
-    if (!tc::make_map(&ma, x, a.K, rows, 1, a.K, 0, 64, bf) || !tc::make_map(&mb, dy, a.N, rows, 1, a.N, 0, 64, bf))
-        return cudaErrorInvalidValue;
-    const int64_t tiles = a.groups * ((a.K + tc::kBM - 1) / tc::kBM) * ((a.N + BN - 1) / BN);
-    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(ma, mb, g, tiles, stream);
+    (void)groups;
+    const size_t parts = (size_t)weight_grad_slots(rows, K, N) * K * N * sizeof(float);
+    return parts + (dtype == SPMM_F32 ? plane_bytes(rows * K) + plane_bytes(rows * N) : 0);
 }
 
-cudaError_t launch_weight_grad_tc(const GroupedLaunch &a, cudaStream_t stream)
+cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, cudaStream_t stream)
 {
     tc::GemmArgs g{};
     g.ranges = ranges_of(a);
@@ -187,30 +262,37 @@ cudaError_t launch_weight_grad_tc(const GroupedLaunch &a, cudaStream_t stream)
     g.out = a.out;
     g.ldo = a.N;
     g.out_batch = a.K * a.N;
-    g.bf16 = a.dtype == SPMM_BF16;
-    g.out_type = g.bf16 ? tc::kOutBf16 : tc::kOutF16;
-    g.passes = 1;
     g.status = a.status;
-    switch (tile_columns(a.groups * ((a.K + tc::kBM - 1) / tc::kBM), a.N)) {
-        case 256: return weight_grad_tc<256>(a, g, stream);
-        case 128: return weight_grad_tc<128>(a, g, stream);
-        default: return weight_grad_tc<64>(a, g, stream);
+    set_types(g, a.dtype);
+    const int bn = weight_grad_columns(a.N);
+    g.part_rows = weight_grad_part(a.rows, a.K, a.N, bn);
+    const int64_t slots = weight_grad_slots(a.rows, a.K, a.N);
+    const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: never read
+    char *ws = static_cast<char *>(workspace);
+    if (a.dtype == SPMM_F32 && a.rows > 0) {
+        char *px = ws, *pdy = px + plane_bytes(a.rows * a.K);
+        ws = pdy + plane_bytes(a.rows * a.N);
+        cudaError_t e = split_planes(x, px, 1, a.rows * a.K, Ranges{}, a.status, stream);
+        if (e == cudaSuccess) e = split_planes(dy, pdy, 1, a.rows * a.N, Ranges{}, a.status, stream);
+        if (e != cudaSuccess) return e;
+        x = px;
+        dy = pdy;
+        g.za = g.zb = 1;
     }
-}
-
-}  // namespace
-
-size_t grouped_rows_workspace(int64_t, int64_t, int64_t, int64_t, bool, int) { return 0; }
-size_t grouped_weight_grad_workspace(int64_t, int64_t, int64_t, int64_t, int) { return 0; }
-
-cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *, cudaStream_t stream)
-{
-    return a.dtype == SPMM_F32 ? rows_simt<float>(a, stream) : launch_rows_tc(a, stream);
-}
-
-cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *, cudaStream_t stream)
-{
-    return a.dtype == SPMM_F32 ? weight_grad_simt<float>(a, stream) : launch_weight_grad_tc(a, stream);
+    g.parts = reinterpret_cast<float *>(ws);
+    g.part_slots = slots;
+    cudaError_t e;
+    switch (bn) {
+        case 256: e = weight_grad_tc<256>(a, x, dy, g, stream); break;
+        case 128: e = weight_grad_tc<128>(a, x, dy, g, stream); break;
+        default: e = weight_grad_tc<64>(a, x, dy, g, stream);
+    }
+    if (e != cudaSuccess || slots == 0) return e;
+    switch (a.dtype) {
+        case SPMM_F16: return add_parts<__half>(a, g, stream);
+        case SPMM_BF16: return add_parts<__nv_bfloat16>(a, g, stream);
+        default: return add_parts<float>(a, g, stream);
+    }
 }
 
 }  // namespace spmmb

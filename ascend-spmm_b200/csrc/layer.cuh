@@ -52,34 +52,35 @@ __device__ __forceinline__ void segment_rows(const Ranges &p, int64_t s, int64_t
     *end = e;
 }
 
-// Walks the tiles of all segments in order: `height` rows and `mult` column
-// tiles each.  Every lane of the warp calls it with the same arguments;
-// `tile` must not decrease from call to call.
-struct TileWalk {
-    int64_t base = 0;    // segments before the current 32
-    int64_t before = 0;  // tiles of the segments before `base`
-    int64_t count = -1;  // this lane's segment: its tiles, rows and the tiles before it
-    int64_t begin = 0, end = 0, first = 0;
+// Walks the tiles of all segments in order, `mult` column tiles per `height`
+// rows.  SPLIT (weight gradients): a group's tiles cover its rows in parts of
+// `height`, a group without rows has one, the rows outside the groups none.
+// Every lane of the warp calls it with the same arguments; `tile` must not
+// decrease from call to call.
+template <bool SPLIT> struct TileWalk {
+    int64_t base = 0;      // segments before the current 32
+    int64_t before = 0;    // tiles of the segments before `base`
+    int64_t kept = 0;      // SPLIT: parts of the groups of several parts before `base`
+    int64_t count = -1;    // this lane's segment: its tiles, rows, and what is before it
+    int64_t begin = 0, end = 0, first = 0, parts = 0, slot = 0;
 
     // The segment of `tile` (0 .. groups + 1), its rows and the tile's number
-    // within it; false past the last tile.
-    __device__ __forceinline__ bool find(const Ranges &p, int height, int64_t mult, int64_t tile, DevStatus *status,
-                                         int64_t *seg, int64_t *b, int64_t *e, int64_t *inner)
+    // within it; false past the last tile.  `slots`: parts of the groups of
+    // several parts before this group, -1 where it has a single part.
+    __device__ __forceinline__ bool find(const Ranges &p, int64_t height, int64_t mult, int64_t tile, DevStatus *status,
+                                         int64_t *seg, int64_t *b, int64_t *e, int64_t *inner, int64_t *slots)
     {
         const int lane = threadIdx.x & 31;
         for (;;) {
             if (count < 0) {
                 segment_rows(p, base + lane, &begin, &end, status);
-                count = (end - begin + height - 1) / height * mult;
-                int64_t sum = count;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += v;
-                }
-                first = sum - count;
+                int64_t n = (end - begin + height - 1) / height;
+                if (SPLIT) n = base + lane >= 1 && base + lane <= p.groups ? max(n, (int64_t)1) : 0;
+                count = n * mult;
+                parts = SPLIT && n > 1 ? n : 0;
+                first = before_lane(count);
+                if (SPLIT) slot = before_lane(parts);
             }
-            const int64_t total = __shfl_sync(0xffffffffu, first + count, 31);
             const unsigned hit = __ballot_sync(0xffffffffu, tile - before >= first && tile - before < first + count);
             if (hit) {
                 const int l = __ffs(hit) - 1;
@@ -87,13 +88,28 @@ struct TileWalk {
                 *b = __shfl_sync(0xffffffffu, begin, l);
                 *e = __shfl_sync(0xffffffffu, end, l);
                 *inner = tile - before - __shfl_sync(0xffffffffu, first, l);
+                if (SPLIT) *slots = __shfl_sync(0xffffffffu, parts ? kept + slot : -1, l);
                 return true;
             }
-            before += total;
+            before += __shfl_sync(0xffffffffu, first + count, 31);
+            if (SPLIT) kept += __shfl_sync(0xffffffffu, slot + parts, 31);
             base += 32;
             count = -1;
             if (base >= p.groups + 2) return false;
         }
+    }
+
+private:
+    __device__ __forceinline__ int64_t before_lane(int64_t v)
+    {
+        const int lane = threadIdx.x & 31;
+        int64_t sum = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+        }
+        return sum - v;
     }
 };
 
