@@ -29,6 +29,7 @@
 #include "../../include/spmm_b200.h"
 #include "engine.h"
 #include "layer.cuh"
+#include "layer.h"
 #include "tc.cuh"
 
 namespace spmmb {
@@ -444,8 +445,14 @@ template <int MODE, int BN, bool AMN, bool BMN, int EPI>
 cudaError_t launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, const GemmArgs &a, int64_t tiles, cudaStream_t s)
 {
     auto kernel = gemm_kernel<MODE, BN, AMN, BMN, EPI>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmShape<BN>::kBytes);
-    if (e != cudaSuccess) return e;
+    static PerDevice<bool> ready;   // the attribute outlasts the call
+    bool *done = ready.here();
+    if (!done || !*done) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmShape<BN>::kBytes);
+        if (e != cudaSuccess) return e;
+        if (done) *done = true;
+    }
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count()));
     kernel<<<grid, kGemmThreads, GemmShape<BN>::kBytes, s>>>(ma, mb, a);
     return cudaGetLastError();

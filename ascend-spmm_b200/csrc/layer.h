@@ -12,6 +12,18 @@
 
 namespace spmmb {
 
+// A value per device that is computed once (a kernel's launch attributes).
+// Racing threads compute the same value.
+template <typename T> struct PerDevice {
+    static constexpr int kDevices = 64;
+    T value[kDevices] = {};
+    T *here()   // nullptr: no device, or one out of range
+    {
+        int dev = 0;
+        return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < kDevices ? value + dev : nullptr;
+    }
+};
+
 // ---- layer normalisation (norm.cu) ---------------------------------------
 struct NormLaunch {
     const void *x;

@@ -359,12 +359,16 @@ __global__ void __launch_bounds__(256) norm_params_kernel(const float *part, int
     }
 }
 
-// Blocks that fill the GPU once (a persistent grid), no more than the rows need.
-template <typename K> int64_t grid_of(K kernel, int threads, int64_t turns)
+// Blocks of `kernel` that fill the GPU once (a persistent grid), no more than the rows need.
+template <auto kernel> int64_t grid_of(int threads, int64_t turns)
 {
-    int per_sm = 1;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1)
-        per_sm = 1;
+    static PerDevice<int> resident;
+    int *have = resident.here(), per_sm = have ? *have : 0;
+    if (per_sm < 1) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1)
+            per_sm = 1;
+        if (have) *have = per_sm;
+    }
     return std::max<int64_t>(1, std::min<int64_t>((int64_t)per_sm * device_sm_count(), turns));
 }
 
@@ -374,10 +378,10 @@ template <typename T, int VE, int NV, int TEAM> cudaError_t run_team(const NormA
     constexpr int threads = kBlock<TEAM>, teams = threads / TEAM;
     const int64_t turns = (a.rows + teams - 1) / teams;
     if (backward) {
-        *blocks = std::min(max_blocks, grid_of(norm_backward_kernel<T, VE, NV, TEAM>, threads, turns));
+        *blocks = std::min(max_blocks, grid_of<norm_backward_kernel<T, VE, NV, TEAM>>(threads, turns));
         norm_backward_kernel<T, VE, NV, TEAM><<<(unsigned)*blocks, threads, 0, stream>>>(a);
     } else {
-        *blocks = grid_of(norm_forward_kernel<T, VE, NV, TEAM>, threads, turns);
+        *blocks = grid_of<norm_forward_kernel<T, VE, NV, TEAM>>(threads, turns);
         norm_forward_kernel<T, VE, NV, TEAM><<<(unsigned)*blocks, threads, 0, stream>>>(a);
     }
     return cudaGetLastError();

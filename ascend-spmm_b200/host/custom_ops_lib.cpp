@@ -7,6 +7,7 @@
 // there is no CPU path.  All compute goes through the C ABI of
 // libspmm_b200.so (include/spmm_b200.h) on the current CUDA stream.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -725,7 +726,7 @@ int check_group_ptr(const at::Tensor &ptr, const at::Tensor &x, int64_t groups, 
 }
 
 // x [rows, K] times weight[g] [K, N] (transposed: x [rows, N] times weight[g]^T).
-at::Tensor grouped_matmul(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &group_ptr, bool transposed)
+at::Tensor grouped_rows(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &group_ptr, bool transposed)
 {
     const char *op = "grouped_matmul";
     TORCH_CHECK_CUDA(x);
@@ -770,6 +771,93 @@ at::Tensor grouped_weight_grad(const at::Tensor &x, const at::Tensor &grad, cons
     check_rc(spmm_grouped_weight_grad_launch(xc.data_ptr(), gc.data_ptr(), group_ptr.data_ptr(), dw.data_ptr(), rows,
                                              groups, K, N, itype, dt, ws.data_ptr(), wbytes, stream_of(xc)));
     return dw;
+}
+
+// Autograd nodes of the layer operators: C++ functions, so that a training
+// step's backward pass runs without the interpreter (a Python node costs
+// about 40 us more per forward and backward).  They are differentiable once.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+variable_list once(variable_list grads, const char *op)
+{
+    if (!at::GradMode::is_enabled()) return grads;   // no second derivative was asked for
+    for (at::Tensor &g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);   // so that the error node is on their path
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string("trying to differentiate twice a function that is differentiable once: ") + op, grads.size());
+    return (*error)(std::move(grads));
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor *> ts)
+{
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor *t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const c10::optional<at::Tensor> &weight,
+                              const c10::optional<at::Tensor> &bias, double eps)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [y, mean, rstd] = layer_norm_forward(x, weight, bias, eps, true);
+        ctx->save_for_backward({x, weight.value_or(at::Tensor()), mean, rstd});
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->saved_data["fp32_bias"] = bias.has_value() && bias->scalar_type() == at::kFloat;
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list out(4);
+        if (grads[0].defined()) {
+            at::NoGradGuard none;
+            const bool weight = s[1].defined(), bias = ctx->saved_data["bias"].toBool();
+            // a parameter that was not given has no edge
+            std::tie(out[0], out[1], out[2]) = layer_norm_backward(
+                grads[0], s[0], s[2], s[3], weight ? c10::optional<at::Tensor>(s[1]) : c10::nullopt,
+                ctx->needs_input_grad(0), weight && ctx->needs_input_grad(1),
+                bias && ctx->needs_input_grad(weight ? 2 : 1), ctx->saved_data["fp32_bias"].toBool());
+        }
+        return once(std::move(out), "layer_norm");
+    }
+};
+
+at::Tensor layer_norm(const at::Tensor &x, const c10::optional<at::Tensor> &weight,
+                      const c10::optional<at::Tensor> &bias, double eps)
+{
+    const at::Tensor w = weight.value_or(at::Tensor()), b = bias.value_or(at::Tensor());
+    if (wants_grad({&x, &w, &b})) return LayerNormFunction::apply(x, weight, bias, eps);
+    return std::get<0>(layer_norm_forward(x, weight, bias, eps, false));
+}
+
+struct GroupedMatmulFunction : torch::autograd::Function<GroupedMatmulFunction> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight,
+                              const at::Tensor &group_ptr)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({x, weight, group_ptr});
+        return grouped_rows(x, weight, group_ptr, false);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list out(3);
+        if (grads[0].defined()) {
+            at::NoGradGuard none;
+            if (ctx->needs_input_grad(0)) out[0] = grouped_rows(grads[0], s[1], s[2], true);
+            if (ctx->needs_input_grad(1)) out[1] = grouped_weight_grad(s[0], grads[0], s[2]);
+        }
+        return once(std::move(out), "grouped_matmul");
+    }
+};
+
+at::Tensor grouped_matmul(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &group_ptr, bool transposed)
+{
+    if (!transposed && wants_grad({&x, &weight})) return GroupedMatmulFunction::apply(x, weight, group_ptr);
+    return grouped_rows(x, weight, group_ptr, transposed);
 }
 
 at::Tensor orthogonalize(const at::Tensor &update, int64_t steps, double a, double b, double c, double eps)
@@ -851,6 +939,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("a"), pybind11::arg("window_size") = 16);
     m.def("pack_rows", &pack_rows, "dst[index[i]] = src[i]; other rows zero (pack_node_tensor helper)");
     m.def("restore_rows", &restore_rows, "dst[i] = src[index[i]] (restore_node_tensor helper)");
+    m.def("layer_norm", &layer_norm, "Layer normalisation of the last dimension, differentiable", pybind11::arg("x"),
+          pybind11::arg("weight") = pybind11::none(), pybind11::arg("bias") = pybind11::none(),
+          pybind11::arg("eps") = 1e-5);
     m.def("layer_norm_forward", &layer_norm_forward,
           "Layer normalisation of the last dimension: (y, mean, rstd); mean and rstd only with stats",
           pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("eps") = 1e-5,
@@ -862,7 +953,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("fp32_params") = false);
     m.def("grouped_matmul", &grouped_matmul,
           "Rows group_ptr[g] .. group_ptr[g + 1] of x times weight[g] (its transpose with transposed); widths "
-          "divisible by 16 for FP16 and BF16, by 8 for FP32",
+          "divisible by 16 for FP16 and BF16, by 8 for FP32; differentiable unless transposed",
           pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("group_ptr"), pybind11::arg("transposed") = false);
     m.def("grouped_weight_grad", &grouped_weight_grad, "Gradient of grouped_matmul's weight: x_g^T grad_g per group",
           pybind11::arg("x"), pybind11::arg("grad"), pybind11::arg("group_ptr"));

@@ -35,6 +35,7 @@ from custom_ops_lib import pack_rows as _pack_rows, restore_rows as _restore_row
 from custom_ops_lib import (  # noqa: F401  (layer operators)
     grouped_matmul as _grouped_matmul,
     grouped_weight_grad,
+    layer_norm as _layer_norm,
     layer_norm_backward,
     layer_norm_forward,
     orthogonalize as _orthogonalize,
@@ -115,22 +116,6 @@ def restore_node_tensor(packed_tensor, inv_permutation):
 # --------------------------------------------------------------------------
 # Layer operators around the SpMM (no counterpart in the reference)
 # --------------------------------------------------------------------------
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.fp32_bias = bias is not None and bias.dtype == torch.float32
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dx, dw, db = layer_norm_backward(grad, x, mean, rstd, weight, *ctx.needs_input_grad[:3], ctx.fp32_bias)
-        return dx, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension
     of a CUDA tensor x (fp16, bf16 or fp32, any width), differentiable in x,
@@ -141,25 +126,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     run in a fixed order.  ``layer_norm_forward`` / ``layer_norm_backward`` are
     the two passes by themselves.
     """
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return layer_norm_forward(x, weight, bias, eps, False)[0]
-
-
-class _GroupedMatmul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, group_ptr):
-        ctx.save_for_backward(x, weight, group_ptr)
-        return _grouped_matmul(x, weight, group_ptr, False)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, group_ptr = ctx.saved_tensors
-        dx = _grouped_matmul(grad, weight, group_ptr, True) if ctx.needs_input_grad[0] else None
-        dw = grouped_weight_grad(x, grad, group_ptr) if ctx.needs_input_grad[1] else None
-        return dx, dw, None
+    return _layer_norm(x, weight, bias, eps)
 
 
 def grouped_matmul(x, weight, group_ptr, transposed=False):
@@ -174,8 +141,6 @@ def grouped_matmul(x, weight, group_ptr, transposed=False):
     form); ``grouped_weight_grad`` is the weight's gradient by itself.  A
     malformed range raises the device status instead of a fault.
     """
-    if not transposed and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        return _GroupedMatmul.apply(x, weight, group_ptr)
     return _grouped_matmul(x, weight, group_ptr, transposed)
 
 

@@ -216,3 +216,15 @@ def test_refusals(lib):
         lib.layer_norm_backward(grad[:, :16], x, mean, rstd, w)
     with pytest.raises(RuntimeError, match="one value per row"):
         lib.layer_norm_backward(grad, x, mean[:2], rstd, w)
+
+
+def test_differentiable_once(lib):
+    x, w, b, grad = make(4, 32, F32, F32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    first = torch.autograd.grad(lib.layer_norm(*leaves), leaves, grad, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        first[0].sum().backward()
+    # a frozen parameter gets no gradient, the others keep theirs
+    y = lib.layer_norm(x, w.detach(), b)
+    dx, db = torch.autograd.grad(y, [x, b], grad)
+    assert torch.equal(dx, first[0].detach()) and torch.equal(db, first[2].detach())
