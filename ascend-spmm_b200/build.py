@@ -33,10 +33,10 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               f"-I{INCLUDE}"]
 
-CU_SOURCES = ["status.cu", "gather.cu", "gather_mma.cu", "window.cu", "window_warp.cu", "window_tc.cu", "rows.cu", "cube.cu", "preprocess.cu", "noalloc.cu", "l2plan.cu", "norm.cu", "gemm_tc.cu", "grouped.cu", "ortho.cu", "capi_layers.cu", "capi.cu"]
+CU_SOURCES = ["status.cu", "gather.cu", "gather_mma.cu", "window.cu", "window_warp.cu", "window_tc.cu", "rows.cu", "cube.cu", "preprocess.cu", "noalloc.cu", "l2plan.cu", "norm.cu", "gemm_tc.cu", "grouped.cu", "ortho.cu", "ortho_small.cu", "capi_layers.cu", "capi.cu"]
 HEADERS = ["common.cuh", "engine.h"]
-LAYER_SOURCES = ["norm.cu", "gemm_tc.cu", "grouped.cu", "ortho.cu", "capi_layers.cu"]
-LAYER_HEADERS = ["layer.cuh", "layer.h", "tc.cuh", "gemm_tc.cuh"]
+LAYER_SOURCES = ["norm.cu", "gemm_tc.cu", "grouped.cu", "ortho.cu", "ortho_small.cu", "capi_layers.cu"]
+LAYER_HEADERS = ["layer.cuh", "layer.h", "tc.cuh", "gemm_tc.cuh", "ortho.cuh"]
 
 
 def _newer(target: Path, deps) -> bool:

@@ -159,29 +159,6 @@ template <int MODE, int BN, int EPI> struct Walk {
     }
 };
 
-__device__ __forceinline__ uint4 pack8(const float *v, bool bf16)
-{
-    uint4 w;
-    unsigned *u = reinterpret_cast<unsigned *>(&w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (bf16) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            u[i] = *reinterpret_cast<const unsigned *>(&h);
-        } else {
-            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-            u[i] = *reinterpret_cast<const unsigned *>(&h);
-        }
-    }
-    return w;
-}
-
-__device__ __forceinline__ void st_shared16(unsigned at, uint4 v)
-{
-    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                 : "memory");
-}
-
 template <int MODE, int BN, bool AMN, bool BMN, int EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,

@@ -13,8 +13,9 @@
 // products take the high part, the term a X both.  Otherwise the rounding of
 // X would be multiplied by a in every step along the directions whose
 // singular values are still small: 5e-3 after five steps on a low-rank update
-// with noise, 2e-4 with the low part.  Powers of two scale the stored values
-// away from fp16's subnormals and leave a factor of 100 below its maximum.
+// with noise, 2e-4 with the low part.
+//
+// Small matrices run in one launch: ortho_small.cu.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
@@ -23,13 +24,13 @@
 #include "gemm_tc.cuh"
 #include "layer.cuh"
 #include "layer.h"
+#include "ortho.cuh"
 
 namespace spmmb {
 
 namespace {
 
-constexpr float kScaleX = 512.f, kScaleG = 256.f, kScaleP = 256.f;   // stored = value * scale
-constexpr int kParts = 64;                                           // partial sums of squares per matrix, at most
+constexpr int kParts = 64;   // partial sums of squares per matrix, at most
 
 int64_t pad8(int64_t x) { return (x + 7) & ~int64_t(7); }
 
@@ -176,11 +177,12 @@ cudaError_t update(const OrthoLaunch &o, const Space &w, tc::GemmArgs g, const _
 
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int)
 {
-    return Space(batch, m, n, nullptr).bytes(batch);
+    return ortho_small_eligible(m, n) ? 0 : Space(batch, m, n, nullptr).bytes(batch);
 }
 
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
+    if (ortho_small_eligible(o.m, o.n)) return launch_ortho_small(o, stream);
     const Space w(o.batch, o.m, o.n, workspace);
     switch (o.dtype) {
         case SPMM_F16: start<__half>(o, w, stream); break;

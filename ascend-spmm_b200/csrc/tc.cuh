@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_bf16.h>
 
 #include "common.cuh"
 
@@ -104,6 +105,30 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v)
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Eight fp32 values as fp16 or bf16.
+__device__ __forceinline__ uint4 pack8(const float *v, bool bf16)
+{
+    uint4 w;
+    unsigned *u = reinterpret_cast<unsigned *>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (bf16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *reinterpret_cast<const unsigned *>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            u[i] = *reinterpret_cast<const unsigned *>(&h);
+        }
+    }
+    return w;
+}
+
+__device__ __forceinline__ void st_shared16(unsigned at, uint4 v)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
 }
 
 // Shared-memory matrix descriptor (sm100): start address, leading and stride
