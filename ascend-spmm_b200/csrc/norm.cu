@@ -10,9 +10,7 @@
 // and dy and writes dx.  A team of lanes owns a row and keeps it in
 // registers, so the mean and then the centred squares are summed from
 // registers in fp32 (no E[x^2] - E[x]^2, whose cancellation would lose rows
-// with a large mean) and each element crosses memory once.  A team is 8
-// lanes for rows of up to sixteen 16-byte vectors, a warp up to 128 vectors,
-// a block above.
+// with a large mean) and each element crosses memory once.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
@@ -27,14 +25,9 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 
-// VE consecutive elements as one load or store.
-template <int BYTES> struct Raw;
-template <> struct Raw<16> { using Type = uint4; };
-template <> struct Raw<4> { using Type = unsigned; };
-template <> struct Raw<2> { using Type = unsigned short; };
-
+// A 16-byte vector of a row.
 template <typename T, int VE> union Pack {
-    typename Raw<sizeof(T) * VE>::Type raw;
+    uint4 raw;
     T e[VE];
     __device__ Pack() {}
 };
@@ -45,44 +38,40 @@ template <typename T, int VE> __device__ __forceinline__ void unpack(const Pack<
     for (int i = 0; i < VE; ++i) f[i] = elem_f32<T>(p.e[i]);
 }
 
-// VE parameters (weight or bias) starting at column c: of the rows' type or fp32.
-template <typename T, int VE>
-__device__ __forceinline__ void load_params(const void *p, bool f32, int64_t c, float *f)
+template <typename T> __device__ __forceinline__ float load_param(const void *p, bool f32, int64_t c)
 {
-    if (f32) {
-        const float *q = static_cast<const float *>(p) + c;
-        if constexpr (VE % 4 == 0) {
-#pragma unroll
-            for (int i = 0; i < VE / 4; ++i) {
-                const float4 v = __ldg(reinterpret_cast<const float4 *>(q) + i);
-                f[4 * i] = v.x; f[4 * i + 1] = v.y; f[4 * i + 2] = v.z; f[4 * i + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < VE; ++i) f[i] = __ldg(q + i);
-        }
-    } else {
-        Pack<T, VE> v;
-        v.raw = __ldg(reinterpret_cast<const decltype(v.raw) *>(static_cast<const T *>(p) + c));
-        unpack<T, VE>(v, f);
-    }
+    return f32 ? __ldg(static_cast<const float *>(p) + c) : elem_f32<T>(static_cast<const T *>(p)[c]);
 }
 
-// Sum over the lanes of a team of at most a warp, or over a block through
-// `red` (one float per warp; the caller alternates two buffers so that one
-// barrier per sum is enough).
-template <int TEAM> __device__ __forceinline__ float team_sum(float v, float *red)
+// Sums of N values over a team: shuffles within a warp, then, for a team of
+// several warps, one exchange through `red` behind a barrier of the team's
+// own threads.  The caller alternates two `red` buffers, so that one barrier
+// per sum is enough.
+template <int TEAM, int BLOCK> __device__ __forceinline__ void team_barrier(int team)
+{
+    if constexpr (TEAM == BLOCK) __syncthreads();
+    else asm volatile("bar.sync %0, %1;\n" ::"r"(team + 1), "n"(TEAM) : "memory");
+}
+template <int TEAM, int BLOCK, int N> __device__ __forceinline__ void team_sum(float (&v)[N], float (*red)[N], int team)
 {
 #pragma unroll
-    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-    if constexpr (TEAM > 32) {
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = 0.f;
+    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
-        for (int w = 0; w < TEAM / 32; ++w) v += red[w];
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kFull, v[i], o);
+    if constexpr (TEAM > 32) {
+        constexpr int kWarps = TEAM / 32;
+        float(*mine)[N] = red + team * kWarps;
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) mine[threadIdx.x % TEAM >> 5][i] = v[i];
+        team_barrier<TEAM, BLOCK>(team);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += mine[w][i];
     }
-    return v;
 }
 
 struct NormArgs {
@@ -95,77 +84,197 @@ struct NormArgs {
     bool pf32;               // weight and bias are fp32
 };
 
-// Threads per block for a team size.
-template <int TEAM> constexpr int kBlock = TEAM > 32 ? TEAM : 128;
+// What a lane holds of its team's rows: NV 16-byte vectors, and with ODD
+// (rows that start anywhere in a vector) NS single elements.  An odd row is a
+// head of single elements up to the first vector boundary, whole vectors, and
+// a tail of single elements.  A team only takes rows that start at the same
+// place in a vector (its row stride is a multiple of VE), so each lane keeps
+// its columns, and their parameters, for all its rows.
+template <typename T, int NV_, int TEAM_, bool ODD_> struct Part {
+    static constexpr int NV = NV_, TEAM = TEAM_, VE = 16 / sizeof(T);
+    static constexpr bool ODD = ODD_;
+    static constexpr int NS = !ODD ? 0 : TEAM < 16 ? 2 : 1, KS = NS ? NS : 1;
+    int width, vec, vectors;   // vec: first column of vector 0; vectors: this lane's
+    int single[KS];            // column of single element k, -1 for none
 
-template <typename T, int VE, int NV, int TEAM>
-__global__ void __launch_bounds__(kBlock<TEAM>) norm_forward_kernel(const NormArgs a)
+    __device__ __forceinline__ Part(int64_t row, int64_t w, int t) : width((int)w)
+    {
+        int head = 0, body = width / VE;
+        if constexpr (ODD) {
+            head = min((VE - (int)(row * w % VE)) % VE, width);
+            body = (width - head) / VE;
+            const int tail = width - head - body * VE;
+            if constexpr (NS == 2) {
+                single[0] = t < head ? t : -1;
+                single[1] = t < tail ? width - tail + t : -1;
+            } else {
+                single[0] = t < 8 ? (t < head ? t : -1) : t - 8 < tail ? width - tail + t - 8 : -1;
+            }
+        }
+        vec = head + t * VE;
+        vectors = t < body ? (body - t + TEAM - 1) / TEAM : 0;
+    }
+    __device__ __forceinline__ int col(int i) const { return vec + i * TEAM * VE; }
+    __device__ __forceinline__ int elements() const
+    {
+        int n = vectors * VE;
+        for (int k = 0; k < NS; ++k) n += single[k] >= 0;
+        return n;
+    }
+};
+
+// One row's elements of a lane.
+template <typename P, typename T> struct Row {
+    Pack<T, P::VE> v[P::NV];
+    T s[P::KS];
+    __device__ __forceinline__ void load(const T *x, int64_t r, int64_t rows, const P &p)
+    {
+        if (r >= rows) return;
+        const T *q = x + r * p.width;
+#pragma unroll
+        for (int i = 0; i < P::NV; ++i)
+            if (i < p.vectors) v[i].raw = __ldcs(reinterpret_cast<const uint4 *>(q + p.col(i)));
+#pragma unroll
+        for (int k = 0; k < P::NS; ++k)
+            if (p.single[k] >= 0) s[k] = q[p.single[k]];
+    }
+};
+
+// Parameters of the lane's columns (`none` where there is no such array).
+template <typename P, typename T> struct Params {
+    float v[P::NV][P::VE], s[P::KS];
+    __device__ __forceinline__ Params(const void *p, bool f32, float none, const P &part)
+    {
+#pragma unroll
+        for (int i = 0; i < P::NV; ++i) {
+            if (!P::ODD && p && i < part.vectors) {
+                if (f32) {
+#pragma unroll
+                    for (int e = 0; e < P::VE; e += 4) {
+                        const float *q = static_cast<const float *>(p) + part.col(i) + e;
+                        const float4 u = __ldg(reinterpret_cast<const float4 *>(q));
+                        v[i][e] = u.x; v[i][e + 1] = u.y; v[i][e + 2] = u.z; v[i][e + 3] = u.w;
+                    }
+                } else {
+                    Pack<T, P::VE> u;
+                    u.raw = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p) + part.col(i)));
+                    unpack<T, P::VE>(u, v[i]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < P::VE; ++e)
+                    v[i][e] = p && i < part.vectors ? load_param<T>(p, f32, part.col(i) + e) : none;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < P::NS; ++k) s[k] = p && part.single[k] >= 0 ? load_param<T>(p, f32, part.single[k]) : none;
+    }
+};
+
+template <typename T, int NV, int TEAM, int BLOCK, bool ODD>
+__global__ void __launch_bounds__(BLOCK) norm_forward_kernel(const NormArgs a)
 {
-    __shared__ float red[2][32];
-    constexpr int kTeams = kBlock<TEAM> / TEAM;
+    using P = Part<T, NV, TEAM, ODD>;
+    constexpr int kTeams = BLOCK / TEAM, VE = P::VE, kLanes = TEAM < 32 ? TEAM : 32;
+    __shared__ float red[2][BLOCK / 32][2], count[BLOCK / 32];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const float inv = 1.f / (float)a.width;
     const T *x = static_cast<const T *>(a.x);
-    T *y = static_cast<T *>(a.y);
-    // every lane of a warp (every thread of a block team) takes the same number of turns
-    for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < a.rows; r0 += (int64_t)gridDim.x * kTeams) {
-        const int64_t r = r0 + team;
-        const bool on = r < a.rows;
-        const T *xr = x + r * a.width;
-        Pack<T, VE> v[NV];
+    const int64_t stride = (int64_t)gridDim.x * kTeams;
+    int64_t r = (int64_t)blockIdx.x * kTeams + team;
+    const P part(r, a.width, t);
+    Row<P, T> row, next;
+    row.load(x, r, a.rows, part);
+    const Params<P, T> w(a.w, a.pf32, 1.f, part), b(a.b, a.pf32, 0.f, part);
+    float inv_n = 0.f;   // of the warp's elements of a row
+    if constexpr (TEAM > 32) {
+        float n = (float)part.elements();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t c = (int64_t)(t + i * TEAM) * VE;
-            if (on && c < a.width) v[i].raw = __ldcs(reinterpret_cast<const decltype(v[i].raw) *>(xr + c));
-        }
-        float s = 0.f;
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(kFull, n, o);
+        inv_n = n > 0.f ? 1.f / n : 0.f;
+        count[threadIdx.x >> 5] = n;   // read behind the first row's barrier
+    }
+    int turn = 0;
+    // every lane of a warp (every thread of a block) takes the same number of turns
+    for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < a.rows; r0 += stride, r += stride, turn ^= 1) {
+        next.load(x, r + stride, a.rows, part);   // in flight while this row is worked on
+        const bool on = r < a.rows;
+        // the team's (a wider team: the warp's) sum, then its squares around its own mean
+        float s = 0.f, q = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (on && (int64_t)(t + i * TEAM) * VE < a.width) {
+            if (on && i < part.vectors) {
                 float f[VE];
-                unpack<T, VE>(v[i], f);
+                unpack<T, VE>(row.v[i], f);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) s += f[e];
             }
-        const float mean = team_sum<TEAM>(s, red[0]) * inv;
-        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < P::NS; ++k)
+            if (on && part.single[k] >= 0) s += elem_f32<T>(row.s[k]);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+        float mean = s * (TEAM > 32 ? inv_n : inv);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (on && (int64_t)(t + i * TEAM) * VE < a.width) {
+            if (on && i < part.vectors) {
                 float f[VE];
-                unpack<T, VE>(v[i], f);
+                unpack<T, VE>(row.v[i], f);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) s = fmaf(f[e] - mean, f[e] - mean, s);
+                for (int e = 0; e < VE; ++e) q = fmaf(f[e] - mean, f[e] - mean, q);
             }
-        const float rstd = 1.f / sqrtf(team_sum<TEAM>(s, red[1]) * inv + a.eps);
-        if (!on) continue;
-        if (a.mean && t == 0) {
-            a.mean[r] = mean;
-            a.rstd[r] = rstd;
+#pragma unroll
+        for (int k = 0; k < P::NS; ++k)
+            if (on && part.single[k] >= 0) {
+                const float d = elem_f32<T>(row.s[k]) - mean;
+                q = fmaf(d, d, q);
+            }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) q += __shfl_xor_sync(kFull, q, o);
+        if constexpr (TEAM > 32) {
+            // join the warps behind one barrier: squares moved to the common mean
+            // (sum (x - M)^2 = sum (x - m)^2 + n (m - M)^2)
+            constexpr int kWarps = TEAM / 32;
+            float(*mine)[2] = red[turn] + team * kWarps;
+            if ((threadIdx.x & 31) == 0) {
+                mine[t >> 5][0] = mean;
+                mine[t >> 5][1] = q;
+            }
+            team_barrier<TEAM, BLOCK>(team);
+            s = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) s = fmaf(count[team * kWarps + k], mine[k][0], s);
+            mean = s * inv;
+            q = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const float d = mine[k][0] - mean;
+                q += fmaf(count[team * kWarps + k] * d, d, mine[k][1]);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t c = (int64_t)(t + i * TEAM) * VE;
-            if (c >= a.width) continue;
-            float f[VE], p[VE];
-            unpack<T, VE>(v[i], f);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) f[e] = (f[e] - mean) * rstd;
-            if (a.w) {
-                load_params<T, VE>(a.w, a.pf32, c, p);
-#pragma unroll
-                for (int e = 0; e < VE; ++e) f[e] *= p[e];
+        const float rstd = 1.f / sqrtf(q * inv + a.eps);
+        if (on) {
+            if (a.mean && t == 0) {
+                a.mean[r] = mean;
+                a.rstd[r] = rstd;
             }
-            if (a.b) {
-                load_params<T, VE>(a.b, a.pf32, c, p);
+            T *y = static_cast<T *>(a.y) + r * part.width;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) f[e] += p[e];
+            for (int i = 0; i < NV; ++i) {
+                if (i >= part.vectors) continue;
+                float f[VE];
+                unpack<T, VE>(row.v[i], f);
+                Pack<T, VE> o;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o.e[e] = elem_of<T>(fmaf((f[e] - mean) * rstd, w.v[i][e], b.v[i][e]));
+                __stcs(reinterpret_cast<uint4 *>(y + part.col(i)), o.raw);
             }
-            Pack<T, VE> o;
 #pragma unroll
-            for (int e = 0; e < VE; ++e) o.e[e] = elem_of<T>(f[e]);
-            __stcs(reinterpret_cast<decltype(o.raw) *>(y + r * a.width + c), o.raw);
+            for (int k = 0; k < P::NS; ++k)
+                if (part.single[k] >= 0)
+                    y[part.single[k]] = elem_of<T>(fmaf((elem_f32<T>(row.s[k]) - mean) * rstd, w.s[k], b.s[k]));
         }
+        row = next;
     }
 }
 
@@ -173,28 +282,30 @@ __global__ void __launch_bounds__(kBlock<TEAM>) norm_forward_kernel(const NormAr
 template <typename T>
 __global__ void __launch_bounds__(512) norm_forward_wide_kernel(const NormArgs a)
 {
-    __shared__ float red[2][32];
+    __shared__ float red[2][16][1];
     const float inv = 1.f / (float)a.width;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + r * a.width;
         T *y = static_cast<T *>(a.y) + r * a.width;
-        float s = 0.f;
-        for (int64_t c = threadIdx.x; c < a.width; c += 512) s += elem_f32<T>(x[c]);
-        const float mean = team_sum<512>(s, red[0]) * inv;
-        s = 0.f;
+        float s[1] = {0.f};
+        for (int64_t c = threadIdx.x; c < a.width; c += 512) s[0] += elem_f32<T>(x[c]);
+        team_sum<512, 512>(s, red[0], 0);
+        const float mean = s[0] * inv;
+        s[0] = 0.f;
         for (int64_t c = threadIdx.x; c < a.width; c += 512) {
             const float d = elem_f32<T>(x[c]) - mean;
-            s = fmaf(d, d, s);
+            s[0] = fmaf(d, d, s[0]);
         }
-        const float rstd = 1.f / sqrtf(team_sum<512>(s, red[1]) * inv + a.eps);
+        team_sum<512, 512>(s, red[1], 0);
+        const float rstd = 1.f / sqrtf(s[0] * inv + a.eps);
         if (a.mean && threadIdx.x == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
         for (int64_t c = threadIdx.x; c < a.width; c += 512) {
-            float f = (elem_f32<T>(x[c]) - mean) * rstd, p;
-            if (a.w) { load_params<T, 1>(a.w, a.pf32, c, &p); f *= p; }
-            if (a.b) { load_params<T, 1>(a.b, a.pf32, c, &p); f += p; }
+            float f = (elem_f32<T>(x[c]) - mean) * rstd;
+            if (a.w) { f *= load_param<T>(a.w, a.pf32, c); }
+            if (a.b) { f += load_param<T>(a.b, a.pf32, c); }
             y[c] = elem_of<T>(f);
         }
     }
@@ -203,108 +314,121 @@ __global__ void __launch_bounds__(512) norm_forward_wide_kernel(const NormArgs a
 // Backward: the lane that holds a column holds it for every row of its team,
 // so dw and db accumulate in its registers; the teams of a block are added
 // through shared memory and the block writes one partial row.
-template <typename T, int VE, int NV, int TEAM>
-__global__ void __launch_bounds__(kBlock<TEAM>) norm_backward_kernel(const NormArgs a)
+template <typename T, int NV, int TEAM, int BLOCK, bool ODD>
+__global__ void __launch_bounds__(BLOCK) norm_backward_kernel(const NormArgs a)
 {
-    __shared__ float red[2][2][32];
-    constexpr int kTeams = kBlock<TEAM> / TEAM;
+    using P = Part<T, NV, TEAM, ODD>;
+    constexpr int kTeams = BLOCK / TEAM, VE = P::VE;
+    __shared__ float red[2][BLOCK / 32][2];
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const float inv = 1.f / (float)a.width;
     const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy);
-    T *dx = static_cast<T *>(a.y);
-    float dw[NV][VE], db[NV][VE];
+    const int64_t stride = (int64_t)gridDim.x * kTeams;
+    int64_t r = (int64_t)blockIdx.x * kTeams + team;
+    const P part(r, a.width, t);
+    Row<P, T> vx, vg, nx, ng;
+    vx.load(x, r, a.rows, part);
+    vg.load(dy, r, a.rows, part);
+    float mean = r < a.rows ? a.mean[r] : 0.f, rstd = r < a.rows ? a.rstd[r] : 0.f;
+    const Params<P, T> w(a.w, a.pf32, 1.f, part);
+    float dw[NV][VE], db[NV][VE], dws[P::KS], dbs[P::KS];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < VE; ++e) dw[i][e] = db[i][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < P::KS; ++k) dws[k] = dbs[k] = 0.f;
     int turn = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < a.rows; r0 += (int64_t)gridDim.x * kTeams, turn ^= 1) {
-        const int64_t r = r0 + team;
-        const bool on = r < a.rows;
-        Pack<T, VE> vx[NV], vg[NV];
+    for (int64_t r0 = (int64_t)blockIdx.x * kTeams; r0 < a.rows; r0 += stride, r += stride, turn ^= 1) {
+        const bool on = r < a.rows, more = r + stride < a.rows;
+        nx.load(x, r + stride, a.rows, part);   // in flight while this row is worked on
+        ng.load(dy, r + stride, a.rows, part);
+        const float next_mean = more ? a.mean[r + stride] : 0.f, next_rstd = more ? a.rstd[r + stride] : 0.f;
+        float s[2] = {0.f, 0.f};
+        auto add = [&](float f, float g, float wv, float &dwv, float &dbv) {
+            const float xh = (f - mean) * rstd, gw = g * wv;
+            dwv = fmaf(g, xh, dwv);
+            dbv += g;
+            s[0] += gw;
+            s[1] = fmaf(gw, xh, s[1]);
+        };
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int64_t c = (int64_t)(t + i * TEAM) * VE;
-            if (on && c < a.width) {
-                vx[i].raw = __ldcs(reinterpret_cast<const decltype(vx[i].raw) *>(x + r * a.width + c));
-                vg[i].raw = __ldcs(reinterpret_cast<const decltype(vg[i].raw) *>(dy + r * a.width + c));
-            }
+            if (!on || i >= part.vectors) continue;
+            float f[VE], g[VE];
+            unpack<T, VE>(vx.v[i], f);
+            unpack<T, VE>(vg.v[i], g);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) add(f[e], g[e], w.v[i][e], dw[i][e], db[i][e]);
         }
-        const float mean = on ? a.mean[r] : 0.f, rstd = on ? a.rstd[r] : 0.f;
-        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t c = (int64_t)(t + i * TEAM) * VE;
-            if (on && c < a.width) {
-                float f[VE], g[VE], p[VE];
-                unpack<T, VE>(vx[i], f);
-                unpack<T, VE>(vg[i], g);
-                if (a.w) load_params<T, VE>(a.w, a.pf32, c, p);
+        for (int k = 0; k < P::NS; ++k)
+            if (on && part.single[k] >= 0) add(elem_f32<T>(vx.s[k]), elem_f32<T>(vg.s[k]), w.s[k], dws[k], dbs[k]);
+        if (a.y) {   // the same for every thread
+            team_sum<TEAM, BLOCK>(s, red[turn], team);
+            const float c1 = s[0] * inv, c2 = s[1] * inv;
+            auto grad = [&](float f, float g, float wv) {
+                const float xh = (f - mean) * rstd;
+                return elem_of<T>(rstd * (g * wv - c1 - xh * c2));
+            };
+            T *dx = static_cast<T *>(a.y) + r * part.width;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    const float xh = (f[e] - mean) * rstd;
-                    dw[i][e] = fmaf(g[e], xh, dw[i][e]);
-                    db[i][e] += g[e];
-                    const float gw = a.w ? g[e] * p[e] : g[e];
-                    s1 += gw;
-                    s2 = fmaf(gw, xh, s2);
-                }
+            for (int i = 0; i < NV; ++i) {
+                if (!on || i >= part.vectors) continue;
+                float f[VE], g[VE];
+                unpack<T, VE>(vx.v[i], f);
+                unpack<T, VE>(vg.v[i], g);
+                Pack<T, VE> o;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o.e[e] = grad(f[e], g[e], w.v[i][e]);
+                __stcs(reinterpret_cast<uint4 *>(dx + part.col(i)), o.raw);
             }
-        }
-        if (!a.y) continue;   // the same for every thread: only dw and db wanted
-        const float c1 = team_sum<TEAM>(s1, red[turn][0]) * inv, c2 = team_sum<TEAM>(s2, red[turn][1]) * inv;
-        if (!on) continue;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int64_t c = (int64_t)(t + i * TEAM) * VE;
-            if (c >= a.width) continue;
-            float f[VE], g[VE], p[VE];
-            unpack<T, VE>(vx[i], f);
-            unpack<T, VE>(vg[i], g);
-            if (a.w) load_params<T, VE>(a.w, a.pf32, c, p);
-            Pack<T, VE> o;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                const float xh = (f[e] - mean) * rstd, gw = a.w ? g[e] * p[e] : g[e];
-                o.e[e] = elem_of<T>(rstd * (gw - c1 - xh * c2));
-            }
-            __stcs(reinterpret_cast<decltype(o.raw) *>(dx + r * a.width + c), o.raw);
+            for (int k = 0; k < P::NS; ++k)
+                if (on && part.single[k] >= 0)
+                    dx[part.single[k]] = grad(elem_f32<T>(vx.s[k]), elem_f32<T>(vg.s[k]), w.s[k]);
         }
+        vx = nx;
+        vg = ng;
+        mean = next_mean;
+        rstd = next_rstd;
     }
     if (!a.part) return;
-    float *pw = a.part + (int64_t)blockIdx.x * 2 * a.width, *pb = pw + a.width;
-    if constexpr (kTeams == 1) {
+    float *pw = a.part + (int64_t)blockIdx.x * 2 * a.width;
+    auto put = [&](float *at, const float (&v)[NV][VE], const float (&single)[P::KS]) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-                const int64_t c = (int64_t)(t + i * TEAM) * VE + e;
-                if (c < a.width) { pw[c] = dw[i][e]; pb[c] = db[i][e]; }
-            }
+            for (int e = 0; e < VE; ++e)
+                if (i < part.vectors) at[part.col(i) + e] = v[i][e];
+#pragma unroll
+        for (int k = 0; k < P::NS; ++k)
+            if (part.single[k] >= 0) at[part.single[k]] = single[k];
+    };
+    if constexpr (kTeams == 1) {
+        put(pw, dw, dws);
+        put(pw + a.width, db, dbs);
     } else {
-        __shared__ float sums[kTeams][TEAM * VE + 1];
-        for (int which = 0; which < 2; ++which)
+        __shared__ float sums[kTeams][TEAM * NV * VE + 15];   // by column
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+            if (which) put(sums[team], db, dbs);
+            else put(sums[team], dw, dws);
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.width; c += BLOCK) {
+                float v = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < VE; ++e) sums[team][t * VE + e] = which ? db[i][e] : dw[i][e];
-                __syncthreads();
-                for (int j = threadIdx.x; j < TEAM * VE; j += kBlock<TEAM>) {
-                    float v = 0.f;
-#pragma unroll
-                    for (int k = 0; k < kTeams; ++k) v += sums[k][j];
-                    const int64_t c = (int64_t)i * TEAM * VE + j;
-                    if (c < a.width) (which ? pb : pw)[c] = v;
-                }
+                for (int k = 0; k < kTeams; ++k) v += sums[k][c];
+                pw[which * a.width + c] = v;
             }
+        }
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormArgs a)
 {
-    __shared__ float red[2][2][32];
+    __shared__ float red[2][16][2];
     const float inv = 1.f / (float)a.width;
     float *pw = a.part ? a.part + (int64_t)blockIdx.x * 2 * a.width : nullptr;
     if (pw)
@@ -314,48 +438,51 @@ __global__ void __launch_bounds__(512) norm_backward_wide_kernel(const NormArgs 
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
         const T *x = static_cast<const T *>(a.x) + r * a.width, *dy = static_cast<const T *>(a.dy) + r * a.width;
         const float mean = a.mean[r], rstd = a.rstd[r];
-        float s1 = 0.f, s2 = 0.f;
+        float s[2] = {0.f, 0.f};
         for (int64_t c = threadIdx.x; c < a.width; c += 512) {
             const float g = elem_f32<T>(dy[c]), xh = (elem_f32<T>(x[c]) - mean) * rstd;
-            float p = 1.f;
-            if (a.w) load_params<T, 1>(a.w, a.pf32, c, &p);
-            s1 += g * p;
-            s2 = fmaf(g * p, xh, s2);
+            const float p = a.w ? load_param<T>(a.w, a.pf32, c) : 1.f;
+            s[0] += g * p;
+            s[1] = fmaf(g * p, xh, s[1]);
             if (pw) {   // this thread's own columns
                 pw[c] = fmaf(g, xh, pw[c]);
                 pw[a.width + c] += g;
             }
         }
         if (!a.y) continue;
-        const float c1 = team_sum<512>(s1, red[turn][0]) * inv, c2 = team_sum<512>(s2, red[turn][1]) * inv;
+        team_sum<512, 512>(s, red[turn], 0);
+        const float c1 = s[0] * inv, c2 = s[1] * inv;
         T *dx = static_cast<T *>(a.y) + r * a.width;
         for (int64_t c = threadIdx.x; c < a.width; c += 512) {
             const float xh = (elem_f32<T>(x[c]) - mean) * rstd;
-            float p = 1.f;
-            if (a.w) load_params<T, 1>(a.w, a.pf32, c, &p);
+            const float p = a.w ? load_param<T>(a.w, a.pf32, c) : 1.f;
             dx[c] = elem_of<T>(rstd * (elem_f32<T>(dy[c]) * p - c1 - xh * c2));
         }
     }
 }
 
-// Adds the blocks' partial rows: 32 columns per block, 8 partial rows at a
+// Adds the blocks' partial rows: 32 columns per block, 32 partial rows at a
 // time, in an order that depends on the number of partials alone.
 template <typename P>
-__global__ void __launch_bounds__(256) norm_params_kernel(const float *part, int blocks, int64_t width, P *dw, P *db)
+__global__ void __launch_bounds__(1024) norm_params_kernel(const float *part, int blocks, int64_t width, P *dw, P *db)
 {
-    __shared__ float sums[8][33];
+    __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;   // over dw's columns, then db's
     float s = 0.f;
-    if (c < 2 * width)
-        for (int k = row; k < blocks; k += 8) s += part[(int64_t)k * 2 * width + c];
+    if (c < 2 * width) {
+#pragma unroll 8
+        for (int k = row; k < blocks; k += 32) s += part[(int64_t)k * 2 * width + c];
+    }
     sums[row][lane] = s;
     __syncthreads();
-    if (row == 0 && c < 2 * width) {
+    s = sums[lane][row];   // column `row` of the block, its 32 sums across the lanes
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += sums[k][lane];
-        P *out = c < width ? dw : db;
-        if (out) out[c < width ? c : c - width] = elem_of<P>(s);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+    const int64_t d = (int64_t)blockIdx.x * 32 + row;
+    if (lane == 0 && d < 2 * width) {
+        P *out = d < width ? dw : db;
+        if (out) out[d < width ? d : d - width] = elem_of<P>(s);
     }
 }
 
@@ -372,43 +499,56 @@ template <auto kernel> int64_t grid_of(int threads, int64_t turns)
     return std::max<int64_t>(1, std::min<int64_t>((int64_t)per_sm * device_sm_count(), turns));
 }
 
-template <typename T, int VE, int NV, int TEAM> cudaError_t run_team(const NormArgs &a, bool backward, int64_t max_blocks,
-                                                                     int64_t *blocks, cudaStream_t stream)
+template <typename T, int NV, int TEAM, bool ODD, bool BACKWARD>
+cudaError_t run_team(const NormArgs &a, int64_t max_blocks, int64_t *blocks, cudaStream_t stream)
 {
-    constexpr int threads = kBlock<TEAM>, teams = threads / TEAM;
-    const int64_t turns = (a.rows + teams - 1) / teams;
-    if (backward) {
-        *blocks = std::min(max_blocks, grid_of<norm_backward_kernel<T, VE, NV, TEAM>>(threads, turns));
-        norm_backward_kernel<T, VE, NV, TEAM><<<(unsigned)*blocks, threads, 0, stream>>>(a);
-    } else {
-        *blocks = grid_of<norm_forward_kernel<T, VE, NV, TEAM>>(threads, turns);
-        norm_forward_kernel<T, VE, NV, TEAM><<<(unsigned)*blocks, threads, 0, stream>>>(a);
-    }
+    constexpr int kBlock = TEAM < 256 ? 256 : TEAM, kTeams = kBlock / TEAM, VE = 16 / sizeof(T);
+    const int64_t turns = (a.rows + kTeams - 1) / kTeams;
+    constexpr auto kernel = [] {
+        if constexpr (BACKWARD) return norm_backward_kernel<T, NV, TEAM, kBlock, ODD>;
+        else return norm_forward_kernel<T, NV, TEAM, kBlock, ODD>;
+    }();
+    *blocks = grid_of<kernel>(kBlock, turns);
+    if (BACKWARD) *blocks = std::min(max_blocks, *blocks);
+    // a team's rows must start at the same place in a vector
+    constexpr int kStep = VE / kTeams > 1 ? VE / kTeams : 1;
+    if (ODD && *blocks < turns) *blocks = std::max<int64_t>(kStep, *blocks / kStep * kStep);
+    kernel<<<(unsigned)*blocks, kBlock, 0, stream>>>(a);
     return cudaGetLastError();
+}
+
+// Vectors per lane, measured (fp16, 524287 x 1024; GB/s of 6538): forward 4 on
+// a warp 6284, 2 on two warps 5312 (its two sums need a barrier); backward,
+// which also holds two accumulators per column, 2 on two warps 5967, 4 on a
+// warp 5390.
+template <typename T, bool ODD, bool BACKWARD>
+cudaError_t run_width(const NormArgs &a, int64_t max_blocks, int64_t *blocks, cudaStream_t s, bool *wide)
+{
+    constexpr int V = 16 / sizeof(T), NV = BACKWARD ? 2 : 4;
+    const int64_t v = a.width / V;   // whole vectors of a row, at most
+    if (v <= 8) return run_team<T, 1, 8, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 16) return run_team<T, 2, 8, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 16 * NV) return run_team<T, NV, 16, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 32 * NV) return run_team<T, NV, 32, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 64 * NV) return run_team<T, NV, 64, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 128 * NV) return run_team<T, NV, 128, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 256 * NV) return run_team<T, NV, 256, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (v <= 512 * NV) return run_team<T, NV, 512, ODD, BACKWARD>(a, max_blocks, blocks, s);
+    if (BACKWARD && v <= 2048) return run_team<T, 2, 1024, ODD, true>(a, max_blocks, blocks, s);
+    *wide = true;
+    return cudaSuccess;
 }
 
 template <typename T> cudaError_t run_norm(const NormArgs &a, bool backward, int64_t max_blocks, int64_t *blocks,
                                            cudaStream_t s)
 {
-    constexpr int V = 16 / sizeof(T);
-    if (a.width % V == 0) {   // rows of whole 16-byte vectors
-        const int64_t v = a.width / V;
-        if (v <= 8) return run_team<T, V, 1, 8>(a, backward, max_blocks, blocks, s);
-        if (v <= 16) return run_team<T, V, 2, 8>(a, backward, max_blocks, blocks, s);
-        if (v <= 32) return run_team<T, V, 1, 32>(a, backward, max_blocks, blocks, s);
-        if (v <= 64) return run_team<T, V, 2, 32>(a, backward, max_blocks, blocks, s);
-        if (v <= 128) return run_team<T, V, 4, 32>(a, backward, max_blocks, blocks, s);
-        if (v <= 256) return run_team<T, V, 2, 128>(a, backward, max_blocks, blocks, s);
-        if (v <= 512) return run_team<T, V, 2, 256>(a, backward, max_blocks, blocks, s);
-        if (v <= 1024) return run_team<T, V, 2, 512>(a, backward, max_blocks, blocks, s);
-        if (v <= 2048) return run_team<T, V, 2, 1024>(a, backward, max_blocks, blocks, s);
-    } else {                  // rows that start at any element
-        if (a.width <= 32) return run_team<T, 1, 4, 8>(a, backward, max_blocks, blocks, s);
-        if (a.width <= 128) return run_team<T, 1, 4, 32>(a, backward, max_blocks, blocks, s);
-        if (a.width <= 1024) return run_team<T, 1, 8, 128>(a, backward, max_blocks, blocks, s);
-        if (a.width <= 4096) return run_team<T, 1, 8, 512>(a, backward, max_blocks, blocks, s);
-        if (a.width <= 8192) return run_team<T, 1, 8, 1024>(a, backward, max_blocks, blocks, s);
-    }
+    bool wide = false;
+    const bool odd = a.width % (16 / sizeof(T)) != 0;
+    const cudaError_t e = backward ? odd ? run_width<T, true, true>(a, max_blocks, blocks, s, &wide)
+                                           : run_width<T, false, true>(a, max_blocks, blocks, s, &wide)
+                          : odd ? run_width<T, true, false>(a, max_blocks, blocks, s, &wide)
+                                  : run_width<T, false, false>(a, max_blocks, blocks, s, &wide);
+    if (!wide) return e;
     *blocks = std::min<int64_t>(a.rows, 2 * device_sm_count());
     if (backward) {
         *blocks = std::min(*blocks, max_blocks);
@@ -458,17 +598,17 @@ cudaError_t launch_norm_backward(const NormLaunch &n, const void *grad, void *dw
     const unsigned grid = (unsigned)((2 * n.width + 31) / 32);
     switch (n.param_dtype) {
         case SPMM_F16:
-            norm_params_kernel<__half><<<grid, 256, 0, stream>>>(a.part, (int)blocks, n.width,
+            norm_params_kernel<__half><<<grid, 1024, 0, stream>>>(a.part, (int)blocks, n.width,
                                                                  static_cast<__half *>(dweight),
                                                                  static_cast<__half *>(dbias));
             break;
         case SPMM_BF16:
-            norm_params_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a.part, (int)blocks, n.width,
+            norm_params_kernel<__nv_bfloat16><<<grid, 1024, 0, stream>>>(a.part, (int)blocks, n.width,
                                                                         static_cast<__nv_bfloat16 *>(dweight),
                                                                         static_cast<__nv_bfloat16 *>(dbias));
             break;
         default:
-            norm_params_kernel<float><<<grid, 256, 0, stream>>>(a.part, (int)blocks, n.width,
+            norm_params_kernel<float><<<grid, 1024, 0, stream>>>(a.part, (int)blocks, n.width,
                                                                 static_cast<float *>(dweight),
                                                                 static_cast<float *>(dbias));
     }
