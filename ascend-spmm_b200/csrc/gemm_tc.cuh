@@ -210,43 +210,46 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     };
 
     if (warp == 0) {
-        // ---- TMA warp: one lane issues
+        // ---- TMA warp: all lanes find the tile, one issues its copies
         unsigned slice = 0;   // slices issued
         for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
-            for (int pass = 0; pass < a.passes && ok; ++pass) {
-                const int za = (int)t.batch_a + a.pa[pass] * a.za, zb = (int)t.batch_b + a.pb[pass] * a.zb;
-                for (int64_t k = t.k0; k < t.k1; k += kBK, ++slice) {
-                    const unsigned st = slice % S::kStages;
-                    if (!bar_wait(empty + 8 * st, (slice / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
-                    if (lane == 0) {
+            const int n = (int)((t.k1 - t.k0 + kBK - 1) / kBK);
+            if (elect()) {
+                const int row0 = (int)t.row0, col0 = (int)t.col0;
+                for (int pass = 0; pass < a.passes && ok; ++pass) {
+                    const int za = (int)t.batch_a + a.pa[pass] * a.za, zb = (int)t.batch_b + a.pb[pass] * a.zb;
+                    int k = (int)t.k0;
+                    for (int i = 0; i < n; ++i, k += kBK) {
+                        const unsigned at = slice + pass * n + i, st = at % S::kStages;
+                        if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
                         const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA, bar = full + 8 * st;
                         bar_expect(bar, S::kA + S::kB);
                         if constexpr (AMN) {
 #pragma unroll
-                            for (int i = 0; i < kBM / 64; ++i)
-                                tma_load(sa + i * 8192, &map_a, (int)t.row0 + 64 * i, (int)k, za, bar);
+                            for (int c = 0; c < kBM / 64; ++c) tma_load(sa + c * 8192, &map_a, row0 + 64 * c, k, za, bar);
                         } else {
-                            tma_load(sa, &map_a, (int)k, (int)t.row0, za, bar);
+                            tma_load(sa, &map_a, k, row0, za, bar);
                         }
                         if constexpr (BMN) {
 #pragma unroll
-                            for (int i = 0; i < BN / 64; ++i)
-                                tma_load(sb + i * 8192, &map_b, (int)t.col0 + 64 * i, (int)k, zb, bar);
+                            for (int c = 0; c < BN / 64; ++c) tma_load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb, bar);
                         } else {
-                            tma_load(sb, &map_b, (int)k, (int)t.col0, zb, bar);
+                            tma_load(sb, &map_b, k, col0, zb, bar);
                         }
                     }
-                    __syncwarp();
                 }
             }
+            __syncwarp();
+            slice += a.passes * n;
+            ok = *abort == 0;
         }
-        if (!ok)   // the copies in flight land before the block leaves (bounded)
-            for (unsigned s = slice > S::kStages ? slice - S::kStages : 0; s < slice; ++s) {
+        if (!ok)   // the copies in flight land before the block leaves (bounded; a slice never issued runs out)
+            for (unsigned s = slice > 2 * S::kStages ? slice - 2 * S::kStages : 0; s < slice; ++s) {
                 volatile int never = 0;
-                bar_wait(full + 8 * (s % S::kStages), s / S::kStages & 1u, &never);
+                if (!bar_wait(full + 8 * (s % S::kStages), s / S::kStages & 1u, &never)) break;
             }
     } else if (warp == 1) {
-        // ---- MMA warp
+        // ---- MMA warp: one lane issues
         const unsigned idesc = idesc16(a.bf16, AMN, BMN, kBM, BN);
         // byte strides of the operands' layouts: K-major, 8 rows of 128 bytes per
         // swizzle atom; MN-major, atoms of 64 rows or columns x 8 deep, 8 KB apart
@@ -254,45 +257,60 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const uint64_t db = BMN ? desc128(base + S::kA, 8192, 1024) : desc128(base + S::kA, 16, 1024);
         constexpr unsigned step_a = (AMN ? 2048 : 32) >> 4, step_b = (BMN ? 2048 : 32) >> 4;
         unsigned slice = 0, used = 0;
+        // The products of the slice at position `at` (depth elements deep).
+        auto multiply = [&](unsigned at, int depth, unsigned d, bool first) {
+            const unsigned st = at % S::kStages, off = st * (S::kA + S::kB) >> 4;
+            if (depth == kBK) {
+#pragma unroll
+                for (int i = 0; i < kBK / 16; ++i)
+                    mma(d, da + off + i * step_a, db + off + i * step_b, idesc, first && i == 0 ? 0u : 1u);
+            } else {
+                for (int i = 0; i * 16 < depth; ++i)
+                    mma(d, da + off + i * step_a, db + off + i * step_b, idesc, first && i == 0 ? 0u : 1u);
+            }
+            commit(empty + 8 * st);
+        };
+        auto landed = [&](unsigned at) { return bar_wait(full + 8 * (at % S::kStages), at / S::kStages & 1u, abort); };
         for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
-            if (t.k0 >= t.k1) continue;
-            const unsigned acc = used & 1u;
-            if (!bar_wait(acc_empty + 8 * acc, (used >> 1 & 1u) ^ 1u, abort)) { give_up(2); break; }
+            const int depth = (int)(t.k1 - t.k0), n = (depth + kBK - 1) / kBK;
+            if (n <= 0) continue;
+            // kRagged: a last slice that ends within 16 rows needs the whole warp
+            const bool ragged = MODE == kRagged && (depth & 15);
+            const int whole = ragged ? n - 1 : n;
+            const unsigned d = tmem + (used & 1u) * BN;
+            if (!bar_wait(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) { give_up(2); break; }
             fence_after();
-            unsigned first = 1;
-            for (int pass = 0; pass < a.passes && ok; ++pass)
-                for (int64_t k = t.k0; k < t.k1; k += kBK, ++slice) {
-                    const unsigned st = slice % S::kStages;
-                    if (!bar_wait(full + 8 * st, slice / S::kStages & 1u, abort)) { give_up(3); break; }
-                    const int depth = (int)min((int64_t)kBK, t.k1 - k);
-                    if (MODE == kRagged && (depth & 15)) {
-                        // rows [depth, next 16) of both operands: zero
-                        const unsigned at = base + st * (S::kA + S::kB);
-                        const int pad = 16 - (depth & 15), quads = pad * 8;   // 16-byte pieces of a 64-wide column block
-                        for (int i = lane; i < quads * ((S::kA + S::kB) / 8192); i += 32)
-                            st_shared16(at + i / quads * 8192 + depth * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
-                        fence_async();
-                        __syncwarp();
+            for (int pass = 0; pass < a.passes; ++pass, slice += n) {
+                if (elect())
+                    for (int i = 0; i < whole; ++i) {
+                        if (!landed(slice + i)) { give_up(3); break; }
+                        multiply(slice + i, min(kBK, depth - i * kBK), d, pass == 0 && i == 0);
                     }
-                    fence_after();
-                    if (lane == 0) {
-                        const unsigned off = st * (S::kA + S::kB) >> 4;
-                        for (int i = 0; i * 16 < depth; ++i) {
-                            mma(tmem + acc * BN, da + off + i * step_a, db + off + i * step_b, idesc, first ? 0u : 1u);
-                            first = 0;
-                        }
-                        commit(empty + 8 * st);
-                    }
+                __syncwarp();
+                if (ragged && *abort == 0) {
+                    const unsigned at = slice + n - 1, st = at % S::kStages;
+                    if (!landed(at)) give_up(3);
+                    // the rows past the group's end, up to the next multiple of 16, of both operands: zero
+                    const unsigned buf = base + st * (S::kA + S::kB);
+                    const int deep = depth - (n - 1) * kBK;
+                    const int quads = (16 - (deep & 15)) * 8;   // 16-byte pieces of a 64-wide column block
+                    for (int i = lane; i < quads * ((S::kA + S::kB) / 8192); i += 32)
+                        st_shared16(buf + i / quads * 8192 + deep * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
+                    fence_async();
+                    __syncwarp();
+                    if (elect()) multiply(at, deep, d, pass == 0 && n == 1);
                     __syncwarp();
                 }
+            }
+            ok = *abort == 0;
             if (!ok) break;
-            if (lane == 0) commit(acc_full + 8 * acc);
+            if (elect()) commit(acc_full + 8 * (used & 1u));
             __syncwarp();
             ++used;
         }
         if (!ok) {   // every product issued is complete before TMEM is freed (bounded)
             volatile int never = 0;
-            if (lane == 0) commit(done);
+            if (elect()) commit(done);
             __syncwarp();
             bar_wait(done, 0, &never);
         }

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(SmallShape<R>::kThreads, 1) ortho_small_kernel
             put8_split(base + S::kHi + at, base + S::kLo + at, x + 8 * j);
         }
         publish();
-        if (threadIdx.x == 0) {
+        if (warp == 0 && tc::elect()) {
             for (int k = 0; k < kr; ++k) {   // the small products first
                 tc::mma(tmem + kG, hi + along(k), lo + along(k), kSquare, k > 0);
                 tc::mma(tmem + kG, lo + along(k), hi + along(k), kSquare, 1);
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(SmallShape<R>::kThreads, 1) ortho_small_kernel
             }
         }
         publish();
-        if (threadIdx.x == 0) {
+        if (warp == 0 && tc::elect()) {
             for (int k = 0; k < ks; ++k) {
                 tc::mma(tmem + kGG, pa + along(k), pb + along(k), kSquare, k > 0);
                 tc::mma(tmem + kGG, pb + along(k), pa + along(k), kSquare, 1);
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(SmallShape<R>::kThreads, 1) ortho_small_kernel
             }
         }
         publish();
-        if (threadIdx.x == 0) {
+        if (warp == 0 && tc::elect()) {
             for (int k = 0; k < ks; ++k) {
                 tc::mma(tmem + kX, pb + along(k), hi_mn + down(k), kWide, k > 0);
                 tc::mma(tmem + kX, pa + along(k), lo_mn + down(k), kWide, 1);

@@ -10,6 +10,16 @@
 namespace spmmb {
 namespace tc {
 
+// True in one lane of a converged warp, always the same one.  The instructions
+// that take their operands in uniform registers (TMA loads, tcgen05.mma and
+// commit) are issued behind it: behind a plain lane == 0 the compiler has to
+// serialise over the lanes that might be active.
+__device__ __forceinline__ bool elect()
+{
+    unsigned one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ void bar_init(unsigned bar, unsigned count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
@@ -27,10 +37,10 @@ __device__ __forceinline__ void bar_expect(unsigned bar, unsigned bytes)
 __device__ __forceinline__ bool bar_try(unsigned bar, unsigned parity)
 {
     unsigned ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
                  "selp.u32 %0, 1, 0, p;\n\t}\n"
                  : "=r"(ok)
-                 : "r"(bar), "r"(parity), "r"(20000)
+                 : "r"(bar), "r"(parity)
                  : "memory");
     return ok != 0;
 }
