@@ -27,21 +27,18 @@ EncodeTiled encoder()
     return f;
 }
 
-}  // namespace
-
-bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
-              int64_t batch_stride, int box_rows, bool bf16)
+bool encode_map(CUtensorMap *map, const void *p, CUtensorMapDataType type, int size, int64_t inner, int64_t rows,
+                int64_t batch, int64_t ld, int64_t batch_stride, int box_inner, int box_rows, CUtensorMapSwizzle swizzle)
 {
     const EncodeTiled encode = encoder();
     if (!encode) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)batch};
-    const cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)((batch > 1 ? batch_stride : ld) * 2)};
-    const cuuint32_t box[3] = {kBK, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
-    const auto type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)((batch > 1 ? batch_stride : ld) * size)};
+    const cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
     for (int attempt = 0; attempt < 2; ++attempt) {
         const CUresult r = encode(map, type, 3, const_cast<void *>(p), dims, strides, box, step,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r == CUDA_SUCCESS) return true;
         // a thread that has made no runtime call yet (an autograd worker) has no
         // current context: setting its device binds the primary one
@@ -50,6 +47,26 @@ bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int6
             return false;
     }
     return false;
+}
+
+}  // namespace
+
+bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
+              int64_t batch_stride, int box_rows, bool bf16)
+{
+    return encode_map(map, p, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, inner, rows,
+                      batch, ld, batch_stride, kBK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+bool make_out_map(CUtensorMap *map, void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
+                  int64_t batch_stride, int out_type)
+{
+    if (out_type == kOutF32)
+        return encode_map(map, p, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, inner, rows, batch, ld, batch_stride, 32, 32,
+                          CU_TENSOR_MAP_SWIZZLE_128B);
+    return encode_map(map, p,
+                      out_type == kOutBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                      inner, rows, batch, ld, batch_stride, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 }  // namespace tc

@@ -3,9 +3,9 @@
 //
 // A persistent block per SM walks output tiles of 128 x BN.  One warp issues
 // the TMA loads of 64-deep slices into a ring of stages, one warp the
-// tcgen05.mma of each slice, and four warps read a finished accumulator out
-// of TMEM, round it and store it while the next tile's products run into the
-// other accumulator.  Operands may be stored with the reduction contiguous
+// tcgen05.mma of each slice, and eight warps read a finished accumulator out
+// of TMEM, round it and store it by TMA (32 rows x 32 columns at a time)
+// while the next tile's products run into the other accumulator.  Operands may be stored with the reduction contiguous
 // (K-major) or with the rows or columns contiguous (MN-major): both layouts
 // are read as they lie, so no product needs a transposed copy.
 //
@@ -45,8 +45,7 @@ struct GemmArgs {
     int64_t m, n, k;          // kRows: n, k; kRagged: m, n; kDense: all
     int64_t batch;            // kDense
     int64_t part_rows;        // kRagged: a multiple of 64
-    float *parts;             // kRagged: [part_slots][m][n], the parts of groups of several
-    int64_t part_slots;
+    int64_t part_slots;       // kRagged: parts in the second output map ([part_slots][m][n])
     void *out;
     int64_t ldo, out_batch;   // elements
     int out_type;
@@ -58,25 +57,24 @@ struct GemmArgs {
     // kGram: x = alpha * accumulator; kPoly, kUpdate: x = alpha * accumulator
     // + beta * (in + in_lo), `in` laid out as the output.  kGram and kPoly
     // are symmetric and also write the transposed tile; kUpdate writes x as
-    // fp16 and, to out_lo, the rest that the rounding left (out_lo null: x
-    // alone, in the output's type).
+    // fp16 and, with `low`, the rest that the rounding left through the
+    // second output map (else x alone, in the output's type).
     float alpha, beta;
     const __half *in, *in_lo;
-    __half *out_lo;
+    bool low;
     int64_t ldi, in_batch;
     DevStatus *status;
 };
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kGemmThreads = 192;   // TMA warp, MMA warp, four epilogue warps
+constexpr int kEpiWarps = 8, kGemmThreads = 64 + 32 * kEpiWarps;   // TMA warp, MMA warp, epilogue warps
 
 template <int BN> struct GemmShape {
     static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int kChunk = 256;                           // bytes of a row staged at a time
-    static constexpr int kPitch = kChunk + 16;                   // odd in 16-byte units: no bank conflicts
     static constexpr int kStageOff = kStages * (kA + kB);
-    static constexpr int kBarOff = kStageOff + kBM * kPitch;
+    static constexpr int kStaging = 4096;                        // of an epilogue warp
+    static constexpr int kBarOff = kStageOff + kEpiWarps * kStaging;
     static constexpr int kFull = kBarOff, kEmpty = kFull + 8 * kStages, kAccFull = kEmpty + 8 * kStages;
     static constexpr int kAccEmpty = kAccFull + 16, kDone = kAccEmpty + 16, kTmem = kDone + 8, kAbort = kTmem + 4;
     static constexpr int kBytes = kAbort + 4;
@@ -88,7 +86,7 @@ template <int BN> struct GemmShape {
 struct Tile {
     int64_t batch_a, batch_b, row0, col0;   // operand batch, first row and column
     int64_t k0, k1;                         // range of the reduction (k0 == k1: zeros)
-    int64_t out;                            // element offset of the tile in `out` (in `parts`)
+    int64_t out_row, out_z;                 // first row and batch index in the output
     bool part;                              // kRagged: one part of several
     int rows, cols;                         // what is stored
     bool mirror;                            // kGram, kPoly: also the transposed tile
@@ -113,7 +111,8 @@ template <int MODE, int BN, int EPI> struct Walk {
             o->k0 = 0;
             o->k1 = seg >= 1 && seg <= a.ranges.groups ? a.k : 0;
             o->rows = (int)min((int64_t)kBM, e - o->row0);
-            o->out = o->row0 * a.ldo + o->col0;
+            o->out_row = o->row0;
+            o->out_z = 0;
         } else if constexpr (MODE == kRagged) {
             int64_t seg, b, e, inner, slots;
             if (!ranges.find(a.ranges, a.part_rows, mt * nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
@@ -129,7 +128,8 @@ template <int MODE, int BN, int EPI> struct Walk {
                 o->k1 = o->k0;
                 o->rows = 0;
             }
-            o->out = (o->part ? (slots + p) * a.m * a.n : (seg - 1) * a.out_batch) + o->row0 * a.n + o->col0;
+            o->out_row = o->row0;
+            o->out_z = o->part ? slots + p : seg - 1;
         } else {
             const bool half = EPI == kGram || EPI == kPoly;   // symmetric: the tiles on and below the diagonal
             const int64_t per = half ? mt * (mt + 1) / 2 : mt * nt;
@@ -151,7 +151,8 @@ template <int MODE, int BN, int EPI> struct Walk {
             o->k0 = 0;
             o->k1 = a.k;
             o->rows = (int)min((int64_t)kBM, a.m - o->row0);
-            o->out = q * a.out_batch + o->row0 * a.ldo + o->col0;
+            o->out_row = o->row0;
+            o->out_z = q;
             o->mirror = half && i != j;
         }
         o->cols = (int)min((int64_t)BN, a.n - o->col0);
@@ -162,6 +163,7 @@ template <int MODE, int BN, int EPI> struct Walk {
 template <int MODE, int BN, bool AMN, bool BMN, int EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+            const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_p,
             const __grid_constant__ GemmArgs a)
 {
     using S = GemmShape<BN>;
@@ -179,7 +181,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(acc_full + 8 * i, 1);
-            bar_init(acc_empty + 8 * i, 4);
+            bar_init(acc_empty + 8 * i, kEpiWarps);
         }
         bar_init(done, 1);
         // a misaligned stage ring would break the swizzle: give up before any copy
@@ -188,6 +190,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         prefetch_map(&map_a);
         prefetch_map(&map_b);
+        prefetch_map(&map_o);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(base + S::kTmem),
@@ -199,6 +202,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     __syncthreads();
     fence_after();
     const unsigned tmem = *reinterpret_cast<volatile unsigned *>(smem + S::kTmem);
+    let_next_kernel_start();
+    wait_for_earlier_kernels();   // nothing above reads or writes global memory
 
     Walk<MODE, BN, EPI> walk(a);
     Tile t;
@@ -315,13 +320,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             bar_wait(done, 0, &never);
         }
     } else {
-        // ---- epilogue warps: TMEM lanes 32 (warp % 4) .. + 31 are rows of the tile
-        const int row = (warp & 3) * 32 + lane;
-        const unsigned stage = base + S::kStageOff + row * S::kPitch;
-        const unsigned lanes = tmem + ((unsigned)((warp & 3) * 32) << 16);
+        // ---- epilogue warps: TMEM lanes 32 (warp % 4) .. + 31 are rows of the
+        // tile; of the two warps of a lane quarter one takes the even and one
+        // the odd blocks of 32 columns
+        const int row0 = (warp & 3) * 32, row = row0 + lane, parity = (warp - 2) / 4;
+        const unsigned stage = base + S::kStageOff + (warp - 2) * S::kStaging;
+        const unsigned lanes = tmem + ((unsigned)row0 << 16);
         const int out_size = a.out_type == kOutF32 ? 4 : 2;
-        // rows that do not start on 16 bytes cannot be bulk-copied
-        const bool bulk = (a.ldo * out_size & 15) == 0 && (a.out_batch * out_size & 15) == 0;
+        // an output whose rows do not start on 16 bytes has no tensor map
+        const bool mapped = (a.ldo * out_size & 15) == 0;
+        // a 16-byte piece in a row of the staged 64-byte (fp32: 128-byte) wide block, swizzled as its map
+        const unsigned swz2 = (unsigned)(lane >> 1 & 3), swz4 = (unsigned)(lane & 7);
         unsigned used = 0;
         for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
             const bool zero = t.k0 >= t.k1;
@@ -332,88 +341,113 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 ++used;
             }
             const bool on = row < t.rows, part = MODE == kRagged && t.part;
-            const int es = part ? 4 : out_size;
-            // kUpdate stages 64 columns of the high and of the low part side by side
-            const int chunk = EPI == kUpdate ? 64 : S::kChunk / es;
-            char *out = part ? reinterpret_cast<char *>(a.parts) : static_cast<char *>(a.out);
-            for (int c0 = 0; c0 < t.cols; c0 += chunk) {
-                bulk_wait_read();
-                if (EPI == kUpdate && !bulk) __syncwarp();   // the warp reads its rows' staging across lanes below
-                for (int c = 0; c < chunk && c0 + c < t.cols; c += 32) {
-                    float v[32];
-                    if (zero) {
+            const bool wide = part || out_size == 4;
+            const int y = (int)t.out_row + row0, z = (int)t.out_z;
+            // a group's last rows share the block with the next group's: no box for them
+            const bool boxed = (part || mapped) && (MODE != kRows || row0 + 32 <= t.rows);
+            for (int c = parity * 32; c < t.cols && row0 < t.rows; c += 64) {
+                float v[32];
+                if (zero) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-                    } else {
-                        tmem_ld32(lanes + acc * BN + c0 + c, v);
-                    }
-                    if constexpr (EPI != kStore) {
-                        const int64_t at = t.batch_a * a.in_batch + (t.row0 + row) * a.ldi + t.col0 + c0 + c;
+                    for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                } else {
+                    tmem_ld32(lanes + acc * BN + c, v);
+                }
+                if constexpr (EPI != kStore) {
+                    const int64_t at = t.batch_a * a.in_batch + (t.row0 + row) * a.ldi + t.col0 + c;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-                            if (EPI != kGram && on && t.col0 + c0 + c + i < a.ldi) {
-                                hi = *reinterpret_cast<const uint4 *>(a.in + at + i);
-                                if (EPI == kUpdate) lo = *reinterpret_cast<const uint4 *>(a.in_lo + at + i);
-                            }
-                            float h[8], l[8];
-                            unpack16<__half>(hi, h);
-                            unpack16<__half>(lo, l);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                v[i + e] = EPI == kGram ? a.alpha * v[i + e]
-                                                        : fmaf(a.alpha, v[i + e], a.beta * (h[e] + l[e]));
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                        if (EPI != kGram && on && t.col0 + c + i < a.ldi) {
+                            hi = *reinterpret_cast<const uint4 *>(a.in + at + i);
+                            if (EPI == kUpdate) lo = *reinterpret_cast<const uint4 *>(a.in_lo + at + i);
                         }
-                    }
-                    if (es == 4) {
+                        float h[8], l[8];
+                        unpack16<__half>(hi, h);
+                        unpack16<__half>(lo, l);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            st_shared16(stage + c * 4 + i * 16,
+                        for (int e = 0; e < 8; ++e)
+                            v[i + e] = EPI == kGram ? a.alpha * v[i + e]
+                                                    : fmaf(a.alpha, v[i + e], a.beta * (h[e] + l[e]));
+                    }
+                }
+                const int x = (int)t.col0 + c;
+                if (boxed) {
+                    __syncwarp();
+                    if (elect()) bulk_wait_read<0>();   // the staging's last store has read it
+                    __syncwarp();
+                    if (wide) {
+#pragma unroll
+                        for (unsigned i = 0; i < 8; ++i)
+                            st_shared16(stage + lane * 128 + ((i ^ swz4) << 4),
                                         make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
                                                    __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])));
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (unsigned i = 0; i < 4; ++i) {
                             const uint4 w = pack8(v + 8 * i, a.out_type == kOutBf16);
-                            st_shared16(stage + c * 2 + i * 16, w);
-                            if (EPI == kUpdate && a.out_lo) {   // what the high part's rounding left
+                            const unsigned at = stage + lane * 64 + ((i ^ swz2) << 4);
+                            st_shared16(at, w);
+                            if (EPI == kUpdate && a.low) {   // what the high part's rounding left
                                 float h[8];
                                 unpack16<__half>(w, h);
 #pragma unroll
                                 for (int e = 0; e < 8; ++e) h[e] = v[8 * i + e] - h[e];
-                                st_shared16(stage + 128 + c * 2 + i * 16, pack8(h, false));
+                                st_shared16(at + 2048, pack8(h, false));
+                            }
+                        }
+                        if ((EPI == kGram || EPI == kPoly) && t.mirror) {
+                            // transposed: column c + i of the tile is a row of 32 elements
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(
+                                                 stage + 2048 + i * 64 + (((lane >> 3) ^ (i >> 1 & 3)) << 4) +
+                                                 (lane & 7) * 2),
+                                             "h"(__half_as_ushort(__float2half_rn(v[i])))
+                                             : "memory");
+                        }
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (elect()) {
+                        tma_store(part ? &map_p : &map_o, stage, x, y, z);
+                        if (EPI == kUpdate && a.low) tma_store(&map_p, stage + 2048, x, y, z);
+                        if ((EPI == kGram || EPI == kPoly) && t.mirror) tma_store(&map_o, stage + 2048, y, x, z);
+                        bulk_commit();
+                    }
+                } else if (MODE == kRows) {   // each lane its row
+                    if (on) {
+                        char *o = static_cast<char *>(a.out) + ((t.out_row + row) * a.ldo + x) * out_size;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (c + 8 * i >= t.cols) break;
+                            if (out_size == 4) {
+                                float4 *q = reinterpret_cast<float4 *>(o) + 2 * i;
+                                q[0] = make_float4(v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3]);
+                                q[1] = make_float4(v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]);
+                            } else {
+                                reinterpret_cast<uint4 *>(o)[i] = pack8(v + 8 * i, a.out_type == kOutBf16);
                             }
                         }
                     }
-                    if ((EPI == kGram || EPI == kPoly) && t.mirror && on) {
-                        // lanes hold consecutive rows: 64 contiguous bytes per column
-                        __half *o = static_cast<__half *>(a.out) + t.batch_a * a.out_batch +
-                                    (t.col0 + c0 + c) * a.ldo + t.row0 + row;
+                } else {   // kUpdate's result with rows of any alignment: 16-bit, row by row across the lanes
+                    __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (c0 + c + i < t.cols) o[i * a.ldo] = __float2half_rn(v[i]);
-                    }
-                }
-                const int cols = min(chunk, t.cols - c0);
-                if (EPI != kUpdate || bulk) {
-                    // a row's last 16-byte piece may end in the padding of its leading dimension
-                    const unsigned bytes = (unsigned)(cols * es + 15) & ~15u;
-                    if (on) {
-                        const int64_t at = t.out + row * a.ldo + c0;
-                        fence_async();
-                        bulk_store(out + at * es, stage, bytes);
-                        if (EPI == kUpdate && a.out_lo) bulk_store(a.out_lo + at, stage + 128, bytes);
-                    }
-                    bulk_commit();
-                } else {
-                    __syncwarp();
-                    for (int r = 0; r < 32 && (warp & 3) * 32 + r < t.rows; ++r) {
-                        const unsigned char *src = smem + S::kStageOff + ((warp & 3) * 32 + r) * S::kPitch;
-                        unsigned short *o = static_cast<unsigned short *>(a.out) + t.out +
-                                            ((warp & 3) * 32 + r) * a.ldo + c0;
-                        for (int c = lane; c < cols; c += 32) o[c] = reinterpret_cast<const unsigned short *>(src)[c];
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 w = pack8(v + 8 * i, a.out_type == kOutBf16);
+                        const unsigned at = stage + lane * 68 + i * 16;   // an odd number of words apart
+                        asm volatile("st.shared.u32 [%0], %1;\n\tst.shared.u32 [%0+4], %2;\n\t"
+                                     "st.shared.u32 [%0+8], %3;\n\tst.shared.u32 [%0+12], %4;\n" ::"r"(at),
+                                     "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                                     : "memory");
                     }
                     __syncwarp();
+                    const unsigned char *src = smem + S::kStageOff + (warp - 2) * S::kStaging;
+                    unsigned short *o = static_cast<unsigned short *>(a.out) + t.out_z * a.out_batch +
+                                        (t.out_row + row0) * a.ldo + x;
+                    if (c + lane < t.cols)
+                        for (int r = 0; r < 32 && row0 + r < t.rows; ++r)
+                            o[r * a.ldo + lane] = *reinterpret_cast<const unsigned short *>(src + r * 68 + lane * 2);
                 }
             }
             if (!zero) {
@@ -435,9 +469,33 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 // read in boxes of 64 elements x box_rows, 128-byte swizzled, zero outside.
 bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
               int64_t batch_stride, int box_rows, bool bf16);
+// Tensor map of an output, written in boxes of 32 x 32 elements.
+bool make_out_map(CUtensorMap *map, void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
+                  int64_t batch_stride, int out_type);
+
+// Launch that lets the kernel's set-up overlap the kernel before it.
+template <typename K, typename... A>
+cudaError_t launch_overlapped(K kernel, unsigned grid, int threads, int smem, cudaStream_t stream, const A &...args)
+{
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+struct Maps {
+    CUtensorMap a, b, o, p;
+};
 
 template <int MODE, int BN, bool AMN, bool BMN, int EPI>
-cudaError_t launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, const GemmArgs &a, int64_t tiles, cudaStream_t s)
+cudaError_t launch_gemm(const Maps &m, const GemmArgs &a, int64_t tiles, cudaStream_t s)
 {
     auto kernel = gemm_kernel<MODE, BN, AMN, BMN, EPI>;
     static PerDevice<bool> ready;   // the attribute outlasts the call
@@ -449,8 +507,7 @@ cudaError_t launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, const Gemm
         if (done) *done = true;
     }
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count()));
-    kernel<<<grid, kGemmThreads, GemmShape<BN>::kBytes, s>>>(ma, mb, a);
-    return cudaGetLastError();
+    return launch_overlapped(kernel, grid, kGemmThreads, GemmShape<BN>::kBytes, s, m.a, m.b, m.o, m.p, a);
 }
 
 }  // namespace tc

@@ -109,14 +109,16 @@ template <int BN>
 cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::GemmArgs &g, int64_t row_tiles,
                     cudaStream_t stream)
 {
-    CUtensorMap ma, mb;
+    tc::Maps m;
     const int64_t planes = g.passes > 1 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
     const int64_t tiles = row_tiles * ((g.n + BN - 1) / BN);
-    if (!tc::make_map(&ma, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
-        !tc::make_map(&mb, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? BN : 64, g.bf16))
+    if (!tc::make_map(&m.a, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
+        !tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? BN : 64, g.bf16) ||
+        !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
         return cudaErrorInvalidValue;
-    if (a.transposed) return tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(ma, mb, g, tiles, stream);
-    return tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(ma, mb, g, tiles, stream);
+    m.p = m.o;
+    if (a.transposed) return tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(m, g, tiles, stream);
+    return tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(m, g, tiles, stream);
 }
 
 // Rows of one part of a weight gradient: a group's rows are one reduction
@@ -185,27 +187,32 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, T *o
     }
 }
 
-template <typename T> cudaError_t add_parts(const GroupedLaunch &a, const tc::GemmArgs &g, cudaStream_t stream)
+template <typename T> cudaError_t add_parts(const GroupedLaunch &a, const float *parts, const tc::GemmArgs &g, cudaStream_t stream)
 {
     const int64_t elems = a.K * a.N;
     const int64_t per = std::max<int64_t>(1, 16 * device_sm_count() / a.groups);
     const unsigned blocks = (unsigned)std::min((elems + 1023) / 1024, per);
     const dim3 grid(blocks, (unsigned)std::min<int64_t>(a.groups, 65535));
-    add_parts_kernel<T><<<grid, 256, 0, stream>>>(g.parts, static_cast<T *>(a.out), elems, g.part_rows, g.part_slots,
+    add_parts_kernel<T><<<grid, 256, 0, stream>>>(parts, static_cast<T *>(a.out), elems, g.part_rows, g.part_slots,
                                                   g.ranges, a.status);
     return cudaGetLastError();
 }
 
 template <int BN>
-cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy, tc::GemmArgs &g, cudaStream_t stream)
+cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy, float *parts, tc::GemmArgs &g,
+                           cudaStream_t stream)
 {
-    CUtensorMap ma, mb;
+    tc::Maps m;
     const int64_t planes = g.passes > 1 ? kPlanes : 1, rows = std::max<int64_t>(a.rows, 1);
-    if (!tc::make_map(&ma, x, a.K, rows, planes, a.K, rows * a.K, 64, g.bf16) ||
-        !tc::make_map(&mb, dy, a.N, rows, planes, a.N, rows * a.N, 64, g.bf16))
+    if (!tc::make_map(&m.a, x, a.K, rows, planes, a.K, rows * a.K, 64, g.bf16) ||
+        !tc::make_map(&m.b, dy, a.N, rows, planes, a.N, rows * a.N, 64, g.bf16) ||
+        !tc::make_out_map(&m.o, a.out, a.N, a.K, a.groups, a.N, a.K * a.N, g.out_type))
+        return cudaErrorInvalidValue;
+    m.p = m.o;
+    if (g.part_slots > 0 && !tc::make_out_map(&m.p, parts, a.N, a.K, g.part_slots, a.N, a.K * a.N, tc::kOutF32))
         return cudaErrorInvalidValue;
     const int64_t tiles = (a.groups + a.rows / g.part_rows) * ((a.K + tc::kBM - 1) / tc::kBM) * ((a.N + BN - 1) / BN);
-    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(ma, mb, g, tiles, stream);
+    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(m, g, tiles, stream);
 }
 
 }  // namespace
@@ -279,19 +286,19 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
         dy = pdy;
         g.za = g.zb = 1;
     }
-    g.parts = reinterpret_cast<float *>(ws);
+    float *parts = reinterpret_cast<float *>(ws);
     g.part_slots = slots;
     cudaError_t e;
     switch (bn) {
-        case 256: e = weight_grad_tc<256>(a, x, dy, g, stream); break;
-        case 128: e = weight_grad_tc<128>(a, x, dy, g, stream); break;
-        default: e = weight_grad_tc<64>(a, x, dy, g, stream);
+        case 256: e = weight_grad_tc<256>(a, x, dy, parts, g, stream); break;
+        case 128: e = weight_grad_tc<128>(a, x, dy, parts, g, stream); break;
+        default: e = weight_grad_tc<64>(a, x, dy, parts, g, stream);
     }
     if (e != cudaSuccess || slots == 0) return e;
     switch (a.dtype) {
-        case SPMM_F16: return add_parts<__half>(a, g, stream);
-        case SPMM_BF16: return add_parts<__nv_bfloat16>(a, g, stream);
-        default: return add_parts<float>(a, g, stream);
+        case SPMM_F16: return add_parts<__half>(a, parts, g, stream);
+        case SPMM_BF16: return add_parts<__nv_bfloat16>(a, parts, g, stream);
+        default: return add_parts<float>(a, parts, g, stream);
     }
 }
 

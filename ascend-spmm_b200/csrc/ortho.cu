@@ -155,22 +155,22 @@ template <typename T> void start(const OrthoLaunch &o, const Space &w, cudaStrea
 }
 
 template <int BN>
-cudaError_t update(const OrthoLaunch &o, const Space &w, tc::GemmArgs g, const __half *x, cudaStream_t stream)
+cudaError_t update(const OrthoLaunch &o, const Space &w, const tc::GemmArgs &g, const __half *x, tc::Maps &m,
+                   cudaStream_t stream)
 {
     const bool tall = o.m > o.n;
     const int64_t side = std::min(o.m, o.n);
-    CUtensorMap ma, mb;
     const int64_t tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM) * ((o.n + BN - 1) / BN);
     if (tall) {   // X P: P is symmetric, read with the reduction contiguous
-        if (!tc::make_map(&ma, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tc::kBM, false) ||
-            !tc::make_map(&mb, w.poly, side, side, o.batch, w.lds, side * w.lds, BN, false))
+        if (!tc::make_map(&m.a, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tc::kBM, false) ||
+            !tc::make_map(&m.b, w.poly, side, side, o.batch, w.lds, side * w.lds, BN, false))
             return cudaErrorInvalidValue;
-        return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate>(ma, mb, g, tiles, stream);
+        return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate>(m, g, tiles, stream);
     }
-    if (!tc::make_map(&ma, w.poly, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false) ||
-        !tc::make_map(&mb, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, 64, false))
+    if (!tc::make_map(&m.a, w.poly, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false) ||
+        !tc::make_map(&m.b, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, 64, false))
         return cudaErrorInvalidValue;
-    return tc::launch_gemm<tc::kDense, BN, false, true, tc::kUpdate>(ma, mb, g, tiles, stream);
+    return tc::launch_gemm<tc::kDense, BN, false, true, tc::kUpdate>(m, g, tiles, stream);
 }
 
 }  // namespace
@@ -195,10 +195,12 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
     const int64_t mt = (side + tc::kBM - 1) / tc::kBM, half = o.batch * mt * (mt + 1) / 2;
     for (int i = 0; i < o.steps && e == cudaSuccess; ++i) {
         const __half *x = w.hi[i & 1];
-        CUtensorMap mx, mg;
-        if (!tc::make_map(&mx, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tall ? 64 : tc::kBM, false) ||
-            !tc::make_map(&mg, w.gram, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false))
+        tc::Maps m;
+        if (!tc::make_map(&m.a, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tall ? 64 : tc::kBM, false) ||
+            !tc::make_out_map(&m.o, w.gram, side, side, o.batch, w.lds, side * w.lds, tc::kOutF16))
             return cudaErrorInvalidValue;
+        m.b = m.a;
+        m.p = m.o;
         tc::GemmArgs g{};
         g.batch = o.batch;
         g.passes = 1;
@@ -211,8 +213,8 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.ldo = w.lds;
         g.out_batch = side * w.lds;
         g.alpha = kScaleG / (kScaleX * kScaleX);
-        e = tall ? tc::launch_gemm<tc::kDense, 128, true, true, tc::kGram>(mx, mx, g, half, stream)
-                 : tc::launch_gemm<tc::kDense, 128, false, false, tc::kGram>(mx, mx, g, half, stream);
+        e = tall ? tc::launch_gemm<tc::kDense, 128, true, true, tc::kGram>(m, g, half, stream)
+                 : tc::launch_gemm<tc::kDense, 128, false, false, tc::kGram>(m, g, half, stream);
         if (e != cudaSuccess) break;
         // P = b G + c G G
         g.k = side;
@@ -222,7 +224,11 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.out = w.poly;
         g.alpha = o.c * (kScaleP / (kScaleG * kScaleG));
         g.beta = o.b * (kScaleP / kScaleG);
-        e = tc::launch_gemm<tc::kDense, 128, false, false, tc::kPoly>(mg, mg, g, half, stream);
+        if (!tc::make_map(&m.a, w.gram, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false) ||
+            !tc::make_out_map(&m.o, w.poly, side, side, o.batch, w.lds, side * w.lds, tc::kOutF16))
+            return cudaErrorInvalidValue;
+        m.b = m.a;
+        e = tc::launch_gemm<tc::kDense, 128, false, false, tc::kPoly>(m, g, half, stream);
         if (e != cudaSuccess) break;
         // X <- a X + P X (X P); the last step writes the result
         const bool last = i + 1 == o.steps;
@@ -233,17 +239,21 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.ldi = w.ldx;
         g.in_batch = o.m * w.ldx;
         g.out = last ? o.out : static_cast<void *>(w.hi[i + 1 & 1]);
-        g.out_lo = last ? nullptr : w.lo;
+        g.low = !last;
         g.ldo = last ? o.n : w.ldx;
         g.out_batch = o.m * g.ldo;
         g.out_type = last ? tc::kOutBf16 : tc::kOutF16;
         g.alpha = last ? 1.f / (kScaleP * kScaleX) : 1.f / kScaleP;
         g.beta = last ? o.a / kScaleX : o.a;
+        const bool mapped = (g.ldo * 2 & 15) == 0;   // else the result's rows have no map
+        if ((mapped && !tc::make_out_map(&m.o, g.out, o.n, o.m, o.batch, g.ldo, g.out_batch, g.out_type)) ||
+            (!last && !tc::make_out_map(&m.p, w.lo, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tc::kOutF16)))
+            return cudaErrorInvalidValue;
         const int64_t row_tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM);
         const int sms = device_sm_count();
-        if (o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms) e = update<256>(o, w, g, x, stream);
-        else if (o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms) e = update<128>(o, w, g, x, stream);
-        else e = update<64>(o, w, g, x, stream);
+        if (o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms) e = update<256>(o, w, g, x, m, stream);
+        else if (o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms) e = update<128>(o, w, g, x, m, stream);
+        else e = update<64>(o, w, g, x, m, stream);
     }
     return e;
 }

@@ -74,15 +74,25 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map)
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
 }
 
-// `bytes` (a multiple of 16) of shared memory to global memory, by one thread.
-__device__ __forceinline__ void bulk_store(void *dst, unsigned src, unsigned bytes)
+// A box of shared memory to a tensor map's tile (clipped at the tensor's end), by one thread.
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, unsigned src, int x, int y, int z)
 {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(src), "r"(bytes)
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n" ::"l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(src)
                  : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
+// All but the N latest stores of this thread have read their shared memory.
+template <int N> __device__ __forceinline__ void bulk_wait_read()
+{
+    asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
+// Programmatic dependent launch: the kernels before this one in the stream
+// are complete and their writes visible; the next may start its set-up.
+__device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;\n"); }
 
 // D[tmem] (+)= A B over 16 elements of the reduction; acc == 0 overwrites D.
 __device__ __forceinline__ void mma(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc)
