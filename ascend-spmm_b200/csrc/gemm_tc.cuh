@@ -1,7 +1,8 @@
 // Dense products on the fifth-generation tensor cores for the layer
 // operators: 16-bit operands brought in by TMA, fp32 accumulators in TMEM.
 //
-// A persistent block per SM walks output tiles of 128 x BN.  One warp issues
+// A persistent block per SM walks output tiles of 128 x bn (bn <= BN, so that
+// a width just above a multiple of BN is cut into equal tiles).  One warp issues
 // the TMA loads of 64-deep slices into a ring of stages, one warp the
 // tcgen05.mma of each slice, and eight warps read a finished accumulator out
 // of TMEM, round it and store it by TMA (32 rows x 32 columns at a time)
@@ -43,6 +44,7 @@ enum OutType { kOutF16, kOutBf16, kOutF32 };
 struct GemmArgs {
     Ranges ranges;            // kRows, kRagged
     int64_t m, n, k;          // kRows: n, k; kRagged: m, n; kDense: all
+    int bn;                   // columns of a tile, at most the kernel's BN: a multiple of 32 (16 for a single one)
     int64_t batch;            // kDense
     int64_t part_rows;        // kRagged: a multiple of 64
     int64_t part_slots;       // kRagged: parts in the second output map ([part_slots][m][n])
@@ -69,6 +71,9 @@ struct GemmArgs {
 constexpr int kBM = 128, kBK = 64;
 constexpr int kEpiWarps = 8, kGemmThreads = 64 + 32 * kEpiWarps;   // TMA warp, MMA warp, epilogue warps
 
+constexpr int kSorted = 256;   // most groups that a weight gradient sorts
+constexpr int kAsked = 4;      // tiles asked for and not yet done by every warp
+
 template <int BN> struct GemmShape {
     static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
@@ -77,9 +82,59 @@ template <int BN> struct GemmShape {
     static constexpr int kBarOff = kStageOff + kEpiWarps * kStaging;
     static constexpr int kFull = kBarOff, kEmpty = kFull + 8 * kStages, kAccFull = kEmpty + 8 * kStages;
     static constexpr int kAccEmpty = kAccFull + 16, kDone = kAccEmpty + 16, kTmem = kDone + 8, kAbort = kTmem + 4;
-    static constexpr int kBytes = kAbort + 4;
+    // kRagged: the groups in descending order of length (see Order)
+    static constexpr int kOrder = kAbort + 4, kFirst = kOrder + 2 * kSorted, kSlot = kFirst + 4 * (kSorted + 1);
+    static constexpr int kAnswer = (kSlot + 4 * kSorted + 15) / 16 * 16, kAskFull = kAnswer + 16 * kAsked;
+    static constexpr int kAskEmpty = kAskFull + 8 * kAsked, kBytes = kAskEmpty + 8 * kAsked;
     static constexpr int kCols = 2 * BN;                         // TMEM columns of the two accumulators
     static_assert(kBytes <= 232448, "shared memory of a block");
+};
+
+// The tiles of a block, for one of its warps.  kRows and kDense deal them out
+// in turn.  kRagged, whose tiles differ in length, launches a block per tile,
+// and a running block takes over those that have not started, one after the
+// other: the TMA warp asks, a few tiles ahead of the others (ring of kAsked).
+template <int MODE, int BN> struct Turns {
+    using S = GemmShape<BN>;
+    const unsigned base;
+    volatile int *const abort;
+    const bool asks;       // the TMA warp
+    int64_t tile;
+    unsigned turn = 0;
+
+    __device__ Turns(unsigned base, volatile int *abort, bool asks)
+        : base(base), abort(abort), asks(asks), tile(blockIdx.x)
+    {
+    }
+    // Warp-wide, at the start of the current tile.
+    __device__ __forceinline__ bool ask()
+    {
+        if (MODE != kRagged || !asks) return true;
+        const unsigned slot = turn % kAsked;
+        if (!bar_wait(base + S::kAskEmpty + 8 * slot, (turn / kAsked & 1u) ^ 1u, abort)) return false;
+        if (elect()) {
+            fence_async();   // the slot's last answer was read before
+            bar_expect(base + S::kAskFull + 8 * slot, 16);
+            ask_for_block(base + S::kAnswer + 16 * slot, base + S::kAskFull + 8 * slot);
+        }
+        __syncwarp();
+        return true;
+    }
+    // Warp-wide: goes to the next tile; tile < 0 past the last.  False if a wait ran out.
+    __device__ __forceinline__ bool next()
+    {
+        if (MODE != kRagged) {
+            tile += gridDim.x;
+            return true;
+        }
+        const unsigned slot = turn % kAsked;
+        if (!bar_wait(base + S::kAskFull + 8 * slot, turn / kAsked & 1u, abort)) return false;
+        tile = block_given(base + S::kAnswer + 16 * slot);
+        __syncwarp();
+        if (elect()) bar_arrive(base + S::kAskEmpty + 8 * slot);
+        ++turn;
+        return true;
+    }
 };
 
 // One output tile as each role sees it.
@@ -92,20 +147,75 @@ struct Tile {
     bool mirror;                            // kGram, kPoly: also the transposed tile
 };
 
+// A weight gradient's groups by length, longest first: its tiles take as long
+// as their group's rows (of a part), and handed out in this order to the
+// blocks as they become free they end within one short tile of each other.
+// Up to kSorted groups; more of them even out by themselves.
+struct Order {
+    const unsigned short *group;   // [groups], nullptr: not sorted
+    const int *first;              // [groups + 1] tiles before the group of this rank
+    const int *slot;               // [groups] by group: its first part's slot, -1 with a single part
+};
+
+// Every thread of the block; `length`: kSorted ints of scratch.
+__device__ __forceinline__ void sort_groups(const GemmArgs &a, int tiles, unsigned short *group, int *first, int *slot,
+                                            int *length)
+{
+    const int n = (int)a.ranges.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int g = threadIdx.x; g < n; g += blockDim.x) {
+        int64_t b, e;
+        segment_rows(a.ranges, g + 1, &b, &e, a.status);
+        length[g] = (int)(e - b);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < n; g += blockDim.x) {
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += length[i] > length[g] || (length[i] == length[g] && i < g);
+        group[rank] = (unsigned short)g;
+    }
+    __syncthreads();
+    if (warp < 2) {   // warp 0: tiles by rank; warp 1: slots by group
+        int before = 0;
+        for (int base = 0; base < n; base += 32) {
+            const int i = base + lane;
+            int v = 0;
+            if (i < n) {
+                const int parts = (int)((length[warp ? i : group[i]] + a.part_rows - 1) / a.part_rows);
+                v = warp ? (parts > 1 ? parts : 0) : max(parts, 1) * tiles;
+            }
+            int sum = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
+            }
+            if (i < n) (warp ? slot : first)[i] = warp && v == 0 ? -1 : before + sum - v;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (warp == 0 && lane == 0) first[n] = before;
+    }
+    __syncthreads();
+}
+
 template <int MODE, int BN, int EPI> struct Walk {
     const GemmArgs &a;
+    const Order order;
     TileWalk<MODE == kRagged> ranges;
     int64_t mt, nt;
-    __device__ Walk(const GemmArgs &a) : a(a), mt((a.m + kBM - 1) / kBM), nt((a.n + BN - 1) / BN) {}
+    int rank = 0;
+    __device__ Walk(const GemmArgs &a, const Order &order)
+        : a(a), order(order), mt((a.m + kBM - 1) / kBM), nt((a.n + a.bn - 1) / a.bn)
+    {
+    }
 
-    // Warp-wide; `t` must not decrease.  False past the last tile.
+    // Warp-wide: the tile of index t; false past the last tile.
     __device__ __forceinline__ bool at(int64_t t, Tile *o)
     {
         if constexpr (MODE == kRows) {
             int64_t seg, b, e, inner, slots;
             if (!ranges.find(a.ranges, kBM, nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
             o->row0 = b + inner / nt * kBM;
-            o->col0 = inner % nt * BN;
+            o->col0 = inner % nt * a.bn;
             o->batch_a = 0;
             o->batch_b = seg - 1;
             o->k0 = 0;
@@ -115,12 +225,23 @@ template <int MODE, int BN, int EPI> struct Walk {
             o->out_z = 0;
         } else if constexpr (MODE == kRagged) {
             int64_t seg, b, e, inner, slots;
-            if (!ranges.find(a.ranges, a.part_rows, mt * nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
+            if (order.group) {
+                const int groups = (int)a.ranges.groups;
+                if (rank >= groups || order.first[rank] > t) rank = 0;
+                while (rank < groups && order.first[rank + 1] <= t) ++rank;
+                if (rank >= groups) return false;
+                seg = order.group[rank] + 1;
+                inner = t - order.first[rank];
+                slots = order.slot[seg - 1];
+                segment_rows(a.ranges, seg, &b, &e, a.status);
+            } else if (!ranges.find(a.ranges, a.part_rows, mt * nt, t, a.status, &seg, &b, &e, &inner, &slots)) {
+                return false;
+            }
             const int64_t p = inner / (mt * nt), i = inner % (mt * nt);
             o->k0 = b + p * a.part_rows;
             o->k1 = min(e, o->k0 + a.part_rows);
             o->row0 = i / nt * kBM;
-            o->col0 = i % nt * BN;
+            o->col0 = i % nt * a.bn;
             o->batch_a = o->batch_b = 0;
             o->rows = (int)min((int64_t)kBM, a.m - o->row0);
             o->part = slots >= 0;
@@ -147,7 +268,7 @@ template <int MODE, int BN, int EPI> struct Walk {
             }
             o->batch_a = o->batch_b = q;
             o->row0 = i * kBM;
-            o->col0 = j * BN;
+            o->col0 = j * a.bn;
             o->k0 = 0;
             o->k1 = a.k;
             o->rows = (int)min((int64_t)kBM, a.m - o->row0);
@@ -155,7 +276,7 @@ template <int MODE, int BN, int EPI> struct Walk {
             o->out_z = q;
             o->mirror = half && i != j;
         }
-        o->cols = (int)min((int64_t)BN, a.n - o->col0);
+        o->cols = (int)min((int64_t)a.bn, a.n - o->col0);
         return true;
     }
 };
@@ -184,6 +305,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             bar_init(acc_empty + 8 * i, kEpiWarps);
         }
         bar_init(done, 1);
+        for (int i = 0; i < kAsked; ++i) {
+            bar_init(base + S::kAskFull + 8 * i, 1);
+            bar_init(base + S::kAskEmpty + 8 * i, 2 + kEpiWarps);
+        }
         // a misaligned stage ring would break the swizzle: give up before any copy
         *abort = (base & 1023u) ? 1 : 0;
         if (base & 1023u) raise_status(a.status, SPMM_DEV_TIMEOUT, -1);
@@ -205,7 +330,19 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     let_next_kernel_start();
     wait_for_earlier_kernels();   // nothing above reads or writes global memory
 
-    Walk<MODE, BN, EPI> walk(a);
+    Order order{};
+    if constexpr (MODE == kRagged)
+        if (a.ranges.groups <= kSorted) {
+            unsigned short *group = reinterpret_cast<unsigned short *>(smem + S::kOrder);
+            int *first = reinterpret_cast<int *>(smem + S::kFirst), *slot = reinterpret_cast<int *>(smem + S::kSlot);
+            sort_groups(a, (int)((a.m + kBM - 1) / kBM * ((a.n + a.bn - 1) / a.bn)), group, first, slot,
+                        reinterpret_cast<int *>(smem + S::kStageOff));
+            order = Order{group, first, slot};
+        }
+    Walk<MODE, BN, EPI> walk(a, order);
+    // the columns of B that a slice brings in (MN-major: in blocks of 64), and its bytes
+    const int b_blocks = BMN ? (a.bn + 63) / 64 : 0;
+    const unsigned slice_bytes = S::kA + (BMN ? b_blocks * 8192 : a.bn * 128);
     Tile t;
     bool ok = *abort == 0;
     auto give_up = [&](int code) {
@@ -217,7 +354,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (warp == 0) {
         // ---- TMA warp: all lanes find the tile, one issues its copies
         unsigned slice = 0;   // slices issued
-        for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
+        Turns<MODE, BN> turns(base, abort, true);
+        for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
+            if (!turns.ask()) { give_up(6); break; }
+            if (!walk.at(turns.tile, &t)) {
+                if (MODE == kRagged) continue;
+                break;
+            }
             const int n = (int)((t.k1 - t.k0 + kBK - 1) / kBK);
             if (elect()) {
                 const int row0 = (int)t.row0, col0 = (int)t.col0;
@@ -228,7 +371,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         const unsigned at = slice + pass * n + i, st = at % S::kStages;
                         if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
                         const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA, bar = full + 8 * st;
-                        bar_expect(bar, S::kA + S::kB);
+                        bar_expect(bar, slice_bytes);
                         if constexpr (AMN) {
 #pragma unroll
                             for (int c = 0; c < kBM / 64; ++c) tma_load(sa + c * 8192, &map_a, row0 + 64 * c, k, za, bar);
@@ -237,7 +380,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         }
                         if constexpr (BMN) {
 #pragma unroll
-                            for (int c = 0; c < BN / 64; ++c) tma_load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb, bar);
+                            for (int c = 0; c < BN / 64; ++c)
+                                if (c < b_blocks) tma_load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb, bar);
                         } else {
                             tma_load(sb, &map_b, k, col0, zb, bar);
                         }
@@ -248,14 +392,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             slice += a.passes * n;
             ok = *abort == 0;
         }
-        if (!ok)   // the copies in flight land before the block leaves (bounded; a slice never issued runs out)
+        if (!ok) {   // copies and an answer in flight land before the block leaves (bounded; one never issued runs out)
+            volatile int no = 0;
+            if (MODE == kRagged) bar_wait(base + S::kAskFull + 8 * (turns.turn % kAsked), turns.turn / kAsked & 1u, &no);
             for (unsigned s = slice > 2 * S::kStages ? slice - 2 * S::kStages : 0; s < slice; ++s) {
                 volatile int never = 0;
                 if (!bar_wait(full + 8 * (s % S::kStages), s / S::kStages & 1u, &never)) break;
             }
+        }
     } else if (warp == 1) {
         // ---- MMA warp: one lane issues
-        const unsigned idesc = idesc16(a.bf16, AMN, BMN, kBM, BN);
+        const unsigned idesc = idesc16(a.bf16, AMN, BMN, kBM, a.bn);
         // byte strides of the operands' layouts: K-major, 8 rows of 128 bytes per
         // swizzle atom; MN-major, atoms of 64 rows or columns x 8 deep, 8 KB apart
         const uint64_t da = AMN ? desc128(base, 8192, 1024) : desc128(base, 16, 1024);
@@ -276,7 +423,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             commit(empty + 8 * st);
         };
         auto landed = [&](unsigned at) { return bar_wait(full + 8 * (at % S::kStages), at / S::kStages & 1u, abort); };
-        for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
+        Turns<MODE, BN> turns(base, abort, false);
+        for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
+            if (!walk.at(turns.tile, &t)) {
+                if (MODE == kRagged) continue;
+                break;
+            }
             const int depth = (int)(t.k1 - t.k0), n = (depth + kBK - 1) / kBK;
             if (n <= 0) continue;
             // kRagged: a last slice that ends within 16 rows needs the whole warp
@@ -299,7 +451,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                     const unsigned buf = base + st * (S::kA + S::kB);
                     const int deep = depth - (n - 1) * kBK;
                     const int quads = (16 - (deep & 15)) * 8;   // 16-byte pieces of a 64-wide column block
-                    for (int i = lane; i < quads * ((S::kA + S::kB) / 8192); i += 32)
+                    for (int i = lane; i < quads * (S::kA / 8192 + b_blocks); i += 32)
                         st_shared16(buf + i / quads * 8192 + deep * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
                     fence_async();
                     __syncwarp();
@@ -332,7 +484,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // a 16-byte piece in a row of the staged 64-byte (fp32: 128-byte) wide block, swizzled as its map
         const unsigned swz2 = (unsigned)(lane >> 1 & 3), swz4 = (unsigned)(lane & 7);
         unsigned used = 0;
-        for (int64_t tile = blockIdx.x; ok && walk.at(tile, &t); tile += gridDim.x) {
+        Turns<MODE, BN> turns(base, abort, false);
+        for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
+            if (!walk.at(turns.tile, &t)) {
+                if (MODE == kRagged) continue;
+                break;
+            }
             const bool zero = t.k0 >= t.k1;
             const unsigned acc = used & 1u;
             if (!zero) {
@@ -506,7 +663,8 @@ cudaError_t launch_gemm(const Maps &m, const GemmArgs &a, int64_t tiles, cudaStr
         if (e != cudaSuccess) return e;
         if (done) *done = true;
     }
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count()));
+    const int64_t most = MODE == kRagged ? INT32_MAX : device_sm_count();
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min(tiles, most));
     return launch_overlapped(kernel, grid, kGemmThreads, GemmShape<BN>::kBytes, s, m.a, m.b, m.o, m.p, a);
 }
 

@@ -6,6 +6,7 @@
 // The group of a row tile is found on the device from the row ranges, so no
 // length crosses to the host and a launch can be captured in a graph.
 #include <algorithm>
+#include <climits>
 
 #include "../../include/spmm_b200.h"
 #include "common.cuh"
@@ -83,14 +84,26 @@ size_t plane_bytes(int64_t elems) { return ((size_t)elems * kPlanes * 2 + 255) &
 
 // ---- launches --------------------------------------------------------------
 
-// Columns per tile: the widest that the output's width fills and that still
-// gives every SM a tile (a narrower tile reads the row operand more often).
+// Columns per tile (a multiple of 16 of at most 256): the cut into equal
+// tiles with the least turns x time.  A 64-deep slice of a tile takes about
+// as long as 70 + bn columns (0.19 us at 64, 0.46 us at 256): its rows are
+// read however narrow it is.
 int tile_columns(int64_t row_tiles, int64_t width)
 {
-    const int sms = device_sm_count();
-    if (width > 128 && row_tiles * ((width + 255) / 256) >= sms) return 256;
-    if (width > 64 && row_tiles * ((width + 127) / 128) >= sms) return 128;
-    return 64;
+    const int64_t sms = device_sm_count();
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int64_t n = (width + 255) / 256; n <= (width + 63) / 64; ++n) {
+        const int64_t step = n > 1 ? 32 : 16;   // a tile is stored 32 columns at a time
+        const int64_t bn = ((width + n - 1) / n + step - 1) / step * step;
+        const int64_t cost = (row_tiles * n + sms - 1) / sms * (bn + 70);
+        if (cost < least) {
+            least = cost;
+            best = (int)bn;
+        }
+        if (n > 64 && bn <= 128) break;   // very wide outputs: narrower tiles gain nothing more
+    }
+    return best;
 }
 
 void set_types(tc::GemmArgs &g, int dtype)
@@ -111,9 +124,9 @@ cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::Ge
 {
     tc::Maps m;
     const int64_t planes = g.passes > 1 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
-    const int64_t tiles = row_tiles * ((g.n + BN - 1) / BN);
+    const int64_t tiles = row_tiles * ((g.n + g.bn - 1) / g.bn);
     if (!tc::make_map(&m.a, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
-        !tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? BN : 64, g.bf16) ||
+        !tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? g.bn : 64, g.bf16) ||
         !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
         return cudaErrorInvalidValue;
     m.p = m.o;
@@ -132,7 +145,14 @@ int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn)
     return (std::max<int64_t>(512, even) + 63) & ~int64_t(63);
 }
 
-int weight_grad_columns(int64_t N) { return N > 128 ? 256 : N > 64 ? 128 : 64; }
+// Equal tiles of at most 256 columns: the reduction is cut where there are
+// too few of them, so they need not be narrower.
+int weight_grad_columns(int64_t N)
+{
+    const int64_t n = (N + 255) / 256;
+    const int64_t step = n > 1 ? 32 : 16;   // a tile is stored 32 columns at a time
+    return (int)(((N + n - 1) / n + step - 1) / step * step);
+}
 
 // A group of n > 1 parts has more than (n - 1) part rows, so n <= 2 rows / part.
 int64_t weight_grad_slots(int64_t rows, int64_t K, int64_t N)
@@ -211,7 +231,8 @@ cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy
     m.p = m.o;
     if (g.part_slots > 0 && !tc::make_out_map(&m.p, parts, a.N, a.K, g.part_slots, a.N, a.K * a.N, tc::kOutF32))
         return cudaErrorInvalidValue;
-    const int64_t tiles = (a.groups + a.rows / g.part_rows) * ((a.K + tc::kBM - 1) / tc::kBM) * ((a.N + BN - 1) / BN);
+    const int64_t tiles = (a.groups + a.rows / g.part_rows) * ((a.K + tc::kBM - 1) / tc::kBM) *
+                          ((a.N + g.bn - 1) / g.bn);
     return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(m, g, tiles, stream);
 }
 
@@ -246,11 +267,10 @@ cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStr
     }
     // every group can end in a partial tile; the rows outside the groups too
     const int64_t row_tiles = std::min(a.rows, (a.rows + tc::kBM - 1) / tc::kBM + a.groups + 1);
-    switch (tile_columns(row_tiles, g.n)) {
-        case 256: return rows_tc<256>(a, x, w, g, row_tiles, stream);
-        case 128: return rows_tc<128>(a, x, w, g, row_tiles, stream);
-        default: return rows_tc<64>(a, x, w, g, row_tiles, stream);
-    }
+    g.bn = tile_columns(row_tiles, g.n);
+    if (g.bn <= 64) return rows_tc<64>(a, x, w, g, row_tiles, stream);
+    if (g.bn <= 128) return rows_tc<128>(a, x, w, g, row_tiles, stream);
+    return rows_tc<256>(a, x, w, g, row_tiles, stream);
 }
 
 size_t grouped_weight_grad_workspace(int64_t rows, int64_t groups, int64_t K, int64_t N, int dtype)
@@ -271,8 +291,8 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
     g.out_batch = a.K * a.N;
     g.status = a.status;
     set_types(g, a.dtype);
-    const int bn = weight_grad_columns(a.N);
-    g.part_rows = weight_grad_part(a.rows, a.K, a.N, bn);
+    g.bn = weight_grad_columns(a.N);
+    g.part_rows = weight_grad_part(a.rows, a.K, a.N, g.bn);
     const int64_t slots = weight_grad_slots(a.rows, a.K, a.N);
     const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: never read
     char *ws = static_cast<char *>(workspace);
@@ -289,11 +309,9 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
     float *parts = reinterpret_cast<float *>(ws);
     g.part_slots = slots;
     cudaError_t e;
-    switch (bn) {
-        case 256: e = weight_grad_tc<256>(a, x, dy, parts, g, stream); break;
-        case 128: e = weight_grad_tc<128>(a, x, dy, parts, g, stream); break;
-        default: e = weight_grad_tc<64>(a, x, dy, parts, g, stream);
-    }
+    if (g.bn <= 64) e = weight_grad_tc<64>(a, x, dy, parts, g, stream);
+    else if (g.bn <= 128) e = weight_grad_tc<128>(a, x, dy, parts, g, stream);
+    else e = weight_grad_tc<256>(a, x, dy, parts, g, stream);
     if (e != cudaSuccess || slots == 0) return e;
     switch (a.dtype) {
         case SPMM_F16: return add_parts<__half>(a, parts, g, stream);

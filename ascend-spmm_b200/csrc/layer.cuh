@@ -55,8 +55,8 @@ __device__ __forceinline__ void segment_rows(const Ranges &p, int64_t s, int64_t
 // Walks the tiles of all segments in order, `mult` column tiles per `height`
 // rows.  SPLIT (weight gradients): a group's tiles cover its rows in parts of
 // `height`, a group without rows has one, the rows outside the groups none.
-// Every lane of the warp calls it with the same arguments; `tile` must not
-// decrease from call to call.
+// Every lane of the warp calls it with the same arguments; it goes on from the
+// last tile's place.
 template <bool SPLIT> struct TileWalk {
     int64_t base = 0;      // segments before the current 32
     int64_t before = 0;    // tiles of the segments before `base`
@@ -71,6 +71,10 @@ template <bool SPLIT> struct TileWalk {
                                          int64_t *seg, int64_t *b, int64_t *e, int64_t *inner, int64_t *slots)
     {
         const int lane = threadIdx.x & 31;
+        if (tile < before) {
+            base = before = kept = 0;
+            count = -1;
+        }
         for (;;) {
             if (count < 0) {
                 segment_rows(p, base + lane, &begin, &end, status);

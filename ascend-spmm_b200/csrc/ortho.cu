@@ -154,22 +154,18 @@ template <typename T> void start(const OrthoLaunch &o, const Space &w, cudaStrea
         o.steps == 0 ? static_cast<__nv_bfloat16 *>(o.out) : nullptr);
 }
 
+// The tensor maps of a call, each encoded once.
+struct OrthoMaps {
+    CUtensorMap square[2], x[2];            // X as the operands of G and of the update, by buffer
+    CUtensorMap gram, poly;                 // G and P as operands
+    CUtensorMap gram_out, poly_out, x_out[2], low_out, out;
+};
+
 template <int BN>
-cudaError_t update(const OrthoLaunch &o, const Space &w, const tc::GemmArgs &g, const __half *x, tc::Maps &m,
-                   cudaStream_t stream)
+cudaError_t update(const OrthoLaunch &o, const tc::Maps &m, const tc::GemmArgs &g, cudaStream_t stream)
 {
-    const bool tall = o.m > o.n;
-    const int64_t side = std::min(o.m, o.n);
-    const int64_t tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM) * ((o.n + BN - 1) / BN);
-    if (tall) {   // X P: P is symmetric, read with the reduction contiguous
-        if (!tc::make_map(&m.a, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tc::kBM, false) ||
-            !tc::make_map(&m.b, w.poly, side, side, o.batch, w.lds, side * w.lds, BN, false))
-            return cudaErrorInvalidValue;
-        return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate>(m, g, tiles, stream);
-    }
-    if (!tc::make_map(&m.a, w.poly, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false) ||
-        !tc::make_map(&m.b, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, 64, false))
-        return cudaErrorInvalidValue;
+    const int64_t tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM) * ((o.n + g.bn - 1) / g.bn);
+    if (o.m > o.n) return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate>(m, g, tiles, stream);
     return tc::launch_gemm<tc::kDense, BN, false, true, tc::kUpdate>(m, g, tiles, stream);
 }
 
@@ -190,17 +186,33 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         default: start<float>(o, w, stream);
     }
     cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || o.steps == 0) return e;
     const bool tall = o.m > o.n;
-    const int64_t side = std::min(o.m, o.n), long_side = std::max(o.m, o.n);
+    const int64_t side = std::min(o.m, o.n), long_side = std::max(o.m, o.n), sq = side * w.lds, all = o.m * w.ldx;
     const int64_t mt = (side + tc::kBM - 1) / tc::kBM, half = o.batch * mt * (mt + 1) / 2;
+    // columns of an update's tile
+    const int64_t row_tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM);
+    const int sms = device_sm_count();
+    const int bn = o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms  ? 256
+                   : o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms ? 128
+                                                                        : 64;
+    // a result whose rows do not start on 16 bytes has no map
+    const bool mapped = (o.n & 7) == 0;
+    OrthoMaps M;
+    bool fine = tc::make_map(&M.gram, w.gram, side, side, o.batch, w.lds, sq, tc::kBM, false) &&
+                tc::make_map(&M.poly, w.poly, side, side, o.batch, w.lds, sq, tall ? bn : tc::kBM, false) &&
+                tc::make_out_map(&M.gram_out, w.gram, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
+                tc::make_out_map(&M.poly_out, w.poly, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
+                tc::make_out_map(&M.low_out, w.lo, o.n, o.m, o.batch, w.ldx, all, tc::kOutF16);
+    for (int i = 0; i < 2 && fine; ++i)   // tall: G reads X down its rows, the update along them; wide: the reverse
+        fine = tc::make_map(&M.square[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tall ? 64 : tc::kBM, false) &&
+               tc::make_map(&M.x[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tall ? tc::kBM : 64, false) &&
+               tc::make_out_map(&M.x_out[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kOutF16);
+    M.out = M.x_out[0];
+    if (fine && mapped) fine = tc::make_out_map(&M.out, o.out, o.n, o.m, o.batch, o.n, o.m * o.n, tc::kOutBf16);
+    if (!fine) return cudaErrorInvalidValue;
     for (int i = 0; i < o.steps && e == cudaSuccess; ++i) {
-        const __half *x = w.hi[i & 1];
-        tc::Maps m;
-        if (!tc::make_map(&m.a, x, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tall ? 64 : tc::kBM, false) ||
-            !tc::make_out_map(&m.o, w.gram, side, side, o.batch, w.lds, side * w.lds, tc::kOutF16))
-            return cudaErrorInvalidValue;
-        m.b = m.a;
-        m.p = m.o;
+        const int now = i & 1, next = now ^ 1;
         tc::GemmArgs g{};
         g.batch = o.batch;
         g.passes = 1;
@@ -209,10 +221,12 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         // G = X X^T (X^T X)
         g.m = g.n = side;
         g.k = long_side;
+        g.bn = 128;
         g.out = w.gram;
         g.ldo = w.lds;
-        g.out_batch = side * w.lds;
+        g.out_batch = sq;
         g.alpha = kScaleG / (kScaleX * kScaleX);
+        tc::Maps m{M.square[now], M.square[now], M.gram_out, M.gram_out};
         e = tall ? tc::launch_gemm<tc::kDense, 128, true, true, tc::kGram>(m, g, half, stream)
                  : tc::launch_gemm<tc::kDense, 128, false, false, tc::kGram>(m, g, half, stream);
         if (e != cudaSuccess) break;
@@ -220,40 +234,33 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.k = side;
         g.in = w.gram;
         g.ldi = w.lds;
-        g.in_batch = side * w.lds;
+        g.in_batch = sq;
         g.out = w.poly;
         g.alpha = o.c * (kScaleP / (kScaleG * kScaleG));
         g.beta = o.b * (kScaleP / kScaleG);
-        if (!tc::make_map(&m.a, w.gram, side, side, o.batch, w.lds, side * w.lds, tc::kBM, false) ||
-            !tc::make_out_map(&m.o, w.poly, side, side, o.batch, w.lds, side * w.lds, tc::kOutF16))
-            return cudaErrorInvalidValue;
-        m.b = m.a;
+        m = tc::Maps{M.gram, M.gram, M.poly_out, M.poly_out};
         e = tc::launch_gemm<tc::kDense, 128, false, false, tc::kPoly>(m, g, half, stream);
         if (e != cudaSuccess) break;
         // X <- a X + P X (X P); the last step writes the result
         const bool last = i + 1 == o.steps;
         g.m = o.m;
         g.n = o.n;
-        g.in = x;
+        g.bn = bn;
+        g.in = w.hi[now];
         g.in_lo = w.lo;
         g.ldi = w.ldx;
-        g.in_batch = o.m * w.ldx;
-        g.out = last ? o.out : static_cast<void *>(w.hi[i + 1 & 1]);
+        g.in_batch = all;
+        g.out = last ? o.out : static_cast<void *>(w.hi[next]);
         g.low = !last;
         g.ldo = last ? o.n : w.ldx;
         g.out_batch = o.m * g.ldo;
         g.out_type = last ? tc::kOutBf16 : tc::kOutF16;
         g.alpha = last ? 1.f / (kScaleP * kScaleX) : 1.f / kScaleP;
         g.beta = last ? o.a / kScaleX : o.a;
-        const bool mapped = (g.ldo * 2 & 15) == 0;   // else the result's rows have no map
-        if ((mapped && !tc::make_out_map(&m.o, g.out, o.n, o.m, o.batch, g.ldo, g.out_batch, g.out_type)) ||
-            (!last && !tc::make_out_map(&m.p, w.lo, o.n, o.m, o.batch, w.ldx, o.m * w.ldx, tc::kOutF16)))
-            return cudaErrorInvalidValue;
-        const int64_t row_tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM);
-        const int sms = device_sm_count();
-        if (o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms) e = update<256>(o, w, g, x, m, stream);
-        else if (o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms) e = update<128>(o, w, g, x, m, stream);
-        else e = update<64>(o, w, g, x, m, stream);
+        m = tc::Maps{tall ? M.x[now] : M.poly, tall ? M.poly : M.x[now], last ? M.out : M.x_out[next], M.low_out};
+        if (bn == 256) e = update<256>(o, m, g, stream);
+        else if (bn == 128) e = update<128>(o, m, g, stream);
+        else e = update<64>(o, m, g, stream);
     }
     return e;
 }

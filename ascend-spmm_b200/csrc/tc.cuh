@@ -89,6 +89,30 @@ template <int N> __device__ __forceinline__ void bulk_wait_read()
 }
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
+// Cluster launch control: takes a block of the grid that has not started yet
+// over from the hardware; the 16-byte answer at `answer` arrives on `bar`.
+__device__ __forceinline__ void ask_for_block(unsigned answer, unsigned bar)
+{
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(
+                     answer),
+                 "r"(bar)
+                 : "memory");
+}
+// The block's index, -1 if none was left.
+__device__ __forceinline__ int64_t block_given(unsigned answer)
+{
+    unsigned ok, x = 0;
+    asm volatile("{\n\t.reg .b128 r;\n\t.reg .b64 lo, hi;\n\t.reg .pred p;\n\t"
+                 "ld.shared.v2.b64 {lo, hi}, [%2];\n\tmov.b128 r, {lo, hi};\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}\n"
+                 : "=r"(ok), "=r"(x)
+                 : "r"(answer)
+                 : "memory");
+    return ok ? (int64_t)x : -1;
+}
+
 // Programmatic dependent launch: the kernels before this one in the stream
 // are complete and their writes visible; the next may start its set-up.
 __device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
