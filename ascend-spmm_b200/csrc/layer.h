@@ -71,7 +71,7 @@ struct OrthoLaunch {
 };
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int dtype);
 // One block per matrix, no workspace (ortho_small.cu).
-bool ortho_small_eligible(int64_t m, int64_t n);
+bool ortho_small_eligible(int64_t m, int64_t n, int steps, float a);
 cudaError_t launch_ortho_small(const OrthoLaunch &o, cudaStream_t stream);
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream);
 

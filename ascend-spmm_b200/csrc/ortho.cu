@@ -173,12 +173,12 @@ cudaError_t update(const OrthoLaunch &o, const tc::Maps &m, const tc::GemmArgs &
 
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int)
 {
-    return ortho_small_eligible(m, n) ? 0 : Space(batch, m, n, nullptr).bytes(batch);
+    return Space(batch, m, n, nullptr).bytes(batch);
 }
 
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
-    if (ortho_small_eligible(o.m, o.n)) return launch_ortho_small(o, stream);
+    if (ortho_small_eligible(o.m, o.n, o.steps, o.a)) return launch_ortho_small(o, stream);
     const Space w(o.batch, o.m, o.n, workspace);
     switch (o.dtype) {
         case SPMM_F16: start<__half>(o, w, stream); break;

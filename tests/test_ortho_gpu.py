@@ -133,3 +133,16 @@ def test_refusals(lib):
         lib.orthogonalize(u, coefficients=(float("nan"), 0.0, 0.0))
     with pytest.raises(RuntimeError, match="eps must not be negative"):
         lib.orthogonalize(u, eps=-1.0)
+
+
+@pytest.mark.parametrize("m,n", [(8, 300), (128, 257), (513, 128), (100, 2000), (4096, 32), (64, 4097), (129, 600)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_thin_matrices(lib, m, n, dtype):
+    """A short side of at most 128, in several chunks of the long one, and just past both limits."""
+    check(lib, gradient(2, m, n, dtype, seed=m))
+
+
+@pytest.mark.parametrize("steps", [1, 2, 8, 9])
+def test_step_counts_of_thin_matrices(lib, steps):
+    check(lib, gradient(2, 96, 300, F32, seed=steps, decay=0.5), steps=steps)
+    check(lib, gradient(2, 30, 20, F32, seed=steps, decay=0.5), steps=steps)
