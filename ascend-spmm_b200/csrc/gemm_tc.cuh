@@ -37,8 +37,11 @@ namespace spmmb {
 namespace tc {
 
 enum Mode { kRows, kRagged, kDense };
-// Epilogues of kDense: see ortho.cu.
-enum Epi { kStore, kGram, kPoly, kUpdate };
+// kStoreSum: fp32 products.  The tensor core truncates each step into its
+// accumulator, which adds up to 1e-6 over 100 steps; so an accumulator takes
+// kSumSlices slices and the epilogue warps add them in registers, rounding to
+// nearest.  The others but kStore are kDense's: see ortho.cu.
+enum Epi { kStore, kStoreSum, kGram, kPoly, kUpdate };
 enum OutType { kOutF16, kOutBf16, kOutF32 };
 
 struct GemmArgs {
@@ -69,6 +72,7 @@ struct GemmArgs {
 };
 
 constexpr int kBM = 128, kBK = 64;
+constexpr int kSumSlices = 8;
 constexpr int kEpiWarps = 8, kGemmThreads = 64 + 32 * kEpiWarps;   // TMA warp, MMA warp, epilogue warps
 
 constexpr int kSorted = 256;   // most groups that a weight gradient sorts
@@ -363,30 +367,33 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
             const int n = (int)((t.k1 - t.k0 + kBK - 1) / kBK);
             if (elect()) {
-                const int row0 = (int)t.row0, col0 = (int)t.col0;
-                for (int pass = 0; pass < a.passes && ok; ++pass) {
-                    const int za = (int)t.batch_a + a.pa[pass] * a.za, zb = (int)t.batch_b + a.pb[pass] * a.zb;
-                    int k = (int)t.k0;
-                    for (int i = 0; i < n; ++i, k += kBK) {
-                        const unsigned at = slice + pass * n + i, st = at % S::kStages;
-                        if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
-                        const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA, bar = full + 8 * st;
-                        bar_expect(bar, slice_bytes);
-                        if constexpr (AMN) {
+                const int row0 = (int)t.row0, col0 = (int)t.col0, sum = EPI == kStoreSum ? kSumSlices : n;
+                unsigned at = slice;
+                for (int s0 = 0; s0 < n && ok; s0 += sum)
+                    for (int pass = 0; pass < a.passes && ok; ++pass) {
+                        const int za = (int)t.batch_a + a.pa[pass] * a.za, zb = (int)t.batch_b + a.pb[pass] * a.zb;
+                        int k = (int)t.k0 + s0 * kBK;
+                        for (int i = s0; i < min(s0 + sum, n); ++i, ++at, k += kBK) {
+                            const unsigned st = at % S::kStages;
+                            if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
+                            const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA, bar = full + 8 * st;
+                            bar_expect(bar, slice_bytes);
+                            if constexpr (AMN) {
 #pragma unroll
-                            for (int c = 0; c < kBM / 64; ++c) tma_load(sa + c * 8192, &map_a, row0 + 64 * c, k, za, bar);
-                        } else {
-                            tma_load(sa, &map_a, k, row0, za, bar);
-                        }
-                        if constexpr (BMN) {
+                                for (int c = 0; c < kBM / 64; ++c)
+                                    tma_load(sa + c * 8192, &map_a, row0 + 64 * c, k, za, bar);
+                            } else {
+                                tma_load(sa, &map_a, k, row0, za, bar);
+                            }
+                            if constexpr (BMN) {
 #pragma unroll
-                            for (int c = 0; c < BN / 64; ++c)
-                                if (c < b_blocks) tma_load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb, bar);
-                        } else {
-                            tma_load(sb, &map_b, k, col0, zb, bar);
+                                for (int c = 0; c < BN / 64; ++c)
+                                    if (c < b_blocks) tma_load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb, bar);
+                            } else {
+                                tma_load(sb, &map_b, k, col0, zb, bar);
+                            }
                         }
                     }
-                }
             }
             __syncwarp();
             slice += a.passes * n;
@@ -434,36 +441,39 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // kRagged: a last slice that ends within 16 rows needs the whole warp
             const bool ragged = MODE == kRagged && (depth & 15);
             const int whole = ragged ? n - 1 : n;
-            const unsigned d = tmem + (used & 1u) * BN;
-            if (!bar_wait(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) { give_up(2); break; }
-            fence_after();
-            for (int pass = 0; pass < a.passes; ++pass, slice += n) {
-                if (elect())
-                    for (int i = 0; i < whole; ++i) {
-                        if (!landed(slice + i)) { give_up(3); break; }
-                        multiply(slice + i, min(kBK, depth - i * kBK), d, pass == 0 && i == 0);
+            const int sum = EPI == kStoreSum ? kSumSlices : n;
+            for (int s0 = 0; s0 < n && ok; s0 += sum, ++used) {
+                const unsigned d = tmem + (used & 1u) * BN;
+                if (!bar_wait(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) { give_up(2); break; }
+                fence_after();
+                const int s1 = min(s0 + sum, n);
+                for (int pass = 0; pass < a.passes; ++pass, slice += s1 - s0) {
+                    if (elect())
+                        for (int i = s0; i < min(s1, whole); ++i) {
+                            if (!landed(slice + i - s0)) { give_up(3); break; }
+                            multiply(slice + i - s0, min(kBK, depth - i * kBK), d, pass == 0 && i == s0);
+                        }
+                    __syncwarp();
+                    if (ragged && s1 == n && *abort == 0) {
+                        const unsigned at = slice + s1 - s0 - 1, st = at % S::kStages;
+                        if (!landed(at)) give_up(3);
+                        // the rows past the group's end, up to the next multiple of 16, of both operands: zero
+                        const unsigned buf = base + st * (S::kA + S::kB);
+                        const int deep = depth - (n - 1) * kBK;
+                        const int quads = (16 - (deep & 15)) * 8;   // 16-byte pieces of a 64-wide column block
+                        for (int i = lane; i < quads * (S::kA / 8192 + b_blocks); i += 32)
+                            st_shared16(buf + i / quads * 8192 + deep * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
+                        fence_async();
+                        __syncwarp();
+                        if (elect()) multiply(at, deep, d, pass == 0 && n - 1 == s0);
+                        __syncwarp();
                     }
-                __syncwarp();
-                if (ragged && *abort == 0) {
-                    const unsigned at = slice + n - 1, st = at % S::kStages;
-                    if (!landed(at)) give_up(3);
-                    // the rows past the group's end, up to the next multiple of 16, of both operands: zero
-                    const unsigned buf = base + st * (S::kA + S::kB);
-                    const int deep = depth - (n - 1) * kBK;
-                    const int quads = (16 - (deep & 15)) * 8;   // 16-byte pieces of a 64-wide column block
-                    for (int i = lane; i < quads * (S::kA / 8192 + b_blocks); i += 32)
-                        st_shared16(buf + i / quads * 8192 + deep * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
-                    fence_async();
-                    __syncwarp();
-                    if (elect()) multiply(at, deep, d, pass == 0 && n == 1);
-                    __syncwarp();
                 }
+                ok = *abort == 0;
+                if (!ok) break;
+                if (elect()) commit(acc_full + 8 * (used & 1u));
+                __syncwarp();
             }
-            ok = *abort == 0;
-            if (!ok) break;
-            if (elect()) commit(acc_full + 8 * (used & 1u));
-            __syncwarp();
-            ++used;
         }
         if (!ok) {   // every product issued is complete before TMEM is freed (bounded)
             volatile int never = 0;
@@ -490,27 +500,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (MODE == kRagged) continue;
                 break;
             }
-            const bool zero = t.k0 >= t.k1;
-            const unsigned acc = used & 1u;
-            if (!zero) {
-                if (!bar_wait(acc_full + 8 * acc, used >> 1 & 1u, abort)) { give_up(4); break; }
-                fence_after();
-                ++used;
-            }
+            const int n = (int)max((t.k1 - t.k0 + kBK - 1) / kBK, (int64_t)0);
             const bool on = row < t.rows, part = MODE == kRagged && t.part;
             const bool wide = part || out_size == 4;
             const int y = (int)t.out_row + row0, z = (int)t.out_z;
             // a group's last rows share the block with the next group's: no box for them
             const bool boxed = (part || mapped) && (MODE != kRows || row0 + 32 <= t.rows);
-            for (int c = parity * 32; c < t.cols && row0 < t.rows; c += 64) {
-                float v[32];
-                if (zero) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0.f;
-                } else {
-                    tmem_ld32(lanes + acc * BN + c, v);
-                }
-                if constexpr (EPI != kStore) {
+            const bool any = row0 < t.rows;   // the warp has rows of the tile
+            // 32 columns from c on: the epilogue's arithmetic and the store
+            auto emit = [&](int c, float (&v)[32]) {
+                if constexpr (EPI != kStore && EPI != kStoreSum) {
                     const int64_t at = t.batch_a * a.in_batch + (t.row0 + row) * a.ldi + t.col0 + c;
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
@@ -606,11 +605,61 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         for (int r = 0; r < 32 && row0 + r < t.rows; ++r)
                             o[r * a.ldo + lane] = *reinterpret_cast<const unsigned short *>(src + r * 68 + lane * 2);
                 }
-            }
-            if (!zero) {
+            };
+            auto take = [&]() {   // the next accumulator
+                const unsigned acc = used & 1u;
+                if (!bar_wait(acc_full + 8 * acc, used >> 1 & 1u, abort)) { give_up(4); return 0u; }
+                fence_after();
+                return lanes + acc * BN;
+            };
+            auto give_back = [&]() {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(acc_empty + 8 * acc);
+                if (lane == 0) bar_arrive(acc_empty + 8 * (used & 1u));
+                ++used;
+            };
+            if constexpr (EPI == kStoreSum) {
+                float v[BN / 64][32];
+#pragma unroll
+                for (int b = 0; b < BN / 64; ++b)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[b][i] = 0.f;
+                for (int s0 = 0; s0 < n; s0 += kSumSlices) {
+                    const unsigned from = take();
+                    if (!ok) break;
+#pragma unroll
+                    for (int b = 0; b < BN / 64; ++b) {
+                        const int c = parity * 32 + 64 * b;
+                        if (any && c < t.cols) {
+                            float w[32];
+                            tmem_ld32(from + c, w);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[b][i] += w[i];
+                        }
+                    }
+                    give_back();
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int b = 0; b < BN / 64; ++b) {
+                    const int c = parity * 32 + 64 * b;
+                    if (any && c < t.cols) emit(c, v[b]);
+                }
+            } else {
+                unsigned from = 0;
+                if (n > 0) from = take();
+                if (!ok) break;
+                for (int c = parity * 32; c < t.cols && any; c += 64) {
+                    float v[32];
+                    if (n > 0) {
+                        tmem_ld32(from + c, v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                    }
+                    emit(c, v);
+                }
+                if (n > 0) give_back();
             }
         }
         bulk_wait();

@@ -130,8 +130,11 @@ cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::Ge
         !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
         return cudaErrorInvalidValue;
     m.p = m.o;
-    if (a.transposed) return tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(m, g, tiles, stream);
-    return tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(m, g, tiles, stream);
+    if (g.passes > 1)
+        return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStoreSum>(m, g, tiles, stream)
+                            : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStoreSum>(m, g, tiles, stream);
+    return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(m, g, tiles, stream)
+                        : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(m, g, tiles, stream);
 }
 
 // Rows of one part of a weight gradient: a group's rows are one reduction
@@ -233,7 +236,8 @@ cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy
         return cudaErrorInvalidValue;
     const int64_t tiles = (a.groups + a.rows / g.part_rows) * ((a.K + tc::kBM - 1) / tc::kBM) *
                           ((a.N + g.bn - 1) / g.bn);
-    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(m, g, tiles, stream);
+    return g.passes > 1 ? tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStoreSum>(m, g, tiles, stream)
+                        : tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(m, g, tiles, stream);
 }
 
 }  // namespace
