@@ -35,22 +35,30 @@ __host__ __device__ Ranges ranges_of(const GroupedLaunch &a)
 constexpr int kPlanes = 3, kPasses = 6;
 constexpr unsigned char kPassA[kPasses] = {0, 2, 1, 0, 1, 0}, kPassB[kPasses] = {2, 0, 1, 1, 0, 0};
 
-// One thread splits 8 elements.  ranges.ptr set: src is [groups][elems] and
-// groups without rows are skipped.
-__global__ void __launch_bounds__(256) split_planes_kernel(const float *src, __nv_bfloat16 *dst, int64_t elems,
-                                                           int64_t plane, int64_t groups, Ranges ranges,
+// An operand to split: src [groups][elems], planes `plane` apart.  `skip`:
+// groups without rows are left out.
+struct Split {
+    const float *src;
+    __nv_bfloat16 *dst;
+    int64_t elems, plane, groups;
+    bool skip;
+};
+
+// One thread splits 8 elements at a time; blockIdx.z: which operand.
+__global__ void __launch_bounds__(256) split_planes_kernel(const Split first, const Split second, Ranges ranges,
                                                            DevStatus *status)
 {
-    for (int64_t g = blockIdx.y; g < groups; g += gridDim.y) {
-        if (ranges.ptr) {
+    const Split &s = blockIdx.z ? second : first;
+    for (int64_t g = blockIdx.y; g < s.groups; g += gridDim.y) {
+        if (s.skip) {
             int64_t b, e;
             segment_rows(ranges, g + 1, &b, &e, status);
             if (b == e) continue;
         }
-        const int64_t at = g * elems;
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < elems; i += (int64_t)gridDim.x * 2048) {
-            const float4 u = __ldg(reinterpret_cast<const float4 *>(src + at + i));
-            const float4 w = __ldg(reinterpret_cast<const float4 *>(src + at + i) + 1);
+        const int64_t at = g * s.elems;
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < s.elems; i += (int64_t)gridDim.x * 2048) {
+            const float4 u = __ldg(reinterpret_cast<const float4 *>(s.src + at + i));
+            const float4 w = __ldg(reinterpret_cast<const float4 *>(s.src + at + i) + 1);
             float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int p = 0; p < kPlanes; ++p) {
@@ -62,21 +70,23 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const float *src, __n
                     if (isinf(__bfloat162float(h[k])) && !isinf(v[k])) h[k] = __float2bfloat16_rz(v[k]);
                     v[k] = isfinite(v[k]) ? v[k] - __bfloat162float(h[k]) : 0.f;
                 }
-                *reinterpret_cast<uint4 *>(dst + p * plane + at + i) = *reinterpret_cast<const uint4 *>(h);
+                *reinterpret_cast<uint4 *>(s.dst + p * s.plane + at + i) = *reinterpret_cast<const uint4 *>(h);
             }
         }
     }
 }
 
-cudaError_t split_planes(const void *src, void *dst, int64_t batch, int64_t elems, const Ranges &ranges,
-                         DevStatus *status, cudaStream_t stream)
+// The rows operand (x) and a second one: rows too, or the weights of `groups` groups.
+cudaError_t split_planes(const void *x, void *px, int64_t x_elems, const void *w, void *pw, int64_t w_elems,
+                         int64_t groups, bool skip, const Ranges &ranges, DevStatus *status, cudaStream_t stream)
 {
-    if (batch * elems == 0) return cudaSuccess;
-    const int64_t per = std::max<int64_t>(1, 8 * device_sm_count() / batch);
-    const int64_t blocks = std::min((elems + 2047) / 2048, per);
-    const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(batch, 65535));
-    split_planes_kernel<<<grid, 256, 0, stream>>>(static_cast<const float *>(src), static_cast<__nv_bfloat16 *>(dst),
-                                                  elems, batch * elems, batch, ranges, status);
+    const Split a{static_cast<const float *>(x), static_cast<__nv_bfloat16 *>(px), x_elems, x_elems, 1, false};
+    const Split b{static_cast<const float *>(w), static_cast<__nv_bfloat16 *>(pw), w_elems, groups * w_elems, groups, skip};
+    const int64_t y = std::max<int64_t>(1, std::min<int64_t>(groups, 65535));
+    const int64_t most = 8 * (int64_t)device_sm_count();   // blocks that fill the GPU
+    // wide enough for x alone, whose blocks of the other groups return at once
+    const int64_t blocks = std::max<int64_t>(1, std::min((std::max(x_elems, w_elems) + 2047) / 2048, most));
+    split_planes_kernel<<<dim3((unsigned)blocks, (unsigned)y, 2), 256, 0, stream>>>(a, b, ranges, status);
     return cudaGetLastError();
 }
 
@@ -261,8 +271,8 @@ cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStr
     const void *x = a.x, *w = a.groups > 0 ? a.w : a.x;   // no group: the weight is never read
     if (a.dtype == SPMM_F32) {
         char *px = static_cast<char *>(workspace), *pw = px + plane_bytes(a.rows * g.k);
-        cudaError_t e = split_planes(x, px, 1, a.rows * g.k, Ranges{}, a.status, stream);
-        if (e == cudaSuccess) e = split_planes(a.w, pw, a.groups, a.K * a.N, g.ranges, a.status, stream);
+        const cudaError_t e = split_planes(x, px, a.rows * g.k, a.w, pw, a.K * a.N, a.groups, true, g.ranges, a.status,
+                                           stream);
         if (e != cudaSuccess) return e;
         x = px;
         w = a.groups > 0 ? pw : px;
@@ -303,8 +313,8 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
     if (a.dtype == SPMM_F32 && a.rows > 0) {
         char *px = ws, *pdy = px + plane_bytes(a.rows * a.K);
         ws = pdy + plane_bytes(a.rows * a.N);
-        cudaError_t e = split_planes(x, px, 1, a.rows * a.K, Ranges{}, a.status, stream);
-        if (e == cudaSuccess) e = split_planes(dy, pdy, 1, a.rows * a.N, Ranges{}, a.status, stream);
+        const cudaError_t e = split_planes(x, px, a.rows * a.K, dy, pdy, a.rows * a.N, 1, false, g.ranges, a.status,
+                                           stream);
         if (e != cudaSuccess) return e;
         x = px;
         dy = pdy;
