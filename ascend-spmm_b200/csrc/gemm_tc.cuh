@@ -78,9 +78,10 @@ constexpr int kEpiWarps = 8, kGemmThreads = 64 + 32 * kEpiWarps;   // TMA warp, 
 constexpr int kSorted = 256;   // most groups that a weight gradient sorts
 constexpr int kAsked = 4;      // tiles asked for and not yet done by every warp
 
-template <int BN> struct GemmShape {
-    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2;
-    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+template <int BN, bool PAIR = false> struct GemmShape {
+    static constexpr int kA = kBM * kBK * 2, kB = (PAIR ? BN / 2 : BN) * kBK * 2;
+    static constexpr int kStages = PAIR ? 6 : BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kRows = PAIR ? 2 * kBM : kBM;           // of a tile
     static constexpr int kStageOff = kStages * (kA + kB);
     static constexpr int kStaging = 4096;                        // of an epilogue warp
     static constexpr int kBarOff = kStageOff + kEpiWarps * kStaging;
@@ -98,8 +99,9 @@ template <int BN> struct GemmShape {
 // in turn.  kRagged, whose tiles differ in length, launches a block per tile,
 // and a running block takes over those that have not started, one after the
 // other: the TMA warp asks, a few tiles ahead of the others (ring of kAsked).
-template <int MODE, int BN> struct Turns {
-    using S = GemmShape<BN>;
+template <int MODE, int BN, bool PAIR> struct Turns {
+    using S = GemmShape<BN, PAIR>;
+    static constexpr int kBlocks = PAIR ? 2 : 1;   // per tile
     const unsigned base;
     volatile int *const abort;
     const bool asks;       // the TMA warp
@@ -107,7 +109,7 @@ template <int MODE, int BN> struct Turns {
     unsigned turn = 0;
 
     __device__ Turns(unsigned base, volatile int *abort, bool asks)
-        : base(base), abort(abort), asks(asks), tile(blockIdx.x)
+        : base(base), abort(abort), asks(asks), tile(blockIdx.x / kBlocks)
     {
     }
     // Warp-wide, at the start of the current tile.
@@ -128,12 +130,13 @@ template <int MODE, int BN> struct Turns {
     __device__ __forceinline__ bool next()
     {
         if (MODE != kRagged) {
-            tile += gridDim.x;
+            tile += gridDim.x / kBlocks;
             return true;
         }
         const unsigned slot = turn % kAsked;
         if (!bar_wait(base + S::kAskFull + 8 * slot, turn / kAsked & 1u, abort)) return false;
         tile = block_given(base + S::kAnswer + 16 * slot);
+        fence_async();
         __syncwarp();
         if (elect()) bar_arrive(base + S::kAskEmpty + 8 * slot);
         ++turn;
@@ -201,14 +204,15 @@ __device__ __forceinline__ void sort_groups(const GemmArgs &a, int tiles, unsign
     __syncthreads();
 }
 
-template <int MODE, int BN, int EPI> struct Walk {
+template <int MODE, int EPI, bool PAIR> struct Walk {
+    static constexpr int kHeight = PAIR ? 2 * kBM : kBM;   // rows of a tile
     const GemmArgs &a;
     const Order order;
     TileWalk<MODE == kRagged> ranges;
     int64_t mt, nt;
     int rank = 0;
     __device__ Walk(const GemmArgs &a, const Order &order)
-        : a(a), order(order), mt((a.m + kBM - 1) / kBM), nt((a.n + a.bn - 1) / a.bn)
+        : a(a), order(order), mt((a.m + kHeight - 1) / kHeight), nt((a.n + a.bn - 1) / a.bn)
     {
     }
 
@@ -217,14 +221,14 @@ template <int MODE, int BN, int EPI> struct Walk {
     {
         if constexpr (MODE == kRows) {
             int64_t seg, b, e, inner, slots;
-            if (!ranges.find(a.ranges, kBM, nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
-            o->row0 = b + inner / nt * kBM;
+            if (!ranges.find(a.ranges, kHeight, nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
+            o->row0 = b + inner / nt * kHeight;
             o->col0 = inner % nt * a.bn;
             o->batch_a = 0;
             o->batch_b = seg - 1;
             o->k0 = 0;
             o->k1 = seg >= 1 && seg <= a.ranges.groups ? a.k : 0;
-            o->rows = (int)min((int64_t)kBM, e - o->row0);
+            o->rows = (int)min((int64_t)kHeight, e - o->row0);
             o->out_row = o->row0;
             o->out_z = 0;
         } else if constexpr (MODE == kRagged) {
@@ -244,10 +248,10 @@ template <int MODE, int BN, int EPI> struct Walk {
             const int64_t p = inner / (mt * nt), i = inner % (mt * nt);
             o->k0 = b + p * a.part_rows;
             o->k1 = min(e, o->k0 + a.part_rows);
-            o->row0 = i / nt * kBM;
+            o->row0 = i / nt * kHeight;
             o->col0 = i % nt * a.bn;
             o->batch_a = o->batch_b = 0;
-            o->rows = (int)min((int64_t)kBM, a.m - o->row0);
+            o->rows = (int)min((int64_t)kHeight, a.m - o->row0);
             o->part = slots >= 0;
             if (o->part && slots + p >= a.part_slots) {   // only overlapping (malformed) ranges can need more
                 o->k1 = o->k0;
@@ -271,33 +275,45 @@ template <int MODE, int BN, int EPI> struct Walk {
                 j = r % nt;
             }
             o->batch_a = o->batch_b = q;
-            o->row0 = i * kBM;
+            o->row0 = i * kHeight;
             o->col0 = j * a.bn;
             o->k0 = 0;
             o->k1 = a.k;
-            o->rows = (int)min((int64_t)kBM, a.m - o->row0);
+            o->rows = (int)min((int64_t)kHeight, a.m - o->row0);
             o->out_row = o->row0;
             o->out_z = q;
             o->mirror = half && i != j;
         }
         o->cols = (int)min((int64_t)a.bn, a.n - o->col0);
+        if (PAIR) {   // this block's half of the rows
+            const int skip = (int)cluster_rank() * kBM;
+            o->row0 += skip;
+            o->out_row += skip;
+            o->rows = max(0, min(kBM, o->rows - skip));
+        }
         return true;
     }
 };
 
-template <int MODE, int BN, bool AMN, bool BMN, int EPI>
+// PAIR: two blocks share a tile of 256 rows (tcgen05.mma.cta_group::2).  Each
+// brings in its 128 rows of A and half of the columns of B, so a slice of
+// 256 columns costs a block 32 KB instead of 48 KB; the first block's MMA
+// warp issues the products of both, and each block stores its own rows.
+template <int MODE, int BN, bool AMN, bool BMN, int EPI, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_p,
             const __grid_constant__ GemmArgs a)
 {
-    using S = GemmShape<BN>;
+    static_assert(!PAIR || MODE != kRagged, "a group's zeros are written by one block");
+    using S = GemmShape<BN, PAIR>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort = reinterpret_cast<volatile int *>(smem + S::kAbort);
     const unsigned full = base + S::kFull, empty = base + S::kEmpty;
     const unsigned acc_full = base + S::kAccFull, acc_empty = base + S::kAccEmpty, done = base + S::kDone;
+    const unsigned peer = PAIR ? cluster_rank() : 0;   // 0: the pair's first block
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
@@ -306,7 +322,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(acc_full + 8 * i, 1);
-            bar_init(acc_empty + 8 * i, kEpiWarps);
+            bar_init(acc_empty + 8 * i, PAIR ? 2 * kEpiWarps : kEpiWarps);
         }
         bar_init(done, 1);
         for (int i = 0; i < kAsked; ++i) {
@@ -321,11 +337,22 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         prefetch_map(&map_b);
         prefetch_map(&map_o);
     }
+    if (PAIR) {   // the barriers of both blocks are set up
+        __syncthreads();
+        cluster_sync();
+    }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(base + S::kTmem),
-                     "r"(S::kCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(base + S::kTmem),
+                         "r"(S::kCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(base + S::kTmem),
+                         "r"(S::kCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        }
     }
     fence_before();
     __syncthreads();
@@ -339,14 +366,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (a.ranges.groups <= kSorted) {
             unsigned short *group = reinterpret_cast<unsigned short *>(smem + S::kOrder);
             int *first = reinterpret_cast<int *>(smem + S::kFirst), *slot = reinterpret_cast<int *>(smem + S::kSlot);
-            sort_groups(a, (int)((a.m + kBM - 1) / kBM * ((a.n + a.bn - 1) / a.bn)), group, first, slot,
+            sort_groups(a, (int)((a.m + S::kRows - 1) / S::kRows * ((a.n + a.bn - 1) / a.bn)), group, first, slot,
                         reinterpret_cast<int *>(smem + S::kStageOff));
             order = Order{group, first, slot};
         }
-    Walk<MODE, BN, EPI> walk(a, order);
+    Walk<MODE, EPI, PAIR> walk(a, order);
     // the columns of B that a slice brings in (MN-major: in blocks of 64), and its bytes
-    const int b_blocks = BMN ? (a.bn + 63) / 64 : 0;
-    const unsigned slice_bytes = S::kA + (BMN ? b_blocks * 8192 : a.bn * 128);
+    const int b_cols = PAIR ? BN / 2 : a.bn, b_blocks = BMN ? (b_cols + 63) / 64 : 0;
+    const unsigned slice_bytes = S::kA + (BMN ? b_blocks * 8192 : b_cols * 128);
     Tile t;
     bool ok = *abort == 0;
     auto give_up = [&](int code) {
@@ -358,7 +385,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (warp == 0) {
         // ---- TMA warp: all lanes find the tile, one issues its copies
         unsigned slice = 0;   // slices issued
-        Turns<MODE, BN> turns(base, abort, true);
+        Turns<MODE, BN, PAIR> turns(base, abort, true);
         for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
             if (!turns.ask()) { give_up(6); break; }
             if (!walk.at(turns.tile, &t)) {
@@ -367,7 +394,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             }
             const int n = (int)((t.k1 - t.k0 + kBK - 1) / kBK);
             if (elect()) {
-                const int row0 = (int)t.row0, col0 = (int)t.col0, sum = EPI == kStoreSum ? kSumSlices : n;
+                const int row0 = (int)t.row0, col0 = (int)t.col0 + (PAIR ? (int)peer * b_cols : 0);
+                const int sum = EPI == kStoreSum ? kSumSlices : n;
                 unsigned at = slice;
                 for (int s0 = 0; s0 < n && ok; s0 += sum)
                     for (int pass = 0; pass < a.passes && ok; ++pass) {
@@ -376,21 +404,26 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                         for (int i = s0; i < min(s0 + sum, n); ++i, ++at, k += kBK) {
                             const unsigned st = at % S::kStages;
                             if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
-                            const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA, bar = full + 8 * st;
-                            bar_expect(bar, slice_bytes);
+                            const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA;
+                            // a pair's slice, both halves, arrives on the first block's barrier
+                            const unsigned bar = PAIR ? in_block(full + 8 * st, 0) : full + 8 * st;
+                            if (peer == 0) bar_expect(full + 8 * st, PAIR ? 2 * slice_bytes : slice_bytes);
+                            auto load = [&](unsigned dst, const CUtensorMap *map, int x, int y, int z) {
+                                if constexpr (PAIR) tma_load_pair(dst, map, x, y, z, bar);
+                                else tma_load(dst, map, x, y, z, bar);
+                            };
                             if constexpr (AMN) {
 #pragma unroll
-                                for (int c = 0; c < kBM / 64; ++c)
-                                    tma_load(sa + c * 8192, &map_a, row0 + 64 * c, k, za, bar);
+                                for (int c = 0; c < kBM / 64; ++c) load(sa + c * 8192, &map_a, row0 + 64 * c, k, za);
                             } else {
-                                tma_load(sa, &map_a, k, row0, za, bar);
+                                load(sa, &map_a, k, row0, za);
                             }
                             if constexpr (BMN) {
 #pragma unroll
                                 for (int c = 0; c < BN / 64; ++c)
-                                    if (c < b_blocks) tma_load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb, bar);
+                                    if (c < b_blocks) load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb);
                             } else {
-                                tma_load(sb, &map_b, k, col0, zb, bar);
+                                load(sb, &map_b, k, col0, zb);
                             }
                         }
                     }
@@ -409,7 +442,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
     } else if (warp == 1) {
         // ---- MMA warp: one lane issues
-        const unsigned idesc = idesc16(a.bf16, AMN, BMN, kBM, a.bn);
+        const unsigned idesc = idesc16(a.bf16, AMN, BMN, S::kRows, PAIR ? BN : a.bn);
         // byte strides of the operands' layouts: K-major, 8 rows of 128 bytes per
         // swizzle atom; MN-major, atoms of 64 rows or columns x 8 deep, 8 KB apart
         const uint64_t da = AMN ? desc128(base, 8192, 1024) : desc128(base, 16, 1024);
@@ -417,20 +450,30 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         constexpr unsigned step_a = (AMN ? 2048 : 32) >> 4, step_b = (BMN ? 2048 : 32) >> 4;
         unsigned slice = 0, used = 0;
         // The products of the slice at position `at` (depth elements deep).
+        auto mul = [&](unsigned d, uint64_t x, uint64_t y, unsigned add) {
+            if constexpr (PAIR) mma_pair(d, x, y, idesc, add);
+            else mma(d, x, y, idesc, add);
+        };
+        auto finish = [&](unsigned bar) {
+            if constexpr (PAIR) commit_pair(bar);
+            else commit(bar);
+        };
         auto multiply = [&](unsigned at, int depth, unsigned d, bool first) {
             const unsigned st = at % S::kStages, off = st * (S::kA + S::kB) >> 4;
             if (depth == kBK) {
 #pragma unroll
                 for (int i = 0; i < kBK / 16; ++i)
-                    mma(d, da + off + i * step_a, db + off + i * step_b, idesc, first && i == 0 ? 0u : 1u);
+                    mul(d, da + off + i * step_a, db + off + i * step_b, first && i == 0 ? 0u : 1u);
             } else {
                 for (int i = 0; i * 16 < depth; ++i)
-                    mma(d, da + off + i * step_a, db + off + i * step_b, idesc, first && i == 0 ? 0u : 1u);
+                    mul(d, da + off + i * step_a, db + off + i * step_b, first && i == 0 ? 0u : 1u);
             }
-            commit(empty + 8 * st);
+            finish(empty + 8 * st);
         };
-        auto landed = [&](unsigned at) { return bar_wait(full + 8 * (at % S::kStages), at / S::kStages & 1u, abort); };
-        Turns<MODE, BN> turns(base, abort, false);
+        auto landed = [&](unsigned at) {
+            return bar_wait<PAIR>(full + 8 * (at % S::kStages), at / S::kStages & 1u, abort);
+        };
+        Turns<MODE, BN, PAIR> turns(base, abort, false);
         for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
             if (!walk.at(turns.tile, &t)) {
                 if (MODE == kRagged) continue;
@@ -444,11 +487,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const int sum = EPI == kStoreSum ? kSumSlices : n;
             for (int s0 = 0; s0 < n && ok; s0 += sum, ++used) {
                 const unsigned d = tmem + (used & 1u) * BN;
-                if (!bar_wait(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) { give_up(2); break; }
+                if (peer == 0 && !bar_wait<PAIR>(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) {
+                    give_up(2);
+                    break;
+                }
                 fence_after();
                 const int s1 = min(s0 + sum, n);
                 for (int pass = 0; pass < a.passes; ++pass, slice += s1 - s0) {
-                    if (elect())
+                    if (peer == 0 && elect())
                         for (int i = s0; i < min(s1, whole); ++i) {
                             if (!landed(slice + i - s0)) { give_up(3); break; }
                             multiply(slice + i - s0, min(kBK, depth - i * kBK), d, pass == 0 && i == s0);
@@ -471,15 +517,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 }
                 ok = *abort == 0;
                 if (!ok) break;
-                if (elect()) commit(acc_full + 8 * (used & 1u));
+                if (peer == 0 && elect()) finish(acc_full + 8 * (used & 1u));
                 __syncwarp();
             }
         }
         if (!ok) {   // every product issued is complete before TMEM is freed (bounded)
             volatile int never = 0;
-            if (elect()) commit(done);
-            __syncwarp();
-            bar_wait(done, 0, &never);
+            if (peer == 0) {
+                if (elect()) finish(done);
+                __syncwarp();
+                bar_wait(done, 0, &never);
+            }
         }
     } else {
         // ---- epilogue warps: TMEM lanes 32 (warp % 4) .. + 31 are rows of the
@@ -494,7 +542,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         // a 16-byte piece in a row of the staged 64-byte (fp32: 128-byte) wide block, swizzled as its map
         const unsigned swz2 = (unsigned)(lane >> 1 & 3), swz4 = (unsigned)(lane & 7);
         unsigned used = 0;
-        Turns<MODE, BN> turns(base, abort, false);
+        Turns<MODE, BN, PAIR> turns(base, abort, false);
         for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
             if (!walk.at(turns.tile, &t)) {
                 if (MODE == kRagged) continue;
@@ -608,14 +656,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             };
             auto take = [&]() {   // the next accumulator
                 const unsigned acc = used & 1u;
-                if (!bar_wait(acc_full + 8 * acc, used >> 1 & 1u, abort)) { give_up(4); return 0u; }
+                if (!bar_wait<PAIR>(acc_full + 8 * acc, used >> 1 & 1u, abort)) { give_up(4); return 0u; }
                 fence_after();
                 return lanes + acc * BN;
             };
             auto give_back = [&]() {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(acc_empty + 8 * (used & 1u));
+                if (lane == 0) {
+                    if (PAIR) bar_arrive_cluster(in_block(acc_empty + 8 * (used & 1u), 0));
+                    else bar_arrive(acc_empty + 8 * (used & 1u));
+                }
                 ++used;
             };
             if constexpr (EPI == kStoreSum) {
@@ -666,9 +717,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
     fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();   // neither block's memory or barriers are used any more
     fence_after();
-    if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::kCols) : "memory");
+    if (warp == 1) {
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::kCols) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::kCols) : "memory");
+    }
 }
 
 // Tensor map of a 16-bit operand [batch][rows][inner] (strides in elements),
@@ -681,18 +737,22 @@ bool make_out_map(CUtensorMap *map, void *p, int64_t inner, int64_t rows, int64_
 
 // Launch that lets the kernel's set-up overlap the kernel before it.
 template <typename K, typename... A>
-cudaError_t launch_overlapped(K kernel, unsigned grid, int threads, int smem, cudaStream_t stream, const A &...args)
+cudaError_t launch_overlapped(K kernel, unsigned grid, unsigned cluster, int threads, int smem, cudaStream_t stream,
+                              const A &...args)
 {
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
@@ -700,21 +760,22 @@ struct Maps {
     CUtensorMap a, b, o, p;
 };
 
-template <int MODE, int BN, bool AMN, bool BMN, int EPI>
+template <int MODE, int BN, bool AMN, bool BMN, int EPI, bool PAIR = false>
 cudaError_t launch_gemm(const Maps &m, const GemmArgs &a, int64_t tiles, cudaStream_t s)
 {
-    auto kernel = gemm_kernel<MODE, BN, AMN, BMN, EPI>;
+    using S = GemmShape<BN, PAIR>;
+    auto kernel = gemm_kernel<MODE, BN, AMN, BMN, EPI, PAIR>;
     static PerDevice<bool> ready;   // the attribute outlasts the call
     bool *done = ready.here();
     if (!done || !*done) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GemmShape<BN>::kBytes);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
         if (e != cudaSuccess) return e;
         if (done) *done = true;
     }
-    const int64_t most = MODE == kRagged ? INT32_MAX : device_sm_count();
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min(tiles, most));
-    return launch_overlapped(kernel, grid, kGemmThreads, GemmShape<BN>::kBytes, s, m.a, m.b, m.o, m.p, a);
+    constexpr int kBlocks = PAIR ? 2 : 1;   // per tile
+    const int64_t most = MODE == kRagged ? INT32_MAX / 2 : device_sm_count() / kBlocks;
+    const unsigned grid = kBlocks * (unsigned)std::max<int64_t>(1, std::min(tiles, most));
+    return launch_overlapped(kernel, grid, kBlocks, kGemmThreads, S::kBytes, s, m.a, m.b, m.o, m.p, a);
 }
 
 }  // namespace tc

@@ -128,7 +128,7 @@ void set_types(tc::GemmArgs &g, int dtype)
     }
 }
 
-template <int BN>
+template <int BN, bool PAIR = false>
 cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::GemmArgs &g, int64_t row_tiles,
                     cudaStream_t stream)
 {
@@ -136,15 +136,36 @@ cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::Ge
     const int64_t planes = g.passes > 1 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
     const int64_t tiles = row_tiles * ((g.n + g.bn - 1) / g.bn);
     if (!tc::make_map(&m.a, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
-        !tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? g.bn : 64, g.bf16) ||
+        !tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? PAIR ? BN / 2 : g.bn : 64,
+                      g.bf16) ||
         !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
         return cudaErrorInvalidValue;
     m.p = m.o;
-    if (g.passes > 1)
-        return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStoreSum>(m, g, tiles, stream)
-                            : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStoreSum>(m, g, tiles, stream);
-    return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore>(m, g, tiles, stream)
-                        : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore>(m, g, tiles, stream);
+    if constexpr (!PAIR)
+        if (g.passes > 1)
+            return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStoreSum>(m, g, tiles, stream)
+                                : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStoreSum>(m, g, tiles, stream);
+    return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore, PAIR>(m, g, tiles, stream)
+                        : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStore, PAIR>(m, g, tiles, stream);
+}
+
+// Row tiles, at most: every group can end in a partial one; the rows outside
+// the groups too.
+int64_t row_tiles_of(const GroupedLaunch &a, int height)
+{
+    return std::min(a.rows, (a.rows + height - 1) / height + a.groups + 1);
+}
+
+// Whether pairs of blocks take tiles of 256 rows.  They pay where the products
+// bound the kernel and groups are long enough that their last tile's missing
+// rows do not matter: 65536 rows in 64 groups, K = 1024, N = 2048, bf16, 244 us
+// alone and 212 us in pairs with even groups, 253 and 236 us with uneven ones;
+// 100003 rows of 46 groups, K = 128, N = 256 (bound by memory) 18 and 22 us.
+// A weight gradient gained nothing (276 and 281 us) and has no such form.
+bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
+{
+    return g.passes == 1 && g.k >= 512 && g.n % 256 == 0 && a.rows >= 512 * std::max<int64_t>(a.groups, 1) &&
+           a.rows / 256 * (g.n / 256) >= 2 * device_sm_count();
 }
 
 // Rows of one part of a weight gradient: a group's rows are one reduction
@@ -279,8 +300,11 @@ cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStr
         g.za = 1;
         g.zb = (int)a.groups;
     }
-    // every group can end in a partial tile; the rows outside the groups too
-    const int64_t row_tiles = std::min(a.rows, (a.rows + tc::kBM - 1) / tc::kBM + a.groups + 1);
+    if (pair_rows(a, g)) {
+        g.bn = 256;
+        return rows_tc<256, true>(a, x, w, g, row_tiles_of(a, 2 * tc::kBM), stream);
+    }
+    const int64_t row_tiles = row_tiles_of(a, tc::kBM);
     g.bn = tile_columns(row_tiles, g.n);
     if (g.bn <= 64) return rows_tc<64>(a, x, w, g, row_tiles, stream);
     if (g.bn <= 128) return rows_tc<128>(a, x, w, g, row_tiles, stream);

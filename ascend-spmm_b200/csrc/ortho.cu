@@ -30,7 +30,7 @@ namespace spmmb {
 
 namespace {
 
-constexpr int kParts = 64;   // partial sums of squares per matrix, at most
+constexpr int kParts = 512;   // partial sums of squares per matrix, at most
 
 int64_t pad8(int64_t x) { return (x + 7) & ~int64_t(7); }
 
@@ -133,7 +133,7 @@ struct Space {
         lds = pad8(side);
         x = (batch * m * ldx + 127) & ~int64_t(127);
         s = (batch * side * lds + 127) & ~int64_t(127);
-        parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts, m * n / 8192));
+        parts = (int)std::max<int64_t>(1, std::min({(int64_t)kParts, m * n / 8192, 2048 / batch}));
         hi[0] = static_cast<__half *>(ws);
         hi[1] = hi[0] + x;
         lo = hi[1] + x;
@@ -161,12 +161,13 @@ struct OrthoMaps {
     CUtensorMap gram_out, poly_out, x_out[2], low_out, out;
 };
 
-template <int BN>
+template <int BN, bool PAIR = false>
 cudaError_t update(const OrthoLaunch &o, const tc::Maps &m, const tc::GemmArgs &g, cudaStream_t stream)
 {
-    const int64_t tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM) * ((o.n + g.bn - 1) / g.bn);
-    if (o.m > o.n) return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate>(m, g, tiles, stream);
-    return tc::launch_gemm<tc::kDense, BN, false, true, tc::kUpdate>(m, g, tiles, stream);
+    const int64_t height = PAIR ? 2 * tc::kBM : tc::kBM;
+    const int64_t tiles = o.batch * ((o.m + height - 1) / height) * ((o.n + g.bn - 1) / g.bn);
+    if (o.m > o.n) return tc::launch_gemm<tc::kDense, BN, false, false, tc::kUpdate, PAIR>(m, g, tiles, stream);
+    return tc::launch_gemm<tc::kDense, BN, false, true, tc::kUpdate, PAIR>(m, g, tiles, stream);
 }
 
 }  // namespace
@@ -196,11 +197,12 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
     const int bn = o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms  ? 256
                    : o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms ? 128
                                                                         : 64;
+    const bool pair = bn == 256;   // 4096 x 2048: 373 us alone, 362 in pairs; 4096 x 4096: 1360 and 1259
     // a result whose rows do not start on 16 bytes has no map
     const bool mapped = (o.n & 7) == 0;
     OrthoMaps M;
     bool fine = tc::make_map(&M.gram, w.gram, side, side, o.batch, w.lds, sq, tc::kBM, false) &&
-                tc::make_map(&M.poly, w.poly, side, side, o.batch, w.lds, sq, tall ? bn : tc::kBM, false) &&
+                tc::make_map(&M.poly, w.poly, side, side, o.batch, w.lds, sq, tall ? pair ? bn / 2 : bn : tc::kBM, false) &&
                 tc::make_out_map(&M.gram_out, w.gram, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
                 tc::make_out_map(&M.poly_out, w.poly, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
                 tc::make_out_map(&M.low_out, w.lo, o.n, o.m, o.batch, w.ldx, all, tc::kOutF16);
@@ -258,7 +260,8 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.alpha = last ? 1.f / (kScaleP * kScaleX) : 1.f / kScaleP;
         g.beta = last ? o.a / kScaleX : o.a;
         m = tc::Maps{tall ? M.x[now] : M.poly, tall ? M.poly : M.x[now], last ? M.out : M.x_out[next], M.low_out};
-        if (bn == 256) e = update<256>(o, m, g, stream);
+        if (pair) e = update<256, true>(o, m, g, stream);
+        else if (bn == 256) e = update<256>(o, m, g, stream);
         else if (bn == 128) e = update<128>(o, m, g, stream);
         else e = update<64>(o, m, g, stream);
     }

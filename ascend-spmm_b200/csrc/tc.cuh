@@ -44,14 +44,27 @@ __device__ __forceinline__ bool bar_try(unsigned bar, unsigned parity)
                  : "memory");
     return ok != 0;
 }
+// As bar_try, with what another block of the cluster released visible too.
+__device__ __forceinline__ bool bar_try_cluster(unsigned bar, unsigned parity)
+{
+    unsigned ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}\n"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
 // Bounded wait: false after about 2 s, or as soon as another warp of the
 // block has given up (*abort).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, volatile int *abort)
 {
-    if (bar_try(bar, parity)) return true;
+    auto done = [&] { return CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
+    if (done()) return true;
     const long long t0 = clock64();
     for (int i = 0; i < (1 << 24); ++i) {
-        if (bar_try(bar, parity)) return true;
+        if (done()) return true;
         if (*abort || clock64() - t0 > (1ll << 32)) break;
     }
     return false;
@@ -184,6 +197,52 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v)
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// ---- pairs of blocks (clusters of two) -------------------------------------
+__device__ __forceinline__ unsigned cluster_rank()
+{
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+// The address of this block's shared memory `addr` in block `rank` of the cluster.
+__device__ __forceinline__ unsigned in_block(unsigned addr, unsigned rank)
+{
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(unsigned remote)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// As tma_load, into this block, arriving on a barrier of either block of the pair.
+__device__ __forceinline__ void tma_load_pair(unsigned dst, const CUtensorMap *map, int x, int y, int z, unsigned bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+                 "[%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+// D over both blocks' TMEM: 256 rows, each block's A 128 of them and its B half of the columns.
+__device__ __forceinline__ void mma_pair(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+// Arrival on the same barrier of both blocks.
+__device__ __forceinline__ void commit_pair(unsigned bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+                     bar),
+                 "h"((unsigned short)3)
+                 : "memory");
+}
 // Eight fp32 values as fp16 or bf16.
 __device__ __forceinline__ uint4 pack8(const float *v, bool bf16)
 {
