@@ -555,24 +555,34 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // a group's last rows share the block with the next group's: no box for them
             const bool boxed = (part || mapped) && (MODE != kRows || row0 + 32 <= t.rows);
             const bool any = row0 < t.rows;   // the warp has rows of the tile
-            // 32 columns from c on: the epilogue's arithmetic and the store
-            auto emit = [&](int c, float (&v)[32]) {
-                if constexpr (EPI != kStore && EPI != kStoreSum) {
-                    const int64_t at = t.batch_a * a.in_batch + (t.row0 + row) * a.ldi + t.col0 + c;
+            // kPoly, kUpdate: what is added to 32 columns from c on
+            struct Addend {
+                uint4 hi[4], lo[4];
+            };
+            auto fetch = [&](int c, Addend &p) {
+                const int64_t at = t.batch_a * a.in_batch + (t.row0 + row) * a.ldi + t.col0 + c;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-                        if (EPI != kGram && on && t.col0 + c + i < a.ldi) {
-                            hi = *reinterpret_cast<const uint4 *>(a.in + at + i);
-                            if (EPI == kUpdate) lo = *reinterpret_cast<const uint4 *>(a.in_lo + at + i);
-                        }
+                for (int i = 0; i < 4; ++i) {
+                    p.hi[i] = p.lo[i] = make_uint4(0, 0, 0, 0);
+                    if (!on || t.col0 + c + 8 * i >= a.ldi) continue;
+                    p.hi[i] = *reinterpret_cast<const uint4 *>(a.in + at + 8 * i);
+                    if (EPI == kUpdate) p.lo[i] = *reinterpret_cast<const uint4 *>(a.in_lo + at + 8 * i);
+                }
+            };
+            // 32 columns from c on: the epilogue's arithmetic and the store
+            auto emit = [&](int c, float (&v)[32], const Addend &p) {
+                if constexpr (EPI == kGram) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] *= a.alpha;
+                } else if constexpr (EPI == kPoly || EPI == kUpdate) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
                         float h[8], l[8];
-                        unpack16<__half>(hi, h);
-                        unpack16<__half>(lo, l);
+                        unpack16<__half>(p.hi[i], h);
+                        unpack16<__half>(p.lo[i], l);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            v[i + e] = EPI == kGram ? a.alpha * v[i + e]
-                                                    : fmaf(a.alpha, v[i + e], a.beta * (h[e] + l[e]));
+                            v[8 * i + e] = fmaf(a.alpha, v[8 * i + e], a.beta * (h[e] + l[e]));
                     }
                 }
                 const int x = (int)t.col0 + c;
@@ -694,13 +704,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                 for (int b = 0; b < BN / 64; ++b) {
                     const int c = parity * 32 + 64 * b;
-                    if (any && c < t.cols) emit(c, v[b]);
+                    if (any && c < t.cols) emit(c, v[b], Addend{});
                 }
             } else {
+                constexpr bool kAdds = EPI == kPoly || EPI == kUpdate;
+                // the first columns' addend is read while the products run, the next ones' a block ahead
+                Addend now, next;
+                if (kAdds && any) fetch(parity * 32, now);
                 unsigned from = 0;
                 if (n > 0) from = take();
                 if (!ok) break;
                 for (int c = parity * 32; c < t.cols && any; c += 64) {
+                    if (kAdds && c + 64 < t.cols) fetch(c + 64, next);
                     float v[32];
                     if (n > 0) {
                         tmem_ld32(from + c, v);
@@ -708,7 +723,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = 0.f;
                     }
-                    emit(c, v);
+                    emit(c, v, now);
+                    now = next;
                 }
                 if (n > 0) give_back();
             }

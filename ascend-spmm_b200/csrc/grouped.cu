@@ -42,36 +42,39 @@ struct Split {
     __nv_bfloat16 *dst;
     int64_t elems, plane, groups;
     bool skip;
+    __host__ __device__ int64_t chunks() const { return (elems + 2047) / 2048; }   // of a group
 };
 
-// One thread splits 8 elements at a time; blockIdx.z: which operand.
+// Chunks of 2048 elements, of the first operand and then of the second; a
+// thread splits 8 elements.
 __global__ void __launch_bounds__(256) split_planes_kernel(const Split first, const Split second, Ranges ranges,
                                                            DevStatus *status)
 {
-    const Split &s = blockIdx.z ? second : first;
-    for (int64_t g = blockIdx.y; g < s.groups; g += gridDim.y) {
+    const int64_t firsts = first.groups * first.chunks(), total = firsts + second.groups * second.chunks();
+    for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const Split &s = item < firsts ? first : second;
+        const int64_t chunk = item < firsts ? item : item - firsts, g = chunk / s.chunks();
         if (s.skip) {
             int64_t b, e;
             segment_rows(ranges, g + 1, &b, &e, status);
             if (b == e) continue;
         }
-        const int64_t at = g * s.elems;
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < s.elems; i += (int64_t)gridDim.x * 2048) {
-            const float4 u = __ldg(reinterpret_cast<const float4 *>(s.src + at + i));
-            const float4 w = __ldg(reinterpret_cast<const float4 *>(s.src + at + i) + 1);
-            float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+        const int64_t in_group = chunk % s.chunks() * 2048 + threadIdx.x * 8, i = g * s.elems + in_group;
+        if (in_group >= s.elems) continue;
+        const float4 u = __ldg(reinterpret_cast<const float4 *>(s.src + i));
+        const float4 w = __ldg(reinterpret_cast<const float4 *>(s.src + i) + 1);
+        float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int p = 0; p < kPlanes; ++p) {
-                __align__(16) __nv_bfloat16 h[8];
+        for (int p = 0; p < kPlanes; ++p) {
+            __align__(16) __nv_bfloat16 h[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    h[k] = __float2bfloat16_rn(v[k]);
-                    // next to fp32's maximum, rounding up would leave the range
-                    if (isinf(__bfloat162float(h[k])) && !isinf(v[k])) h[k] = __float2bfloat16_rz(v[k]);
-                    v[k] = isfinite(v[k]) ? v[k] - __bfloat162float(h[k]) : 0.f;
-                }
-                *reinterpret_cast<uint4 *>(s.dst + p * s.plane + at + i) = *reinterpret_cast<const uint4 *>(h);
+            for (int k = 0; k < 8; ++k) {
+                h[k] = __float2bfloat16_rn(v[k]);
+                // next to fp32's maximum, rounding up would leave the range
+                if (isinf(__bfloat162float(h[k])) && !isinf(v[k])) h[k] = __float2bfloat16_rz(v[k]);
+                v[k] = isfinite(v[k]) ? v[k] - __bfloat162float(h[k]) : 0.f;
             }
+            *reinterpret_cast<uint4 *>(s.dst + p * s.plane + i) = *reinterpret_cast<const uint4 *>(h);
         }
     }
 }
@@ -82,11 +85,8 @@ cudaError_t split_planes(const void *x, void *px, int64_t x_elems, const void *w
 {
     const Split a{static_cast<const float *>(x), static_cast<__nv_bfloat16 *>(px), x_elems, x_elems, 1, false};
     const Split b{static_cast<const float *>(w), static_cast<__nv_bfloat16 *>(pw), w_elems, groups * w_elems, groups, skip};
-    const int64_t y = std::max<int64_t>(1, std::min<int64_t>(groups, 65535));
-    const int64_t most = 8 * (int64_t)device_sm_count();   // blocks that fill the GPU
-    // wide enough for x alone, whose blocks of the other groups return at once
-    const int64_t blocks = std::max<int64_t>(1, std::min((std::max(x_elems, w_elems) + 2047) / 2048, most));
-    split_planes_kernel<<<dim3((unsigned)blocks, (unsigned)y, 2), 256, 0, stream>>>(a, b, ranges, status);
+    const int64_t blocks = std::min(a.chunks() + groups * b.chunks(), 16 * (int64_t)device_sm_count());
+    split_planes_kernel<<<(unsigned)std::max<int64_t>(1, blocks), 256, 0, stream>>>(a, b, ranges, status);
     return cudaGetLastError();
 }
 
@@ -200,29 +200,27 @@ template <typename T>
 __global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, T *out, int64_t elems, int64_t part_rows,
                                                         int64_t slots, Ranges ranges, DevStatus *status)
 {
-    __shared__ int64_t range[2];
+    __shared__ int64_t before;
     for (int64_t g = blockIdx.y; g < ranges.groups; g += gridDim.y) {
-        if (threadIdx.x < 32) {   // the parts of the groups before g, and its own
-            int64_t before = 0, own = 0;
-            for (int64_t base = 0; base <= g; base += 32) {
-                const int64_t s = base + threadIdx.x;
-                int64_t b = 0, e = 0;
-                if (s <= g) segment_rows(ranges, s + 1, &b, &e, status);
-                int64_t n = (e - b + part_rows - 1) / part_rows;
-                n = n > 1 ? n : 0;
-                if (s == g) own = n;
-                int64_t sum = s < g ? n : 0;
+        auto parts_of = [&](int64_t group) {
+            int64_t b, e;
+            segment_rows(ranges, group + 1, &b, &e, status);
+            const int64_t n = (e - b + part_rows - 1) / part_rows;
+            return n > 1 ? n : 0;
+        };
+        const int64_t n = parts_of(g);
+        if (n == 0) continue;   // the same for the whole block
+        if (threadIdx.x < 32) {   // the parts of the groups before g
+            int64_t sum = 0;
+            for (int64_t i = threadIdx.x; i < g; i += 32) sum += parts_of(i);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                before += sum;
-            }
-            own = __shfl_sync(0xffffffffu, own, (int)(g & 31));
-            if (threadIdx.x == 0) { range[0] = before; range[1] = own; }
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (threadIdx.x == 0) before = sum;
         }
         __syncthreads();
-        const int64_t first = range[0], n = range[1];
+        const int64_t first = before;
         __syncthreads();
-        if (n == 0 || first + n > slots) continue;
+        if (first + n > slots) continue;
         for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < elems; i += (int64_t)gridDim.x * 1024) {
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4

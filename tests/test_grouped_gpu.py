@@ -230,3 +230,51 @@ def test_refusals(lib):
         lib.grouped_matmul(x[:, :16].float(), w[:, :16, :12].float(), ptr)
     with pytest.raises(RuntimeError, match="same number of rows"):
         lib.grouped_weight_grad(x, grad[:4], ptr)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("groups", [255, 256, 257, 3000])
+def test_many_groups(lib, groups, dtype):
+    """More groups than the weight gradient sorts, some of them long enough to be summed in parts."""
+    g = torch.Generator().manual_seed(groups)
+    sizes = torch.randint(0, 7, (groups,), generator=g)
+    sizes[groups // 3], sizes[groups - 2] = 3000, 2100
+    check(lib, *make(sizes.tolist(), 48, 32, dtype, seed=groups))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_pairs_of_blocks(lib, dtype):
+    """Long groups and wide weights, where two blocks share a tile of 256 rows; groups that end anywhere in it."""
+    check(lib, *make([5000, 3000, 129, 0, 1, 255, 12000, 257], 512, 1024, dtype, seed=11))
+    x, w, ptr, grad = make([9001, 9007], 1024, 512, dtype, seed=12, before=300, after=77)
+    x[:300], x[-77:] = float("nan"), float("inf")
+    y = lib.grouped_matmul(x, w, ptr)
+    assert not bool(y[:300].any()) and not bool(y[-77:].any())
+    assert_within(y[300:-77], *(t[300:-77] for t in grouped_reference(x, w, ptr)))
+    dx = lib.grouped_matmul(grad, w, ptr, transposed=True)
+    assert_within(dx, *grouped_reference(grad, w, ptr, True))
+
+
+def test_one_long_group_and_wide_weights(lib):
+    """A weight gradient in many parts, tiles of several widths."""
+    for K, N in ((16, 544), (272, 80), (1024, 256)):
+        x, w, ptr, grad = make([40000, 0, 5], K, N, F16, seed=K)
+        assert_within(lib.grouped_weight_grad(x, grad, ptr), *weight_grad_reference(x, grad, ptr))
+
+
+def test_fp32_extremes(lib):
+    """Values over fp32's range: the planes of a split operand keep its exponents; infinities and NaN give
+    non-finite results in their rows alone."""
+    x, w, ptr, grad = make([40, 30], 64, 48, F32, seed=13)
+    big = x * 1e30
+    assert_within(lib.grouped_matmul(big, w, ptr), *grouped_reference(big, w, ptr))
+    small = x * 1e-25
+    assert_within(lib.grouped_matmul(small, w, ptr), *grouped_reference(small, w, ptr))
+    top = torch.full((70, 64), 3.4028234e38, device="cuda")
+    one = torch.zeros(2, 64, 48, device="cuda")
+    one[:, 0] = 0.5
+    assert torch.equal(lib.grouped_matmul(top, one, ptr), torch.full((70, 48), 1.7014117e38, device="cuda"))
+    x[3, 5] = float("inf")
+    y = lib.grouped_matmul(x, w, ptr)
+    rows = torch.arange(70, device="cuda") != 3
+    assert not bool(y[3].isfinite().any()) and bool(y[rows].isfinite().all())
