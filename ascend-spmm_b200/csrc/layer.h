@@ -70,9 +70,13 @@ struct OrthoLaunch {
     DevStatus *status;
 };
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int dtype);
-// One block per matrix, no workspace (ortho_small.cu).
+// A shorter side of at most 128 (ortho_small.cu).
 bool ortho_small_eligible(int64_t m, int64_t n, int steps, float a);
-cudaError_t launch_ortho_small(const OrthoLaunch &o, cudaStream_t stream);
+size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n);
+cudaError_t launch_ortho_small(const OrthoLaunch &o, void *workspace, cudaStream_t stream);
+// Sums of squares of each matrix in parts (ortho.cu): squares [batch][parts].
+int ortho_square_parts(int64_t batch, int64_t m, int64_t n);
+cudaError_t launch_ortho_squares(const OrthoLaunch &o, double *squares, cudaStream_t stream);
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream);
 
 }  // namespace spmmb

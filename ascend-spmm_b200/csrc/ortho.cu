@@ -133,7 +133,7 @@ struct Space {
         lds = pad8(side);
         x = (batch * m * ldx + 127) & ~int64_t(127);
         s = (batch * side * lds + 127) & ~int64_t(127);
-        parts = (int)std::max<int64_t>(1, std::min({(int64_t)kParts, m * n / 8192, 2048 / batch}));
+        parts = ortho_square_parts(batch, m, n);
         hi[0] = static_cast<__half *>(ws);
         hi[1] = hi[0] + x;
         lo = hi[1] + x;
@@ -147,7 +147,6 @@ struct Space {
 template <typename T> void start(const OrthoLaunch &o, const Space &w, cudaStream_t stream)
 {
     const T *u = static_cast<const T *>(o.update);
-    ortho_squares_kernel<T><<<dim3(w.parts, (unsigned)o.batch), 256, 0, stream>>>(u, o.m * o.n, w.part);
     const int64_t items = o.m * (w.ldx / 8);
     ortho_split_kernel<T><<<dim3((unsigned)((items + 255) / 256), (unsigned)o.batch), 256, 0, stream>>>(
         u, w.part, w.parts, o.eps, o.m, o.n, w.ldx, w.hi[0], w.lo,
@@ -172,21 +171,46 @@ cudaError_t update(const OrthoLaunch &o, const tc::Maps &m, const tc::GemmArgs &
 
 }  // namespace
 
+int ortho_square_parts(int64_t batch, int64_t m, int64_t n)
+{
+    return (int)std::max<int64_t>(1, std::min({(int64_t)kParts, m * n / 8192, 2048 / batch}));
+}
+
+cudaError_t launch_ortho_squares(const OrthoLaunch &o, double *squares, cudaStream_t stream)
+{
+    const dim3 grid(ortho_square_parts(o.batch, o.m, o.n), (unsigned)o.batch);
+    const int64_t elems = o.m * o.n;
+    switch (o.dtype) {
+        case SPMM_F16:
+            ortho_squares_kernel<<<grid, 256, 0, stream>>>(static_cast<const __half *>(o.update), elems, squares);
+            break;
+        case SPMM_BF16:
+            ortho_squares_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(o.update), elems, squares);
+            break;
+        default: ortho_squares_kernel<<<grid, 256, 0, stream>>>(static_cast<const float *>(o.update), elems, squares);
+    }
+    return cudaGetLastError();
+}
+
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int)
 {
-    return Space(batch, m, n, nullptr).bytes(batch);
+    // which form runs depends on the steps too: room for either
+    return std::max(Space(batch, m, n, nullptr).bytes(batch),
+                    std::min(m, n) <= 128 ? ortho_small_workspace(batch, m, n) : 0);
 }
 
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
-    if (ortho_small_eligible(o.m, o.n, o.steps, o.a)) return launch_ortho_small(o, stream);
+    if (ortho_small_eligible(o.m, o.n, o.steps, o.a)) return launch_ortho_small(o, workspace, stream);
     const Space w(o.batch, o.m, o.n, workspace);
+    cudaError_t e = launch_ortho_squares(o, w.part, stream);
+    if (e != cudaSuccess) return e;
     switch (o.dtype) {
         case SPMM_F16: start<__half>(o, w, stream); break;
         case SPMM_BF16: start<__nv_bfloat16>(o, w, stream); break;
         default: start<float>(o, w, stream);
     }
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess || o.steps == 0) return e;
     const bool tall = o.m > o.n;
     const int64_t side = std::min(o.m, o.n), long_side = std::max(o.m, o.n), sq = side * w.lds, all = o.m * w.ldx;

@@ -1,5 +1,5 @@
-// Orthogonalised updates of matrices whose shorter side s is at most 128: all
-// steps of one matrix in one block, one launch.
+// Orthogonalised updates of matrices whose shorter side s is at most 128: the
+// steps of one matrix run in one block.
 //
 // Every step multiplies X from the left by the same polynomial of its own
 // G = X X^T, so with T = a I + b G + c G G
@@ -13,7 +13,10 @@
 // latencies (105 us for 128 x 64); the products on X were most of the rest.
 //
 // The block holds 128 x 128 matrices in shared memory and their accumulators
-// in TMEM; X passes through in chunks of 256 columns.  A tall matrix is held
+// in TMEM; X passes through in chunks of 256 columns.  A short X stays in one
+// block and one launch (kAll); of a long one many blocks form G in parts
+// (kGram), one runs the steps and leaves Q in memory (kSteps), and many apply
+// it (kApply): 30 x 4000 in one block takes 125 us, in parts 54 us.  A tall matrix is held
 // as its transpose.  X as the second operand of Q X is MN-major: the bytes of
 // a K-major [rows][64] tile are also those of an MN-major tile whose
 // reduction runs down the rows.
@@ -49,8 +52,8 @@ constexpr int kAtom = kSide * 128;       // bytes of [128 rows][64 columns] fp16
 // and below it one of Q, so that [G | Q] is one operand of 256 rows.  A chunk
 // of X lies where it overlaps neither Q nor itself: high parts over T, low
 // parts over G.
-constexpr int kG = 0, kQ = kAtom, kPartGQ = 4 * kAtom, kStepGQ = 2 * kAtom;
-constexpr int kT = 8 * kAtom, kPartT = 2 * kAtom, kStepT = kAtom;
+constexpr int kG_ = 0, kQ_ = kAtom, kPartGQ = 4 * kAtom, kStepGQ = 2 * kAtom;
+constexpr int kT_ = 8 * kAtom, kPartT = 2 * kAtom, kStepT = kAtom;
 constexpr int kBar = 12 * kAtom, kTmem = kBar + 8, kAbort = kTmem + 4, kRed = kAbort + 4, kBytes = kRed + 8 * kWarps;
 static_assert(kBytes <= 232448, "shared memory of a block");
 
@@ -100,8 +103,20 @@ __device__ __forceinline__ void load_chunk(float (&x)[64], const T *u, int s, in
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLaunch o, float scale_q)
+enum Phase { kAll, kGram, kSteps, kApply };
+
+// What the phases of a long matrix leave for each other.
+struct Between {
+    const double *squares;   // [batch][square_parts]
+    int square_parts;
+    float *gram;             // [batch][parts][128][128], in kScaleX^2 units
+    int parts;
+    int64_t per;             // columns of a part, a multiple of kChunk
+    uint4 *q;                // [batch][2][128][16]: Q's parts, 8 columns each
+};
+
+template <typename T, int PHASE>
+__global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLaunch o, float scale_q, const Between w)
 {
     extern __shared__ __align__(1024) unsigned char smem[];
     const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
@@ -112,7 +127,12 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
     const int64_t r = max(o.m, o.n);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + kAbort);
     const unsigned bar = base + kBar;
-    const T *u = static_cast<const T *>(o.update) + (int64_t)blockIdx.x * o.m * o.n;
+    const int64_t matrix = blockIdx.y;
+    const T *u = static_cast<const T *>(o.update) + matrix * o.m * o.n;
+    // the columns of this block
+    const int64_t c_begin = PHASE == kAll ? 0 : blockIdx.x * w.per;
+    const int64_t c_end = PHASE == kAll ? r : min(r, c_begin + w.per);
+    const bool reload = PHASE != kAll || r > kChunk;   // x holds one chunk
 
     if (threadIdx.x == 0) {
         tc::bar_init(bar, 1);
@@ -129,10 +149,14 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
     // ---- the norm: squares in 64 bits (an fp32 update's can leave fp32's range)
     float x[64];
     double sum = 0.0;
-    for (int64_t c = 0; c < r; c += kChunk) {
-        load_chunk<T>(x, u, s, r, tall, row, share, c);
+    if constexpr (PHASE == kAll) {
+        for (int64_t c = 0; c < r; c += kChunk) {
+            load_chunk<T>(x, u, s, r, tall, row, share, c);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) sum += (double)x[i] * (double)x[i];
+            for (int i = 0; i < 64; ++i) sum += (double)x[i] * (double)x[i];
+        }
+    } else if constexpr (PHASE != kSteps) {
+        for (int i = threadIdx.x; i < w.square_parts; i += kThreads) sum += w.squares[matrix * w.square_parts + i];
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
@@ -174,9 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
         return Operand{tc::desc128(base + at, 16, 1024), tc::desc128(base + at + part, 16, 1024), 2, (unsigned)step >> 4,
                        2, (unsigned)step >> 4};
     };
-    const Operand g = k_major(kG, kPartGQ, kStepGQ), q = k_major(kQ, kPartGQ, kStepGQ), t = k_major(kT, kPartT, kStepT);
-    const Operand xk{tc::desc128(base + kT, 16, 1024), tc::desc128(base + kG, 16, 1024), 2, kAtom >> 4, 2, kStepGQ >> 4};
-    const Operand xn{tc::desc128(base + kT, kAtom, 1024), tc::desc128(base + kG, kStepGQ, 1024), 128, 512, 128, 512};
+    const Operand g = k_major(kG_, kPartGQ, kStepGQ), q = k_major(kQ_, kPartGQ, kStepGQ), t = k_major(kT_, kPartT, kStepT);
+    const Operand xk{tc::desc128(base + kT_, 16, 1024), tc::desc128(base + kG_, 16, 1024), 2, kAtom >> 4, 2, kStepGQ >> 4};
+    const Operand xn{tc::desc128(base + kT_, kAtom, 1024), tc::desc128(base + kG_, kStepGQ, 1024), 128, 512, 128, 512};
     // d (+)= A B over n 16-deep steps, the small products first; by one thread.
     auto product = [&](unsigned d, const Operand &a, const Operand &b, int n, unsigned idesc, bool add) {
         for (int k = 0; k < n; ++k) {
@@ -206,30 +230,67 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
     };
     // The chunk at column c to shared memory (x already holds an only chunk).
     auto stage = [&](int64_t c) {
-        if (r > kChunk) load_chunk<T>(x, u, s, r, tall, row, share, c);
+        if (reload) load_chunk<T>(x, u, s, r, tall, row, share, c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float v[8];
             if ((share + 4 * i) * 8 >= ((r - c + 63) & ~int64_t(63))) break;   // past the last atom that is read
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = x[8 * i + e] * scale * kScaleX;
-            put_split(base + kT + piece(row, share + 4 * i, kAtom), base + kG + piece(row, share + 4 * i, kStepGQ), v);
+            put_split(base + kT_ + piece(row, share + 4 * i, kAtom), base + kG_ + piece(row, share + 4 * i, kStepGQ), v);
         }
         publish();
     };
 
-    if (o.steps > 0) {
-        for (int64_t c = 0; c < r && ok; c += kChunk) {
-            stage(c);
-            if (warp == 0 && tc::elect()) {
-                product(tmem + kAccG, xk, xk, (int)(min(r - c, (int64_t)kChunk) + 15) / 16, square, c > 0);
-                tc::commit(bar);
-            }
-            ok = finished();
-        }
-        if (ok) move(kAccG, kScaleG / (kScaleX * kScaleX), kG, kPartGQ, kStepGQ);
+    if (PHASE != kApply && o.steps > 0) {
         float unit_g = 1.f / (kScaleX * kScaleX);   // value of kAccG's units
-        for (int step = 0; step < o.steps && ok; ++step) {
+        float given[PHASE == kSteps ? 32 : 1];      // kSteps: this thread's part of the first G, in those units
+        if constexpr (PHASE != kSteps) {
+            for (int64_t c = c_begin; c < c_end && ok; c += kChunk) {
+                stage(c);
+                if (warp == 0 && tc::elect()) {
+                    product(tmem + kAccG, xk, xk, (int)(min(r - c, (int64_t)kChunk) + 15) / 16, square, c > c_begin);
+                    tc::commit(bar);
+                }
+                ok = finished();
+            }
+        }
+        if constexpr (PHASE == kGram) {
+            float v[32];
+            tc::tmem_ld8x4(lanes + kAccG + share * 8, 32, v);
+            float *to = w.gram + ((matrix * w.parts + blockIdx.x) * kSide + row) * kSide;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (ok && row < s && share + 4 * j < pieces)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4)
+                        *reinterpret_cast<float4 *>(to + (share + 4 * j) * 8 + e) =
+                            make_float4(v[8 * j + e], v[8 * j + e + 1], v[8 * j + e + 2], v[8 * j + e + 3]);
+        } else if constexpr (PHASE == kSteps) {   // the parts, in their order
+#pragma unroll
+            for (int i = 0; i < 32; ++i) given[i] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (share + 4 * j >= pieces) break;
+                // G is symmetric: read down its columns, so that the lanes read one line
+                const int col = (share + 4 * j) * 8;
+                const float *from = w.gram + (matrix * w.parts * kSide + col) * kSide + row;
+                if (row < s)
+#pragma unroll 4
+                    for (int k = 0; k < w.parts; ++k)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (col + e < s) given[8 * j + e] += __ldg(from + ((int64_t)k * kSide + e) * kSide);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = given[8 * j + e] * (kScaleG / (kScaleX * kScaleX));
+                const unsigned at = base + kG_ + piece(row, share + 4 * j, kStepGQ);
+                put_split(at, at + kPartGQ, v);
+            }
+        } else if (ok) {
+            move(kAccG, kScaleG / (kScaleX * kScaleX), kG_, kPartGQ, kStepGQ);
+        }
+        for (int step = 0; PHASE != kGram && step < o.steps && ok; ++step) {
             const bool first = step == 0, last = step + 1 == o.steps;
             publish();
             if (warp == 0 && tc::elect()) {
@@ -240,23 +301,28 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
             const float fg = o.b * unit_g, fgg = o.c / (kScaleG * kScaleG);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float v[8], w[8];
+                float v[8], gg[8];
                 const int col = (share + 4 * j) * 8;
                 if (share + 4 * j >= pieces) break;   // the same for the whole warp
-                tc::tmem_ld8(lanes + kAccG + col, v);
-                tc::tmem_ld8(lanes + kAccGG + col, w);
+                if (PHASE == kSteps && first) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = given[PHASE == kSteps ? 8 * j + e : 0];
+                } else {
+                    tc::tmem_ld8(lanes + kAccG + col, v);
+                }
+                tc::tmem_ld8(lanes + kAccGG + col, gg);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[e] = fmaf(fg, v[e], fgg * w[e]);
+                    v[e] = fmaf(fg, v[e], fgg * gg[e]);
                     if (row == col + e && row < s) v[e] += o.a;
-                    w[e] = v[e] * scale_q;
+                    gg[e] = v[e] * scale_q;
                     v[e] *= kScaleP;
                 }
-                const unsigned at = base + kT + piece(row, share + 4 * j, kStepT);
+                const unsigned at = base + kT_ + piece(row, share + 4 * j, kStepT);
                 put_split(at, at + kPartT, v);
                 if (first) {   // Q = T
-                    const unsigned to = base + kQ + piece(row, share + 4 * j, kStepGQ);
-                    put_split(to, to + kPartGQ, w);
+                    const unsigned to = base + kQ_ + piece(row, share + 4 * j, kStepGQ);
+                    put_split(to, to + kPartGQ, gg);
                 }
             }
             if (first && last) break;
@@ -271,9 +337,9 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
                 tc::commit(bar);
             }
             if (!(ok = finished())) break;
-            if (!first) move(kAccW + 128, 1.f / kScaleP, kQ, kPartGQ, kStepGQ);
+            if (!first) move(kAccW + 128, 1.f / kScaleP, kQ_, kPartGQ, kStepGQ);
             if (last) break;
-            move(kAccW, 1.f / kScaleP, kG, kPartGQ, kStepGQ);   // H
+            move(kAccW, 1.f / kScaleP, kG_, kPartGQ, kStepGQ);   // H
             publish();
             if (warp == 0 && tc::elect()) {
                 product(tmem + kAccG, g, t, ks, square, false);
@@ -281,14 +347,27 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
             }
             if (!(ok = finished())) break;
             unit_g = 1.f / (kScaleG * kScaleP);
-            move(kAccG, 1.f / kScaleP, kG, kPartGQ, kStepGQ);
+            move(kAccG, 1.f / kScaleP, kG_, kPartGQ, kStepGQ);
         }
         __syncthreads();   // T of a single step is written before X takes its place
     }
 
+    // ---- Q between the phases: part, row, piece
+    if constexpr (PHASE == kSteps || PHASE == kApply) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int part = i & 1, j = share + 4 * (i >> 1);
+            uint4 *at = w.q + ((matrix * 2 + part) * kSide + row) * 16 + j;
+            uint4 *mine = reinterpret_cast<uint4 *>(smem + kQ_ + part * kPartGQ + piece(row, j, kStepGQ));
+            if (j >= pieces) break;
+            if (PHASE == kApply) *mine = *at;
+            else if (ok) *at = *mine;   // this thread's own
+        }
+    }
+
     // ---- the result
-    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(o.out) + (int64_t)blockIdx.x * o.m * o.n;
-    for (int64_t c0 = 0; c0 < r && ok; c0 += kChunk) {
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(o.out) + matrix * o.m * o.n;
+    for (int64_t c0 = c_begin; (PHASE == kAll || PHASE == kApply) && c0 < c_end && ok; c0 += kChunk) {
         const int cols = (int)min(r - c0, (int64_t)kChunk);
         if (o.steps > 0) {
             stage(c0);
@@ -297,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
                 tc::commit(bar);
             }
             if (!(ok = finished())) break;
-        } else if (r > kChunk) {
+        } else if (reload) {
             load_chunk<T>(x, u, s, r, tall, row, share, c0);
         }
         const float f = o.steps > 0 ? 1.f / (scale_q * kScaleX) : scale;
@@ -324,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
                         out[tall ? (c0 + col + e) * s + row : row * r + c0 + col + e] = __float2bfloat16_rn(v[e]);
             }
         }
-        if (r > kChunk) {   // the accumulator and the chunk are read before the next one
+        if (c0 + kChunk < c_end) {   // the accumulator and the chunk are read before the next one
             tc::fence_before();
             __syncthreads();
             tc::fence_after();
@@ -332,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
     }
 
     if (!ok && threadIdx.x == 0) {
-        raise_status(o.status, SPMM_DEV_TIMEOUT, blockIdx.x);
+        raise_status(o.status, SPMM_DEV_TIMEOUT, matrix);
         // the products issued are complete before TMEM is freed (bounded)
         volatile int never = 0;
         tc::bar_wait(bar, parity ^ 1u, &never);
@@ -344,9 +423,10 @@ __global__ void __launch_bounds__(kThreads, 1) ortho_small_kernel(const OrthoLau
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
 
-template <typename T> cudaError_t run_small(const OrthoLaunch &o, float scale_q, cudaStream_t stream)
+template <typename T, int PHASE>
+cudaError_t run_phase(const OrthoLaunch &o, float scale_q, const Between &w, int64_t blocks, cudaStream_t stream)
 {
-    auto kernel = ortho_small_kernel<T>;
+    auto kernel = ortho_small_kernel<T, PHASE>;
     static PerDevice<bool> ready;
     bool *done = ready.here();
     if (!done || !*done) {
@@ -354,7 +434,7 @@ template <typename T> cudaError_t run_small(const OrthoLaunch &o, float scale_q,
         if (e != cudaSuccess) return e;
         if (done) *done = true;
     }
-    kernel<<<(unsigned)o.batch, kThreads, kBytes, stream>>>(o, scale_q);
+    kernel<<<dim3((unsigned)blocks, (unsigned)o.batch), kThreads, kBytes, stream>>>(o, scale_q, w);
     return cudaGetLastError();
 }
 
@@ -366,21 +446,64 @@ float q_scale(int steps, float a)
     return (float)std::min(256.0, std::exp2(std::floor(std::log2(32768.0 / largest))));
 }
 
-}  // namespace
-
-// The longer side: one block reads the whole matrix three times.
-bool ortho_small_eligible(int64_t m, int64_t n, int steps, float a)
+// Blocks of a matrix in parts (1: one block does it all).  A block alone takes
+// about 7 us more for every chunk (128 x 256 49 us), the four launches of a
+// matrix in parts 90 us whatever its length (128 x 1024 to 128 x 4096).  With
+// as many matrices as half the SMs they fill the GPU by themselves until a
+// matrix is very long.
+int64_t parts_of(int64_t batch, int64_t m, int64_t n)
 {
-    return std::min(m, n) <= kSide && std::max(m, n) <= 4096 && q_scale(steps, a) > 0.f;
+    const int64_t r = std::max(m, n), chunks = (r + kChunk - 1) / kChunk;
+    return chunks <= 6 || (chunks <= 16 && batch > device_sm_count() / 2) ? 1 : std::min<int64_t>(chunks, 64);
 }
 
-cudaError_t launch_ortho_small(const OrthoLaunch &o, cudaStream_t stream)
+Between between(int64_t batch, int64_t m, int64_t n, void *workspace)
+{
+    Between w{};
+    const int64_t parts = parts_of(batch, m, n), chunks = (std::max(m, n) + kChunk - 1) / kChunk;
+    if (parts == 1) return w;
+    const int64_t each = (chunks + parts - 1) / parts;
+    w.per = each * kChunk;
+    w.parts = (int)((chunks + each - 1) / each);
+    w.square_parts = ortho_square_parts(batch, m, n);
+    w.q = static_cast<uint4 *>(workspace);
+    w.gram = reinterpret_cast<float *>(w.q + batch * 2 * kSide * 16);
+    w.squares = reinterpret_cast<const double *>(w.gram + batch * w.parts * kSide * kSide);
+    return w;
+}
+
+template <typename T> cudaError_t run_small(const OrthoLaunch &o, float scale_q, void *workspace, cudaStream_t stream)
+{
+    const Between w = between(o.batch, o.m, o.n, workspace);
+    if (w.parts == 0) return run_phase<T, kAll>(o, scale_q, w, 1, stream);
+    cudaError_t e = launch_ortho_squares(o, const_cast<double *>(w.squares), stream);
+    if (e == cudaSuccess && o.steps > 0) e = run_phase<T, kGram>(o, scale_q, w, w.parts, stream);
+    if (e == cudaSuccess && o.steps > 0) e = run_phase<T, kSteps>(o, scale_q, w, 1, stream);
+    if (e == cudaSuccess) e = run_phase<T, kApply>(o, scale_q, w, w.parts, stream);
+    return e;
+}
+
+}  // namespace
+
+bool ortho_small_eligible(int64_t m, int64_t n, int steps, float a)
+{
+    return std::min(m, n) <= kSide && q_scale(steps, a) > 0.f;
+}
+
+size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n)
+{
+    const Between w = between(batch, m, n, nullptr);
+    return w.parts == 0 ? 0
+                        : (size_t)batch * (2 * kSide * 256 + (size_t)w.parts * kSide * kSide * 4 + 8 * w.square_parts);
+}
+
+cudaError_t launch_ortho_small(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
     const float scale_q = q_scale(o.steps, o.a);
     switch (o.dtype) {
-        case SPMM_F16: return run_small<__half>(o, scale_q, stream);
-        case SPMM_BF16: return run_small<__nv_bfloat16>(o, scale_q, stream);
-        default: return run_small<float>(o, scale_q, stream);
+        case SPMM_F16: return run_small<__half>(o, scale_q, workspace, stream);
+        case SPMM_BF16: return run_small<__nv_bfloat16>(o, scale_q, workspace, stream);
+        default: return run_small<float>(o, scale_q, workspace, stream);
     }
 }
 

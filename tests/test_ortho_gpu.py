@@ -142,6 +142,14 @@ def test_thin_matrices(lib, m, n, dtype):
     check(lib, gradient(2, m, n, dtype, seed=m))
 
 
+@pytest.mark.parametrize("batch,m,n", [(1, 30, 4000), (3, 769, 128), (2, 17, 20000), (90, 40, 1100), (2, 1, 5000)])
+def test_long_thin_matrices(lib, batch, m, n):
+    """One matrix over many blocks, and many matrices over one block each."""
+    check(lib, gradient(batch, m, n, F32, seed=m))
+    check(lib, gradient(batch, m, n, BF16, seed=m), steps=1)
+    check(lib, gradient(batch, m, n, F16, seed=m), steps=0)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 8, 9])
 def test_step_counts_of_thin_matrices(lib, steps):
     check(lib, gradient(2, 96, 300, F32, seed=steps, decay=0.5), steps=steps)
