@@ -447,14 +447,15 @@ float q_scale(int steps, float a)
 }
 
 // Blocks of a matrix in parts (1: one block does it all).  A block alone takes
-// about 7 us more for every chunk (128 x 256 49 us), the four launches of a
-// matrix in parts 90 us whatever its length (128 x 1024 to 128 x 4096).  With
+// about 28 us more for every chunk (128 x 256 49 us, 128 x 1024 134 us), the
+// four launches of a matrix in parts 92 us whatever its length (128 x 1024 to
+// 128 x 4096).  With
 // as many matrices as half the SMs they fill the GPU by themselves until a
 // matrix is very long.
 int64_t parts_of(int64_t batch, int64_t m, int64_t n)
 {
     const int64_t r = std::max(m, n), chunks = (r + kChunk - 1) / kChunk;
-    return chunks <= 6 || (chunks <= 16 && batch > device_sm_count() / 2) ? 1 : std::min<int64_t>(chunks, 64);
+    return chunks <= 2 || (chunks <= 16 && batch > device_sm_count() / 2) ? 1 : std::min<int64_t>(chunks, 64);
 }
 
 Between between(int64_t batch, int64_t m, int64_t n, void *workspace)
