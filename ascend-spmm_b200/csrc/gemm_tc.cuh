@@ -59,6 +59,10 @@ struct GemmArgs {
     // operands (plane p of A starts at batch index p * za, of B at p * zb).
     int passes, za, zb;
     unsigned char pa[6], pb[6];
+    // MN-major operands whose map has the blocks of 64 rows or columns as a
+    // dimension (make_blocked_map): a slice is one copy instead of one per
+    // block, and the issuing lane keeps up with the tensor core
+    bool blocked_a, blocked_b;
     // kGram: x = alpha * accumulator; kPoly, kUpdate: x = alpha * accumulator
     // + beta * (in + in_lo), `in` laid out as the output.  kGram and kPoly
     // are symmetric and also write the transposed tile; kUpdate writes x as
@@ -412,18 +416,26 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                                 if constexpr (PAIR) tma_load_pair(dst, map, x, y, z, bar);
                                 else tma_load(dst, map, x, y, z, bar);
                             };
-                            if constexpr (AMN) {
+                            auto load_blocks = [&](unsigned dst, const CUtensorMap *map, int x, int z) {
+                                if constexpr (PAIR) tma_load4_pair(dst, map, 0, k, x / 64, z, bar);
+                                else tma_load4(dst, map, 0, k, x / 64, z, bar);
+                            };
+                            if (!AMN) {
+                                load(sa, &map_a, k, row0, za);
+                            } else if (a.blocked_a) {
+                                load_blocks(sa, &map_a, row0, za);
+                            } else {
 #pragma unroll
                                 for (int c = 0; c < kBM / 64; ++c) load(sa + c * 8192, &map_a, row0 + 64 * c, k, za);
-                            } else {
-                                load(sa, &map_a, k, row0, za);
                             }
-                            if constexpr (BMN) {
+                            if (!BMN) {
+                                load(sb, &map_b, k, col0, zb);
+                            } else if (a.blocked_b) {
+                                load_blocks(sb, &map_b, col0, zb);
+                            } else {
 #pragma unroll
                                 for (int c = 0; c < BN / 64; ++c)
                                     if (c < b_blocks) load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb);
-                            } else {
-                                load(sb, &map_b, k, col0, zb);
                             }
                         }
                     }
@@ -747,6 +759,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 // read in boxes of 64 elements x box_rows, 128-byte swizzled, zero outside.
 bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
               int64_t batch_stride, int box_rows, bool bf16);
+// As make_map for an MN-major operand read in boxes of `blocks` x 64 rows x 64
+// elements: [batch][inner / 64][rows][64].  Only for an inner extent of whole
+// blocks; others have a box per block.
+bool make_blocked_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
+                      int64_t batch_stride, int blocks, bool bf16);
+// An MN-major operand whose tiles are `tile` wide: the blocked map where it
+// can be, else the plain one; *blocked says which.
+inline bool make_mn_map(CUtensorMap *map, bool *blocked, const void *p, int64_t inner, int64_t rows, int64_t batch,
+                        int64_t ld, int64_t batch_stride, int tile, bool bf16)
+{
+    *blocked = inner % 64 == 0 && (tile % 64 == 0 || tile >= inner);
+    return *blocked ? make_blocked_map(map, p, inner, rows, batch, ld, batch_stride, (tile + 63) / 64, bf16)
+                    : make_map(map, p, inner, rows, batch, ld, batch_stride, 64, bf16);
+}
 // Tensor map of an output, written in boxes of 32 x 32 elements.
 bool make_out_map(CUtensorMap *map, void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
                   int64_t batch_stride, int out_type);

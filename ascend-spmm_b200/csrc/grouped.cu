@@ -135,9 +135,11 @@ cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::Ge
     tc::Maps m;
     const int64_t planes = g.passes > 1 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
     const int64_t tiles = row_tiles * ((g.n + g.bn - 1) / g.bn);
+    const int cols = PAIR ? BN / 2 : g.bn;   // of the weight that a block brings in
     if (!tc::make_map(&m.a, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
-        !tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, a.transposed ? PAIR ? BN / 2 : g.bn : 64,
-                      g.bf16) ||
+        !(a.transposed ? tc::make_map(&m.b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, cols, g.bf16)
+                       : tc::make_mn_map(&m.b, &g.blocked_b, w, a.N, a.K, planes * groups, a.N, a.K * a.N, cols,
+                                         g.bf16)) ||
         !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
         return cudaErrorInvalidValue;
     m.p = m.o;
@@ -256,8 +258,8 @@ cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy
 {
     tc::Maps m;
     const int64_t planes = g.passes > 1 ? kPlanes : 1, rows = std::max<int64_t>(a.rows, 1);
-    if (!tc::make_map(&m.a, x, a.K, rows, planes, a.K, rows * a.K, 64, g.bf16) ||
-        !tc::make_map(&m.b, dy, a.N, rows, planes, a.N, rows * a.N, 64, g.bf16) ||
+    if (!tc::make_mn_map(&m.a, &g.blocked_a, x, a.K, rows, planes, a.K, rows * a.K, tc::kBM, g.bf16) ||
+        !tc::make_mn_map(&m.b, &g.blocked_b, dy, a.N, rows, planes, a.N, rows * a.N, g.bn, g.bf16) ||
         !tc::make_out_map(&m.o, a.out, a.N, a.K, a.groups, a.N, a.K * a.N, g.out_type))
         return cudaErrorInvalidValue;
     m.p = m.o;

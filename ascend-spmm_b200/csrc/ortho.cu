@@ -230,9 +230,13 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
                 tc::make_out_map(&M.gram_out, w.gram, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
                 tc::make_out_map(&M.poly_out, w.poly, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
                 tc::make_out_map(&M.low_out, w.lo, o.n, o.m, o.batch, w.ldx, all, tc::kOutF16);
+    bool blocked_square = false, blocked_x = false;
     for (int i = 0; i < 2 && fine; ++i)   // tall: G reads X down its rows, the update along them; wide: the reverse
-        fine = tc::make_map(&M.square[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tall ? 64 : tc::kBM, false) &&
-               tc::make_map(&M.x[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tall ? tc::kBM : 64, false) &&
+        fine = (tall ? tc::make_mn_map(&M.square[i], &blocked_square, w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false)
+                     : tc::make_map(&M.square[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false)) &&
+               (tall ? tc::make_map(&M.x[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false)
+                     : tc::make_mn_map(&M.x[i], &blocked_x, w.hi[i], o.n, o.m, o.batch, w.ldx, all, pair ? bn / 2 : bn,
+                                       false)) &&
                tc::make_out_map(&M.x_out[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kOutF16);
     M.out = M.x_out[0];
     if (fine && mapped) fine = tc::make_out_map(&M.out, o.out, o.n, o.m, o.batch, o.n, o.m * o.n, tc::kOutBf16);
@@ -252,6 +256,7 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.ldo = w.lds;
         g.out_batch = sq;
         g.alpha = kScaleG / (kScaleX * kScaleX);
+        g.blocked_a = g.blocked_b = blocked_square;
         tc::Maps m{M.square[now], M.square[now], M.gram_out, M.gram_out};
         e = tall ? tc::launch_gemm<tc::kDense, 128, true, true, tc::kGram>(m, g, half, stream)
                  : tc::launch_gemm<tc::kDense, 128, false, false, tc::kGram>(m, g, half, stream);
@@ -281,6 +286,8 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.ldo = last ? o.n : w.ldx;
         g.out_batch = o.m * g.ldo;
         g.out_type = last ? tc::kOutBf16 : tc::kOutF16;
+        g.blocked_a = false;
+        g.blocked_b = blocked_x;
         g.alpha = last ? 1.f / (kScaleP * kScaleX) : 1.f / kScaleP;
         g.beta = last ? o.a / kScaleX : o.a;
         m = tc::Maps{tall ? M.x[now] : M.poly, tall ? M.poly : M.x[now], last ? M.out : M.x_out[next], M.low_out};

@@ -82,6 +82,14 @@ __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, i
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
+// A box of a four-dimensional map.
+__device__ __forceinline__ void tma_load4(unsigned dst, const CUtensorMap *map, int x, int y, int z, int w, unsigned bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map)
 {
     asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
@@ -225,6 +233,14 @@ __device__ __forceinline__ void tma_load_pair(unsigned dst, const CUtensorMap *m
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
                  "[%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load4_pair(unsigned dst, const CUtensorMap *map, int x, int y, int z, int w,
+                                               unsigned bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+                 "[%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
                  : "memory");
 }
 // D over both blocks' TMEM: 256 rows, each block's A 128 of them and its B half of the columns.
