@@ -79,7 +79,7 @@ constexpr int kBM = 128, kBK = 64;
 constexpr int kSumSlices = 8;
 constexpr int kEpiWarps = 8, kGemmThreads = 64 + 32 * kEpiWarps;   // TMA warp, MMA warp, epilogue warps
 
-constexpr int kSorted = 256;   // most groups that a weight gradient sorts
+constexpr int kSorted = 128;   // most groups that a weight gradient sorts
 constexpr int kAsked = 4;      // tiles asked for and not yet done by every warp
 
 template <int BN, bool PAIR = false> struct GemmShape {
@@ -93,7 +93,8 @@ template <int BN, bool PAIR = false> struct GemmShape {
     static constexpr int kAccEmpty = kAccFull + 16, kDone = kAccEmpty + 16, kTmem = kDone + 8, kAbort = kTmem + 4;
     // kRagged: the groups in descending order of length (see Order)
     static constexpr int kOrder = kAbort + 4, kFirst = kOrder + 2 * kSorted, kSlot = kFirst + 4 * (kSorted + 1);
-    static constexpr int kAnswer = (kSlot + 4 * kSorted + 15) / 16 * 16, kAskFull = kAnswer + 16 * kAsked;
+    static constexpr int kBegin = kSlot + 4 * kSorted, kLength = kBegin + 4 * kSorted;
+    static constexpr int kAnswer = (kLength + 4 * kSorted + 15) / 16 * 16, kAskFull = kAnswer + 16 * kAsked;
     static constexpr int kAskEmpty = kAskFull + 8 * kAsked, kBytes = kAskEmpty + 8 * kAsked;
     static constexpr int kCols = 2 * BN;                         // TMEM columns of the two accumulators
     static_assert(kBytes <= 232448, "shared memory of a block");
@@ -166,16 +167,18 @@ struct Order {
     const unsigned short *group;   // [groups], nullptr: not sorted
     const int *first;              // [groups + 1] tiles before the group of this rank
     const int *slot;               // [groups] by group: its first part's slot, -1 with a single part
+    const int *begin, *length;     // [groups] by group: its rows
 };
 
-// Every thread of the block; `length`: kSorted ints of scratch.
+// Every thread of the block.
 __device__ __forceinline__ void sort_groups(const GemmArgs &a, int tiles, unsigned short *group, int *first, int *slot,
-                                            int *length)
+                                            int *begin, int *length)
 {
     const int n = (int)a.ranges.groups, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int g = threadIdx.x; g < n; g += blockDim.x) {
         int64_t b, e;
         segment_rows(a.ranges, g + 1, &b, &e, a.status);
+        begin[g] = (int)b;
         length[g] = (int)(e - b);
     }
     __syncthreads();
@@ -213,10 +216,10 @@ template <int MODE, int EPI, bool PAIR> struct Walk {
     const GemmArgs &a;
     const Order order;
     TileWalk<MODE == kRagged> ranges;
-    int64_t mt, nt;
+    unsigned mt, nt;   // tiles down and across (an output that fits the GPU has fewer than 2^32 tiles)
     int rank = 0;
     __device__ Walk(const GemmArgs &a, const Order &order)
-        : a(a), order(order), mt((a.m + kHeight - 1) / kHeight), nt((a.n + a.bn - 1) / a.bn)
+        : a(a), order(order), mt((unsigned)((a.m + kHeight - 1) / kHeight)), nt((unsigned)((a.n + a.bn - 1) / a.bn))
     {
     }
 
@@ -226,8 +229,8 @@ template <int MODE, int EPI, bool PAIR> struct Walk {
         if constexpr (MODE == kRows) {
             int64_t seg, b, e, inner, slots;
             if (!ranges.find(a.ranges, kHeight, nt, t, a.status, &seg, &b, &e, &inner, &slots)) return false;
-            o->row0 = b + inner / nt * kHeight;
-            o->col0 = inner % nt * a.bn;
+            o->row0 = b + (int64_t)((unsigned)inner / nt) * kHeight;
+            o->col0 = (int64_t)((unsigned)inner % nt) * a.bn;
             o->batch_a = 0;
             o->batch_b = seg - 1;
             o->k0 = 0;
@@ -245,15 +248,17 @@ template <int MODE, int EPI, bool PAIR> struct Walk {
                 seg = order.group[rank] + 1;
                 inner = t - order.first[rank];
                 slots = order.slot[seg - 1];
-                segment_rows(a.ranges, seg, &b, &e, a.status);
-            } else if (!ranges.find(a.ranges, a.part_rows, mt * nt, t, a.status, &seg, &b, &e, &inner, &slots)) {
+                b = order.begin[seg - 1];
+                e = b + order.length[seg - 1];
+            } else if (!ranges.find(a.ranges, a.part_rows, (int64_t)mt * nt, t, a.status, &seg, &b, &e, &inner, &slots)) {
                 return false;
             }
-            const int64_t p = inner / (mt * nt), i = inner % (mt * nt);
+            const int64_t p = (unsigned)inner / (mt * nt);
+            const unsigned i = (unsigned)inner % (mt * nt);
             o->k0 = b + p * a.part_rows;
             o->k1 = min(e, o->k0 + a.part_rows);
-            o->row0 = i / nt * kHeight;
-            o->col0 = i % nt * a.bn;
+            o->row0 = (int64_t)(i / nt) * kHeight;
+            o->col0 = (int64_t)(i % nt) * a.bn;
             o->batch_a = o->batch_b = 0;
             o->rows = (int)min((int64_t)kHeight, a.m - o->row0);
             o->part = slots >= 0;
@@ -265,12 +270,12 @@ template <int MODE, int EPI, bool PAIR> struct Walk {
             o->out_z = o->part ? slots + p : seg - 1;
         } else {
             const bool half = EPI == kGram || EPI == kPoly;   // symmetric: the tiles on and below the diagonal
-            const int64_t per = half ? mt * (mt + 1) / 2 : mt * nt;
+            const unsigned per = half ? mt * (mt + 1) / 2 : mt * nt;
             if (t >= a.batch * per) return false;
-            const int64_t q = t / per, r = t % per;
-            int64_t i, j;
+            const unsigned q = (unsigned)t / per, r = (unsigned)t % per;
+            unsigned i, j;
             if (half) {
-                i = (int64_t)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
+                i = (unsigned)((sqrtf(8.f * (float)r + 1.f) - 1.f) * 0.5f);
                 while (i * (i + 1) / 2 > r) --i;
                 while ((i + 1) * (i + 2) / 2 <= r) ++i;
                 j = r - i * (i + 1) / 2;
@@ -279,8 +284,8 @@ template <int MODE, int EPI, bool PAIR> struct Walk {
                 j = r % nt;
             }
             o->batch_a = o->batch_b = q;
-            o->row0 = i * kHeight;
-            o->col0 = j * a.bn;
+            o->row0 = (int64_t)i * kHeight;
+            o->col0 = (int64_t)j * a.bn;
             o->k0 = 0;
             o->k1 = a.k;
             o->rows = (int)min((int64_t)kHeight, a.m - o->row0);
@@ -370,9 +375,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (a.ranges.groups <= kSorted) {
             unsigned short *group = reinterpret_cast<unsigned short *>(smem + S::kOrder);
             int *first = reinterpret_cast<int *>(smem + S::kFirst), *slot = reinterpret_cast<int *>(smem + S::kSlot);
-            sort_groups(a, (int)((a.m + S::kRows - 1) / S::kRows * ((a.n + a.bn - 1) / a.bn)), group, first, slot,
-                        reinterpret_cast<int *>(smem + S::kStageOff));
-            order = Order{group, first, slot};
+            int *begin = reinterpret_cast<int *>(smem + S::kBegin), *length = reinterpret_cast<int *>(smem + S::kLength);
+            sort_groups(a, (int)((a.m + S::kRows - 1) / S::kRows * ((a.n + a.bn - 1) / a.bn)), group, first, slot, begin,
+                        length);
+            order = Order{group, first, slot, begin, length};
         }
     Walk<MODE, EPI, PAIR> walk(a, order);
     // the columns of B that a slice brings in (MN-major: in blocks of 64), and its bytes

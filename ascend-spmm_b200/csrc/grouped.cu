@@ -163,7 +163,7 @@ int64_t row_tiles_of(const GroupedLaunch &a, int height)
 // rows do not matter: 65536 rows in 64 groups, K = 1024, N = 2048, bf16, 244 us
 // alone and 212 us in pairs with even groups, 253 and 236 us with uneven ones;
 // 100003 rows of 46 groups, K = 128, N = 256 (bound by memory) 18 and 22 us.
-// A weight gradient gained nothing (276 and 281 us) and has no such form.
+// A weight gradient gained almost nothing (274 and 272 us) and has no such form.
 bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
 {
     return g.passes == 1 && g.k >= 512 && g.n % 256 == 0 && a.rows >= 512 * std::max<int64_t>(a.groups, 1) &&
@@ -172,8 +172,10 @@ bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
 
 // Rows of one part of a weight gradient: a group's rows are one reduction
 // unless that leaves SMs idle.  Six units of work per SM bound what an
-// unlucky SM has left at the end; 512 rows are the least that pay for
-// storing and adding a tile in fp32.
+// unlucky SM has left at the end; more, smaller parts cost more than they
+// even out, since each stores its tiles in fp32 and they are read again to be
+// added (65537 uneven rows of 64 groups, K = 1024, N = 2048: parts of 4736
+// rows 272 us, of 2880 rows 346 us).  512 rows are the least.
 int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn)
 {
     const int64_t tiles = ((K + tc::kBM - 1) / tc::kBM) * ((N + bn - 1) / bn);
