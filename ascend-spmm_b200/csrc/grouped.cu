@@ -170,17 +170,21 @@ bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
            a.rows / 256 * (g.n / 256) >= 2 * device_sm_count();
 }
 
-// Rows of one part of a weight gradient: a group's rows are one reduction
-// unless that leaves SMs idle.  Six units of work per SM bound what an
-// unlucky SM has left at the end; more, smaller parts cost more than they
-// even out, since each stores its tiles in fp32 and they are read again to be
-// added (65537 uneven rows of 64 groups, K = 1024, N = 2048: parts of 4736
-// rows 272 us, of 2880 rows 346 us).  512 rows are the least.
-int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn)
+// Rows of one part of a weight gradient.  A group's rows are one reduction
+// unless it would keep one SM busy for longer than the others together: parts
+// of two thirds of an SM's share of the work end within about that much of
+// each other.  More and smaller parts cost more than they even out, since
+// each stores its tiles in fp32 and they are read again to be added; measured
+// with a sixth, two thirds and the whole of the share: 65537 uneven rows of 64
+// groups, K = 1024, N = 2048 413, 331 and 326 us; of 64 even groups, K = N =
+// 512 122, 64 and 64 us; 65536 rows of 8 groups 78, 61 and 83 us.  The least
+// rows that pay: 512, in fp32 (six passes over each) 1024 (20011 rows, K =
+// 256, N = 264: 85 us with 512, 68 us).
+int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn, int dtype)
 {
     const int64_t tiles = ((K + tc::kBM - 1) / tc::kBM) * ((N + bn - 1) / bn);
-    const int64_t even = rows * tiles / (6 * device_sm_count());
-    return (std::max<int64_t>(512, even) + 63) & ~int64_t(63);
+    const int64_t part = rows * tiles * 2 / (3 * device_sm_count());
+    return (std::max<int64_t>(dtype == SPMM_F32 ? 1024 : 512, part) + 63) & ~int64_t(63);
 }
 
 // Equal tiles of at most 256 columns: the reduction is cut where there are
@@ -193,9 +197,9 @@ int weight_grad_columns(int64_t N)
 }
 
 // A group of n > 1 parts has more than (n - 1) part rows, so n <= 2 rows / part.
-int64_t weight_grad_slots(int64_t rows, int64_t K, int64_t N)
+int64_t weight_grad_slots(int64_t rows, int64_t K, int64_t N, int dtype)
 {
-    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N));
+    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N), dtype);
     return rows <= part ? 0 : 2 * rows / part;
 }
 
@@ -316,7 +320,7 @@ cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStr
 size_t grouped_weight_grad_workspace(int64_t rows, int64_t groups, int64_t K, int64_t N, int dtype)
 {
     (void)groups;
-    const size_t parts = (size_t)weight_grad_slots(rows, K, N) * K * N * sizeof(float);
+    const size_t parts = (size_t)weight_grad_slots(rows, K, N, dtype) * K * N * sizeof(float);
     return parts + (dtype == SPMM_F32 ? plane_bytes(rows * K) + plane_bytes(rows * N) : 0);
 }
 
@@ -332,8 +336,8 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
     g.status = a.status;
     set_types(g, a.dtype);
     g.bn = weight_grad_columns(a.N);
-    g.part_rows = weight_grad_part(a.rows, a.K, a.N, g.bn);
-    const int64_t slots = weight_grad_slots(a.rows, a.K, a.N);
+    g.part_rows = weight_grad_part(a.rows, a.K, a.N, g.bn, a.dtype);
+    const int64_t slots = weight_grad_slots(a.rows, a.K, a.N, a.dtype);
     const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: never read
     char *ws = static_cast<char *>(workspace);
     if (a.dtype == SPMM_F32 && a.rows > 0) {
