@@ -74,10 +74,11 @@ struct GemmArgs {
     bool blocked_a, blocked_b;
     // kGram: x = alpha * accumulator; kPoly, kUpdate: x = alpha * accumulator
     // + beta * (in + in_lo), `in` laid out as the output.  kGram and kPoly
-    // are symmetric and also write the transposed tile; kUpdate writes x as
-    // fp16 and, with `low`, the rest that the rounding left through the
+    // are symmetric and, with `symmetric`, compute one of two mirrored tiles
+    // and write it twice; kUpdate writes x as fp16 and, with `low`, the rest that the rounding left through the
     // second output map (else x alone, in the output's type).
     float alpha, beta;
+    bool symmetric;           // kGram, kPoly: only the tiles on and below the diagonal (bn == 128)
     const __half *in, *in_lo;
     bool low;
     int64_t ldi, in_batch;
@@ -278,7 +279,7 @@ template <int MODE, int EPI, bool PAIR> struct Walk {
             o->out_row = o->row0;
             o->out_z = o->part ? slots + p : seg - 1;
         } else {
-            const bool half = EPI == kGram || EPI == kPoly;   // symmetric: the tiles on and below the diagonal
+            const bool half = a.symmetric;   // the tiles on and below the diagonal
             const unsigned per = half ? mt * (mt + 1) / 2 : mt * nt;
             if (t >= a.batch * per) return false;
             const unsigned q = (unsigned)t / per, r = (unsigned)t % per;

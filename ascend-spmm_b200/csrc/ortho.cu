@@ -23,6 +23,7 @@
 // products.  Three of 601 x 1023 152 us: fifteen dependent products of 8 to 12
 // us, of which the reduction's slices are 2 to 4.
 #include <algorithm>
+#include <climits>
 
 #include "../../include/spmm_b200.h"
 #include "common.cuh"
@@ -159,12 +160,51 @@ template <typename T> void start(const OrthoLaunch &o, const Space &w, cudaStrea
         o.steps == 0 ? static_cast<__nv_bfloat16 *>(o.out) : nullptr);
 }
 
+// Columns of a tile of a symmetric product.  In tiles of 128 x 128 one of two
+// mirrored ones is computed and stored twice; where narrower tiles of the
+// whole square fit one turn of the GPU, their shorter products and single
+// store win (1024 x 1024: 231 us in halves, 161 with 64 columns; 5 of 512 x
+// 512: 125 and, with 96, 121; but 2 of 1024 x 1024, more than one turn, 158
+// and 179).
+int square_columns(int64_t row_tiles, int64_t side, int sms)
+{
+    for (int bn : {64, 96})
+        if (row_tiles * ((side + bn - 1) / bn) <= sms) return bn;
+    return 128;
+}
+
+// Columns of an update's tile: the width with the least turns x time, a slice
+// of a tile taking about as long as 70 + bn columns.  12 of 700 x 700: 240 us
+// with 128 (3 turns), 259 with 256 (2); 30 of 200 x 900: 220 (4) and 210 (2);
+// 601 x 1000: 134 and, with 64, 124 (one turn each).
+int update_columns(int64_t row_tiles, int64_t width, int sms)
+{
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int bn : {64, 96, 128, 256}) {
+        const int64_t cost = (row_tiles * ((width + bn - 1) / bn) + sms - 1) / sms * (bn + 70);
+        if (cost < least) {
+            least = cost;
+            best = bn;
+        }
+    }
+    return best;
+}
+
 // The tensor maps of a call, each encoded once.
 struct OrthoMaps {
     CUtensorMap square[2], x[2];            // X as the operands of G and of the update, by buffer
+    CUtensorMap square_b[2], gram_b;        // the second operand of G and of G G: tiles of another width
     CUtensorMap gram, poly;                 // G and P as operands
     CUtensorMap gram_out, poly_out, x_out[2], low_out, out;
 };
+
+template <int BN>
+cudaError_t gram(bool tall, const tc::Maps &m, const tc::GemmArgs &g, int64_t tiles, cudaStream_t stream)
+{
+    return tall ? tc::launch_gemm<tc::kDense, BN, true, true, tc::kGram>(m, g, tiles, stream)
+                : tc::launch_gemm<tc::kDense, BN, false, false, tc::kGram>(m, g, tiles, stream);
+}
 
 template <int BN, bool PAIR = false>
 cudaError_t update(const OrthoLaunch &o, const tc::Maps &m, const tc::GemmArgs &g, cudaStream_t stream)
@@ -220,26 +260,34 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
     if (e != cudaSuccess || o.steps == 0) return e;
     const bool tall = o.m > o.n;
     const int64_t side = std::min(o.m, o.n), long_side = std::max(o.m, o.n), sq = side * w.lds, all = o.m * w.ldx;
-    const int64_t mt = (side + tc::kBM - 1) / tc::kBM, half = o.batch * mt * (mt + 1) / 2;
-    // columns of an update's tile
-    const int64_t row_tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM);
     const int sms = device_sm_count();
-    const int bn = o.n > 128 && row_tiles * ((o.n + 255) / 256) >= sms  ? 256
-                   : o.n > 64 && row_tiles * ((o.n + 127) / 128) >= sms ? 128
-                                                                        : 64;
-    const bool pair = bn == 256;   // 4096 x 2048: 373 us alone, 362 in pairs; 4096 x 4096: 1360 and 1259
+    const int64_t mt = (side + tc::kBM - 1) / tc::kBM;
+    const int square_bn = square_columns(o.batch * mt, side, sms);
+    const bool whole = square_bn < tc::kBM;
+    const int64_t square_tiles = whole ? o.batch * mt * ((side + square_bn - 1) / square_bn) : o.batch * mt * (mt + 1) / 2;
+    const int64_t row_tiles = o.batch * ((o.m + tc::kBM - 1) / tc::kBM);
+    const int bn = update_columns(row_tiles, o.n, sms);
+    // Two SMs share a tile where the products are deep and take several turns
+    // (4 of 2048 x 2048: 879 us alone, 780 in pairs; 4096 x 4096: 1572 and
+    // 1332; but 3 of 1024 x 4096: 369 and 381, one 2048 x 2048: 245 and 252).
+    const bool pair = bn == 256 && side > 1024 && row_tiles * ((o.n + 255) / 256) > sms;
     // a result whose rows do not start on 16 bytes has no map
     const bool mapped = (o.n & 7) == 0;
     OrthoMaps M;
     bool fine = tc::make_map(&M.gram, w.gram, side, side, o.batch, w.lds, sq, tc::kBM, false) &&
+                tc::make_map(&M.gram_b, w.gram, side, side, o.batch, w.lds, sq, square_bn, false) &&
                 tc::make_map(&M.poly, w.poly, side, side, o.batch, w.lds, sq, tall ? pair ? bn / 2 : bn : tc::kBM, false) &&
                 tc::make_out_map(&M.gram_out, w.gram, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
                 tc::make_out_map(&M.poly_out, w.poly, side, side, o.batch, w.lds, sq, tc::kOutF16) &&
                 tc::make_out_map(&M.low_out, w.lo, o.n, o.m, o.batch, w.ldx, all, tc::kOutF16);
-    bool blocked_square = false, blocked_x = false;
+    bool blocked_square = false, blocked_square_b = false, blocked_x = false;
     for (int i = 0; i < 2 && fine; ++i)   // tall: G reads X down its rows, the update along them; wide: the reverse
-        fine = (tall ? tc::make_mn_map(&M.square[i], &blocked_square, w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false)
-                     : tc::make_map(&M.square[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false)) &&
+        fine = (tall ? tc::make_mn_map(&M.square[i], &blocked_square, w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM,
+                                       false) &&
+                           tc::make_mn_map(&M.square_b[i], &blocked_square_b, w.hi[i], o.n, o.m, o.batch, w.ldx, all,
+                                           square_bn, false)
+                     : tc::make_map(&M.square[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false) &&
+                           tc::make_map(&M.square_b[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, square_bn, false)) &&
                (tall ? tc::make_map(&M.x[i], w.hi[i], o.n, o.m, o.batch, w.ldx, all, tc::kBM, false)
                      : tc::make_mn_map(&M.x[i], &blocked_x, w.hi[i], o.n, o.m, o.batch, w.ldx, all, pair ? bn / 2 : bn,
                                        false)) &&
@@ -257,15 +305,16 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         // G = X X^T (X^T X)
         g.m = g.n = side;
         g.k = long_side;
-        g.bn = 128;
+        g.bn = square_bn;
         g.out = w.gram;
         g.ldo = w.lds;
         g.out_batch = sq;
         g.alpha = kScaleG / (kScaleX * kScaleX);
-        g.blocked_a = g.blocked_b = blocked_square;
-        tc::Maps m{M.square[now], M.square[now], M.gram_out, M.gram_out};
-        e = tall ? tc::launch_gemm<tc::kDense, 128, true, true, tc::kGram>(m, g, half, stream)
-                 : tc::launch_gemm<tc::kDense, 128, false, false, tc::kGram>(m, g, half, stream);
+        g.symmetric = !whole;
+        g.blocked_a = blocked_square;
+        g.blocked_b = blocked_square_b;
+        tc::Maps m{M.square[now], M.square_b[now], M.gram_out, M.gram_out};
+        e = square_bn == 64 ? gram<64>(tall, m, g, square_tiles, stream) : gram<128>(tall, m, g, square_tiles, stream);
         if (e != cudaSuccess) break;
         // P = b G + c G G
         g.k = side;
@@ -275,11 +324,14 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.out = w.poly;
         g.alpha = o.c * (kScaleP / (kScaleG * kScaleG));
         g.beta = o.b * (kScaleP / kScaleG);
-        m = tc::Maps{M.gram, M.gram, M.poly_out, M.poly_out};
-        e = tc::launch_gemm<tc::kDense, 128, false, false, tc::kPoly>(m, g, half, stream);
+        m = tc::Maps{M.gram, M.gram_b, M.poly_out, M.poly_out};
+        e = square_bn == 64
+                ? tc::launch_gemm<tc::kDense, 64, false, false, tc::kPoly>(m, g, square_tiles, stream)
+                : tc::launch_gemm<tc::kDense, 128, false, false, tc::kPoly>(m, g, square_tiles, stream);
         if (e != cudaSuccess) break;
         // X <- a X + P X (X P); the last step writes the result
         const bool last = i + 1 == o.steps;
+        g.symmetric = false;
         g.m = o.m;
         g.n = o.n;
         g.bn = bn;
@@ -298,8 +350,8 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.beta = last ? o.a / kScaleX : o.a;
         m = tc::Maps{tall ? M.x[now] : M.poly, tall ? M.poly : M.x[now], last ? M.out : M.x_out[next], M.low_out};
         if (pair) e = update<256, true>(o, m, g, stream);
-        else if (bn == 256) e = update<256>(o, m, g, stream);
-        else if (bn == 128) e = update<128>(o, m, g, stream);
+        else if (bn > 128) e = update<256>(o, m, g, stream);
+        else if (bn > 64) e = update<128>(o, m, g, stream);
         else e = update<64>(o, m, g, stream);
     }
     return e;
