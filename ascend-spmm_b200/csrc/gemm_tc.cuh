@@ -46,10 +46,13 @@ namespace spmmb {
 namespace tc {
 
 enum Mode { kRows, kRagged, kDense };
-// kStoreSum: fp32 products.  The tensor core truncates each step into its
-// accumulator, which adds up to 1e-6 over 100 steps; so an accumulator takes
-// kSumSlices slices and the epilogue warps add them in registers, rounding to
-// nearest.  The others but kStore are kDense's: see ortho.cu.
+// kStoreSum: fp32 operands in three bf16 planes h, m, l each.  A slice brings
+// in the planes once, a ring stage each, for its six products h l, l h, m m,
+// h m, m h and h h.  The tensor core truncates each step into its accumulator,
+// so an accumulator takes one slice, the smallest products first, and the
+// epilogue warps add the slices in registers, rounding to nearest (K = 4096:
+// error 1.4e-7, with two slices 5e-7 and 6 % less time, with four 1.2e-6).
+// The others but kStore are kDense's: see ortho.cu.
 enum Epi { kStore, kStoreSum, kGram, kPoly, kUpdate };
 enum OutType { kOutF16, kOutBf16, kOutF32 };
 
@@ -64,10 +67,7 @@ struct GemmArgs {
     int64_t ldo, out_batch;   // elements
     int out_type;
     bool bf16;                // operand type (else fp16)
-    // The reduction is run `passes` times over planes pa[i], pb[i] of the
-    // operands (plane p of A starts at batch index p * za, of B at p * zb).
-    int passes, za, zb;
-    unsigned char pa[6], pb[6];
+    int za, zb;               // kStoreSum: plane p of A starts at batch index p * za, of B at p * zb
     // MN-major operands whose map has the blocks of 64 rows or columns as a
     // dimension (make_blocked_map): a slice is one copy instead of one per
     // block, and the issuing lane keeps up with the tensor core
@@ -75,8 +75,9 @@ struct GemmArgs {
     // kGram: x = alpha * accumulator; kPoly, kUpdate: x = alpha * accumulator
     // + beta * (in + in_lo), `in` laid out as the output.  kGram and kPoly
     // are symmetric and, with `symmetric`, compute one of two mirrored tiles
-    // and write it twice; kUpdate writes x as fp16 and, with `low`, the rest that the rounding left through the
-    // second output map (else x alone, in the output's type).
+    // and write it twice; kUpdate writes x as fp16 and, with `low`, the rest
+    // that the rounding left through the second output map (else x alone, in
+    // the output's type).
     float alpha, beta;
     bool symmetric;           // kGram, kPoly: only the tiles on and below the diagonal (bn == 128)
     const __half *in, *in_lo;
@@ -86,7 +87,6 @@ struct GemmArgs {
 };
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kSumSlices = 8;
 constexpr int kEpiWarps = 8, kGemmThreads = 64 + 32 * kEpiWarps;   // TMA warp, MMA warp, epilogue warps
 
 constexpr int kSorted = 128;   // most groups that a weight gradient sorts
@@ -326,6 +326,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 {
     static_assert(!PAIR || MODE != kRagged, "a group's zeros are written by one block");
     using S = GemmShape<BN, PAIR>;
+    constexpr int kParts = EPI == kStoreSum ? 3 : 1;   // ring stages of a slice
+    static_assert(S::kStages >= 2 * kParts, "a slice arrives while another is multiplied");
     extern __shared__ __align__(1024) unsigned char smem[];
     const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -415,49 +417,48 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const int n = (int)((t.k1 - t.k0 + kBK - 1) / kBK);
             if (elect()) {
                 const int row0 = (int)t.row0, col0 = (int)t.col0 + (PAIR ? (int)peer * b_cols : 0);
-                const int sum = EPI == kStoreSum ? kSumSlices : n;
                 unsigned at = slice;
-                for (int s0 = 0; s0 < n && ok; s0 += sum)
-                    for (int pass = 0; pass < a.passes && ok; ++pass) {
-                        const int za = (int)t.batch_a + a.pa[pass] * a.za, zb = (int)t.batch_b + a.pb[pass] * a.zb;
-                        int k = (int)t.k0 + s0 * kBK;
-                        for (int i = s0; i < min(s0 + sum, n); ++i, ++at, k += kBK) {
-                            const unsigned st = at % S::kStages;
-                            if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
-                            const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA;
-                            // a pair's slice, both halves, arrives on the first block's barrier
-                            const unsigned bar = PAIR ? in_block(full + 8 * st, 0) : full + 8 * st;
-                            if (peer == 0) bar_expect(full + 8 * st, PAIR ? 2 * slice_bytes : slice_bytes);
-                            auto load = [&](unsigned dst, const CUtensorMap *map, int x, int y, int z) {
-                                if constexpr (PAIR) tma_load_pair(dst, map, x, y, z, bar);
-                                else tma_load(dst, map, x, y, z, bar);
-                            };
-                            auto load_blocks = [&](unsigned dst, const CUtensorMap *map, int x, int z) {
-                                if constexpr (PAIR) tma_load4_pair(dst, map, 0, k, x / 64, z, bar);
-                                else tma_load4(dst, map, 0, k, x / 64, z, bar);
-                            };
-                            if (!AMN) {
-                                load(sa, &map_a, k, row0, za);
-                            } else if (a.blocked_a) {
-                                load_blocks(sa, &map_a, row0, za);
-                            } else {
+                int k = (int)t.k0;
+                for (int i = 0; i < n && ok; ++i, k += kBK)
 #pragma unroll
-                                for (int c = 0; c < kBM / 64; ++c) load(sa + c * 8192, &map_a, row0 + 64 * c, k, za);
-                            }
-                            if (!BMN) {
-                                load(sb, &map_b, k, col0, zb);
-                            } else if (a.blocked_b) {
-                                load_blocks(sb, &map_b, col0, zb);
-                            } else {
+                    for (int j = 0; j < kParts; ++j, ++at) {
+                        const int plane = kParts == 1 ? 0 : (j + 2) % 3;   // l, h, m: l is done with first
+                        const int za = (int)t.batch_a + plane * a.za, zb = (int)t.batch_b + plane * a.zb;
+                        const unsigned st = at % S::kStages;
+                        if (!bar_wait(empty + 8 * st, (at / S::kStages & 1u) ^ 1u, abort)) { give_up(1); break; }
+                        const unsigned sa = base + st * (S::kA + S::kB), sb = sa + S::kA;
+                        // a pair's slice, both halves, arrives on the first block's barrier
+                        const unsigned bar = PAIR ? in_block(full + 8 * st, 0) : full + 8 * st;
+                        if (peer == 0) bar_expect(full + 8 * st, PAIR ? 2 * slice_bytes : slice_bytes);
+                        auto load = [&](unsigned dst, const CUtensorMap *map, int x, int y, int z) {
+                            if constexpr (PAIR) tma_load_pair(dst, map, x, y, z, bar);
+                            else tma_load(dst, map, x, y, z, bar);
+                        };
+                        auto load_blocks = [&](unsigned dst, const CUtensorMap *map, int x, int z) {
+                            if constexpr (PAIR) tma_load4_pair(dst, map, 0, k, x / 64, z, bar);
+                            else tma_load4(dst, map, 0, k, x / 64, z, bar);
+                        };
+                        if (!AMN) {
+                            load(sa, &map_a, k, row0, za);
+                        } else if (a.blocked_a) {
+                            load_blocks(sa, &map_a, row0, za);
+                        } else {
 #pragma unroll
-                                for (int c = 0; c < BN / 64; ++c)
-                                    if (c < b_blocks) load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb);
-                            }
+                            for (int c = 0; c < kBM / 64; ++c) load(sa + c * 8192, &map_a, row0 + 64 * c, k, za);
+                        }
+                        if (!BMN) {
+                            load(sb, &map_b, k, col0, zb);
+                        } else if (a.blocked_b) {
+                            load_blocks(sb, &map_b, col0, zb);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < BN / 64; ++c)
+                                if (c < b_blocks) load(sb + c * 8192, &map_b, col0 + 64 * c, k, zb);
                         }
                     }
             }
             __syncwarp();
-            slice += a.passes * n;
+            slice += kParts * n;
             ok = *abort == 0;
         }
         if (!ok) {   // copies and an answer in flight land before the block leaves (bounded; one never issued runs out)
@@ -477,7 +478,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         const uint64_t db = BMN ? desc128(base + S::kA, 8192, 1024) : desc128(base + S::kA, 16, 1024);
         constexpr unsigned step_a = (AMN ? 2048 : 32) >> 4, step_b = (BMN ? 2048 : 32) >> 4;
         unsigned slice = 0, used = 0;
-        // The products of the slice at position `at` (depth elements deep).
         auto mul = [&](unsigned d, uint64_t x, uint64_t y, unsigned add) {
             if constexpr (PAIR) mma_pair(d, x, y, idesc, add);
             else mma(d, x, y, idesc, add);
@@ -486,20 +486,44 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             if constexpr (PAIR) commit_pair(bar);
             else commit(bar);
         };
-        auto multiply = [&](unsigned at, int depth, unsigned d, bool first) {
-            const unsigned st = at % S::kStages, off = st * (S::kA + S::kB) >> 4;
+        auto product = [&](unsigned at_a, unsigned at_b, int depth, unsigned d, bool first) {
+            const unsigned off_a = at_a % S::kStages * (S::kA + S::kB) >> 4;
+            const unsigned off_b = at_b % S::kStages * (S::kA + S::kB) >> 4;
             if (depth == kBK) {
 #pragma unroll
                 for (int i = 0; i < kBK / 16; ++i)
-                    mul(d, da + off + i * step_a, db + off + i * step_b, first && i == 0 ? 0u : 1u);
+                    mul(d, da + off_a + i * step_a, db + off_b + i * step_b, first && i == 0 ? 0u : 1u);
             } else {
                 for (int i = 0; i * 16 < depth; ++i)
-                    mul(d, da + off + i * step_a, db + off + i * step_b, first && i == 0 ? 0u : 1u);
+                    mul(d, da + off_a + i * step_a, db + off_b + i * step_b, first && i == 0 ? 0u : 1u);
             }
-            finish(empty + 8 * st);
         };
         auto landed = [&](unsigned at) {
             return bar_wait<PAIR>(full + 8 * (at % S::kStages), at / S::kStages & 1u, abort);
+        };
+        auto release = [&](unsigned at) { finish(empty + 8 * (at % S::kStages)); };
+        // The products of the slice at ring position `at` (depth elements deep);
+        // false if a wait ran out.
+        auto multiply = [&](unsigned at, int depth, unsigned d, bool first) {
+            if constexpr (kParts == 1) {
+                if (!landed(at)) return false;
+                product(at, at, depth, d, first);
+                release(at);
+            } else {   // the smallest first
+                const unsigned l = at, h = at + 1, m = at + 2;
+                if (!landed(l) || !landed(h)) return false;
+                product(h, l, depth, d, first);
+                product(l, h, depth, d, false);
+                release(l);
+                if (!landed(m)) return false;
+                product(m, m, depth, d, false);
+                product(h, m, depth, d, false);
+                product(m, h, depth, d, false);
+                product(h, h, depth, d, false);
+                release(h);
+                release(m);
+            }
+            return true;
         };
         Turns<MODE, BN, PAIR> turns(base, abort, false);
         for (; ok && turns.tile >= 0; turns.next() ? void() : give_up(5)) {
@@ -512,7 +536,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // kRagged: a last slice that ends within 16 rows needs the whole warp
             const bool ragged = MODE == kRagged && (depth & 15);
             const int whole = ragged ? n - 1 : n;
-            const int sum = EPI == kStoreSum ? kSumSlices : n;
+            const int sum = EPI == kStoreSum ? 1 : n;   // slices of an accumulator
             for (int s0 = 0; s0 < n && ok; s0 += sum, ++used) {
                 const unsigned d = tmem + (used & 1u) * BN;
                 if (peer == 0 && !bar_wait<PAIR>(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) {
@@ -521,27 +545,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 }
                 fence_after();
                 const int s1 = min(s0 + sum, n);
-                for (int pass = 0; pass < a.passes; ++pass, slice += s1 - s0) {
-                    if (peer == 0 && elect())
-                        for (int i = s0; i < min(s1, whole); ++i) {
-                            if (!landed(slice + i - s0)) { give_up(3); break; }
-                            multiply(slice + i - s0, min(kBK, depth - i * kBK), d, pass == 0 && i == s0);
+                if (peer == 0 && elect())
+                    for (int i = s0; i < min(s1, whole); ++i)
+                        if (!multiply(slice + kParts * (i - s0), min(kBK, depth - i * kBK), d, i == s0)) {
+                            give_up(3);
+                            break;
                         }
-                    __syncwarp();
-                    if (ragged && s1 == n && *abort == 0) {
-                        const unsigned at = slice + s1 - s0 - 1, st = at % S::kStages;
-                        if (!landed(at)) give_up(3);
-                        // the rows past the group's end, up to the next multiple of 16, of both operands: zero
-                        const unsigned buf = base + st * (S::kA + S::kB);
-                        const int deep = depth - (n - 1) * kBK;
-                        const int quads = (16 - (deep & 15)) * 8;   // 16-byte pieces of a 64-wide column block
+                __syncwarp();
+                slice += kParts * (s1 - s0);
+                if (ragged && s1 == n && *abort == 0) {
+                    const unsigned at = slice - kParts;
+                    // the rows past the group's end, up to the next multiple of 16, of both operands: zero
+                    const int deep = depth - (n - 1) * kBK;
+                    const int quads = (16 - (deep & 15)) * 8;   // 16-byte pieces of a 64-wide column block
+                    for (int p = 0; p < kParts; ++p) {
+                        if (!landed(at + p)) give_up(3);
+                        const unsigned buf = base + (at + p) % S::kStages * (S::kA + S::kB);
                         for (int i = lane; i < quads * (S::kA / 8192 + b_blocks); i += 32)
                             st_shared16(buf + i / quads * 8192 + deep * 128 + i % quads * 16, make_uint4(0, 0, 0, 0));
-                        fence_async();
-                        __syncwarp();
-                        if (elect()) multiply(at, deep, d, pass == 0 && n - 1 == s0);
-                        __syncwarp();
                     }
+                    fence_async();
+                    __syncwarp();
+                    if (elect() && !multiply(at, deep, d, n - 1 == s0)) give_up(3);
+                    __syncwarp();
                 }
                 ok = *abort == 0;
                 if (!ok) break;
@@ -713,7 +739,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 for (int b = 0; b < BN / 64; ++b)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[b][i] = 0.f;
-                for (int s0 = 0; s0 < n; s0 += kSumSlices) {
+                for (int i = 0; i < n; ++i) {
                     const unsigned from = take();
                     if (!ok) break;
 #pragma unroll
@@ -723,7 +749,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                             float w[32];
                             tmem_ld32(from + c, w);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[b][i] += w[i];
+                            for (int e = 0; e < 32; ++e) v[b][e] += w[e];
                         }
                     }
                     give_back();
@@ -795,11 +821,11 @@ bool make_out_map(CUtensorMap *map, void *p, int64_t inner, int64_t rows, int64_
 
 // Launch that lets the kernel's set-up overlap the kernel before it.
 template <typename K, typename... A>
-cudaError_t launch_overlapped(K kernel, unsigned grid, unsigned cluster, int threads, int smem, cudaStream_t stream,
+cudaError_t launch_overlapped(K kernel, dim3 grid, unsigned cluster, int threads, int smem, cudaStream_t stream,
                               const A &...args)
 {
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
+    config.gridDim = grid;
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;

@@ -10,7 +10,7 @@
 // uneven rows of 64 groups, K = 1024, N = 2048 236, 231, 267 (275 GFLOP each:
 // the products, at the power limit's clock); fp16, 100003 rows of 46 groups, K
 // = 256, N = 128 16, 18, 27 (77 MB each: memory, and for the weight the parts);
-// fp32, 20011 rows of 8 groups, K = 256, N = 264 51, 55, 70 (about 17 of each
+// fp32, 20011 rows of 8 groups, K = 256, N = 264 39, 40, 56 (12 to 20 of each
 // is splitting the operands); bf16, 9 rows of 32 groups, K = 1024, N = 512 10,
 // half of it the fixed cost of a launch, its first copies and its last store.
 #include <algorithm>
@@ -39,9 +39,11 @@ __host__ __device__ Ranges ranges_of(const GroupedLaunch &a)
 // exponents) and the product is run as the six plane products above 2^-24 of
 // the result, the smallest first:  h l, l h, m m, h m, m h, h h.  That is six
 // bf16 products, about four times the rate of fp32 FMAs.  An infinite x has
-// zero m and l planes; its products with zero planes are NaN.
-constexpr int kPlanes = 3, kPasses = 6;
-constexpr unsigned char kPassA[kPasses] = {0, 2, 1, 0, 1, 0}, kPassB[kPasses] = {2, 0, 1, 1, 0, 0};
+// zero m and l planes; its products with zero planes are NaN.  The six
+// products share a slice's planes in shared memory: bringing each product's
+// two operands in by themselves took half as long again (51, 55 and 69 us for
+// 39, 40 and 56 in the case above), bound by those copies.
+constexpr int kPlanes = 3;
 
 // An operand to split: src [groups][elems], planes `plane` apart.  `skip`:
 // groups without rows are left out.
@@ -102,16 +104,20 @@ size_t plane_bytes(int64_t elems) { return ((size_t)elems * kPlanes * 2 + 255) &
 
 // ---- launches --------------------------------------------------------------
 
-// Columns per tile (a multiple of 16 of at most 256): the cut into equal
+// The widest tile: of fp32's planes two slices fit the ring with 128 columns.
+constexpr int kWidest = 256, kWidestSum = 128;
+int widest(int dtype) { return dtype == SPMM_F32 ? kWidestSum : kWidest; }
+
+// Columns per tile (a multiple of 16 of at most `most`): the cut into equal
 // tiles with the least turns x time.  A 64-deep slice of a tile takes about
 // as long as 70 + bn columns (0.19 us at 64, 0.46 us at 256): its rows are
 // read however narrow it is.
-int tile_columns(int64_t row_tiles, int64_t width)
+int tile_columns(int64_t row_tiles, int64_t width, int most)
 {
     const int64_t sms = device_sm_count();
     int best = 0;
     int64_t least = INT64_MAX;
-    for (int64_t n = (width + 255) / 256; n <= (width + 63) / 64; ++n) {
+    for (int64_t n = (width + most - 1) / most; n <= (width + 63) / 64; ++n) {
         const int64_t step = n > 1 ? 32 : 16;   // a tile is stored 32 columns at a time
         const int64_t bn = ((width + n - 1) / n + step - 1) / step * step;
         const int64_t cost = (row_tiles * n + sms - 1) / sms * (bn + 70);
@@ -129,11 +135,6 @@ void set_types(tc::GemmArgs &g, int dtype)
     const bool f32 = dtype == SPMM_F32;
     g.bf16 = f32 || dtype == SPMM_BF16;
     g.out_type = f32 ? tc::kOutF32 : g.bf16 ? tc::kOutBf16 : tc::kOutF16;
-    g.passes = f32 ? kPasses : 1;
-    if (f32) {
-        std::copy(kPassA, kPassA + kPasses, g.pa);
-        std::copy(kPassB, kPassB + kPasses, g.pb);
-    }
 }
 
 template <int BN, bool PAIR = false>
@@ -141,7 +142,7 @@ cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::Ge
                     cudaStream_t stream)
 {
     tc::Maps m;
-    const int64_t planes = g.passes > 1 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
+    const int64_t planes = a.dtype == SPMM_F32 ? kPlanes : 1, groups = std::max<int64_t>(a.groups, 1);
     const int64_t tiles = row_tiles * ((g.n + g.bn - 1) / g.bn);
     const int cols = PAIR ? BN / 2 : g.bn;   // of the weight that a block brings in
     if (!tc::make_map(&m.a, x, g.k, a.rows, planes, g.k, a.rows * g.k, tc::kBM, g.bf16) ||
@@ -151,8 +152,8 @@ cudaError_t rows_tc(const GroupedLaunch &a, const void *x, const void *w, tc::Ge
         !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
         return cudaErrorInvalidValue;
     m.p = m.o;
-    if constexpr (!PAIR)
-        if (g.passes > 1)
+    if constexpr (BN <= kWidestSum)
+        if (a.dtype == SPMM_F32)
             return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStoreSum>(m, g, tiles, stream)
                                 : tc::launch_gemm<tc::kRows, BN, false, true, tc::kStoreSum>(m, g, tiles, stream);
     return a.transposed ? tc::launch_gemm<tc::kRows, BN, false, false, tc::kStore, PAIR>(m, g, tiles, stream)
@@ -174,7 +175,7 @@ int64_t row_tiles_of(const GroupedLaunch &a, int height)
 // A weight gradient gained almost nothing (274 and 272 us) and has no such form.
 bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
 {
-    return g.passes == 1 && g.k >= 512 && g.n % 256 == 0 && a.rows >= 512 * std::max<int64_t>(a.groups, 1) &&
+    return a.dtype != SPMM_F32 && g.k >= 512 && g.n % 256 == 0 && a.rows >= 512 * std::max<int64_t>(a.groups, 1) &&
            a.rows / 256 * (g.n / 256) >= 2 * device_sm_count();
 }
 
@@ -186,20 +187,22 @@ bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
 // with a sixth, two thirds and the whole of the share: 65537 uneven rows of 64
 // groups, K = 1024, N = 2048 413, 331 and 326 us; of 64 even groups, K = N =
 // 512 122, 64 and 64 us; 65536 rows of 8 groups 78, 61 and 83 us.  The least
-// rows that pay: 512, in fp32 (six passes over each) 1024 (20011 rows, K =
-// 256, N = 264: 85 us with 512, 68 us).
+// rows that pay: 512, in fp32 (six products of each) 384 (4000 rows of 3
+// groups, K = N = 256: 35 us with 1024, 25 us; 20000 rows of 8 groups, K = N =
+// 128: 43 and 35 us; 20011 rows of 8 groups, K = 256, N = 264: 55 and 57 us).
 int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn, int dtype)
 {
     const int64_t tiles = ((K + tc::kBM - 1) / tc::kBM) * ((N + bn - 1) / bn);
     const int64_t part = rows * tiles * 2 / (3 * device_sm_count());
-    return (std::max<int64_t>(dtype == SPMM_F32 ? 1024 : 512, part) + 63) & ~int64_t(63);
+    return (std::max<int64_t>(dtype == SPMM_F32 ? 384 : 512, part) + 63) & ~int64_t(63);
 }
 
-// Equal tiles of at most 256 columns: the reduction is cut where there are
+// Equal tiles of the greatest width: the reduction is cut where there are
 // too few of them, so they need not be narrower.
-int weight_grad_columns(int64_t N)
+int weight_grad_columns(int64_t N, int dtype)
 {
-    const int64_t n = (N + 255) / 256;
+    const int most = widest(dtype);
+    const int64_t n = (N + most - 1) / most;
     const int64_t step = n > 1 ? 32 : 16;   // a tile is stored 32 columns at a time
     return (int)(((N + n - 1) / n + step - 1) / step * step);
 }
@@ -207,7 +210,7 @@ int weight_grad_columns(int64_t N)
 // A group of n > 1 parts has more than (n - 1) part rows, so n <= 2 rows / part.
 int64_t weight_grad_slots(int64_t rows, int64_t K, int64_t N, int dtype)
 {
-    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N), dtype);
+    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N, dtype), dtype);
     return rows <= part ? 0 : 2 * rows / part;
 }
 
@@ -217,6 +220,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const float *parts, T *o
                                                         int64_t slots, Ranges ranges, DevStatus *status)
 {
     __shared__ int64_t before;
+    tc::wait_for_earlier_kernels();
     for (int64_t g = blockIdx.y; g < ranges.groups; g += gridDim.y) {
         auto parts_of = [&](int64_t group) {
             int64_t b, e;
@@ -261,9 +265,8 @@ template <typename T> cudaError_t add_parts(const GroupedLaunch &a, const float 
     const int64_t per = std::max<int64_t>(1, 16 * device_sm_count() / a.groups);
     const unsigned blocks = (unsigned)std::min((elems + 1023) / 1024, per);
     const dim3 grid(blocks, (unsigned)std::min<int64_t>(a.groups, 65535));
-    add_parts_kernel<T><<<grid, 256, 0, stream>>>(parts, static_cast<T *>(a.out), elems, g.part_rows, g.part_slots,
-                                                  g.ranges, a.status);
-    return cudaGetLastError();
+    return tc::launch_overlapped(add_parts_kernel<T>, grid, 1, 256, 0, stream, parts, static_cast<T *>(a.out), elems,
+                                 g.part_rows, g.part_slots, g.ranges, a.status);
 }
 
 template <int BN>
@@ -271,7 +274,7 @@ cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy
                            cudaStream_t stream)
 {
     tc::Maps m;
-    const int64_t planes = g.passes > 1 ? kPlanes : 1, rows = std::max<int64_t>(a.rows, 1);
+    const int64_t planes = a.dtype == SPMM_F32 ? kPlanes : 1, rows = std::max<int64_t>(a.rows, 1);
     if (!tc::make_mn_map(&m.a, &g.blocked_a, x, a.K, rows, planes, a.K, rows * a.K, tc::kBM, g.bf16) ||
         !tc::make_mn_map(&m.b, &g.blocked_b, dy, a.N, rows, planes, a.N, rows * a.N, g.bn, g.bf16) ||
         !tc::make_out_map(&m.o, a.out, a.N, a.K, a.groups, a.N, a.K * a.N, g.out_type))
@@ -281,8 +284,10 @@ cudaError_t weight_grad_tc(const GroupedLaunch &a, const void *x, const void *dy
         return cudaErrorInvalidValue;
     const int64_t tiles = (a.groups + a.rows / g.part_rows) * ((a.K + tc::kBM - 1) / tc::kBM) *
                           ((a.N + g.bn - 1) / g.bn);
-    return g.passes > 1 ? tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStoreSum>(m, g, tiles, stream)
-                        : tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(m, g, tiles, stream);
+    if constexpr (BN <= kWidestSum)
+        if (a.dtype == SPMM_F32)
+            return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStoreSum>(m, g, tiles, stream);
+    return tc::launch_gemm<tc::kRagged, BN, true, true, tc::kStore>(m, g, tiles, stream);
 }
 
 }  // namespace
@@ -319,7 +324,7 @@ cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStr
         return rows_tc<256, true>(a, x, w, g, row_tiles_of(a, 2 * tc::kBM), stream);
     }
     const int64_t row_tiles = row_tiles_of(a, tc::kBM);
-    g.bn = tile_columns(row_tiles, g.n);
+    g.bn = tile_columns(row_tiles, g.n, widest(a.dtype));
     if (g.bn <= 64) return rows_tc<64>(a, x, w, g, row_tiles, stream);
     if (g.bn <= 128) return rows_tc<128>(a, x, w, g, row_tiles, stream);
     return rows_tc<256>(a, x, w, g, row_tiles, stream);
@@ -343,7 +348,7 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
     g.out_batch = a.K * a.N;
     g.status = a.status;
     set_types(g, a.dtype);
-    g.bn = weight_grad_columns(a.N);
+    g.bn = weight_grad_columns(a.N, a.dtype);
     g.part_rows = weight_grad_part(a.rows, a.K, a.N, g.bn, a.dtype);
     const int64_t slots = weight_grad_slots(a.rows, a.K, a.N, a.dtype);
     const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: never read

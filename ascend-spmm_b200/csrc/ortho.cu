@@ -299,7 +299,6 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         const int now = i & 1, next = now ^ 1;
         tc::GemmArgs g{};
         g.batch = o.batch;
-        g.passes = 1;
         g.status = o.status;
         g.out_type = tc::kOutF16;
         // G = X X^T (X^T X)
