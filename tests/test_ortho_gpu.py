@@ -61,6 +61,15 @@ def test_batches(lib, batch, m, n):
     assert torch.equal(lib.orthogonalize(u.view(1, batch, m, n))[0], y)
 
 
+@pytest.mark.parametrize("batch,m,n", [(1, 250, 1030), (1, 1031, 250), (5, 512, 500), (5, 500, 510), (2, 1024, 1000),
+                                       (12, 700, 697), (30, 200, 900), (20, 900, 200), (1, 1100, 9000),
+                                       (1, 9001, 1100)])
+def test_tile_widths(lib, batch, m, n):
+    """Sizes on both sides of the rules that choose a product's tiles: one turn of narrow tiles or mirrored ones,
+    updates of 64 to 256 columns, alone and in pairs of SMs."""
+    check(lib, gradient(batch, m, n, BF16, seed=m))
+
+
 @pytest.mark.parametrize("decay", [0.0, 3.0])
 def test_spectra(lib, decay):
     """Flat and steep spectra; low rank plus noise, where an operand's rounding could grow with the small
