@@ -2,8 +2,8 @@
 //   G = X X^T,  P = b G + c G G,  X <- a X + P X
 // on the smaller side s of the matrix (for a tall one G = X^T X and
 // X <- a X + X P, the same polynomial).  Each step is two symmetric s x s
-// products, of which the tiles on and below the diagonal are computed and
-// written twice, and one s x s by s x r product; all run on the tensor cores
+// products, of which (but in small ones) the tiles on and below the diagonal
+// are computed and written twice, and one s x s by s x r product; all run on the tensor cores
 // (gemm_tc.cuh), which read X, G and P as they lie, so nothing is transposed.
 //
 // Precision.  The operands are fp16, not bf16: every singular value stays of
@@ -20,7 +20,7 @@
 // Measured: one 4096 x 2048 update 357 us, 300 GFLOP with the symmetric halves
 // counted once: of a step's 69 us the symmetric products take 20 and 14, the
 // update 33, each about 5 us of launch, first copies and last tile beyond its
-// products.  Three of 601 x 1023 152 us: fifteen dependent products of 8 to 12
+// products.  Three of 601 x 1023 137 us: fifteen dependent products of 8 to 12
 // us, of which the reduction's slices are 2 to 4.
 #include <algorithm>
 #include <climits>
