@@ -70,8 +70,8 @@ struct OrthoLaunch {
     DevStatus *status;
 };
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int dtype);
-// A shorter side of at most 128 (ortho_small.cu).
-bool ortho_small_eligible(int64_t m, int64_t n, int steps, float a);
+// A shorter side of at most 128 and steps that its form computes accurately (ortho_small.cu).
+bool ortho_small_eligible(const OrthoLaunch &o);
 size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n);
 cudaError_t launch_ortho_small(const OrthoLaunch &o, void *workspace, cudaStream_t stream);
 // Sums of squares of each matrix in parts (ortho.cu): squares [batch][parts].

@@ -15,7 +15,8 @@
 // singular values are still small: 5e-3 after five steps on a low-rank update
 // with noise, 2e-4 with the low part.
 //
-// Matrices with a side of at most 128 run in ortho_small.cu.
+// Matrices with a side of at most 128 run in ortho_small.cu, as long as the
+// steps are few enough for it.
 //
 // Measured: one 4096 x 2048 update 357 us, 300 GFLOP with the symmetric halves
 // counted once: of a step's 69 us the symmetric products take 20 and 14, the
@@ -240,14 +241,14 @@ cudaError_t launch_ortho_squares(const OrthoLaunch &o, double *squares, cudaStre
 
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int)
 {
-    // which form runs depends on the steps too: room for either
+    // which form runs depends on the steps and coefficients too: room for either
     return std::max(Space(batch, m, n, nullptr).bytes(batch),
                     std::min(m, n) <= 128 ? ortho_small_workspace(batch, m, n) : 0);
 }
 
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
-    if (ortho_small_eligible(o.m, o.n, o.steps, o.a)) return launch_ortho_small(o, workspace, stream);
+    if (ortho_small_eligible(o)) return launch_ortho_small(o, workspace, stream);
     const Space w(o.batch, o.m, o.n, workspace);
     cudaError_t e = launch_ortho_squares(o, w.part, stream);
     if (e != cudaSuccess) return e;

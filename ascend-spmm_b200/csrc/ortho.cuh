@@ -1,11 +1,51 @@
 // Shared by the two forms of the orthogonalised update (ortho.cu, ortho_small.cu).
 #pragma once
 
+#include <algorithm>
+#include <cmath>
+
 namespace spmmb {
 
 // Stored fp16 operand = value * scale.  Singular values are of order one, so
 // a matrix's elements are of order 1 / sqrt(size): the scales keep them out
 // of fp16's subnormals and leave a factor of 100 below its maximum.
 constexpr float kScaleX = 512.f, kScaleG = 256.f, kScaleP = 256.f;
+
+// Bounds over the singular values s in [0, reach] that a step can meet, with
+// u = s^2 an eigenvalue of G (host, 64 bits).  They start in [0, 1]; with the
+// default coefficients they stay below 1.2024.
+struct OrthoReach {
+    double reach = 1.0;
+    double a, b, c;
+    OrthoReach(double a, double b, double c) : a(a), b(b), c(c) {}
+    // The largest factor of an error of G's eigenvalues in a step G <- T G T,
+    // T = a + b u + c u^2: |d (u T^2) / du|, sampled.
+    double growth() const
+    {
+        double most = 0.0;
+        for (int i = 0; i <= 256; ++i) {
+            const double u = reach * reach * i / 256, t = a + u * (b + u * c), dt = b + 2 * u * c;
+            most = std::max(most, std::fabs(t * (t + 2 * u * dt)));
+        }
+        return most;
+    }
+    // To the next step: the largest |s T(s^2)|, at an end or where its derivative a + 3 b u + 5 c u^2 is zero.
+    void step()
+    {
+        double most = value(reach * reach);
+        const double disc = 9 * b * b - 20 * a * c;
+        if (c != 0.0 && disc >= 0.0)
+            for (const double sign : {-1.0, 1.0}) most = std::max(most, value((-3 * b + sign * std::sqrt(disc)) / (10 * c)));
+        else if (c == 0.0 && b != 0.0)
+            most = std::max(most, value(-a / (3 * b)));
+        reach = most;
+    }
+
+private:
+    double value(double u) const
+    {
+        return u >= 0.0 && u <= reach * reach ? std::sqrt(u) * std::fabs(a + u * (b + u * c)) : 0.0;
+    }
+};
 
 }  // namespace spmmb

@@ -23,11 +23,19 @@
 //
 // Precision: every operand is a high and a low fp16 part and every product
 // takes high x high, high x low and low x high (22 bits).  The error before
-// the result's rounding is 1e-5 for a gradient's spectrum and 4e-4 for a low
-// rank with noise, against 2e-3 and more with 11-bit operands (the
+// the result's rounding is 1e-5 for a gradient's spectrum and up to 8e-4 for a
+// low rank with noise, against 2e-3 and more with 11-bit operands (the
 // coefficients multiply an operand's rounding error by up to four a step).
-// Along a direction without a singular value Q grows to a^steps, which fp16's
-// range has to hold: eight steps with the default coefficients.
+//
+// Where the form ends.  G <- T G T multiplies what was rounded in G along a
+// small singular direction by T^2, a^2 = 11.9 a step with the default
+// coefficients, and nothing ties it to X any more: an eigenvalue of 1e-8
+// that should be zero, of either sign, is of order one eight steps later.  Low
+// rank with noise, 128 x 256: 8e-4 after five steps, 9e-3 after six, 1e-1
+// after seven, NaN after eight (the form of ortho.cu, which works on X itself:
+// 3e-4 to 3e-3).  So the steps' growth of G's error is held to 2^15, five steps
+// with the default coefficients; more go to ortho.cu.  Along a direction
+// without a singular value Q grows to a^steps, which fp16's range has to hold.
 //
 // Measured: 128 x 64 25 us, 46 of 256 x 128 49 us.  About a quarter of the
 // time is the tensor core's; a step is three dependent products, each with a
@@ -490,9 +498,13 @@ template <typename T> cudaError_t run_small(const OrthoLaunch &o, float scale_q,
 
 }  // namespace
 
-bool ortho_small_eligible(int64_t m, int64_t n, int steps, float a)
+bool ortho_small_eligible(const OrthoLaunch &o)
 {
-    return std::min(m, n) <= kSide && q_scale(steps, a) > 0.f;
+    if (std::min(o.m, o.n) > kSide || q_scale(o.steps, o.a) == 0.f) return false;
+    double growth = 1.0;   // of G's error, up to its last use
+    OrthoReach at(o.a, o.b, o.c);
+    for (int i = 0; i + 1 < o.steps; ++i, at.step()) growth *= std::max(1.0, at.growth());
+    return growth <= 32768.0;   // false for NaN
 }
 
 size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n)
