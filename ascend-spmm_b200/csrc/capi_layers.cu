@@ -208,7 +208,7 @@ int spmm_orthogonalize_launch(const void *update, void *out, int64_t batch, int6
     if (m > (1 << 20) || n > (1 << 20) || batch > 65535) return capi_error(SPMM_ERR_ARG, "%s: size too large", op);
     if (steps < 0 || steps > 100) return capi_error(SPMM_ERR_ARG, "%s: steps must be in [0, 100]", op);
     if (!(eps >= 0)) return capi_error(SPMM_ERR_ARG, "%s: eps must not be negative", op);
-    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
+    if (!std::isfinite((float)a) || !std::isfinite((float)b) || !std::isfinite((float)c))
         return capi_error(SPMM_ERR_ARG, "%s: coefficients must be finite", op);
     if (batch == 0 || m == 0 || n == 0) return SPMM_OK;
     if (!update || !out) return capi_error(SPMM_ERR_ARG, "%s: null array", op);

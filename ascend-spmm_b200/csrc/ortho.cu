@@ -7,13 +7,15 @@
 // (gemm_tc.cuh), which read X, G and P as they lie, so nothing is transposed.
 //
 // Precision.  The operands are fp16, not bf16: every singular value stays of
-// order one (the polynomial maps [0, 1.3] into itself), so the elements need
-// no exponent range, and 11 bits instead of 8 take the result's error from
-// 1e-2 to about 2e-3.  X is kept as a high and a low fp16 part (22 bits): the
-// products take the high part, the term a X both.  Otherwise the rounding of
-// X would be multiplied by a in every step along the directions whose
-// singular values are still small: 5e-3 after five steps on a low-rank update
-// with noise, 2e-4 with the low part.
+// order one (they start in [0, 1], the default coefficients take them to at
+// most 1.2024 and map [0, 1.2637] into itself), so the elements need no
+// exponent range, and 11 bits instead of 8 take the result's error from 1e-2
+// to about 2e-3.  Other coefficients may take singular values anywhere: the
+// operands' scales follow what the steps can reach (ortho.cuh).  X is kept as
+// a high and a low fp16 part (22 bits): the products take the high part, the
+// term a X both.  Otherwise the rounding of X would be multiplied by a in
+// every step along the directions whose singular values are still small: 5e-3
+// after five steps on a low-rank update with noise, 2e-4 with the low part.
 //
 // Matrices with a side of at most 128 run in ortho_small.cu, as long as the
 // steps are few enough for it.
@@ -296,8 +298,13 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
     M.out = M.x_out[0];
     if (fine && mapped) fine = tc::make_out_map(&M.out, o.out, o.n, o.m, o.batch, o.n, o.m * o.n, tc::kOutBf16);
     if (!fine) return cudaErrorInvalidValue;
+    OrthoReach at(o.a, o.b, o.c);
+    double scale_x = kScaleX;   // of the stored X; it starts with singular values of at most one
     for (int i = 0; i < o.steps && e == cudaSuccess; ++i) {
         const int now = i & 1, next = now ^ 1;
+        const double scale_g = scale_for(kScaleG, at.reach * at.reach), scale_p = scale_for(kScaleP, at.poly());
+        at.step();
+        const double next_x = i + 1 == o.steps ? 1.0 : scale_for(kScaleX, at.reach);   // the result is not scaled
         tc::GemmArgs g{};
         g.batch = o.batch;
         g.status = o.status;
@@ -309,7 +316,7 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.out = w.gram;
         g.ldo = w.lds;
         g.out_batch = sq;
-        g.alpha = kScaleG / (kScaleX * kScaleX);
+        g.alpha = (float)(scale_g / (scale_x * scale_x));
         g.symmetric = !whole;
         g.blocked_a = blocked_square;
         g.blocked_b = blocked_square_b;
@@ -322,8 +329,8 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.ldi = w.lds;
         g.in_batch = sq;
         g.out = w.poly;
-        g.alpha = o.c * (kScaleP / (kScaleG * kScaleG));
-        g.beta = o.b * (kScaleP / kScaleG);
+        g.alpha = (float)(o.c * (scale_p / (scale_g * scale_g)));
+        g.beta = (float)(o.b * (scale_p / scale_g));
         m = tc::Maps{M.gram, M.gram_b, M.poly_out, M.poly_out};
         e = square_bn == 64
                 ? tc::launch_gemm<tc::kDense, 64, false, false, tc::kPoly>(m, g, square_tiles, stream)
@@ -346,8 +353,9 @@ cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t str
         g.out_type = last ? tc::kOutBf16 : tc::kOutF16;
         g.blocked_a = false;
         g.blocked_b = blocked_x;
-        g.alpha = last ? 1.f / (kScaleP * kScaleX) : 1.f / kScaleP;
-        g.beta = last ? o.a / kScaleX : o.a;
+        g.alpha = (float)(next_x / (scale_p * scale_x));
+        g.beta = (float)(o.a * (next_x / scale_x));
+        scale_x = next_x;
         m = tc::Maps{tall ? M.x[now] : M.poly, tall ? M.poly : M.x[now], last ? M.out : M.x_out[next], M.low_out};
         if (pair) e = update<256, true>(o, m, g, stream);
         else if (bn > 128) e = update<256>(o, m, g, stream);

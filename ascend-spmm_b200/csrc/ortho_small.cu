@@ -35,7 +35,9 @@
 // after seven, NaN after eight (the form of ortho.cu, which works on X itself:
 // 3e-4 to 3e-3).  So the steps' growth of G's error is held to 2^15, five steps
 // with the default coefficients; more go to ortho.cu.  Along a direction
-// without a singular value Q grows to a^steps, which fp16's range has to hold.
+// without a singular value Q grows to a^steps, which fp16's range has to hold,
+// and G, T and T G with their fixed scales too: coefficients that leave it go
+// to ortho.cu, whose scales follow them.
 //
 // Measured: 128 x 64 25 us, 46 of 256 x 128 49 us.  About a quarter of the
 // time is the tensor core's; a step is three dependent products, each with a
@@ -450,12 +452,21 @@ cudaError_t run_phase(const OrthoLaunch &o, float scale_q, const Between &w, int
     return cudaGetLastError();
 }
 
-// A power of two that keeps Q, at most max(1, |a|)^steps, in fp16's range; 0 if none does.
-float q_scale(int steps, float a)
+// A power of two that keeps Q, a product of the steps' T, in fp16's range; 0
+// where an operand would leave it or G's rounding would grow too far.
+float q_scale(const OrthoLaunch &o)
 {
-    const double largest = std::pow(std::max(1.0, std::fabs((double)a)), steps);
-    if (!(largest <= 32768.0)) return 0.f;
-    return (float)std::min(256.0, std::exp2(std::floor(std::log2(32768.0 / largest))));
+    OrthoReach at(o.a, o.b, o.c);
+    double q = 1.0, growth = 1.0;   // growth: of G's error, up to its last use
+    for (int i = 0; i < o.steps; ++i) {
+        const double t = at.factor(), g = at.reach * at.reach;
+        if (!(std::max(t * kScaleP, g * std::max(1.0, t) * kScaleG) <= kMostStored)) return 0.f;
+        q *= std::max(1.0, t);
+        if (i + 1 < o.steps) growth *= std::max(1.0, at.growth());
+        at.step();
+    }
+    if (!(growth <= 32768.0) || !(q <= kMostStored)) return 0.f;
+    return (float)std::min(256.0, std::exp2(std::floor(std::log2(kMostStored / q))));
 }
 
 // Blocks of a matrix in parts (1: one block does it all).  A block alone takes
@@ -498,14 +509,7 @@ template <typename T> cudaError_t run_small(const OrthoLaunch &o, float scale_q,
 
 }  // namespace
 
-bool ortho_small_eligible(const OrthoLaunch &o)
-{
-    if (std::min(o.m, o.n) > kSide || q_scale(o.steps, o.a) == 0.f) return false;
-    double growth = 1.0;   // of G's error, up to its last use
-    OrthoReach at(o.a, o.b, o.c);
-    for (int i = 0; i + 1 < o.steps; ++i, at.step()) growth *= std::max(1.0, at.growth());
-    return growth <= 32768.0;   // false for NaN
-}
+bool ortho_small_eligible(const OrthoLaunch &o) { return std::min(o.m, o.n) <= kSide && q_scale(o) > 0.f; }
 
 size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n)
 {
@@ -516,7 +520,7 @@ size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n)
 
 cudaError_t launch_ortho_small(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
-    const float scale_q = q_scale(o.steps, o.a);
+    const float scale_q = q_scale(o);
     switch (o.dtype) {
         case SPMM_F16: return run_small<__half>(o, scale_q, workspace, stream);
         case SPMM_BF16: return run_small<__nv_bfloat16>(o, scale_q, workspace, stream);
