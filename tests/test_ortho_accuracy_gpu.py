@@ -1,10 +1,11 @@
 """orthogonalize on the GPU where rounding could grow: many steps on low rank
-and steep spectra, coefficients that take the operands out of the range of the
-default ones."""
+and steep spectra, the 22-bit form of thin matrices, coefficients that take
+the operands out of the range of the default ones."""
 
 import pytest
 import torch
 
+from layer_reference import ortho_reference
 from test_ortho_gpu import check, gradient, lib  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -26,6 +27,19 @@ def test_steps_on_low_rank_and_steep_spectra(lib, m, n, steps):  # noqa: F811
         for noise in (1e-2, 1e-3):
             check(lib, low_rank(m, n, rank, noise), steps=steps)
     check(lib, gradient(1, m, n, F32, decay=3.0), steps=steps)
+
+
+@pytest.mark.parametrize("batch,m,n", [(1, 128, 64), (2, 100, 200), (1, 128, 128), (2, 64, 2000), (1, 4000, 30)])
+def test_thin_matrices_keep_their_low_parts(lib, batch, m, n):  # noqa: F811
+    """A side of at most 128, default steps: the error before the result's rounding stays below 2.5e-4 in the norm
+    (operands of two fp16 parts, 22 bits; 11-bit operands alone give 1.5e-3 and more).  The rounding to bf16 is
+    independent of it, so the squares add up; 2 % of the rounding's for the chance of it."""
+    u = gradient(batch, m, n, F32, seed=m)
+    ref = ortho_reference(u)
+    norm = lambda t: t.flatten(-2).norm(dim=-1)  # noqa: E731
+    rounding = norm(ref.to(BF16).double() - ref)
+    err = norm(lib.orthogonalize(u).double() - ref)
+    assert bool((err ** 2 <= 1.02 * rounding ** 2 + (2.5e-4 * norm(ref)) ** 2).all()), (err / norm(ref), rounding / norm(ref))
 
 
 @pytest.mark.parametrize("m,n", [(24, 40), (300, 100), (200, 136), (130, 400)])
