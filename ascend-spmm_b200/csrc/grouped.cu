@@ -190,11 +190,20 @@ bool pair_rows(const GroupedLaunch &a, const tc::GemmArgs &g)
 // rows that pay: 512, in fp32 (six products of each) 384 (4000 rows of 3
 // groups, K = N = 256: 35 us with 1024, 25 us; 20000 rows of 8 groups, K = N =
 // 128: 43 and 35 us; 20011 rows of 8 groups, K = 256, N = 264: 55 and 57 us).
+//
+// At most 16384 rows, whatever the share: the tensor core truncates into its
+// accumulator, up to 2^-22 of what it holds in a step of 16 rows and always
+// towards zero, so over a part of products of one sign up to 2^-13 of the sum
+// is lost (measured 1e-4).  One group of 2^20 rows, K = N = 2048, fp16, was
+// 3.4e-3 too small in parts of 604544 rows, seven roundings to fp16.  The
+// price, where parts were longer: 65536 rows of that group 0.41 -> 0.55 ms,
+// 2^20 rows 6.06 -> 6.21 ms.
+constexpr int64_t kLongestPart = 16384;
 int64_t weight_grad_part(int64_t rows, int64_t K, int64_t N, int bn, int dtype)
 {
     const int64_t tiles = ((K + tc::kBM - 1) / tc::kBM) * ((N + bn - 1) / bn);
     const int64_t part = rows * tiles * 2 / (3 * device_sm_count());
-    return (std::max<int64_t>(dtype == SPMM_F32 ? 384 : 512, part) + 63) & ~int64_t(63);
+    return (std::min(kLongestPart, std::max<int64_t>(dtype == SPMM_F32 ? 384 : 512, part)) + 63) & ~int64_t(63);
 }
 
 // Equal tiles of the greatest width: the reduction is cut where there are
@@ -207,11 +216,12 @@ int weight_grad_columns(int64_t N, int dtype)
     return (int)(((N + n - 1) / n + step - 1) / step * step);
 }
 
-// A group of n > 1 parts has more than (n - 1) part rows, so n <= 2 rows / part.
-int64_t weight_grad_slots(int64_t rows, int64_t K, int64_t N, int dtype)
+// Groups of several parts have more than `part` rows each, and no more than
+// one part beyond the whole ones in their rows.
+int64_t weight_grad_slots(int64_t rows, int64_t groups, int64_t K, int64_t N, int dtype)
 {
-    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N, dtype), dtype);
-    return rows <= part ? 0 : 2 * rows / part;
+    const int64_t part = weight_grad_part(rows, K, N, weight_grad_columns(N, dtype), dtype), whole = rows / part;
+    return rows <= part ? 0 : whole + std::min(groups, whole);
 }
 
 // Adds the parts of each group that has several, in their order.
@@ -332,8 +342,7 @@ cudaError_t launch_grouped_rows(const GroupedLaunch &a, void *workspace, cudaStr
 
 size_t grouped_weight_grad_workspace(int64_t rows, int64_t groups, int64_t K, int64_t N, int dtype)
 {
-    (void)groups;
-    const size_t parts = (size_t)weight_grad_slots(rows, K, N, dtype) * K * N * sizeof(float);
+    const size_t parts = (size_t)weight_grad_slots(rows, groups, K, N, dtype) * K * N * sizeof(float);
     return parts + (dtype == SPMM_F32 ? plane_bytes(rows * K) + plane_bytes(rows * N) : 0);
 }
 
@@ -350,7 +359,7 @@ cudaError_t launch_grouped_weight_grad(const GroupedLaunch &a, void *workspace, 
     set_types(g, a.dtype);
     g.bn = weight_grad_columns(a.N, a.dtype);
     g.part_rows = weight_grad_part(a.rows, a.K, a.N, g.bn, a.dtype);
-    const int64_t slots = weight_grad_slots(a.rows, a.K, a.N, a.dtype);
+    const int64_t slots = weight_grad_slots(a.rows, a.groups, a.K, a.N, a.dtype);
     const void *x = a.rows > 0 ? a.x : a.out, *dy = a.rows > 0 ? a.w : a.out;   // no rows: never read
     char *ws = static_cast<char *>(workspace);
     if (a.dtype == SPMM_F32 && a.rows > 0) {
