@@ -52,7 +52,10 @@ enum Mode { kRows, kRagged, kDense };
 // so an accumulator takes one slice, the smallest products first, and the
 // epilogue warps add the slices in registers, rounding to nearest (K = 4096:
 // error 1.4e-7, with two slices 5e-7 and 6 % less time, with four 1.2e-6).
-// The others but kStore are kDense's: see ortho.cu.
+// The others but kStore are kDense's: see ortho.cu.  kGram, whose products are
+// squares on the diagonal and run down a matrix's long side, takes a new
+// accumulator every 256 slices: in a single one 2^20 columns lost 6e-3 of G
+// and moved a 136-row update by 6e-3, 16384 lose 1e-4.
 enum Epi { kStore, kStoreSum, kGram, kPoly, kUpdate };
 enum OutType { kOutF16, kOutBf16, kOutF32 };
 
@@ -327,6 +330,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     static_assert(!PAIR || MODE != kRagged, "a group's zeros are written by one block");
     using S = GemmShape<BN, PAIR>;
     constexpr int kParts = EPI == kStoreSum ? 3 : 1;   // ring stages of a slice
+    constexpr int kSlices = EPI == kStoreSum ? 1 : EPI == kGram ? 256 : 0;   // of an accumulator, 0: all
     static_assert(S::kStages >= 2 * kParts, "a slice arrives while another is multiplied");
     extern __shared__ __align__(1024) unsigned char smem[];
     const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
@@ -536,7 +540,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             // kRagged: a last slice that ends within 16 rows needs the whole warp
             const bool ragged = MODE == kRagged && (depth & 15);
             const int whole = ragged ? n - 1 : n;
-            const int sum = EPI == kStoreSum ? 1 : n;   // slices of an accumulator
+            const int sum = kSlices ? min(kSlices, n) : n;
             for (int s0 = 0; s0 < n && ok; s0 += sum, ++used) {
                 const unsigned d = tmem + (used & 1u) * BN;
                 if (peer == 0 && !bar_wait<PAIR>(acc_empty + 8 * (used & 1u), (used >> 1 & 1u) ^ 1u, abort)) {
@@ -733,13 +737,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 }
                 ++used;
             };
-            if constexpr (EPI == kStoreSum) {
+            if constexpr (kSlices > 0) {
                 float v[BN / 64][32];
 #pragma unroll
                 for (int b = 0; b < BN / 64; ++b)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[b][i] = 0.f;
-                for (int i = 0; i < n; ++i) {
+                for (int i = 0; i < n; i += kSlices) {
                     const unsigned from = take();
                     if (!ok) break;
 #pragma unroll

@@ -56,3 +56,25 @@ def test_coefficients_beyond_the_operands_range(lib, m, n, coefficients, steps):
 def test_coefficients_that_fp32_cannot_hold_are_refused(lib):  # noqa: F811
     with pytest.raises(RuntimeError, match="finite"):
         lib.orthogonalize(torch.zeros(8, 8, device="cuda"), coefficients=(1.0, 1e300, 0.0))
+
+
+@pytest.mark.parametrize("m,n", [(136, 1 << 20), (1 << 18, 200)])
+def test_a_long_side_of_a_million(lib, m, n):  # noqa: F811
+    """G sums squares along the long side; a matrix unit truncates its accumulator towards zero.  The result's
+    rounding (1.7e-3) and the 11-bit operands' 2e-3 leave the norm of the error below 2^-8."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    side = min(m, n)
+    u = torch.randn(side, max(m, n), generator=g, device="cuda") * torch.logspace(0, -1, side, device="cuda")[:, None]
+    u = (u if m < n else u.T).to(F16)
+    y = lib.orthogonalize(u)
+    # the polynomial of the eigenvalues of X X^T, in 64 bits
+    x = (u if m < n else u.T).double()
+    gram = x @ x.T
+    norm = gram.trace().sqrt() + 1e-7
+    value, basis = torch.linalg.eigh(gram / norm ** 2)
+    factor = torch.ones_like(value)
+    for _ in range(5):
+        t = 3.4445 - 4.7750 * value + 2.0315 * value ** 2
+        factor, value = factor * t, value * t * t
+    ref = (basis * (factor / norm)) @ (basis.T @ x)
+    assert float(((y if m < n else y.T).double() - ref).norm()) <= 2.0 ** -8 * float(ref.norm())
