@@ -38,11 +38,15 @@ __host__ __device__ Ranges ranges_of(const GroupedLaunch &a)
 // operand is written as three bf16 planes x = h + m + l (8 bits each, fp32's
 // exponents) and the product is run as the six plane products above 2^-24 of
 // the result, the smallest first:  h l, l h, m m, h m, m h, h h.  That is six
-// bf16 products, about four times the rate of fp32 FMAs.  An infinite x has
-// zero m and l planes; its products with zero planes are NaN.  The six
-// products share a slice's planes in shared memory: bringing each product's
-// two operands in by themselves took half as long again (51, 55 and 69 us for
-// 39, 40 and 56 in the case above), bound by those copies.
+// bf16 products, about four times the rate of fp32 FMAs.  The six share a
+// slice's planes in shared memory: bringing each product's two operands in by
+// themselves took half as long again (51, 55 and 69 us for 39, 40 and 56 in
+// the case above), bound by those copies.
+//
+// An infinite x is split as h = +-1, m = 0, l = +-infinity.  l meets the other
+// operand's h alone, so the product is an infinity of the right sign, and NaN
+// where the other is zero; an infinite h beside the zero m and l planes of
+// ordinary numbers would make it NaN.
 constexpr int kPlanes = 3;
 
 // An operand to split: src [groups][elems], planes `plane` apart.  `skip`:
@@ -73,16 +77,22 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const Split first, co
         if (in_group >= s.elems) continue;
         const float4 u = __ldg(reinterpret_cast<const float4 *>(s.src + i));
         const float4 w = __ldg(reinterpret_cast<const float4 *>(s.src + i) + 1);
-        float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+        float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w}, last[8];   // last: what only plane l holds
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            last[k] = isinf(v[k]) ? v[k] : 0.f;
+            if (isinf(v[k])) v[k] = copysignf(1.f, v[k]);
+        }
 #pragma unroll
         for (int p = 0; p < kPlanes; ++p) {
             __align__(16) __nv_bfloat16 h[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
+                if (p == kPlanes - 1) v[k] += last[k];
                 h[k] = __float2bfloat16_rn(v[k]);
                 // next to fp32's maximum, rounding up would leave the range
                 if (isinf(__bfloat162float(h[k])) && !isinf(v[k])) h[k] = __float2bfloat16_rz(v[k]);
-                v[k] = isfinite(v[k]) ? v[k] - __bfloat162float(h[k]) : 0.f;
+                v[k] = isnan(v[k]) ? 0.f : v[k] - __bfloat162float(h[k]);
             }
             *reinterpret_cast<uint4 *>(s.dst + p * s.plane + i) = *reinterpret_cast<const uint4 *>(h);
         }

@@ -1,13 +1,45 @@
-"""grouped_matmul and its gradients at the limits of their forms: long sums."""
+"""grouped_matmul and its gradients at the limits of their forms: infinities
+in fp32, long sums."""
 
 import pytest
 import torch
 
-from test_grouped_gpu import lib  # noqa: F401
+from test_grouped_gpu import lib, make  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+def same_kind(got, want, what):
+    """NaN where the reference has NaN, the same infinities; finite values to fp32's accuracy."""
+    got, want = got.cpu().double(), want.cpu()
+    assert torch.equal(got.isnan(), want.isnan()), what
+    assert torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()]), what
+    ok = want.isfinite()
+    assert bool(((got - want)[ok].abs() <= 1e-5 * (1 + want[ok].abs())).all()), what
+
+
+def test_fp32_infinities(lib):  # noqa: F811
+    """An infinity gives what fp32 arithmetic gives: infinities of the products' signs, NaN for infinity times zero,
+    for infinities of both signs and for NaN."""
+    x, w, ptr, grad = make([40, 30], 64, 48, F32, seed=13)
+    inf = float("inf")
+    x[3, 5], x[50, 7] = inf, -inf
+    x[9, 1], x[9, 2] = inf, inf                  # of one sign or of both, by the weight's signs
+    w[0, 5, 11] = 0.0                            # inf * 0
+    w[0, 20, 3], x[4, 20], x[5, 20] = -inf, 0.0, inf
+    w[1, 30, 40], x[60, 30] = float("nan"), 2.0
+    w[0, 5, 12] = 0.5                            # nothing below the highest of its three parts
+    ref = lambda a, b: (a.cpu().double()[:, :, None] * b.cpu().double()[None]).sum(1)  # noqa: E731
+    want = torch.cat([ref(x[:40], w[0]), ref(x[40:], w[1])])
+    assert bool(want[3].isinf().any()) and bool(want[3].isnan().any()) and bool(want[50, :40].isinf().all())
+    same_kind(lib.grouped_matmul(x, w, ptr), want, "y")
+    grad[2, 3], grad[45, 9], grad[33, 3] = inf, -inf, 0.0
+    want = torch.cat([ref(grad[:40], w[0].T), ref(grad[40:], w[1].T)])
+    same_kind(lib.grouped_matmul(grad, w, ptr, transposed=True), want, "dx")
+    want = torch.stack([ref(x[:40].T, grad[:40]), ref(x[40:].T, grad[40:])])
+    same_kind(lib.grouped_weight_grad(x, grad, ptr), want, "dw")
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
