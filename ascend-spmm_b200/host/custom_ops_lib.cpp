@@ -835,20 +835,24 @@ at::Tensor layer_norm(const at::Tensor &x, const c10::optional<at::Tensor> &weig
 
 struct GroupedMatmulFunction : torch::autograd::Function<GroupedMatmulFunction> {
     static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight,
-                              const at::Tensor &group_ptr)
+                              const at::Tensor &group_ptr, bool transposed)
     {
         at::AutoDispatchBelowADInplaceOrView below;
         ctx->save_for_backward({x, weight, group_ptr});
-        return grouped_rows(x, weight, group_ptr, false);
+        ctx->saved_data["transposed"] = transposed;
+        return grouped_rows(x, weight, group_ptr, transposed);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         const variable_list s = ctx->get_saved_variables();
-        variable_list out(3);
+        const bool transposed = ctx->saved_data["transposed"].toBool();
+        variable_list out(4);
         if (grads[0].defined()) {
             at::NoGradGuard none;
-            if (ctx->needs_input_grad(0)) out[0] = grouped_rows(grads[0], s[1], s[2], true);
-            if (ctx->needs_input_grad(1)) out[1] = grouped_weight_grad(s[0], grads[0], s[2]);
+            if (ctx->needs_input_grad(0)) out[0] = grouped_rows(grads[0], s[1], s[2], !transposed);
+            if (ctx->needs_input_grad(1))   // y = x W^T: the roles of x and the gradient change
+                out[1] = transposed ? grouped_weight_grad(grads[0], s[0], s[2])
+                                    : grouped_weight_grad(s[0], grads[0], s[2]);
         }
         return once(std::move(out), "grouped_matmul");
     }
@@ -856,7 +860,7 @@ struct GroupedMatmulFunction : torch::autograd::Function<GroupedMatmulFunction> 
 
 at::Tensor grouped_matmul(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &group_ptr, bool transposed)
 {
-    if (!transposed && wants_grad({&x, &weight})) return GroupedMatmulFunction::apply(x, weight, group_ptr);
+    if (wants_grad({&x, &weight})) return GroupedMatmulFunction::apply(x, weight, group_ptr, transposed);
     return grouped_rows(x, weight, group_ptr, transposed);
 }
 
@@ -953,7 +957,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("fp32_params") = false);
     m.def("grouped_matmul", &grouped_matmul,
           "Rows group_ptr[g] .. group_ptr[g + 1] of x times weight[g] (its transpose with transposed); widths "
-          "divisible by 16 for FP16 and BF16, by 8 for FP32; differentiable unless transposed",
+          "divisible by 16 for FP16 and BF16, by 8 for FP32; differentiable",
           pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("group_ptr"), pybind11::arg("transposed") = false);
     m.def("grouped_weight_grad", &grouped_weight_grad, "Gradient of grouped_matmul's weight: x_g^T grad_g per group",
           pybind11::arg("x"), pybind11::arg("grad"), pybind11::arg("group_ptr"));

@@ -137,9 +137,10 @@ def grouped_matmul(x, weight, group_ptr, transposed=False):
     divisible by 16, fp32 by 8), ``group_ptr`` [groups + 1] int32 or int64 on
     the device, like a CSR row pointer (the relations of a typed graph's
     messages, the experts of routed rows).  ``transposed`` takes x [rows, N] to
-    [rows, K] by ``weight[g].T``.  Differentiable in x and weight (the plain
-    form); ``grouped_weight_grad`` is the weight's gradient by itself.  A
-    malformed range raises the device status instead of a fault.
+    [rows, K] by ``weight[g].T``.  Both are differentiable in x and weight;
+    ``grouped_weight_grad`` is the weight's gradient by itself, without a
+    gradient of its own.  A malformed range raises the device status instead of
+    a fault.
     """
     return _grouped_matmul(x, weight, group_ptr, transposed)
 
