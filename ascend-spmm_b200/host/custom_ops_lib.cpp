@@ -864,7 +864,7 @@ at::Tensor grouped_matmul(const at::Tensor &x, const at::Tensor &weight, const a
     return grouped_rows(x, weight, group_ptr, transposed);
 }
 
-at::Tensor orthogonalize(const at::Tensor &update, int64_t steps, double a, double b, double c, double eps)
+at::Tensor orthogonalize_forward(const at::Tensor &update, int64_t steps, double a, double b, double c, double eps)
 {
     const char *op = "orthogonalize";
     TORCH_CHECK_CUDA(update);
@@ -882,6 +882,29 @@ at::Tensor orthogonalize(const at::Tensor &update, int64_t steps, double a, doub
     check_rc(spmm_orthogonalize_launch(u.data_ptr(), out.data_ptr(), batch, m, n, (int)steps, a, b, c, eps, dt,
                                        ws.data_ptr(), wbytes, stream_of(u)));
     return out;
+}
+
+// An update is made from gradients and applied outside the graph, so there is
+// no derivative: a backward pass that reaches the node raises an error instead
+// of taking the result for a constant.
+struct OrthogonalizeFunction : torch::autograd::Function<OrthogonalizeFunction> {
+    static at::Tensor forward(AutogradContext *, const at::Tensor &update, int64_t steps, double a, double b, double c,
+                              double eps)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return orthogonalize_forward(update, steps, a, b, c, eps);
+    }
+    static variable_list backward(AutogradContext *, variable_list)
+    {
+        TORCH_CHECK(false, "orthogonalize is not differentiable: detach the update, or call it under no_grad");
+        return {};
+    }
+};
+
+at::Tensor orthogonalize(const at::Tensor &update, int64_t steps, double a, double b, double c, double eps)
+{
+    if (wants_grad({&update})) return OrthogonalizeFunction::apply(update, steps, a, b, c, eps);
+    return orthogonalize_forward(update, steps, a, b, c, eps);
 }
 
 // Sticky device status (code, detail), optionally cleared.  Synchronises.

@@ -1,5 +1,5 @@
 """What the layer operators do with gradients beyond the plain backward pass:
-the transposed product's."""
+the transposed product's, an orthogonalised update's."""
 
 import pytest
 import torch
@@ -22,3 +22,14 @@ def test_gradient_of_the_transposed_product(lib, dtype):  # noqa: F811
     dg, dw = torch.autograd.grad(y, [gl, wl], x)
     assert_within(dg, *grouped_reference(x, w, ptr))
     assert_within(dw, *weight_grad_reference(x, grad, ptr))
+
+
+def test_an_orthogonalised_update_refuses_its_backward_pass(lib):  # noqa: F811
+    u = torch.randn(40, 30, device="cuda", requires_grad=True)
+    y = lib.orthogonalize(u)
+    assert y.requires_grad and torch.equal(y.detach(), lib.orthogonalize(u.detach()))
+    for call in (lambda: y.float().sum().backward(), lambda: torch.autograd.grad(y.sum(), [u], allow_unused=True)):
+        with pytest.raises(RuntimeError, match="orthogonalize is not differentiable"):
+            call()
+    with torch.no_grad():
+        assert not lib.orthogonalize(u).requires_grad
