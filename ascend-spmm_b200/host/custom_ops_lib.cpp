@@ -619,6 +619,14 @@ int layer_dtype(const at::Tensor &t, const char *op)
     return -1;
 }
 
+// Tensors with a forward-mode tangent are refused: the result would have none.
+void refuse_tangents(std::initializer_list<const at::Tensor *> ts, const char *op)
+{
+    for (const at::Tensor *t : ts)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op,
+                    " has no forward-mode derivative; take the tangent off its inputs (torch.autograd.forward_ad)");
+}
+
 // A contiguous, 16-byte aligned form of t (t itself where it is one).
 at::Tensor dense16(const at::Tensor &t) { return aligned16(t.contiguous()); }
 
@@ -632,6 +640,7 @@ at::Tensor norm_param(const c10::optional<at::Tensor> &p, const at::Tensor &x, i
                 p->sizes());
     TORCH_CHECK(p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat, "layer_norm: ", name,
                 " must have the dtype of x or FP32");
+    refuse_tangents({&*p}, "layer_norm");
     return dense16(*p);
 }
 
@@ -656,6 +665,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_forward(const at::Tens
     const int dt = layer_dtype(x, "layer_norm");
     const int64_t width = x.size(-1);
     TORCH_CHECK(width >= 1, "layer_norm requires a feature width of at least 1");
+    refuse_tangents({&x}, "layer_norm");
     c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor w = norm_param(weight, x, width, "weight"), b = norm_param(bias, x, width, "bias");
     const int pdt = param_dtype_of(w, b, dt);
@@ -691,6 +701,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(const at::Ten
     const int dt = layer_dtype(x, op);
     const int64_t width = x.size(-1);
     TORCH_CHECK(width >= 1, op, " requires a feature width of at least 1");
+    refuse_tangents({&grad, &x, &mean, &rstd}, op);
     const int64_t rows = x.numel() / width;
     TORCH_CHECK(grad.sizes() == x.sizes() && grad.scalar_type() == x.scalar_type(), op,
                 ": grad must have the shape and dtype of x");
@@ -740,6 +751,7 @@ at::Tensor grouped_rows(const at::Tensor &x, const at::Tensor &weight, const at:
     TORCH_CHECK(x.size(1) == (transposed ? N : K), op, ": x has ", x.size(1), " features, the weight takes ",
                 transposed ? N : K);
     const int itype = check_group_ptr(group_ptr, x, groups, op);
+    refuse_tangents({&x, &weight}, op);
     c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor xc = dense16(x), wc = dense16(weight);
     at::Tensor out = at::empty({rows, transposed ? K : N}, xc.options());
@@ -762,6 +774,7 @@ at::Tensor grouped_weight_grad(const at::Tensor &x, const at::Tensor &grad, cons
     TORCH_CHECK(grad.size(0) == x.size(0), op, ": x and grad must have the same number of rows");
     same_device({&grad}, x, op);
     const int itype = check_group_ptr(group_ptr, x, -1, op);
+    refuse_tangents({&x, &grad}, op);
     const int64_t groups = group_ptr.size(0) - 1, K = x.size(1), N = grad.size(1), rows = x.size(0);
     c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor xc = dense16(x), gc = dense16(grad);
@@ -871,6 +884,7 @@ at::Tensor orthogonalize_forward(const at::Tensor &update, int64_t steps, double
     TORCH_CHECK(update.dim() >= 2, op, ": update must have at least two dimensions");
     const int dt = layer_dtype(update, op);
     TORCH_CHECK(steps >= 0 && steps <= 100, op, ": steps must be in [0, 100]");
+    refuse_tangents({&update}, op);
     c10::cuda::CUDAGuard guard(update.device());
     const at::Tensor u = dense16(update);
     at::Tensor out = at::empty(u.sizes(), u.options().dtype(at::kBFloat16));

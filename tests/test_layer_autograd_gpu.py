@@ -1,8 +1,9 @@
 """What the layer operators do with gradients beyond the plain backward pass:
-the transposed product's, an orthogonalised update's."""
+the transposed product's, an orthogonalised update's, forward-mode tangents."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from layer_reference import assert_within, grouped_reference, weight_grad_reference
 from test_grouped_gpu import lib, make  # noqa: F401
@@ -33,3 +34,19 @@ def test_an_orthogonalised_update_refuses_its_backward_pass(lib):  # noqa: F811
             call()
     with torch.no_grad():
         assert not lib.orthogonalize(u).requires_grad
+
+
+def test_forward_mode_tangents_are_refused(lib):  # noqa: F811
+    x, w, ptr, grad = make([8, 8], 32, 32, F32)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        dw = forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: lib.layer_norm(d), lambda: lib.layer_norm(x, d[0]), lambda: lib.grouped_matmul(d, w, ptr),
+                     lambda: lib.grouped_matmul(x, dw, ptr), lambda: lib.grouped_matmul(d, w, ptr, True),
+                     lambda: lib.grouped_weight_grad(x, d, ptr), lambda: lib.orthogonalize(d),
+                     lambda: lib.layer_norm_forward(d, None, None)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            lib.layer_norm(d)
+    lib.layer_norm(x)
