@@ -43,7 +43,7 @@ class _SparseMatrix:
         self._start = torch.zeros(40, dtype=torch.int32, device=row.device)
 
     def __matmul__(self, x):
-        return _Spmm.apply(x, self)
+        return _Spmm.apply(x, self, False)
 
     def run(self, csr, x):
         ptr, col, val = csr
@@ -51,14 +51,16 @@ class _SparseMatrix:
 
 
 class _Spmm(torch.autograd.Function):
+    """A @ x, or with ``transposed`` A^T @ x: each is the other's gradient, to any order."""
+
     @staticmethod
-    def forward(ctx, x, matrix):
-        ctx.matrix = matrix
-        return matrix.run(matrix.forward_csr, x)
+    def forward(ctx, x, matrix, transposed):
+        ctx.matrix, ctx.transposed = matrix, transposed
+        return matrix.run(matrix.transpose_csr if transposed else matrix.forward_csr, x)
 
     @staticmethod
     def backward(ctx, grad):
-        return ctx.matrix.run(ctx.matrix.transpose_csr, grad), None
+        return _Spmm.apply(grad, ctx.matrix, not ctx.transposed), None, None
 
 
 class RelationalGraph:

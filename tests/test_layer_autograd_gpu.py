@@ -1,5 +1,6 @@
 """What the layer operators do with gradients beyond the plain backward pass:
-the transposed product's, an orthogonalised update's, forward-mode tangents."""
+the transposed product's, an orthogonalised update's, forward-mode tangents,
+second derivatives of the sparse products."""
 
 import pytest
 import torch
@@ -7,6 +8,7 @@ import torch.autograd.forward_ad as forward_ad
 
 from layer_reference import assert_within, grouped_reference, weight_grad_reference
 from test_grouped_gpu import lib, make  # noqa: F401
+from test_relational_gpu import edges, relational  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +52,17 @@ def test_forward_mode_tangents_are_refused(lib):  # noqa: F811
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             lib.layer_norm(d)
     lib.layer_norm(x)
+
+
+def test_sparse_products_are_differentiable_twice(relational):  # noqa: F811
+    """f(x) = |A x|^2: the gradient 2 A^T A x has its own, 2 A^T A v."""
+    n, R = 30, 3
+    graph = relational.RelationalGraph(*edges(n, R, 200, seed=5), n, R)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(n, 16, generator=g, device="cuda", requires_grad=True)
+    v = torch.randn(n, 16, generator=g, device="cuda")
+    y = graph.gather @ x
+    (first,) = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    (second,) = torch.autograd.grad(first, x, v)
+    (want,) = torch.autograd.grad(graph.gather @ x, x, 2 * (graph.gather @ v))
+    assert float((second - want).norm()) <= 1e-5 * float(want.norm()) and float(want.norm()) > 0
