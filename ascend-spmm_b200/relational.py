@@ -65,9 +65,12 @@ class _Spmm(torch.autograd.Function):
 
 class RelationalGraph:
     """Edges ``src[i] -> dst[i]`` of relation ``relation[i]`` with weight
-    ``values[i]`` (fp16 or fp32; distinct triples), on ``num_nodes`` nodes."""
+    ``values[i]`` (fp16 or fp32; distinct triples), on ``num_nodes`` nodes.  The
+    weights are constants of the graph: they get no gradient."""
 
     def __init__(self, relation, src, dst, values, num_nodes: int, num_relations: int, device=None):
+        if values.requires_grad:
+            raise ValueError("values get no gradient: pass them detached")
         device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         relation, src, dst = (t.to(device=device, dtype=torch.int64) for t in (relation, src, dst))
         values = values.to(device)

@@ -1,6 +1,6 @@
 """What the layer operators do with gradients beyond the plain backward pass:
 the transposed product's, an orthogonalised update's, forward-mode tangents,
-second derivatives of the sparse products."""
+second derivatives of the sparse products, edge weights."""
 
 import pytest
 import torch
@@ -66,3 +66,10 @@ def test_sparse_products_are_differentiable_twice(relational):  # noqa: F811
     (second,) = torch.autograd.grad(first, x, v)
     (want,) = torch.autograd.grad(graph.gather @ x, x, 2 * (graph.gather @ v))
     assert float((second - want).norm()) <= 1e-5 * float(want.norm()) and float(want.norm()) > 0
+
+
+def test_edge_weights_that_want_a_gradient_are_refused(relational):  # noqa: F811
+    e = edges(20, 3, 50, seed=4)
+    with pytest.raises(ValueError, match="no gradient"):
+        relational.RelationalGraph(*e[:3], e[3].requires_grad_(True), 20, 3)
+    relational.RelationalGraph(*e[:3], e[3].detach(), 20, 3)
