@@ -120,6 +120,16 @@ class OrthogonalMomentum(torch.optim.Optimizer):
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.9, vector_lr: float = 0.01):
         super().__init__(params, {"lr": lr, "momentum": momentum, "vector_lr": vector_lr})
 
+    def load_state_dict(self, state_dict):
+        """As the base class, which takes saved tensors to their parameter's type; the momentum stays fp32."""
+        super().load_state_dict(state_dict)
+        params = [p for group in self.param_groups for p in group["params"]]
+        names = [name for group in state_dict["param_groups"] for name in group["params"]]
+        for name, p in zip(names, params):
+            saved = state_dict["state"].get(name, {}).get("momentum")
+            if saved is not None:
+                self.state[p]["momentum"] = saved.detach().to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
