@@ -104,7 +104,7 @@ int spmm_layer_norm_launch(const void *x, const void *weight, const void *bias, 
 size_t spmm_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width)
 {
     if (rows <= 0 || width <= 0) return 0;
-    return (size_t)spmmb::norm_backward_blocks(rows) * 2 * (size_t)width * sizeof(float);
+    return (size_t)spmmb::norm_backward_blocks(rows, width) * 2 * (size_t)width * sizeof(float);
 }
 
 int spmm_layer_norm_backward_launch(const void *grad, const void *x, const float *mean, const float *rstd,

@@ -39,7 +39,7 @@ struct NormLaunch {
 cudaError_t launch_norm_forward(const NormLaunch &n, cudaStream_t stream);
 // Blocks that write a partial row of dw and db each (2 * width floats in the
 // workspace).
-int64_t norm_backward_blocks(int64_t rows);
+int64_t norm_backward_blocks(int64_t rows, int64_t width);
 cudaError_t launch_norm_backward(const NormLaunch &n, const void *grad, void *dweight, void *dbias, float *workspace,
                                  cudaStream_t stream);
 

@@ -576,10 +576,13 @@ cudaError_t dispatch(const NormArgs &a, int dtype, bool backward, int64_t max_bl
 
 }  // namespace
 
-int64_t norm_backward_blocks(int64_t rows)
+int64_t norm_backward_blocks(int64_t rows, int64_t width)
 {
-    // at most 16 resident blocks per SM; few rows need no more blocks than rows
-    return std::max<int64_t>(1, std::min<int64_t>(rows, 16 * (int64_t)device_sm_count()));
+    // What an SM's 2048 threads hold of a row's lanes (run_width; 16-bit rows
+    // have the fewest): 8 blocks of 256, 4 of 512, 2 of 1024 threads.  Rows
+    // wider than a block run on 2 of 512.  Few rows need no more blocks than rows.
+    const int64_t per_sm = width / 8 <= 512 ? 8 : width / 8 <= 1024 ? 4 : 2;
+    return std::max<int64_t>(1, std::min<int64_t>(rows, per_sm * device_sm_count()));
 }
 
 cudaError_t launch_norm_forward(const NormLaunch &n, cudaStream_t stream)
@@ -599,7 +602,7 @@ cudaError_t launch_norm_backward(const NormLaunch &n, const void *grad, void *dw
     a.rows = n.rows; a.width = n.width; a.pf32 = n.param_dtype == SPMM_F32;
     a.part = dweight || dbias ? workspace : nullptr;
     int64_t blocks = 0;
-    cudaError_t e = dispatch(a, n.dtype, true, norm_backward_blocks(n.rows), &blocks, stream);
+    cudaError_t e = dispatch(a, n.dtype, true, norm_backward_blocks(n.rows, n.width), &blocks, stream);
     if (e != cudaSuccess || !a.part) return e;
     const unsigned grid = (unsigned)((2 * n.width + 31) / 32);
     switch (n.param_dtype) {
