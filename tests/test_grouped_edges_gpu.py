@@ -1,10 +1,12 @@
 """grouped_matmul and its gradients at the limits of their forms: infinities
-in fp32, long sums."""
+in fp32, long sums, the number of groups that a weight gradient sorts, pairs
+of blocks in both directions."""
 
 import pytest
 import torch
 
-from test_grouped_gpu import lib, make  # noqa: F401
+from layer_reference import assert_within, grouped_reference
+from test_grouped_gpu import check, lib, make  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +60,36 @@ def test_a_million_rows_of_one_group(lib, dtype):  # noqa: F811
         want = x[:, at].double().T @ grad[:, at].double()
         mean = float(((dw[at, at].double() - want) / want).mean())
         assert abs(mean) <= 2.0 ** -13 + 2.0 ** -15, mean
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("groups", [127, 128, 129])
+def test_groups_around_the_sorted_ones(lib, groups, dtype):  # noqa: F811
+    """A weight gradient sorts up to 128 groups; the others are walked in their order."""
+    g = torch.Generator().manual_seed(groups)
+    sizes = torch.randint(0, 7, (groups,), generator=g)
+    sizes[groups // 3], sizes[groups - 2], sizes[groups - 1] = 3000, 2100, 1
+    check(lib, *make(sizes.tolist(), 48, 32, dtype, seed=groups))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_pairs_of_blocks_beside_rows_of_no_group(lib, dtype, transposed):  # noqa: F811
+    """Tiles of 256 rows shared by two blocks (rows / 256 * width / 256 of at least two turns of the GPU, groups of
+    512 rows on average, 512 deep), in both directions, with rows outside every group."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    K, N, width = 512, 768, 512 if transposed else 768
+    rows = -(-2 * sms // (width // 256)) * 256 + 1000
+    sizes = [5000, 0, 1, 129, 255, 257, rows - 300 - 77 - 5642]
+    x, w, ptr, grad = make(sizes, K, N, dtype, seed=12, before=300, after=77)
+    a = grad if transposed else x
+    assert a.shape[0] == rows and rows // 256 * (width // 256) >= 2 * sms and rows >= 512 * len(sizes)
+    a[:300], a[-77:] = float("nan"), float("inf")
+    y = lib.grouped_matmul(a, w, ptr, transposed=transposed)
+    assert not bool(y[:300].any()) and not bool(y[-77:].any())
+    ref, slack = grouped_reference(a, w, ptr, transposed)
+    assert_within(y[300:-77], ref[300:-77], slack[300:-77])
+    # a group's values reach no other: those of the first as NaN
+    a[300:5300] = float("nan")
+    again = lib.grouped_matmul(a, w, ptr, transposed=transposed)
+    assert torch.equal(again[5300:], y[5300:]) and bool(again[300:5300].isnan().all())
