@@ -70,10 +70,11 @@ struct OrthoLaunch {
     DevStatus *status;
 };
 size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int dtype);
-// A shorter side of at most 128 and steps that its form computes accurately (ortho_small.cu).
-bool ortho_small_eligible(const OrthoLaunch &o);
+// A shorter side of at most 128 and steps that its form computes accurately
+// (ortho_small.cu): its scale of Q, else 0.
+float ortho_small_scale(const OrthoLaunch &o);
 size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n);
-cudaError_t launch_ortho_small(const OrthoLaunch &o, void *workspace, cudaStream_t stream);
+cudaError_t launch_ortho_small(const OrthoLaunch &o, float scale_q, void *workspace, cudaStream_t stream);
 // Sums of squares of each matrix in parts (ortho.cu): squares [batch][parts].
 int ortho_square_parts(int64_t batch, int64_t m, int64_t n);
 cudaError_t launch_ortho_squares(const OrthoLaunch &o, double *squares, cudaStream_t stream);

@@ -250,7 +250,8 @@ size_t ortho_workspace(int64_t batch, int64_t m, int64_t n, int)
 
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
 {
-    if (ortho_small_eligible(o)) return launch_ortho_small(o, workspace, stream);
+    const float scale_q = ortho_small_scale(o);
+    if (scale_q > 0.f) return launch_ortho_small(o, scale_q, workspace, stream);
     const Space w(o.batch, o.m, o.n, workspace);
     cudaError_t e = launch_ortho_squares(o, w.part, stream);
     if (e != cudaSuccess) return e;

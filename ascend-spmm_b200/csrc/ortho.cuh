@@ -33,13 +33,14 @@ struct OrthoReach {
     double poly() const { return extreme(0.0); }
     double factor() const { return extreme(a); }
     // The largest factor of an error of G's eigenvalues in a step G <- T G T,
-    // T = a + b u + c u^2: |d (u T^2) / du|, sampled.
+    // T = a + b u + c u^2: |d (u T^2) / du| = |T (a + 3 b u + 5 c u^2)|, sampled.
     double growth() const
     {
         double most = 0.0;
-        for (int i = 0; i <= 256; ++i) {
-            const double u = reach * reach * i / 256, t = a + u * (b + u * c), dt = b + 2 * u * c;
-            most = std::max(most, std::fabs(t * (t + 2 * u * dt)));
+        const double step = reach * reach / 32;
+        for (int i = 0; i <= 32; ++i) {
+            const double u = step * i;
+            most = std::max(most, std::fabs((a + u * (b + u * c)) * (a + u * (3 * b + 5 * u * c))));
         }
         return most;
     }

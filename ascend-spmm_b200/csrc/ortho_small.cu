@@ -452,23 +452,6 @@ cudaError_t run_phase(const OrthoLaunch &o, float scale_q, const Between &w, int
     return cudaGetLastError();
 }
 
-// A power of two that keeps Q, a product of the steps' T, in fp16's range; 0
-// where an operand would leave it or G's rounding would grow too far.
-float q_scale(const OrthoLaunch &o)
-{
-    OrthoReach at(o.a, o.b, o.c);
-    double q = 1.0, growth = 1.0;   // growth: of G's error, up to its last use
-    for (int i = 0; i < o.steps; ++i) {
-        const double t = at.factor(), g = at.reach * at.reach;
-        if (!(std::max(t * kScaleP, g * std::max(1.0, t) * kScaleG) <= kMostStored)) return 0.f;
-        q *= std::max(1.0, t);
-        if (i + 1 < o.steps) growth *= std::max(1.0, at.growth());
-        at.step();
-    }
-    if (!(growth <= 32768.0) || !(q <= kMostStored)) return 0.f;
-    return (float)std::min(256.0, std::exp2(std::floor(std::log2(kMostStored / q))));
-}
-
 // Blocks of a matrix in parts (1: one block does it all).  A block alone takes
 // about 28 us more for every chunk (128 x 256 49 us, 128 x 1024 134 us), the
 // four launches of a matrix in parts 92 us whatever its length (128 x 1024 to
@@ -509,7 +492,24 @@ template <typename T> cudaError_t run_small(const OrthoLaunch &o, float scale_q,
 
 }  // namespace
 
-bool ortho_small_eligible(const OrthoLaunch &o) { return std::min(o.m, o.n) <= kSide && q_scale(o) > 0.f; }
+// A power of two that keeps Q, a product of the steps' T, in fp16's range; 0
+// for a longer side, and where an operand would leave that range or G's
+// rounding would grow too far.
+float ortho_small_scale(const OrthoLaunch &o)
+{
+    if (std::min(o.m, o.n) > kSide) return 0.f;
+    OrthoReach at(o.a, o.b, o.c);
+    double q = 1.0, growth = 1.0;   // growth: of G's error, up to its last use
+    for (int i = 0; i < o.steps; ++i) {
+        const double t = at.factor(), g = at.reach * at.reach;
+        if (!(std::max(t * kScaleP, g * std::max(1.0, t) * kScaleG) <= kMostStored)) return 0.f;
+        q *= std::max(1.0, t);
+        if (i + 1 < o.steps) growth *= std::max(1.0, at.growth());
+        if (!(growth <= 32768.0) || !(q <= kMostStored)) return 0.f;
+        at.step();
+    }
+    return (float)std::min(256.0, std::exp2(std::floor(std::log2(kMostStored / q))));
+}
 
 size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n)
 {
@@ -518,9 +518,8 @@ size_t ortho_small_workspace(int64_t batch, int64_t m, int64_t n)
                         : (size_t)batch * (2 * kSide * 256 + (size_t)w.parts * kSide * kSide * 4 + 8 * w.square_parts);
 }
 
-cudaError_t launch_ortho_small(const OrthoLaunch &o, void *workspace, cudaStream_t stream)
+cudaError_t launch_ortho_small(const OrthoLaunch &o, float scale_q, void *workspace, cudaStream_t stream)
 {
-    const float scale_q = q_scale(o);
     switch (o.dtype) {
         case SPMM_F16: return run_small<__half>(o, scale_q, workspace, stream);
         case SPMM_BF16: return run_small<__nv_bfloat16>(o, scale_q, workspace, stream);
