@@ -46,6 +46,11 @@ namespace spmmb {
 namespace tc {
 
 enum Mode { kRows, kRagged, kDense };
+// The tensor core truncates its accumulator towards zero in every step of 16,
+// by up to 2^-22 of what it holds: 16384 products of one sign lose 1e-4 of
+// their sum, 65536 4e-4, an fp16 result's rounding.  kRagged and kGram end an
+// accumulation there; kRows and the other dense products run over a matrix's
+// width in one.
 // kStoreSum: fp32 operands in three bf16 planes h, m, l each.  A slice brings
 // in the planes once, a ring stage each, for its six products h l, l h, m m,
 // h m, m h and h h.  The tensor core truncates each step into its accumulator,
@@ -175,7 +180,9 @@ struct Tile {
 // A weight gradient's groups by length, longest first: its tiles take as long
 // as their group's rows (of a part), and handed out in this order to the
 // blocks as they become free they end within one short tile of each other.
-// Up to kSorted groups; more of them even out by themselves.
+// Up to kSorted groups, which is what shared memory has room for beside the
+// ring; with more the tiles are handed out in the groups' order (not measured
+// against a sorted one).
 struct Order {
     const unsigned short *group;   // [groups], nullptr: not sorted
     const int *first;              // [groups + 1] tiles before the group of this rank

@@ -7,8 +7,9 @@
 // length crosses to the host and a launch can be captured in a graph.
 //
 // Measured (us; forward, gradient of x, gradient of the weight): bf16, 65537
-// uneven rows of 64 groups, K = 1024, N = 2048 236, 231, 267 (275 GFLOP each:
-// the products, at the power limit's clock); fp16, 100003 rows of 46 groups, K
+// uneven rows of 64 groups, K = 1024, N = 2048 217, 221, 300 in the first
+// passes and 256, 254, 340 after some hundred (275 GFLOP each: the products, at
+// the clock that the power limit leaves); fp16, 100003 rows of 46 groups, K
 // = 256, N = 128 16, 18, 27 (77 MB each: memory, and for the weight the parts);
 // fp32, 20011 rows of 8 groups, K = 256, N = 264 39, 40, 56 (12 to 20 of each
 // is splitting the operands); bf16, 9 rows of 32 groups, K = 1024, N = 512 10,

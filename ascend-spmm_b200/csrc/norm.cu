@@ -17,6 +17,11 @@
 // rows of 1024, forward 332 us 6470, backward 556 us 5790; fp32, 100003 rows
 // of 256, 35 us 5870 and 50 us 6130; bf16, 164110 rows of 1001 (no row starts
 // on a vector), 131 us 5030 and 200 us 4920; 9 rows of 256 2.7 us, the launch.
+// The widest rows are slower, 1 GB of x each, forward and backward GB/s: fp16
+// 8192 2540 and 5510 (the forward form of 512 lanes spills registers), 16384
+// 3060 and 2680; fp32 8192 5950 and 4610; and rows that no block holds, a
+// thread per element in three passes, fp32 16384 1770 and 1020, fp16 33000
+// 1060 and 440.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
@@ -523,10 +528,10 @@ cudaError_t run_team(const NormArgs &a, int64_t max_blocks, int64_t *blocks, cud
     return cudaGetLastError();
 }
 
-// Vectors per lane, measured (fp16, 524287 x 1024; GB/s of 6538): forward 4 on
-// a warp 6284, 2 on two warps 5312 (its two sums need a barrier); backward,
-// which also holds two accumulators per column, 2 on two warps 5967, 4 on a
-// warp 5390.
+// Vectors per lane, measured side by side (fp16, 524287 x 1024; GB/s of 6538,
+// calls back to back): forward 4 on a warp 6390, 2 on two warps 5810 (its two
+// sums need a barrier); backward, which also holds two accumulators per column,
+// 2 on two warps 5770, 4 on a warp 4710.
 template <typename T, bool ODD, bool BACKWARD>
 cudaError_t run_width(const NormArgs &a, int64_t max_blocks, int64_t *blocks, cudaStream_t s, bool *wide)
 {

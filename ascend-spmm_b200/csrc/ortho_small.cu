@@ -453,11 +453,14 @@ cudaError_t run_phase(const OrthoLaunch &o, float scale_q, const Between &w, int
 }
 
 // Blocks of a matrix in parts (1: one block does it all).  A block alone takes
-// about 28 us more for every chunk (128 x 256 49 us, 128 x 1024 134 us), the
-// four launches of a matrix in parts 92 us whatever its length (128 x 1024 to
-// 128 x 4096).  With
-// as many matrices as half the SMs they fill the GPU by themselves until a
-// matrix is very long.
+// about 22 us more for every chunk (128 x 1024 125 us, 128 x 4096 393), the
+// four launches of a matrix in parts 77 and 88 us.  Many matrices fill the GPU
+// by themselves; one block each and in parts, us:
+//   128 x 4096:  64 matrices 422 and 304, 75 423 and 361, 100 426 and 437, 148 433 and 611
+//   128 x 1024:  64 matrices 127 and 110, 75 127 and 137, 100 128 and 143, 148 135 and 187
+//   30 x 4000:   64 matrices 189 and 125, 75 189 and 149, 100 189 and 185, 148 190 and 265
+// Half of the SMs is between the crossovers; up to 200 and 300 matrices the two
+// stay within 8 %.
 int64_t parts_of(int64_t batch, int64_t m, int64_t n)
 {
     const int64_t r = std::max(m, n), chunks = (r + kChunk - 1) / kChunk;

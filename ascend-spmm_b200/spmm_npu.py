@@ -152,8 +152,10 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     orthogonalises its momentum before it is applied to a weight matrix).
 
     ``update`` is fp16, bf16 or fp32; the result is bf16.  The products run on
-    16-bit operands, so fp32 would hold no more of it.  It has no derivative: a
-    backward pass through it raises an error.
+    16-bit operands, so fp32 would hold no more of it: with five steps it is off
+    by 1.7e-3 to 2.5e-3 of its norm (the rounding alone is 1.7e-3), with ten by
+    up to 5e-3, and more with many.  It has no derivative: a backward pass
+    through it raises an error.
     """
     a, b, c = coefficients
     return _orthogonalize(update, steps, a, b, c, eps)
