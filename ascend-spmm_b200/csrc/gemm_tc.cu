@@ -63,6 +63,24 @@ CUtensorMapDataType type16(bool bf16)
 
 }  // namespace
 
+int tile_columns(int64_t row_tiles, int64_t width, int most)
+{
+    const int64_t sms = device_sm_count();
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int64_t n = (width + most - 1) / most; n <= (width + 63) / 64; ++n) {
+        const int64_t step = n > 1 ? 32 : 16;   // a tile is stored 32 columns at a time
+        const int64_t bn = ((width + n - 1) / n + step - 1) / step * step;
+        const int64_t cost = (row_tiles * n + sms - 1) / sms * (bn + 70);
+        if (cost < least) {
+            least = cost;
+            best = (int)bn;
+        }
+        if (n > 64 && bn <= 128) break;   // very wide outputs: narrower tiles gain nothing more
+    }
+    return best;
+}
+
 bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
               int64_t batch_stride, int box_rows, bool bf16)
 {
@@ -76,6 +94,12 @@ bool make_blocked_map(CUtensorMap *map, const void *p, int64_t inner, int64_t ro
     const cuuint64_t strides[3] = {(cuuint64_t)(ld * 2), 128, (cuuint64_t)((batch > 1 ? batch_stride : ld) * 2)};
     const cuuint32_t box[4] = {64, 64, (cuuint32_t)blocks, 1};
     return encode(map, p, type16(bf16), 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+bool make_byte_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int box_rows)
+{
+    return encode_map(map, p, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, inner, rows, batch, inner, rows * inner, 2 * kBK, box_rows,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool make_out_map(CUtensorMap *map, void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,

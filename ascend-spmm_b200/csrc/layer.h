@@ -80,4 +80,88 @@ int ortho_square_parts(int64_t batch, int64_t m, int64_t n);
 cudaError_t launch_ortho_squares(const OrthoLaunch &o, double *squares, cudaStream_t stream);
 cudaError_t launch_ortho(const OrthoLaunch &o, void *workspace, cudaStream_t stream);
 
+// ---- routing to experts (route.cu) ------------------------------------------
+struct RouteLaunch {
+    const void *logits;   // [tokens, n]
+    const float *bias;    // [n], may be null
+    float *weights;       // [tokens, k]
+    int *experts;         // [tokens, k]; read by the backward pass
+    int64_t tokens;
+    int n, k, groups, top_groups, group_best;
+    bool sigmoid, renormalize;
+    float scale;
+    int dtype;
+};
+constexpr int kMostExperts = 1024, kMostChosen = 32, kMostGroups = 32;
+cudaError_t launch_route(const RouteLaunch &r, cudaStream_t stream);
+cudaError_t launch_route_backward(const RouteLaunch &r, const float *grad, void *dlogits, DevStatus *status,
+                                  cudaStream_t stream);
+
+// ---- stable counting sort (bucket.cu) ---------------------------------------
+struct BucketSort {
+    const void *keys;       // [n] by input, int32 or int64
+    bool wide;
+    const int *order_in;    // the inputs in the order to keep (an earlier pass's), -1: none; null: as they are
+    int64_t n;
+    int buckets;            // at most kMostBuckets; a key's bucket is (key >> shift) & mask
+    int shift, mask;
+    int64_t limit;          // keys outside [0, limit) raise the status and are left out
+    int64_t skip;           // this key is left out
+    int *ptr;               // [buckets + 1] first place of each bucket; may be null
+    int *position;          // [n] place of each input, -1 where it is left out; may be null
+    int *order;             // [n] input of each place, -1 past the last
+    DevStatus *status;
+};
+constexpr int kBucketBits = 10, kMostBuckets = 1 << kBucketBits;
+cudaError_t launch_bucket_sort(const BucketSort &a, cudaStream_t stream);
+
+// ---- rows to their experts and back (routed.cu) -------------------------------
+struct RoutedLaunch {
+    const void *x;          // dispatch: [tokens, width]; combine: rows [tokens * k, width]
+    const void *grad;       // combine's backward: [tokens, width]
+    void *out;
+    const int *position;    // [tokens, k]
+    const int *source;      // [tokens * k]
+    const float *weights;   // [tokens, k], may be null: ones
+    float *dweights;        // combine's backward, may be null
+    int64_t tokens, width;
+    int k, dtype;
+    DevStatus *status;
+};
+cudaError_t launch_dispatch(const RoutedLaunch &r, cudaStream_t stream);
+cudaError_t launch_combine(const RoutedLaunch &r, cudaStream_t stream);
+cudaError_t launch_combine_backward(const RoutedLaunch &r, cudaStream_t stream);
+
+// ---- rows of a table (embedding.cu) -------------------------------------------
+struct EmbeddingLaunch {
+    const void *ids;        // [n]
+    const void *in;         // the table [rows, width]; backward: the gradient [n, width]
+    void *out;              // [n, width]; backward: the table's gradient [rows, width]
+    int64_t n, rows, width;
+    float scale;
+    int itype, dtype;
+    DevStatus *status;
+};
+cudaError_t launch_embedding(const EmbeddingLaunch &l, cudaStream_t stream);
+size_t embedding_backward_workspace(int64_t n, int64_t width);
+cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, void *workspace, cudaStream_t stream);
+
+// ---- 8-bit floating point with block scales (fp8.cu) ----------------------------
+struct Fp8Launch {
+    const void *x;          // [rows, K] e4m3
+    const float *x_scale;   // [rows, ceil(K / 128)]
+    const void *w;          // [groups, N, K] e4m3
+    const float *w_scale;   // [groups, ceil(N / 128), ceil(K / 128)]
+    const void *ptr;        // [groups + 1]
+    void *out;              // [rows, N]
+    int64_t rows, groups, K, N;
+    int itype, out_dtype;
+    DevStatus *status;
+};
+cudaError_t launch_quantize_rows(const void *x, void *q, float *scale, int64_t rows, int64_t width, int dtype,
+                                 cudaStream_t stream);
+cudaError_t launch_quantize_weight(const void *w, void *q, float *scale, int64_t groups, int64_t K, int64_t N, int dtype,
+                                   cudaStream_t stream);
+cudaError_t launch_grouped_fp8(const Fp8Launch &a, cudaStream_t stream);
+
 }  // namespace spmmb

@@ -139,13 +139,20 @@ __device__ __forceinline__ int64_t block_given(unsigned answer)
 __device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;\n"); }
 
-// D[tmem] (+)= A B over 16 elements of the reduction; acc == 0 overwrites D.
+// D[tmem] (+)= A B over 16 elements of the reduction (BYTES: 32 of 8 bits); acc == 0 overwrites D.
+template <bool BYTES = false>
 __device__ __forceinline__ void mma(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(acc)
-                 : "memory");
+    if constexpr (BYTES)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                     : "memory");
 }
 // Arrival on `bar` once every mma this thread has issued is complete.
 __device__ __forceinline__ void commit(unsigned bar)
@@ -244,12 +251,19 @@ __device__ __forceinline__ void tma_load4_pair(unsigned dst, const CUtensorMap *
                  : "memory");
 }
 // D over both blocks' TMEM: 256 rows, each block's A 128 of them and its B half of the columns.
+template <bool BYTES = false>
 __device__ __forceinline__ void mma_pair(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(acc)
-                 : "memory");
+    if constexpr (BYTES)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+                     "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                     : "memory");
 }
 // Arrival on the same barrier of both blocks.
 __device__ __forceinline__ void commit_pair(unsigned bar)
@@ -296,6 +310,12 @@ __host__ __device__ constexpr unsigned idesc16(bool bf16, bool a_mn, bool b_mn, 
 {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
            ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
+}
+
+// The same for 8-bit operands, both e4m3 with the reduction contiguous.
+__host__ __device__ constexpr unsigned idesc8(int m, int n)
+{
+    return (1u << 4) | ((unsigned)(n >> 3) << 17) | ((unsigned)(m >> 4) << 24);
 }
 
 }  // namespace tc

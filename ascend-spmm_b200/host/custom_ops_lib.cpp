@@ -921,6 +921,429 @@ at::Tensor orthogonalize(const at::Tensor &update, int64_t steps, double a, doub
     return orthogonalize_forward(update, steps, a, b, c, eps);
 }
 
+// ---------------------------------------------------------------------------
+// Routed experts and learned features (no counterpart in the reference).
+// ---------------------------------------------------------------------------
+struct RouteOptions {
+    int64_t top_k;
+    int scoring;
+    int64_t groups, top_groups, group_best;
+    bool renormalize;
+    double scale;
+};
+
+// (weights [..., top_k] fp32, experts [..., top_k] int32)
+std::tuple<at::Tensor, at::Tensor> route_experts_forward(const at::Tensor &logits,
+                                                         const c10::optional<at::Tensor> &bias, const RouteOptions &o)
+{
+    const char *op = "route_experts";
+    TORCH_CHECK_CUDA(logits);
+    TORCH_CHECK(logits.dim() >= 1, op, ": logits must have at least one dimension");
+    const int dt = layer_dtype(logits, op);
+    const int64_t n = logits.size(-1);
+    refuse_tangents({&logits}, op);
+    at::Tensor b;
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->is_cuda(), op, ": bias must be CUDA tensor");
+        TORCH_CHECK(bias->device() == logits.device(), op, ": all tensors must be on ", logits.device());
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == n, op, ": bias must have shape [", n, "], but got ", bias->sizes());
+        TORCH_CHECK(bias->scalar_type() == at::kFloat, op, ": bias must be FP32");
+    }
+    c10::cuda::CUDAGuard guard(logits.device());
+    if (bias.has_value()) b = dense16(*bias);
+    const at::Tensor x = dense16(logits);
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    TORCH_CHECK(o.top_k >= 1, op, ": top_k must be at least 1");
+    TORCH_CHECK(n >= 1, op, " requires at least one expert");
+    shape.back() = o.top_k;
+    const int64_t tokens = x.numel() / n;
+    at::Tensor w = at::empty(shape, x.options().dtype(at::kFloat)), e = at::empty(shape, x.options().dtype(at::kInt));
+    check_rc(spmm_route_experts_launch(x.data_ptr(), b.defined() ? b.data_ptr<float>() : nullptr, w.data_ptr<float>(),
+                                       e.data_ptr<int>(), tokens, n, o.top_k, o.scoring, o.groups, o.top_groups,
+                                       (int)o.group_best, o.renormalize, o.scale, dt, stream_of(x)));
+    return {w, e};
+}
+
+at::Tensor route_experts_backward(const at::Tensor &logits, const at::Tensor &experts, const at::Tensor &grad,
+                                  int64_t scoring, bool renormalize, double scale)
+{
+    const char *op = "route_experts_backward";
+    c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor x = dense16(logits), g = dense16(grad), e = dense16(experts);
+    at::Tensor dx = at::empty(x.sizes(), x.options());
+    const int64_t n = x.size(-1);
+    check_rc(spmm_route_experts_backward_launch(x.data_ptr(), e.data_ptr<int>(), g.data_ptr<float>(), dx.data_ptr(),
+                                                x.numel() / n, n, e.size(-1), (int)scoring, renormalize, scale,
+                                                layer_dtype(x, op), stream_of(x)));
+    return dx;
+}
+
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &logits, const c10::optional<at::Tensor> &bias,
+                                 const RouteOptions &o)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [w, e] = route_experts_forward(logits, bias, o);
+        ctx->save_for_backward({logits, e});
+        ctx->mark_non_differentiable({e});
+        ctx->saved_data["scoring"] = (int64_t)o.scoring;
+        ctx->saved_data["renormalize"] = o.renormalize;
+        ctx->saved_data["scale"] = o.scale;
+        return {w, e};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list out(3);
+        if (grads[0].defined()) {
+            at::NoGradGuard none;
+            out[0] = route_experts_backward(s[0], s[1], grads[0], ctx->saved_data["scoring"].toInt(),
+                                            ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
+        }
+        return once(std::move(out), "route_experts");
+    }
+};
+
+std::tuple<at::Tensor, at::Tensor> route_experts(const at::Tensor &logits, int64_t top_k,
+                                                 const c10::optional<at::Tensor> &bias, const std::string &scoring,
+                                                 int64_t groups, int64_t top_groups, int64_t group_best,
+                                                 bool renormalize, double scale)
+{
+    TORCH_CHECK(scoring == "softmax" || scoring == "sigmoid", "route_experts: scoring must be softmax or sigmoid, but got ",
+                scoring);
+    TORCH_CHECK(group_best == 1 || group_best == 2, "route_experts: group_best must be 1 or 2");
+    const RouteOptions o{top_k, scoring == "softmax" ? SPMM_SCORE_SOFTMAX : SPMM_SCORE_SIGMOID, groups, top_groups,
+                         group_best, renormalize, scale};
+    if (wants_grad({&logits})) {
+        variable_list out = RouteFunction::apply(logits, bias, o);
+        return {out[0], out[1]};
+    }
+    return route_experts_forward(logits, bias, o);
+}
+
+// (group_ptr [num_experts + 1], position like experts, source [experts.numel()]), int32
+std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(const at::Tensor &experts, int64_t num_experts)
+{
+    const char *op = "expert_plan";
+    TORCH_CHECK_CUDA(experts);
+    TORCH_CHECK(experts.scalar_type() == at::kInt || experts.scalar_type() == at::kLong, op,
+                ": experts must be int32 or int64");
+    TORCH_CHECK(num_experts >= 1 && num_experts <= 1024, op, ": the number of experts must be in [1, 1024]");
+    c10::cuda::CUDAGuard guard(experts.device());
+    const at::Tensor e = experts.contiguous();
+    const auto opt = e.options().dtype(at::kInt);
+    at::Tensor ptr = at::empty({num_experts + 1}, opt), position = at::empty(e.sizes(), opt),
+               source = at::empty({e.numel()}, opt);
+    check_rc(spmm_expert_plan_launch(e.data_ptr(), ptr.data_ptr<int>(), position.data_ptr<int>(), source.data_ptr<int>(),
+                                     e.numel(), num_experts, e.scalar_type() == at::kLong ? SPMM_I64 : SPMM_I32,
+                                     stream_of(e)));
+    return {ptr, position, source};
+}
+
+// position [tokens, k] and source [tokens * k] of expert_plan, beside `like`.
+void check_plan(const at::Tensor &position, const at::Tensor &source, const at::Tensor &like, const char *op)
+{
+    for (const at::Tensor *t : {&position, &source}) {
+        TORCH_CHECK(t->is_cuda(), op, ": position and source must be CUDA tensors");
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), op, ": position and source must be contiguous int32");
+    }
+    same_device({&position, &source}, like, op);
+    TORCH_CHECK(position.dim() == 2 && position.size(1) >= 1, op, ": position must have shape [tokens, choices]");
+    TORCH_CHECK(source.dim() == 1 && source.size(0) == position.numel(), op, ": source must hold one entry per position");
+}
+
+at::Tensor dispatch_rows_forward(const at::Tensor &x, const at::Tensor &position, const at::Tensor &source)
+{
+    const char *op = "dispatch_rows";
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK(x.dim() == 2, op, ": x must be two-dimensional");
+    const int dt = layer_dtype(x, op);
+    check_plan(position, source, x, op);
+    TORCH_CHECK(x.size(0) == position.size(0), op, ": x and position must have the same number of rows");
+    refuse_tangents({&x}, op);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = dense16(x), p = dense16(position), s = dense16(source);
+    at::Tensor rows = at::empty({position.numel(), x.size(1)}, xc.options());
+    check_rc(spmm_dispatch_rows_launch(xc.data_ptr(), p.data_ptr<int>(), s.data_ptr<int>(), rows.data_ptr(), x.size(0),
+                                       position.size(1), x.size(1), dt, stream_of(xc)));
+    return rows;
+}
+
+at::Tensor combine_rows_forward(const at::Tensor &rows, const at::Tensor &position, const at::Tensor &source,
+                                const c10::optional<at::Tensor> &weights)
+{
+    const char *op = "combine_rows";
+    TORCH_CHECK_CUDA(rows);
+    TORCH_CHECK(rows.dim() == 2, op, ": rows must be two-dimensional");
+    const int dt = layer_dtype(rows, op);
+    check_plan(position, source, rows, op);
+    TORCH_CHECK(rows.size(0) == position.numel(), op, ": rows must have one row per position");
+    if (weights.has_value()) {
+        TORCH_CHECK(weights->is_cuda(), op, ": weights must be CUDA tensor");
+        same_device({&*weights}, rows, op);
+        TORCH_CHECK(weights->scalar_type() == at::kFloat && weights->sizes() == position.sizes(), op,
+                    ": weights must be FP32 with the shape of position");
+        refuse_tangents({&*weights}, op);
+    }
+    refuse_tangents({&rows}, op);
+    c10::cuda::CUDAGuard guard(rows.device());
+    at::Tensor w;
+    if (weights.has_value()) w = dense16(*weights);
+    const at::Tensor rc = dense16(rows), p = dense16(position);
+    at::Tensor y = at::empty({position.size(0), rows.size(1)}, rc.options());
+    check_rc(spmm_combine_rows_launch(rc.data_ptr(), p.data_ptr<int>(), w.defined() ? w.data_ptr<float>() : nullptr,
+                                      y.data_ptr(), position.size(0), position.size(1), rows.size(1), dt, stream_of(rc)));
+    return y;
+}
+
+// (drows, dweights); those not wanted are undefined.
+std::tuple<at::Tensor, at::Tensor> combine_rows_backward(const at::Tensor &grad, const at::Tensor &rows,
+                                                         const at::Tensor &position, const at::Tensor &source,
+                                                         const at::Tensor &weights, bool want_rows, bool want_weights)
+{
+    c10::cuda::CUDAGuard guard(grad.device());
+    const at::Tensor g = dense16(grad), r = dense16(rows), p = dense16(position), s = dense16(source), w = dense16(weights);
+    at::Tensor dr, dw;
+    if (want_rows) dr = at::empty({position.numel(), g.size(1)}, g.options());
+    if (want_weights) dw = at::empty(position.sizes(), w.options());
+    check_rc(spmm_combine_rows_backward_launch(
+        g.data_ptr(), r.data_ptr(), p.data_ptr<int>(), s.data_ptr<int>(), w.data_ptr<float>(),
+        want_rows ? dr.data_ptr() : nullptr, want_weights ? dw.data_ptr<float>() : nullptr, position.size(0),
+        position.size(1), g.size(1), layer_dtype(g, "combine_rows_backward"), stream_of(g)));
+    return {dr, dw};
+}
+
+struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &position, const at::Tensor &source)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({position, source});
+        return dispatch_rows_forward(x, position, source);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list out(3);
+        if (grads[0].defined()) {
+            at::NoGradGuard none;
+            out[0] = combine_rows_forward(grads[0], s[0], s[1], c10::nullopt);
+        }
+        return once(std::move(out), "dispatch_rows");
+    }
+};
+
+at::Tensor dispatch_rows(const at::Tensor &x, const at::Tensor &position, const at::Tensor &source)
+{
+    if (wants_grad({&x})) return DispatchFunction::apply(x, position, source);
+    return dispatch_rows_forward(x, position, source);
+}
+
+struct CombineFunction : torch::autograd::Function<CombineFunction> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &rows, const at::Tensor &position,
+                              const at::Tensor &source, const c10::optional<at::Tensor> &weights)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        at::Tensor y = combine_rows_forward(rows, position, source, weights);
+        // the gradient of the rows does not need them
+        ctx->save_for_backward({weights.has_value() && weights->requires_grad() ? rows : at::Tensor(), position, source,
+                                weights.value_or(at::Tensor())});
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list out(4);
+        if (grads[0].defined()) {
+            at::NoGradGuard none;
+            if (!s[3].defined()) {
+                out[0] = dispatch_rows_forward(grads[0], s[1], s[2]);
+            } else {
+                const bool want_weights = s[0].defined() && ctx->needs_input_grad(3);
+                std::tie(out[0], out[3]) = combine_rows_backward(grads[0], want_weights ? s[0] : grads[0], s[1], s[2],
+                                                                 s[3], ctx->needs_input_grad(0), want_weights);
+            }
+        }
+        return once(std::move(out), "combine_rows");
+    }
+};
+
+at::Tensor combine_rows(const at::Tensor &rows, const at::Tensor &position, const at::Tensor &source,
+                        const c10::optional<at::Tensor> &weights)
+{
+    const at::Tensor w = weights.value_or(at::Tensor());
+    if (wants_grad({&rows, &w})) return CombineFunction::apply(rows, position, source, weights);
+    return combine_rows_forward(rows, position, source, weights);
+}
+
+// Index codes of ids: int32 or int64 (contiguous by the caller).
+int id_code(const at::Tensor &ids, const char *op)
+{
+    TORCH_CHECK(ids.is_cuda(), op, ": ids must be CUDA tensor");
+    TORCH_CHECK(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, op, ": ids must be int32 or int64");
+    return ids.scalar_type() == at::kInt ? SPMM_I32 : SPMM_I64;
+}
+
+at::Tensor embedding_forward(const at::Tensor &ids, const at::Tensor &table, double scale)
+{
+    const char *op = "embedding";
+    TORCH_CHECK_CUDA(table);
+    const int itype = id_code(ids, op);
+    same_device({&ids}, table, op);
+    TORCH_CHECK(table.dim() == 2, op, ": table must be two-dimensional");
+    const int dt = layer_dtype(table, op);
+    refuse_tangents({&table}, op);
+    c10::cuda::CUDAGuard guard(table.device());
+    const at::Tensor tc = dense16(table), ic = ids.contiguous();
+    std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
+    shape.push_back(table.size(1));
+    at::Tensor y = at::empty(shape, tc.options());
+    check_rc(spmm_embedding_launch(ic.data_ptr(), tc.data_ptr(), y.data_ptr(), ic.numel(), table.size(0), table.size(1),
+                                   scale, itype, dt, stream_of(tc)));
+    return y;
+}
+
+// dtable [num_rows, width]: the sums of grad's rows by id.
+at::Tensor embedding_grad(const at::Tensor &ids, const at::Tensor &grad, int64_t num_rows, double scale,
+                          const c10::optional<int64_t> &padding_id)
+{
+    const char *op = "embedding_grad";
+    TORCH_CHECK_CUDA(grad);
+    const int itype = id_code(ids, op);
+    same_device({&ids}, grad, op);
+    TORCH_CHECK(grad.dim() == ids.dim() + 1 && grad.sizes().slice(0, ids.dim()) == ids.sizes(), op,
+                ": grad must have the shape of ids and a feature dimension");
+    TORCH_CHECK(num_rows >= 0, op, ": num_rows must not be negative");
+    const int dt = layer_dtype(grad, op);
+    refuse_tangents({&grad}, op);
+    c10::cuda::CUDAGuard guard(grad.device());
+    const at::Tensor gc = dense16(grad), ic = ids.contiguous();
+    const int64_t width = grad.size(-1);
+    at::Tensor d = at::empty({num_rows, width}, gc.options());
+    const size_t wbytes = spmm_embedding_backward_workspace_bytes(ic.numel(), width);
+    at::Tensor ws = workspace(wbytes, gc);
+    check_rc(spmm_embedding_backward_launch(ic.data_ptr(), gc.data_ptr(), d.data_ptr(), ic.numel(), num_rows, width, scale,
+                                            padding_id.value_or(-1), itype, dt, ws.data_ptr(), wbytes, stream_of(gc)));
+    return d;
+}
+
+struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &ids, const at::Tensor &table, double scale,
+                              const c10::optional<int64_t> &padding_id)
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({ids});
+        ctx->saved_data["rows"] = table.size(0);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding_id"] = padding_id.value_or(-1);
+        return embedding_forward(ids, table, scale);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list s = ctx->get_saved_variables();
+        variable_list out(4);
+        if (grads[0].defined()) {
+            at::NoGradGuard none;
+            out[1] = embedding_grad(s[0], grads[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
+                                    ctx->saved_data["padding_id"].toInt());
+        }
+        return once(std::move(out), "embedding");
+    }
+};
+
+at::Tensor embedding(const at::Tensor &ids, const at::Tensor &table, double scale, const c10::optional<int64_t> &padding_id)
+{
+    TORCH_CHECK(table.dim() == 2, "embedding: table must be two-dimensional");
+    TORCH_CHECK(!padding_id.has_value() || (*padding_id >= 0 && *padding_id < table.size(0)),
+                "embedding: padding_id must be a row of the table");
+    if (wants_grad({&table})) return EmbeddingFunction::apply(ids, table, scale, padding_id);
+    return embedding_forward(ids, table, scale);
+}
+
+constexpr int64_t kScaleBlock = 128;
+int64_t scale_blocks(int64_t width) { return (width + kScaleBlock - 1) / kScaleBlock; }
+
+// The 8-bit forms are for serving: an input that wants a gradient is refused.
+void refuse_grad(std::initializer_list<const at::Tensor *> ts, const char *op)
+{
+    refuse_tangents(ts, op);
+    TORCH_CHECK(!wants_grad(ts), op, " is not differentiable: detach its inputs, or call it under no_grad");
+}
+
+// (q [..., width] e4m3, scale [..., ceil(width / 128)] fp32)
+std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor &x)
+{
+    const char *op = "quantize_fp8";
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK(x.dim() >= 1, op, ": x must have at least one dimension");
+    const int dt = layer_dtype(x, op);
+    refuse_grad({&x}, op);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = dense16(x);
+    const int64_t width = x.size(-1);
+    TORCH_CHECK(width >= 1, op, " requires 0 < feature width");
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = scale_blocks(width);
+    at::Tensor q = at::empty(xc.sizes(), xc.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scale = at::empty(shape, xc.options().dtype(at::kFloat));
+    check_rc(spmm_quantize_fp8_launch(xc.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), xc.numel() / width, width, dt,
+                                      stream_of(xc)));
+    return {q, scale};
+}
+
+// weight [groups, K, N] -> (q [groups, N, K] e4m3, scale [groups, ceil(N / 128), ceil(K / 128)] fp32)
+std::tuple<at::Tensor, at::Tensor> quantize_weight_fp8(const at::Tensor &weight)
+{
+    const char *op = "quantize_weight_fp8";
+    TORCH_CHECK_CUDA(weight);
+    TORCH_CHECK(weight.dim() == 3, op, ": weight must be three-dimensional");
+    const int dt = layer_dtype(weight, op);
+    refuse_grad({&weight}, op);
+    c10::cuda::CUDAGuard guard(weight.device());
+    const at::Tensor wc = dense16(weight);
+    const int64_t groups = wc.size(0), K = wc.size(1), N = wc.size(2);
+    at::Tensor q = at::empty({groups, N, K}, wc.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scale = at::empty({groups, scale_blocks(N), scale_blocks(K)}, wc.options().dtype(at::kFloat));
+    check_rc(spmm_quantize_weight_fp8_launch(wc.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), groups, K, N, dt,
+                                             stream_of(wc)));
+    return {q, scale};
+}
+
+// x [rows, K] and weight [groups, N, K] in e4m3 with their scales, as quantize_fp8 and quantize_weight_fp8 give them.
+at::Tensor grouped_matmul_fp8(const at::Tensor &x, const at::Tensor &x_scale, const at::Tensor &weight,
+                              const at::Tensor &weight_scale, const at::Tensor &group_ptr, at::ScalarType out_dtype)
+{
+    const char *op = "grouped_matmul_fp8";
+    TORCH_CHECK_CUDA(x);
+    TORCH_CHECK_CUDA(x_scale);
+    TORCH_CHECK_CUDA(weight);
+    TORCH_CHECK_CUDA(weight_scale);
+    TORCH_CHECK(x.dim() == 2, op, ": x must be two-dimensional");
+    TORCH_CHECK(weight.dim() == 3, op, ": weight must be three-dimensional");
+    TORCH_CHECK(x.scalar_type() == at::kFloat8_e4m3fn && weight.scalar_type() == at::kFloat8_e4m3fn, op,
+                ": x and weight must be float8_e4m3fn");
+    TORCH_CHECK(x_scale.scalar_type() == at::kFloat && weight_scale.scalar_type() == at::kFloat, op, ": scales must be FP32");
+    TORCH_CHECK(out_dtype == at::kHalf || out_dtype == at::kBFloat16 || out_dtype == at::kFloat, op,
+                " supports only FP16, BF16 and FP32 results, but got ", out_dtype);
+    same_device({&x_scale, &weight, &weight_scale}, x, op);
+    const int64_t rows = x.size(0), groups = weight.size(0), N = weight.size(1), K = weight.size(2);
+    TORCH_CHECK(x.size(1) == K, op, ": x has ", x.size(1), " features, the weight takes ", K);
+    TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == rows && x_scale.size(1) == scale_blocks(K), op,
+                ": x_scale must have shape [", rows, ", ", scale_blocks(K), "], but got ", x_scale.sizes());
+    TORCH_CHECK(weight_scale.dim() == 3 && weight_scale.size(0) == groups && weight_scale.size(1) == scale_blocks(N) &&
+                    weight_scale.size(2) == scale_blocks(K),
+                op, ": weight_scale must have shape [", groups, ", ", scale_blocks(N), ", ", scale_blocks(K), "], but got ",
+                weight_scale.sizes());
+    const int itype = check_group_ptr(group_ptr, x, groups, op);
+    refuse_grad({&x, &x_scale, &weight, &weight_scale}, op);
+    c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = dense16(x), wc = dense16(weight), xs = x_scale.contiguous(), ws = weight_scale.contiguous();
+    at::Tensor out = at::empty({rows, N}, xc.options().dtype(out_dtype));
+    check_rc(spmm_grouped_matmul_fp8_launch(xc.data_ptr(), xs.data_ptr<float>(), wc.data_ptr(), ws.data_ptr<float>(),
+                                            group_ptr.data_ptr(), out.data_ptr(), rows, groups, K, N, itype,
+                                            layer_dtype(out, op), stream_of(xc)));
+    return out;
+}
+
 // Sticky device status (code, detail), optionally cleared.  Synchronises.
 std::tuple<int64_t, int64_t> device_status(bool reset)
 {
@@ -1002,6 +1425,31 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           "Newton-Schulz steps on each matrix of update [..., m, n] divided by its Frobenius norm; BF16 result",
           pybind11::arg("update"), pybind11::arg("steps"), pybind11::arg("a"), pybind11::arg("b"), pybind11::arg("c"),
           pybind11::arg("eps"));
+    m.def("route_experts", &route_experts,
+          "Experts of each row of logits and their weights: (weights FP32, experts int32); differentiable in logits",
+          pybind11::arg("logits"), pybind11::arg("top_k"), pybind11::arg("bias"), pybind11::arg("scoring"),
+          pybind11::arg("groups"), pybind11::arg("top_groups"), pybind11::arg("group_best"), pybind11::arg("renormalize"),
+          pybind11::arg("scale"));
+    m.def("expert_plan", &expert_plan, "Stable order of the rows by expert: (group_ptr, position, source), int32",
+          pybind11::arg("experts"), pybind11::arg("num_experts"));
+    m.def("dispatch_rows", &dispatch_rows, "Rows of x in the order of an expert_plan; differentiable", pybind11::arg("x"),
+          pybind11::arg("position"), pybind11::arg("source"));
+    m.def("combine_rows", &combine_rows, "Weighted sums of each row's results back from that order; differentiable",
+          pybind11::arg("rows"), pybind11::arg("position"), pybind11::arg("source"),
+          pybind11::arg("weights") = pybind11::none());
+    m.def("embedding", &embedding, "scale * table[ids]; differentiable in table", pybind11::arg("ids"),
+          pybind11::arg("table"), pybind11::arg("scale") = 1.0, pybind11::arg("padding_id") = pybind11::none());
+    m.def("embedding_grad", &embedding_grad, "Gradient of embedding's table: scale * sums of grad's rows by id",
+          pybind11::arg("ids"), pybind11::arg("grad"), pybind11::arg("num_rows"), pybind11::arg("scale") = 1.0,
+          pybind11::arg("padding_id") = pybind11::none());
+    m.def("quantize_fp8", &quantize_fp8, "Rows in e4m3 with a scale per block of 128: (q, scale)", pybind11::arg("x"));
+    m.def("quantize_weight_fp8", &quantize_weight_fp8,
+          "Weights [groups, K, N] in e4m3 with a scale per block of 128 x 128: (q [groups, N, K], scale)",
+          pybind11::arg("weight"));
+    m.def("grouped_matmul_fp8", &grouped_matmul_fp8,
+          "grouped_matmul of quantised rows and weights; widths divisible by 16", pybind11::arg("x"),
+          pybind11::arg("x_scale"), pybind11::arg("weight"), pybind11::arg("weight_scale"), pybind11::arg("group_ptr"),
+          pybind11::arg("out_dtype"));
     m.def("device_status", &device_status, "Sticky device-side validation status (code, detail)",
           pybind11::arg("reset") = false);
 }

@@ -33,12 +33,21 @@ from custom_ops_lib import (  # noqa: F401  (GPU layout builders)
 )
 from custom_ops_lib import pack_rows as _pack_rows, restore_rows as _restore_rows
 from custom_ops_lib import (  # noqa: F401  (layer operators)
+    combine_rows as _combine_rows,
+    dispatch_rows,
+    embedding as _embedding,
+    embedding_grad,
+    expert_plan as _expert_plan,
     grouped_matmul as _grouped_matmul,
+    grouped_matmul_fp8 as _grouped_matmul_fp8,
     grouped_weight_grad,
     layer_norm as _layer_norm,
     layer_norm_backward,
     layer_norm_forward,
     orthogonalize as _orthogonalize,
+    quantize_fp8 as _quantize_fp8,
+    quantize_weight_fp8 as _quantize_weight_fp8,
+    route_experts as _route_experts,
 )
 
 
@@ -161,12 +170,108 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     return _orthogonalize(update, steps, a, b, c, eps)
 
 
+# --------------------------------------------------------------------------
+# Routed experts and learned features (no counterpart in the reference)
+# --------------------------------------------------------------------------
+def route_experts(logits, top_k, bias=None, scoring="softmax", groups=1, top_groups=1, group_best=1,
+                  renormalize=True, scale=1.0):
+    """The ``top_k`` experts of each row of logits [..., num_experts] (fp16,
+    bf16 or fp32) and their weights: ``(weights, experts)``, fp32 and int32
+    [..., top_k], in descending order.
+
+    The scores are the row's softmax or sigmoid (``scoring``).  ``bias`` (fp32
+    [num_experts], for balance) is added to them for the choice alone.  With
+    ``groups`` > ``top_groups`` the experts are that many ranges of equal size,
+    and only those of the ``top_groups`` ranges with the largest sums of their
+    ``group_best`` (1 or 2) largest values can be chosen.  Equal values go to
+    the lowest index, NaN below all.  ``renormalize`` divides the chosen scores
+    by their sum + 1e-20; ``scale`` multiplies them.  At most 1024 experts, 32
+    chosen ones, 32 groups.
+
+    The weights are differentiable in the logits; the choice is a constant.
+    """
+    return _route_experts(logits, top_k, bias, scoring, groups, top_groups, group_best, renormalize, scale)
+
+
+def expert_plan(experts, num_experts):
+    """The order that brings the rows of each expert together, as int32 tensors
+    on the device: ``(group_ptr, position, source)``.
+
+    ``experts`` (int32 or int64, [rows, choices]; -1: none) is sorted stably.
+    ``group_ptr`` [num_experts + 1] is ``grouped_matmul``'s, ``position`` (like
+    ``experts``) the row of each choice or -1, ``source`` [rows * choices] the
+    choice of each row, -1 behind the last.  ``group_ptr`` differences are the
+    experts' loads.  An expert outside [-1, num_experts) counts as -1 and raises
+    the device status.  At most 1024 experts.
+    """
+    return _expert_plan(experts, num_experts)
+
+
+def combine_rows(rows, position, source, weights=None):
+    """``y[t] = sum_j weights[t, j] * rows[position[t, j]]``: the results of each
+    row's experts added up, in fp32.  ``weights`` is fp32 [rows, choices]
+    (``route_experts``'s) or None for ones; choices without a position add
+    nothing.  Differentiable in rows and weights.
+
+    ``dispatch_rows(x, position, source)`` is the way there: the rows of x in
+    the plan's order, one per choice, zeros behind the last (differentiable).
+    """
+    return _combine_rows(rows, position, source, weights)
+
+
+def embedding(ids, table, scale=1.0, padding_id=None):
+    """``scale * table[ids]`` for ids (int32 or int64, any shape) and a table
+    [rows, width] in fp16, bf16 or fp32, differentiable in table.
+
+    The gradient adds the rows of each id up in fp32 in the order of the ids
+    (no atomics: the same bits every time); the id ``padding_id`` gets none.
+    An id outside the table gives zeros and raises the device status.
+    ``embedding_grad(ids, grad, num_rows, scale, padding_id)`` is the gradient by
+    itself.
+    """
+    return _embedding(ids, table, scale, padding_id)
+
+
+def quantize_fp8(x):
+    """x [..., width] in 8-bit floating point: ``(q, scale)``, q e4m3 like x and
+    fp32 scales [..., ceil(width / 128)], one per block of 128 elements.
+
+    A block's scale is its largest finite magnitude (at least 2^-100) / 448, q
+    the values x / scale rounded to nearest; infinities and NaN become NaN.
+    Widths are divisible by 16.  Not differentiable.
+    """
+    return _quantize_fp8(x)
+
+
+def quantize_weight_fp8(weight):
+    """Weights [groups, K, N] for ``grouped_matmul_fp8``, laid out once: ``(q,
+    scale)``, q e4m3 [groups, N, K] (transposed) and fp32 scales [groups,
+    ceil(N / 128), ceil(K / 128)] of blocks of 128 x 128, as ``quantize_fp8``."""
+    return _quantize_weight_fp8(weight)
+
+
+def grouped_matmul_fp8(x, x_scale, weight, weight_scale, group_ptr, out_dtype=torch.bfloat16):
+    """``grouped_matmul`` of operands in 8 bits (``quantize_fp8``'s rows,
+    ``quantize_weight_fp8``'s weights): each block of 128 products is summed on
+    the tensor cores, the blocks in fp32 times their scales, and the result
+    rounded to ``out_dtype`` (fp16, bf16 or fp32) once.  K and N are divisible
+    by 16.  For serving: not differentiable.
+    """
+    return _grouped_matmul_fp8(x, x_scale, weight, weight_scale, group_ptr, out_dtype)
+
+
 __all__ = [
     "block_level_split",
+    "combine_rows",
     "csr_to_ascend_cube",
     "csr_to_bcsr",
     "csr_to_spmm_cube",
+    "dispatch_rows",
+    "embedding",
+    "embedding_grad",
+    "expert_plan",
     "grouped_matmul",
+    "grouped_matmul_fp8",
     "grouped_weight_grad",
     "layer_norm",
     "layer_norm_backward",
@@ -174,7 +279,10 @@ __all__ = [
     "orthogonalize",
     "pack_node_tensor",
     "preprocess",
+    "quantize_fp8",
+    "quantize_weight_fp8",
     "restore_node_tensor",
+    "route_experts",
     "spmm_ascend_cube",
     "spmm_ascend_cube_aic_without_pipeline",
     "spmm_ascend_cube_aiv_mb",

@@ -52,6 +52,8 @@ enum spmm_status {
 /* SPMM_BF16: layer operators only (the SpMM operators take fp16 and fp32). */
 enum spmm_dtype { SPMM_F16 = 0, SPMM_F32 = 1, SPMM_F64 = 2, SPMM_BF16 = 3 };
 enum spmm_itype { SPMM_I32 = 0, SPMM_I64 = 1 };
+/* How route_experts makes scores of logits. */
+enum spmm_scoring { SPMM_SCORE_SOFTMAX = 0, SPMM_SCORE_SIGMOID = 1 };
 
 /* Device-status codes raised by kernels (see spmm_device_status). */
 enum spmm_device_code {
@@ -376,6 +378,95 @@ size_t spmm_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n, i
 int spmm_orthogonalize_launch(const void *update, void *out, int64_t batch, int64_t m, int64_t n, int steps, double a,
                               double b, double c, double eps, int dtype, void *workspace, size_t workspace_bytes,
                               void *stream);
+
+/* ---------------------------------------------------------------------- */
+/* Routed experts and learned features.  Their row ranges are              */
+/* spmm_grouped_matmul's groups.                                           */
+/* ---------------------------------------------------------------------- */
+
+/* Each row's experts and their weights: with s the softmax or the sigmoid of
+ * the row's logits [tokens, num_experts] (of type dtype) and c = s + bias
+ * (bias [num_experts] or NULL; it takes part in the choice alone),
+ *   groups   the experts are `groups` ranges of equal size; the top_groups
+ *            ranges with the largest sums of their group_best (1 or 2)
+ *            largest c are kept (top_groups == groups: all)
+ *   experts  [tokens, top_k] the top_k largest c of the kept groups, in
+ *            descending order, the lowest index first among equal ones
+ *   weights  [tokens, top_k] s of these, divided by their sum + 1e-20 with
+ *            renormalize, times scale
+ * The choice is that of 64-bit scores (without a bias, of the logits
+ * themselves).  NaN counts as the lowest value in it; a row whose logits are
+ * all -infinity has weights of zero.  At most 1024 experts, 32 chosen ones
+ * and 32 groups. */
+int spmm_route_experts_launch(const void *logits, const float *bias, float *weights, int32_t *experts, int64_t tokens,
+                              int64_t num_experts, int64_t top_k, int scoring, int64_t groups, int64_t top_groups,
+                              int group_best, int renormalize, double scale, int dtype, void *stream);
+/* Gradient of the logits from that of the weights (the experts are taken as
+ * given, each at most once per row).  An expert outside [0, num_experts)
+ * counts as not chosen and raises SPMM_DEV_BAD_COLUMN. */
+int spmm_route_experts_backward_launch(const void *logits, const int32_t *experts, const float *grad, void *dlogits,
+                                       int64_t tokens, int64_t num_experts, int64_t top_k, int scoring,
+                                       int renormalize, double scale, int dtype, void *stream);
+
+/* The order that brings the rows of each expert together (a stable counting
+ * sort of experts [n], n = tokens * choices):
+ *   group_ptr [num_experts + 1]  first row of each expert, and their end
+ *   position  [n]                row of each choice, -1 for an expert of -1
+ *   source    [n]                choice of each row, -1 behind the last row
+ * An expert outside [-1, num_experts) counts as -1 and raises
+ * SPMM_DEV_BAD_COLUMN.  At most 1024 experts. */
+int spmm_expert_plan_launch(const void *experts, int32_t *group_ptr, int32_t *position, int32_t *source, int64_t n,
+                            int64_t num_experts, int itype, void *stream);
+
+/* Rows to their experts and back, k choices per row of x [tokens, width]:
+ *   dispatch  rows[r] = x[source[r] / k], rows without a source are zero
+ *   combine   y[t] = sum_j weights[t, j] * rows[position[t, j]] over the
+ *             choices that have a position (weights NULL: ones)
+ *   backward  of combine: drows[r] = weights[source[r]] * grad[source[r] / k]
+ *             (zero without a source), dweights[t, j] = <rows[position[t, j]], grad[t]>
+ *             (zero without a position); either may be NULL
+ * Dispatch and the combine without weights are each other's gradient.
+ * position and source are spmm_expert_plan's; a position outside
+ * [-1, tokens * k) counts as -1 and raises SPMM_DEV_BAD_COLUMN. */
+int spmm_dispatch_rows_launch(const void *x, const int32_t *position, const int32_t *source, void *rows, int64_t tokens,
+                              int64_t k, int64_t width, int dtype, void *stream);
+int spmm_combine_rows_launch(const void *rows, const int32_t *position, const float *weights, void *y, int64_t tokens,
+                             int64_t k, int64_t width, int dtype, void *stream);
+int spmm_combine_rows_backward_launch(const void *grad, const void *rows, const int32_t *position,
+                                      const int32_t *source, const float *weights, void *drows, float *dweights,
+                                      int64_t tokens, int64_t k, int64_t width, int dtype, void *stream);
+
+/* Rows of a table [rows, width] by id: y[i] = scale * table[ids[i]].  An id
+ * outside [0, rows) gives zeros and raises SPMM_DEV_BAD_COLUMN.
+ * The gradient, dtable[v] = scale * sum of grad[i] over the i with ids[i] == v
+ * (zero for an id that does not occur, for padding_id, which may be -1 for
+ * none), is summed in fp32 in the order of i: no atomics, every row written. */
+int spmm_embedding_launch(const void *ids, const void *table, void *y, int64_t n, int64_t rows, int64_t width,
+                          double scale, int itype, int dtype, void *stream);
+size_t spmm_embedding_backward_workspace_bytes(int64_t n, int64_t width);
+int spmm_embedding_backward_launch(const void *ids, const void *grad, void *dtable, int64_t n, int64_t rows,
+                                   int64_t width, double scale, int64_t padding_id, int itype, int dtype,
+                                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* 8-bit floating point (e4m3, one byte) with a scale for each block of 128:
+ *   rows     x [rows, width] -> q [rows, width], scale [rows, ceil(width / 128)]
+ *   weights  weight [groups, K, N] -> q [groups, N, K] (transposed), scale
+ *            [groups, ceil(N / 128), ceil(K / 128)] of blocks of 128 x 128
+ * A block's scale is its largest finite magnitude (at least 2^-100) / 448 in
+ * fp32, its values x / scale rounded to nearest; infinities and NaN become
+ * NaN.  Widths are divisible by 16. */
+int spmm_quantize_fp8_launch(const void *x, void *q, float *scale, int64_t rows, int64_t width, int dtype, void *stream);
+int spmm_quantize_weight_fp8_launch(const void *weight, void *q, float *scale, int64_t groups, int64_t K, int64_t N,
+                                    int dtype, void *stream);
+
+/* spmm_grouped_matmul of operands in 8 bits as quantised above:
+ *   out[r] = sum over blocks b of x_scale[r, b] * weight_scale[g, n / 128, b]
+ *            * sum over block b of x[r, k] * weight[g, n, k]
+ * in fp32, rounded to out_dtype once.  Ranges as there (rows outside every
+ * group are zero); K and N are divisible by 16. */
+int spmm_grouped_matmul_fp8_launch(const void *x, const float *x_scale, const void *weight, const float *weight_scale,
+                                   const void *group_ptr, void *out, int64_t rows, int64_t groups, int64_t K, int64_t N,
+                                   int itype, int out_dtype, void *stream);
 
 #ifdef __cplusplus
 }
