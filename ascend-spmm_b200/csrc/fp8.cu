@@ -1,7 +1,8 @@
 // Products of row ranges in 8-bit floating point (e4m3) with a scale for each
 // block of 128 elements of the reduction.
 //
-//   rows       s[r, b] = max |x[r, block b]| / 448,  q = e4m3(x / s)
+//   rows       s[b, r] = max |x[r, block b]| / 448,  q = e4m3(x / s); a block's scales lie together, as the
+//              product's lanes read them
 //   weights    s[g, c, b]: the same over blocks of 128 x 128; q is laid out
 //              [groups, N, K], so that both operands have the reduction contiguous
 //   product    y[r] = sum over b of sx[r, b] sw[g, n / 128, b] (q_x q_w over block b)
@@ -9,10 +10,6 @@
 // The scales are fp32, of a maximum of at least 2^-100 over the finite values
 // (smaller ones would make x / s leave fp32's normal range); infinities and
 // NaN become NaN, which e4m3 has.
-//
-// A slice of the product's ring (gemm_tc.cuh) is 128 bytes deep, one block of
-// the scales: each goes into an accumulator of its own, and the epilogue warps
-// add it to their registers times its scales while the next one is computed.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -20,7 +17,7 @@
 #include "../../include/spmm_b200.h"
 #include "common.cuh"
 #include "engine.h"
-#include "gemm_tc.cuh"
+#include "fp8_gemm.cuh"
 #include "layer.cuh"
 #include "layer.h"
 
@@ -34,11 +31,21 @@ constexpr unsigned kFull = 0xffffffffu;
 
 __device__ __forceinline__ float finite_abs(float x) { return isfinite(x) ? fabsf(x) : 0.f; }
 __device__ __forceinline__ float scale_of(float amax) { return __fdiv_rn(fmaxf(amax, kTiny), kLargest); }
-// e4m3 of x / s, to nearest; not finite: NaN.
-__device__ __forceinline__ unsigned char quantized(float x, float s)
+
+// x / s correctly rounded, from the correctly rounded reciprocal of s
+// (Markstein 1990: one residual and one correction of x * (1 / s)).  The scale
+// keeps all of it in fp32's normal range, but for quotients that round to zero in e4m3.  Not
+// finite: NaN (the residual of an infinity is).
+__device__ __forceinline__ float quotient(float x, float s, float inverse)
 {
-    const float v = isfinite(x) ? __fdiv_rn(x, s) : NAN;
-    return (unsigned char)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+    const float q = x * inverse;
+    return copysignf(fmaf(fmaf(-q, s, x), inverse, q), x);   // -0 stays so
+}
+// Two of them in e4m3, to nearest.
+__device__ __forceinline__ unsigned short quantized(float x0, float x1, float s, float inverse)
+{
+    return __nv_cvt_float2_to_fp8x2(make_float2(quotient(x0, s, inverse), quotient(x1, s, inverse)), __NV_SATFINITE,
+                                    __NV_E4M3);
 }
 
 // 16 lanes per block of a row, 8 elements a lane; width is a multiple of 16.
@@ -49,32 +56,36 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *x, unsigned
     const int64_t blocks = (width + kBlock - 1) / kBlock, items = rows * blocks;
     const int lane = threadIdx.x & 15;
     const int64_t step = (int64_t)gridDim.x * (blockDim.x / 16);
-    const int64_t base = (int64_t)blockIdx.x * (blockDim.x / 16);
-    for (int64_t b = base; b < items; b += step) {   // the same number of turns for both halves of a warp
-        const int64_t i = b + threadIdx.x / 16;
-        const int64_t r = i / blocks, c = i % blocks * kBlock + lane * 8;
+    for (int64_t base = (int64_t)blockIdx.x * (blockDim.x / 16); base < items; base += step) {
+        const int64_t i = base + threadIdx.x / 16;   // all lanes of a warp take the same turns
+        const int64_t r = i / blocks, b = i - r * blocks, c = b * kBlock + lane * 8;
         const bool on = i < items && c < width;
-        float f[8];
+        float f[8] = {};
         if (on) {
+            __align__(16) T raw[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = elem_f32<T>(x[r * width + c + e]);
-        } else {
+            for (int v = 0; v < (int)sizeof(raw) / 16; ++v)
+                reinterpret_cast<uint4 *>(raw)[v] = __ldcs(reinterpret_cast<const uint4 *>(x + r * width + c) + v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = 0.f;
+            for (int e = 0; e < 8; ++e) f[e] = elem_f32<T>(raw[e]);
         }
-        float m = 0.f;
+        auto largest = [&](auto of) {
+            float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(f[e]));
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, of(f[e]));   // NaN is not the larger one
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-        const float s = scale_of(m);
-        if (i < items && lane == 0) scale[i] = s;
+            for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+            return m;
+        };
+        float m = largest([](float v) { return fabsf(v); });
+        if (__any_sync(kFull, isinf(m))) m = largest(finite_abs);
+        const float s = scale_of(m), inverse = __frcp_rn(s);
+        if (i < items && lane == 0) scale[b * rows + r] = s;
         if (on) {
-            uint2 raw;
-            unsigned char *o = reinterpret_cast<unsigned char *>(&raw);
+            __align__(8) unsigned short o[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = quantized(f[e], s);
-            *reinterpret_cast<uint2 *>(q + r * width + c) = raw;
+            for (int e = 0; e < 4; ++e) o[e] = quantized(f[2 * e], f[2 * e + 1], s, inverse);
+            *reinterpret_cast<uint2 *>(q + r * width + c) = *reinterpret_cast<const uint2 *>(o);
         }
     }
 }
@@ -101,10 +112,10 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const T *w, unsign
         m = 0.f;
 #pragma unroll
         for (int v = 0; v < 8; ++v) m = fmaxf(m, most[v]);
-        const float s = scale_of(m);
+        const float s = scale_of(m), inverse = __frcp_rn(s);
         if (threadIdx.x == 0) scale[i] = s;
         for (int64_t k = k0 + threadIdx.x / kBlock; k < min(k0 + kBlock, K); k += 2)
-            if (n < N) tile[threadIdx.x % kBlock][k - k0] = quantized(elem_f32<T>(src[k * N]), s);
+            if (n < N) tile[threadIdx.x % kBlock][k - k0] = (unsigned char)quantized(elem_f32<T>(src[k * N]), 0.f, s, inverse);
         __syncthreads();
         for (int r = threadIdx.x / kBlock; r < kBlock && n0 + r < N; r += 2)
             if (k0 + threadIdx.x % kBlock < K)
@@ -127,20 +138,36 @@ template <typename F> cudaError_t by_type(int dtype, F f)
     }
 }
 
-template <int BN, bool PAIR = false>
-cudaError_t fp8_tc(const Fp8Launch &a, tc::GemmArgs &g, int64_t row_tiles, cudaStream_t stream)
+// Row tiles, at most: every group can end in a partial one; the rows outside
+// the groups too.
+int64_t row_tiles_of(const Fp8Launch &l, int height)
 {
-    tc::Maps m;
-    const int64_t tiles = row_tiles * ((g.n + g.bn - 1) / g.bn);
-    const int cols = PAIR ? BN / 2 : g.bn;   // of the weight that a block brings in
-    if (!tc::make_byte_map(&m.a, a.x, a.K, a.rows, 1, tc::kBM) ||
-        !tc::make_byte_map(&m.b, a.groups > 0 ? a.w : a.x, a.K, a.groups > 0 ? a.N : 1, std::max<int64_t>(a.groups, 1),
-                           cols) ||
-        !tc::make_out_map(&m.o, a.out, g.n, a.rows, 1, g.n, 0, g.out_type))
-        return cudaErrorInvalidValue;
-    m.p = m.o;
-    return tc::launch_gemm<tc::kRows, BN, false, false, tc::kStoreScaled, PAIR>(m, g, tiles, stream);
+    return std::min(l.rows, (l.rows + height - 1) / height + l.groups + 1);
 }
+
+template <int BN, bool PAIR = false> cudaError_t launch_tiles(const Fp8Launch &l, const tc::Fp8Args &a, cudaStream_t stream)
+{
+    using S = tc::Fp8Shape<BN, PAIR>;
+    auto kernel = tc::fp8_gemm_kernel<BN, PAIR>;
+    static PerDevice<bool> ready;   // the attribute outlasts the call
+    bool *done = ready.here();
+    if (!done || !*done) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+        if (e != cudaSuccess) return e;
+        if (done) *done = true;
+    }
+    CUtensorMap x, w, out;
+    if (!tc::make_byte_map(&x, l.x, l.K, l.rows, 1, tc::kBM) ||
+        !tc::make_byte_map(&w, l.groups > 0 ? l.w : l.x, l.K, l.groups > 0 ? l.N : 1, std::max<int64_t>(l.groups, 1),
+                           PAIR ? BN / 2 : BN) ||
+        !tc::make_out_map(&out, l.out, l.N, l.rows, 1, l.N, 0, a.out_type))
+        return cudaErrorInvalidValue;
+    constexpr int kBlocks = PAIR ? 2 : 1;   // per tile
+    const int64_t tiles = row_tiles_of(l, kBlocks * tc::kBM) * ((l.N + BN - 1) / BN);
+    const unsigned grid = kBlocks * (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count() / kBlocks));
+    return tc::launch_overlapped(kernel, grid, kBlocks, tc::kFp8Threads, S::kBytes, stream, x, w, out, a);
+}
+
 
 }  // namespace
 
@@ -170,23 +197,21 @@ cudaError_t launch_quantize_weight(const void *w, void *q, float *scale, int64_t
 
 cudaError_t launch_grouped_fp8(const Fp8Launch &a, cudaStream_t stream)
 {
-    tc::GemmArgs g{};
+    tc::Fp8Args g{};
     g.ranges = Ranges{a.ptr, a.itype == SPMM_I64, a.groups, a.rows};
-    g.n = a.N;
-    g.k = a.K;
-    g.out = a.out;
-    g.ldo = a.N;
-    g.out_type = a.out_dtype == SPMM_F32 ? tc::kOutF32 : a.out_dtype == SPMM_BF16 ? tc::kOutBf16 : tc::kOutF16;
+    g.n = (int)a.N;
+    g.blocks_k = (int)((a.K + kBlock - 1) / kBlock);
+    g.blocks_n = (int)((a.N + kBlock - 1) / kBlock);
     g.scale_a = a.x_scale;
     g.scale_b = a.w_scale;
-    g.blocks_k = (a.K + kBlock - 1) / kBlock;
-    g.blocks_n = (a.N + kBlock - 1) / kBlock;
+    g.out = a.out;
+    g.out_type = a.out_dtype == SPMM_F32 ? tc::kOutF32 : a.out_dtype == SPMM_BF16 ? tc::kOutBf16 : tc::kOutF16;
     g.status = a.status;
-    const int64_t row_tiles = std::min(a.rows, (a.rows + tc::kBM - 1) / tc::kBM + a.groups + 1);
-    g.bn = tc::tile_columns(row_tiles, g.n, 256);
-    if (g.bn <= 64) return fp8_tc<64>(a, g, row_tiles, stream);
-    if (g.bn <= 128) return fp8_tc<128>(a, g, row_tiles, stream);
-    return fp8_tc<256>(a, g, row_tiles, stream);
+    // pairs of blocks where groups are long enough that their last tile's missing rows do not matter
+    if (a.N % 256 == 0 && a.rows >= 512 * std::max<int64_t>(a.groups, 1) && a.rows / 256 * (a.N / 256) >= device_sm_count())
+        return launch_tiles<256, true>(a, g, stream);
+    if (row_tiles_of(a, tc::kBM) * ((a.N + 127) / 128) >= device_sm_count()) return launch_tiles<128>(a, g, stream);
+    return launch_tiles<64>(a, g, stream);
 }
 
 }  // namespace spmmb

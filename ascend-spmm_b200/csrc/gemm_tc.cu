@@ -63,24 +63,6 @@ CUtensorMapDataType type16(bool bf16)
 
 }  // namespace
 
-int tile_columns(int64_t row_tiles, int64_t width, int most)
-{
-    const int64_t sms = device_sm_count();
-    int best = 0;
-    int64_t least = INT64_MAX;
-    for (int64_t n = (width + most - 1) / most; n <= (width + 63) / 64; ++n) {
-        const int64_t step = n > 1 ? 32 : 16;   // a tile is stored 32 columns at a time
-        const int64_t bn = ((width + n - 1) / n + step - 1) / step * step;
-        const int64_t cost = (row_tiles * n + sms - 1) / sms * (bn + 70);
-        if (cost < least) {
-            least = cost;
-            best = (int)bn;
-        }
-        if (n > 64 && bn <= 128) break;   // very wide outputs: narrower tiles gain nothing more
-    }
-    return best;
-}
-
 bool make_map(CUtensorMap *map, const void *p, int64_t inner, int64_t rows, int64_t batch, int64_t ld,
               int64_t batch_stride, int box_rows, bool bf16)
 {

@@ -61,10 +61,7 @@ enum Mode { kRows, kRagged, kDense };
 // squares on the diagonal and run down a matrix's long side, takes a new
 // accumulator every 256 slices: in a single one 2^20 columns lost 6e-3 of G
 // and moved a 136-row update by 6e-3, 16384 lose 1e-4.
-// kStoreScaled: 8-bit operands (e4m3).  A slice is 128 elements, the block that
-// shares a scale; an accumulator takes one, and the epilogue warps add it in
-// registers times the row's and the columns' scale of the block.
-enum Epi { kStore, kStoreSum, kStoreScaled, kGram, kPoly, kUpdate };
+enum Epi { kStore, kStoreSum, kGram, kPoly, kUpdate };
 enum OutType { kOutF16, kOutBf16, kOutF32 };
 
 struct GemmArgs {
@@ -94,9 +91,6 @@ struct GemmArgs {
     const __half *in, *in_lo;
     bool low;
     int64_t ldi, in_batch;
-    // kStoreScaled: scale_a [rows][blocks_k], scale_b [batch][blocks_n][blocks_k]
-    const float *scale_a, *scale_b;
-    int64_t blocks_k, blocks_n;
     DevStatus *status;
 };
 
@@ -343,10 +337,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     static_assert(!PAIR || MODE != kRagged, "a group's zeros are written by one block");
     using S = GemmShape<BN, PAIR>;
     constexpr int kParts = EPI == kStoreSum ? 3 : 1;   // ring stages of a slice
-    constexpr bool kBytes8 = EPI == kStoreScaled;
-    static_assert(!kBytes8 || (MODE == kRows && !AMN && !BMN), "8-bit operands have the reduction contiguous");
-    constexpr int kSlices = EPI == kStoreSum || kBytes8 ? 1 : EPI == kGram ? 256 : 0;   // of an accumulator, 0: all
-    constexpr int kDeep = kBytes8 ? 2 * kBK : kBK, kStep = kBytes8 ? 32 : 16;   // elements of a slice, of a product
+    constexpr int kSlices = EPI == kStoreSum ? 1 : EPI == kGram ? 256 : 0;   // of an accumulator, 0: all
     static_assert(S::kStages >= 2 * kParts, "a slice arrives while another is multiplied");
     extern __shared__ __align__(1024) unsigned char smem[];
     const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
@@ -434,12 +425,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (MODE == kRagged) continue;
                 break;
             }
-            const int n = (int)((t.k1 - t.k0 + kDeep - 1) / kDeep);
+            const int n = (int)((t.k1 - t.k0 + kBK - 1) / kBK);
             if (elect()) {
                 const int row0 = (int)t.row0, col0 = (int)t.col0 + (PAIR ? (int)peer * b_cols : 0);
                 unsigned at = slice;
                 int k = (int)t.k0;
-                for (int i = 0; i < n && ok; ++i, k += kDeep)
+                for (int i = 0; i < n && ok; ++i, k += kBK)
 #pragma unroll
                     for (int j = 0; j < kParts; ++j, ++at) {
                         const int plane = kParts == 1 ? 0 : (j + 2) % 3;   // l, h, m: l is done with first
@@ -491,8 +482,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
     } else if (warp == 1) {
         // ---- MMA warp: one lane issues
-        const unsigned idesc = kBytes8 ? idesc8(S::kRows, PAIR ? BN : a.bn)
-                                       : idesc16(a.bf16, AMN, BMN, S::kRows, PAIR ? BN : a.bn);
+        const unsigned idesc = idesc16(a.bf16, AMN, BMN, S::kRows, PAIR ? BN : a.bn);
         // byte strides of the operands' layouts: K-major, 8 rows of 128 bytes per
         // swizzle atom; MN-major, atoms of 64 rows or columns x 8 deep, 8 KB apart
         const uint64_t da = AMN ? desc128(base, 8192, 1024) : desc128(base, 16, 1024);
@@ -500,8 +490,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         constexpr unsigned step_a = (AMN ? 2048 : 32) >> 4, step_b = (BMN ? 2048 : 32) >> 4;
         unsigned slice = 0, used = 0;
         auto mul = [&](unsigned d, uint64_t x, uint64_t y, unsigned add) {
-            if constexpr (PAIR) mma_pair<kBytes8>(d, x, y, idesc, add);
-            else mma<kBytes8>(d, x, y, idesc, add);
+            if constexpr (PAIR) mma_pair(d, x, y, idesc, add);
+            else mma(d, x, y, idesc, add);
         };
         auto finish = [&](unsigned bar) {
             if constexpr (PAIR) commit_pair(bar);
@@ -510,12 +500,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         auto product = [&](unsigned at_a, unsigned at_b, int depth, unsigned d, bool first) {
             const unsigned off_a = at_a % S::kStages * (S::kA + S::kB) >> 4;
             const unsigned off_b = at_b % S::kStages * (S::kA + S::kB) >> 4;
-            if (depth == kDeep) {
+            if (depth == kBK) {
 #pragma unroll
-                for (int i = 0; i < kDeep / kStep; ++i)
+                for (int i = 0; i < kBK / 16; ++i)
                     mul(d, da + off_a + i * step_a, db + off_b + i * step_b, first && i == 0 ? 0u : 1u);
             } else {
-                for (int i = 0; i * kStep < depth; ++i)
+                for (int i = 0; i * 16 < depth; ++i)
                     mul(d, da + off_a + i * step_a, db + off_b + i * step_b, first && i == 0 ? 0u : 1u);
             }
         };
@@ -552,7 +542,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (MODE == kRagged) continue;
                 break;
             }
-            const int depth = (int)(t.k1 - t.k0), n = (depth + kDeep - 1) / kDeep;
+            const int depth = (int)(t.k1 - t.k0), n = (depth + kBK - 1) / kBK;
             if (n <= 0) continue;
             // kRagged: a last slice that ends within 16 rows needs the whole warp
             const bool ragged = MODE == kRagged && (depth & 15);
@@ -568,7 +558,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 const int s1 = min(s0 + sum, n);
                 if (peer == 0 && elect())
                     for (int i = s0; i < min(s1, whole); ++i)
-                        if (!multiply(slice + kParts * (i - s0), min(kDeep, depth - i * kDeep), d, i == s0)) {
+                        if (!multiply(slice + kParts * (i - s0), min(kBK, depth - i * kBK), d, i == s0)) {
                             give_up(3);
                             break;
                         }
@@ -623,7 +613,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 if (MODE == kRagged) continue;
                 break;
             }
-            const int n = (int)max((t.k1 - t.k0 + kDeep - 1) / kDeep, (int64_t)0);
+            const int n = (int)max((t.k1 - t.k0 + kBK - 1) / kBK, (int64_t)0);
             const bool on = row < t.rows, part = MODE == kRagged && t.part;
             const bool wide = part || out_size == 4;
             const int y = (int)t.out_row + row0, z = (int)t.out_z;
@@ -761,16 +751,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[b][i] = 0.f;
                 for (int i = 0; i < n; i += kSlices) {
-                    float scale[kBytes8 ? BN / 64 : 1];   // kStoreScaled: of this slice's blocks of 32 columns
-                    if constexpr (kBytes8) {
-                        const float sa = on ? __ldg(a.scale_a + (t.out_row + row) * a.blocks_k + i) : 0.f;
-#pragma unroll
-                        for (int b = 0; b < BN / 64; ++b) {
-                            const int c = parity * 32 + 64 * b;
-                            if (c < t.cols)
-                                scale[b] = sa * __ldg(a.scale_b + (t.batch_b * a.blocks_n + (t.col0 + c) / (2 * kBK)) * a.blocks_k + i);
-                        }
-                    }
                     const unsigned from = take();
                     if (!ok) break;
 #pragma unroll
@@ -780,10 +760,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                             float w[32];
                             tmem_ld32(from + c, w);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                if constexpr (kBytes8) v[b][e] = fmaf(scale[b], w[e], v[b][e]);
-                                else v[b][e] += w[e];
-                            }
+                            for (int e = 0; e < 32; ++e) v[b][e] += w[e];
                         }
                     }
                     give_back();
@@ -876,12 +853,6 @@ cudaError_t launch_overlapped(K kernel, dim3 grid, unsigned cluster, int threads
     config.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
-
-// Columns per tile (a multiple of 16 of at most `most`): the cut into equal
-// tiles with the least turns x time.  A 64-deep slice of a tile takes about
-// as long as 70 + bn columns (0.19 us at 64, 0.46 us at 256): its rows are
-// read however narrow it is.
-int tile_columns(int64_t row_tiles, int64_t width, int most);
 
 struct Maps {
     CUtensorMap a, b, o, p;

@@ -149,7 +149,7 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
 // ---- 8-bit floating point with block scales (fp8.cu) ----------------------------
 struct Fp8Launch {
     const void *x;          // [rows, K] e4m3
-    const float *x_scale;   // [rows, ceil(K / 128)]
+    const float *x_scale;   // [ceil(K / 128), rows]
     const void *w;          // [groups, N, K] e4m3
     const float *w_scale;   // [groups, ceil(N / 128), ceil(K / 128)]
     const void *ptr;        // [groups + 1]

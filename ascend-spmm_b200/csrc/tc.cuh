@@ -212,6 +212,22 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v)
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// 16 or 32 consecutive columns as above.
+__device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[16])
+{
+    unsigned r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, "
+                 "[%16];\n\ttcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // ---- pairs of blocks (clusters of two) -------------------------------------
 __device__ __forceinline__ unsigned cluster_rank()
 {
@@ -229,6 +245,11 @@ __device__ __forceinline__ unsigned in_block(unsigned addr, unsigned rank)
 __device__ __forceinline__ void bar_arrive_cluster(unsigned remote)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
+}
+// As bar_arrive_cluster, ordering this block's accesses only.
+__device__ __forceinline__ void bar_arrive_peer(unsigned remote)
+{
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
 }
 __device__ __forceinline__ void cluster_sync()
 {
@@ -272,6 +293,14 @@ __device__ __forceinline__ void commit_pair(unsigned bar)
                      bar),
                  "h"((unsigned short)3)
                  : "memory");
+}
+// a += s * w for two fp32 values at once.
+__device__ __forceinline__ void fma2(float &a0, float &a1, float s, float w0, float w1)
+{
+    asm("{\n\t.reg .b64 a, s, w;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 w, {%3, %4};\n\t"
+        "fma.rn.f32x2 a, s, w, a;\n\tmov.b64 {%0, %1}, a;\n\t}\n"
+        : "+f"(a0), "+f"(a1)
+        : "f"(s), "f"(w0), "f"(w1));
 }
 // Eight fp32 values as fp16 or bf16.
 __device__ __forceinline__ uint4 pack8(const float *v, bool bf16)

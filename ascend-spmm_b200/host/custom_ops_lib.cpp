@@ -1269,7 +1269,7 @@ void refuse_grad(std::initializer_list<const at::Tensor *> ts, const char *op)
     TORCH_CHECK(!wants_grad(ts), op, " is not differentiable: detach its inputs, or call it under no_grad");
 }
 
-// (q [..., width] e4m3, scale [..., ceil(width / 128)] fp32)
+// (q [..., width] e4m3, scale [..., ceil(width / 128)] fp32, a transposed view)
 std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor &x)
 {
     const char *op = "quantize_fp8";
@@ -1281,13 +1281,15 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor &x)
     const at::Tensor xc = dense16(x);
     const int64_t width = x.size(-1);
     TORCH_CHECK(width >= 1, op, " requires 0 < feature width");
+    const int64_t rows = xc.numel() / width;
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = scale_blocks(width);
     at::Tensor q = at::empty(xc.sizes(), xc.options().dtype(at::kFloat8_e4m3fn));
-    at::Tensor scale = at::empty(shape, xc.options().dtype(at::kFloat));
-    check_rc(spmm_quantize_fp8_launch(xc.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), xc.numel() / width, width, dt,
+    // the scales of a block lie together: [blocks, rows] in memory
+    at::Tensor scale = at::empty({scale_blocks(width), rows}, xc.options().dtype(at::kFloat));
+    check_rc(spmm_quantize_fp8_launch(xc.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), rows, width, dt,
                                       stream_of(xc)));
-    return {q, scale};
+    return {q, x.dim() == 2 ? scale.t() : rows > 0 ? scale.t().view(shape) : scale.reshape(shape)};
 }
 
 // weight [groups, K, N] -> (q [groups, N, K] e4m3, scale [groups, ceil(N / 128), ceil(K / 128)] fp32)
@@ -1336,7 +1338,7 @@ at::Tensor grouped_matmul_fp8(const at::Tensor &x, const at::Tensor &x_scale, co
     const int itype = check_group_ptr(group_ptr, x, groups, op);
     refuse_grad({&x, &x_scale, &weight, &weight_scale}, op);
     c10::cuda::CUDAGuard guard(x.device());
-    const at::Tensor xc = dense16(x), wc = dense16(weight), xs = x_scale.contiguous(), ws = weight_scale.contiguous();
+    const at::Tensor xc = dense16(x), wc = dense16(weight), xs = x_scale.t().contiguous(), ws = weight_scale.contiguous();
     at::Tensor out = at::empty({rows, N}, xc.options().dtype(out_dtype));
     check_rc(spmm_grouped_matmul_fp8_launch(xc.data_ptr(), xs.data_ptr<float>(), wc.data_ptr(), ws.data_ptr<float>(),
                                             group_ptr.data_ptr(), out.data_ptr(), rows, groups, K, N, itype,

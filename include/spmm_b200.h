@@ -449,7 +449,7 @@ int spmm_embedding_backward_launch(const void *ids, const void *grad, void *dtab
                                    void *workspace, size_t workspace_bytes, void *stream);
 
 /* 8-bit floating point (e4m3, one byte) with a scale for each block of 128:
- *   rows     x [rows, width] -> q [rows, width], scale [rows, ceil(width / 128)]
+ *   rows     x [rows, width] -> q [rows, width], scale [ceil(width / 128), rows]
  *   weights  weight [groups, K, N] -> q [groups, N, K] (transposed), scale
  *            [groups, ceil(N / 128), ceil(K / 128)] of blocks of 128 x 128
  * A block's scale is its largest finite magnitude (at least 2^-100) / 448 in
@@ -460,7 +460,7 @@ int spmm_quantize_weight_fp8_launch(const void *weight, void *q, float *scale, i
                                     int dtype, void *stream);
 
 /* spmm_grouped_matmul of operands in 8 bits as quantised above:
- *   out[r] = sum over blocks b of x_scale[r, b] * weight_scale[g, n / 128, b]
+ *   out[r] = sum over blocks b of x_scale[b, r] * weight_scale[g, n / 128, b]
  *            * sum over block b of x[r, k] * weight[g, n, k]
  * in fp32, rounded to out_dtype once.  Ranges as there (rows outside every
  * group are zero); K and N are divisible by 16. */
