@@ -48,33 +48,39 @@ __device__ __forceinline__ unsigned short quantized(float x0, float x1, float s,
                                     __NV_E4M3);
 }
 
-// 16 lanes per block of a row, 8 elements a lane; width is a multiple of 16.
+// 8 lanes per block of a row, 16 elements a lane (which share the scale's
+// arithmetic); width is a multiple of 16.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *x, unsigned char *q, float *scale, int64_t rows,
                                                             int64_t width)
 {
+    tc::let_next_kernel_start();   // it waits for this one before it reads
     const int64_t blocks = (width + kBlock - 1) / kBlock, items = rows * blocks;
-    const int lane = threadIdx.x & 15;
-    const int64_t step = (int64_t)gridDim.x * (blockDim.x / 16);
-    for (int64_t base = (int64_t)blockIdx.x * (blockDim.x / 16); base < items; base += step) {
-        const int64_t i = base + threadIdx.x / 16;   // all lanes of a warp take the same turns
-        const int64_t r = i / blocks, b = i - r * blocks, c = b * kBlock + lane * 8;
+    const int lane = threadIdx.x & 7;
+    const int64_t step = (int64_t)gridDim.x * (blockDim.x / 8);
+    const int64_t step_rows = step / blocks, step_blocks = step % blocks;   // no division per block
+    int64_t i = (int64_t)blockIdx.x * (blockDim.x / 8) + threadIdx.x / 8;
+    int64_t r = i / blocks, b = i % blocks;
+    for (int64_t base = (int64_t)blockIdx.x * (blockDim.x / 8); base < items; base += step) {
+        // all lanes of a warp take the same turns
+        const int64_t c = b * kBlock + lane * 16;
         const bool on = i < items && c < width;
-        float f[8] = {};
-        if (on) {
-            __align__(16) T raw[8];
+        __align__(16) T raw[16];
 #pragma unroll
-            for (int v = 0; v < (int)sizeof(raw) / 16; ++v)
-                reinterpret_cast<uint4 *>(raw)[v] = __ldcs(reinterpret_cast<const uint4 *>(x + r * width + c) + v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = elem_f32<T>(raw[e]);
+        for (int v = 0; v < (int)sizeof(raw) / 16; ++v) {
+            uint4 &to = reinterpret_cast<uint4 *>(raw)[v];
+            to = make_uint4(0, 0, 0, 0);
+            if (on) to = __ldcs(reinterpret_cast<const uint4 *>(x + r * width + c) + v);
         }
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = elem_f32<T>(raw[e]);
         auto largest = [&](auto of) {
             float m = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, of(f[e]));   // NaN is not the larger one
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, of(f[e]));   // NaN is not the larger one
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+            for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
             return m;
         };
         float m = largest([](float v) { return fabsf(v); });
@@ -82,10 +88,17 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *x, unsigned
         const float s = scale_of(m), inverse = __frcp_rn(s);
         if (i < items && lane == 0) scale[b * rows + r] = s;
         if (on) {
-            __align__(8) unsigned short o[4];
+            __align__(16) unsigned short o[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = quantized(f[2 * e], f[2 * e + 1], s, inverse);
-            *reinterpret_cast<uint2 *>(q + r * width + c) = *reinterpret_cast<const uint2 *>(o);
+            for (int e = 0; e < 8; ++e) o[e] = quantized(f[2 * e], f[2 * e + 1], s, inverse);
+            *reinterpret_cast<uint4 *>(q + r * width + c) = *reinterpret_cast<const uint4 *>(o);
+        }
+        i += step;
+        r += step_rows;
+        b += step_blocks;
+        if (b >= blocks) {
+            b -= blocks;
+            ++r;
         }
     }
 }
@@ -165,7 +178,7 @@ template <int BN, bool PAIR = false> cudaError_t launch_tiles(const Fp8Launch &l
     constexpr int kBlocks = PAIR ? 2 : 1;   // per tile
     const int64_t tiles = row_tiles_of(l, kBlocks * tc::kBM) * ((l.N + BN - 1) / BN);
     const unsigned grid = kBlocks * (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count() / kBlocks));
-    return tc::launch_overlapped(kernel, grid, kBlocks, tc::kFp8Threads, S::kBytes, stream, x, w, out, a);
+    return tc::launch_overlapped(kernel, grid, kBlocks, S::kThreads, S::kBytes, stream, x, w, out, a);
 }
 
 
@@ -177,7 +190,7 @@ cudaError_t launch_quantize_rows(const void *x, void *q, float *scale, int64_t r
     return by_type(dtype, [&](auto type) {
         using T = decltype(type);
         const int64_t items = rows * ((width + kBlock - 1) / kBlock);
-        quantize_rows_kernel<T><<<blocks_for(items, 16), 256, 0, stream>>>(
+        quantize_rows_kernel<T><<<blocks_for(items, 32), 256, 0, stream>>>(
             static_cast<const T *>(x), static_cast<unsigned char *>(q), scale, rows, width);
         return cudaGetLastError();
     });

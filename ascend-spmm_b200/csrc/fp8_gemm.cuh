@@ -6,13 +6,13 @@
 // A persistent block (with PAIR two, on a tile of 256 rows) walks output
 // tiles of 128 x BN.  Warp 0 finds the tiles, hands them to the others through
 // a ring and issues the TMA copies of 128-byte deep slices; a thread of warp 1
-// issues their products; eight warps read the accumulators.  A slice is one
-// block b: its products go into an accumulator of their own, which the
-// epilogue warps add to their registers times the two scales while the next
-// slices run into the others (a sum over blocks cannot stay in TMEM, since the
-// tensor core's own block scales are powers of two).  So P_b is the tensor
-// core's fp32 sum of 128 products, and the blocks are added in fp32 rounded to
-// nearest.
+// issues their products; warp 2 brings the slices' scales into shared memory;
+// the others read the accumulators.  A slice is one block b: its products go
+// into an accumulator of their own, which the epilogue warps add to their
+// registers times the two scales while the next slices run into the others (a
+// sum over blocks cannot stay in TMEM, since the tensor core's own block
+// scales are powers of two).  So P_b is the tensor core's fp32 sum of 128
+// products, and the blocks are added in fp32 rounded to nearest.
 //
 // Every wait is bounded; a wait that runs out raises SPMM_DEV_TIMEOUT, and
 // the block drains its copies and products, frees its TMEM and returns.
@@ -39,48 +39,63 @@ struct Fp8Args {
 };
 
 constexpr int kSlice = 128;           // bytes of a row, the block of a scale
-constexpr int kReaders = 8;           // epilogue warps
-constexpr int kFp8Threads = 64 + 32 * kReaders;
 constexpr int kTiles = 4;             // tiles handed out and not yet taken by every warp
+constexpr int kGroup = 4, kScales = 2;   // slices whose scales are handed over at once; such groups in shared memory
 constexpr int kEnd = -2, kOutside = -1;   // in the place of a group
 
 template <int BN, bool PAIR> struct Fp8Shape {
+    // epilogue warps: each has 32 rows and at most 64 columns in registers
+    static constexpr int kReaders = BN == 256 ? 16 : 8, kOwn = BN / (kReaders / 4);
+    static constexpr int kFirstReader = 4, kThreads = 32 * (kFirstReader + kReaders);   // warp 3 has no work
     static constexpr int kA = kBM * kSlice, kB = (PAIR ? BN / 2 : BN) * kSlice;
-    static constexpr int kStages = 6, kStaging = 4096;             // of an epilogue warp
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 5 : 6, kStaging = 4096;             // of an epilogue warp, twice 32 x 32 16-bit values
     static constexpr int kAccs = BN == 256 ? 2 : 4, kCols = kAccs * BN;
-    static constexpr int kStageOff = kStages * (kA + kB), kTileOff = kStageOff + kReaders * kStaging;
+    static constexpr int kHalves = BN == 256 ? 2 : 1, kScaleBytes = kHalves * kBM * 4;   // of a slice, per block of 128 columns
+    static constexpr int kStageOff = kStages * (kA + kB), kScaleOff = kStageOff + kReaders * kStaging;
+    static constexpr int kTileOff = kScaleOff + kScales * kGroup * kScaleBytes;
     static constexpr int kFull = kTileOff + 16 * kTiles, kEmpty = kFull + 8 * kStages;
     static constexpr int kAccFull = kEmpty + 8 * kStages, kAccEmpty = kAccFull + 8 * kAccs;
     static constexpr int kTileFull = kAccEmpty + 8 * kAccs, kTileEmpty = kTileFull + 8 * kTiles;
-    static constexpr int kDone = kTileEmpty + 8 * kTiles, kTmem = kDone + 8, kAbort = kTmem + 4, kBytes = kAbort + 4;
+    static constexpr int kScaleFull = kTileEmpty + 8 * kTiles, kScaleEmpty = kScaleFull + 8 * kScales;
+    static constexpr int kDone = kScaleEmpty + 8 * kScales, kTmem = kDone + 8, kAbort = kTmem + 4, kBytes = kAbort + 4;
     static_assert(kBytes <= 232448 && kCols <= 512, "shared memory of a block, TMEM of an SM");
 };
 
-// A place in a ring and how often it came round.
+// A place in a ring of N (a power of two) and the parity of its rounds, from one counter.
+template <int N> struct Turn {
+    unsigned count = 0;
+    __device__ __forceinline__ unsigned at() const { return count % N; }
+    __device__ __forceinline__ unsigned parity() const { return count / N & 1u; }
+    __device__ __forceinline__ void next() { ++count; }
+};
+// The same for any N.
 template <int N> struct Ring {
-    unsigned at = 0, turn = 0;
+    unsigned place = 0, turn = 0;
+    __device__ __forceinline__ unsigned at() const { return place; }
+    __device__ __forceinline__ unsigned parity() const { return turn; }
     __device__ __forceinline__ void next()
     {
-        if (++at == N) {
-            at = 0;
+        if (++place == N) {
+            place = 0;
             turn ^= 1u;
         }
     }
 };
 
 template <int BN, bool PAIR>
-__global__ void __launch_bounds__(kFp8Threads, 1)
+__global__ void __launch_bounds__(Fp8Shape<BN, PAIR>::kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_o, const __grid_constant__ Fp8Args a)
 {
     using S = Fp8Shape<BN, PAIR>;
-    constexpr int kHeight = PAIR ? 2 * kBM : kBM;
+    constexpr int kHeight = PAIR ? 2 * kBM : kBM, kReaders = S::kReaders, kFirstReader = S::kFirstReader;
     extern __shared__ __align__(1024) unsigned char smem[];
     const unsigned base = (unsigned)__cvta_generic_to_shared(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort = reinterpret_cast<volatile int *>(smem + S::kAbort);
     const unsigned full = base + S::kFull, empty = base + S::kEmpty;
     const unsigned acc_full = base + S::kAccFull, acc_empty = base + S::kAccEmpty;
+    const unsigned scale_full = base + S::kScaleFull, scale_empty = base + S::kScaleEmpty;
     const unsigned tile_full = base + S::kTileFull, tile_empty = base + S::kTileEmpty, done = base + S::kDone;
     const unsigned peer = PAIR ? cluster_rank() : 0;   // 0: the pair's first block
 
@@ -95,7 +110,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
         for (int i = 0; i < kTiles; ++i) {
             bar_init(tile_full + 8 * i, 1);
-            bar_init(tile_empty + 8 * i, 1 + kReaders);
+            bar_init(tile_empty + 8 * i, 2 + kReaders);
+        }
+        for (int i = 0; i < kScales; ++i) {
+            bar_init(scale_full + 8 * i, 1);
+            bar_init(scale_empty + 8 * i, kReaders);
         }
         bar_init(done, 1);
         // a misaligned stage ring would break the swizzle: give up before any copy
@@ -141,7 +160,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (warp == 0) {
         // ---- finds the tiles and issues their copies
         TileWalk<false> walk;
-        Ring<kTiles> hand;
+        Turn<kTiles> hand;
         Ring<S::kStages> stage;
         unsigned issued = 0;   // slices
         const unsigned nt = (unsigned)((a.n + BN - 1) / BN);
@@ -153,10 +172,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 t = make_int4((int)row, (int)max((int64_t)0, min((int64_t)kBM, e - row)), (int)((unsigned)inner % nt) * BN,
                               seg >= 1 && seg <= a.ranges.groups ? (int)seg - 1 : kOutside);
             }
-            if (!bar_wait(tile_empty + 8 * hand.at, hand.turn ^ 1u, abort)) { give_up(6); break; }
+            if (!bar_wait(tile_empty + 8 * hand.at(), hand.parity() ^ 1u, abort)) { give_up(6); break; }
             if (lane == 0) {
-                tiles[hand.at] = t;
-                bar_arrive(tile_full + 8 * hand.at);
+                tiles[hand.at()] = t;
+                bar_arrive(tile_full + 8 * hand.at());
             }
             __syncwarp();
             hand.next();
@@ -165,17 +184,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (elect()) {
                 const int col = t.z + (PAIR ? (int)peer * (BN / 2) : 0);
                 for (int k = 0; k < a.blocks_k; ++k) {
-                    if (!bar_wait(empty + 8 * stage.at, stage.turn ^ 1u, abort)) { give_up(1); break; }
-                    const unsigned sa = base + stage.at * (S::kA + S::kB), sb = sa + S::kA;
+                    if (!bar_wait(empty + 8 * stage.at(), stage.parity() ^ 1u, abort)) { give_up(1); break; }
+                    const unsigned sa = base + stage.at() * (S::kA + S::kB), sb = sa + S::kA;
                     // a pair's slice, both halves, arrives on the first block's barrier
-                    if (peer == 0) bar_expect(full + 8 * stage.at, (PAIR ? 2 : 1) * (S::kA + S::kB));
+                    if (peer == 0) bar_expect(full + 8 * stage.at(), (PAIR ? 2 : 1) * (S::kA + S::kB));
                     if constexpr (PAIR) {
-                        const unsigned bar = in_block(full + 8 * stage.at, 0);
+                        const unsigned bar = in_block(full + 8 * stage.at(), 0);
                         tma_load_pair(sa, &map_a, k * kSlice, t.x, 0, bar);
                         tma_load_pair(sb, &map_b, k * kSlice, col, t.w, bar);
                     } else {
-                        tma_load(sa, &map_a, k * kSlice, t.x, 0, full + 8 * stage.at);
-                        tma_load(sb, &map_b, k * kSlice, col, t.w, full + 8 * stage.at);
+                        tma_load(sa, &map_a, k * kSlice, t.x, 0, full + 8 * stage.at());
+                        tma_load(sb, &map_b, k * kSlice, col, t.w, full + 8 * stage.at());
                     }
                     stage.next();
                 }
@@ -195,32 +214,32 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (elect()) {
             const unsigned idesc = idesc8(kHeight, BN);
             const uint64_t da = desc128(base, 16, 1024), db = desc128(base + S::kA, 16, 1024);
-            Ring<kTiles> hand;
+            Turn<kTiles> hand;
             Ring<S::kStages> stage;
-            Ring<S::kAccs> acc;
+            Turn<S::kAccs> acc;
             while (ok) {
-                if (!bar_wait(tile_full + 8 * hand.at, hand.turn, abort)) { give_up(7); break; }
-                const int group = tiles[hand.at].w;
-                bar_arrive(tile_empty + 8 * hand.at);
+                if (!bar_wait(tile_full + 8 * hand.at(), hand.parity(), abort)) { give_up(7); break; }
+                const int group = tiles[hand.at()].w;
+                bar_arrive(tile_empty + 8 * hand.at());
                 hand.next();
                 if (group == kEnd) break;
                 if (group < 0 || peer != 0) continue;
                 for (int k = 0; k < a.blocks_k; ++k) {
-                    if (!bar_wait<PAIR>(acc_empty + 8 * acc.at, acc.turn ^ 1u, abort)) { give_up(2); break; }
-                    if (!bar_wait<PAIR>(full + 8 * stage.at, stage.turn, abort)) { give_up(3); break; }
+                    if (!bar_wait(full + 8 * stage.at(), stage.parity(), abort)) { give_up(3); break; }
+                    if (!bar_wait(acc_empty + 8 * acc.at(), acc.parity() ^ 1u, abort)) { give_up(2); break; }
                     fence_after();
-                    const unsigned d = tmem + acc.at * BN, off = stage.at * (S::kA + S::kB) >> 4;
+                    const unsigned d = tmem + acc.at() * BN, off = stage.at() * (S::kA + S::kB) >> 4;
 #pragma unroll
                     for (int i = 0; i < kSlice / 32; ++i) {
                         if constexpr (PAIR) mma_pair<true>(d, da + off + 2 * i, db + off + 2 * i, idesc, i > 0);
                         else mma<true>(d, da + off + 2 * i, db + off + 2 * i, idesc, i > 0);
                     }
                     if constexpr (PAIR) {
-                        commit_pair(acc_full + 8 * acc.at);
-                        commit_pair(empty + 8 * stage.at);
+                        commit_pair(acc_full + 8 * acc.at());
+                        commit_pair(empty + 8 * stage.at());
                     } else {
-                        commit(acc_full + 8 * acc.at);
-                        commit(empty + 8 * stage.at);
+                        commit(acc_full + 8 * acc.at());
+                        commit(empty + 8 * stage.at());
                     }
                     stage.next();
                     acc.next();
@@ -234,46 +253,80 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
         }
         __syncwarp();
-    } else {
-        // ---- epilogue warps: TMEM lanes 32 (warp % 4) .. + 31 are rows of the
-        // tile; of the two warps of a lane quarter each has one half of the columns
-        constexpr int kOwn = BN / 2, kRead = kOwn > 64 ? 16 : 32;   // its columns; read at a time
-        const int row0 = (warp & 3) * 32, first = (warp - 2) / 4 * kOwn;
-        const unsigned stage = base + S::kStageOff + (warp - 2) * S::kStaging;
-        const unsigned lanes = tmem + ((unsigned)row0 << 16) + first;
-        Ring<kTiles> hand;
-        Ring<S::kAccs> acc;
+    } else if (warp == 2) {
+        // ---- the scales of each slice: a row's times that of each block of columns
+        float *const scales = reinterpret_cast<float *>(smem + S::kScaleOff);
+        Turn<kTiles> hand;
+        Turn<kScales> slot;
         while (ok) {
-            if (!bar_wait(tile_full + 8 * hand.at, hand.turn, abort)) { give_up(8); break; }
-            const int4 t = tiles[hand.at];
+            if (!bar_wait(tile_full + 8 * hand.at(), hand.parity(), abort)) { give_up(9); break; }
+            const int4 t = tiles[hand.at()];
             __syncwarp();
-            if (lane == 0) bar_arrive(tile_empty + 8 * hand.at);
+            if (lane == 0) bar_arrive(tile_empty + 8 * hand.at());
+            hand.next();
+            if (t.w == kEnd) break;
+            if (t.w < 0) continue;
+            for (int k0 = 0; k0 < a.blocks_k && ok; k0 += kGroup) {
+                float rows[kGroup][4], cols[kGroup][S::kHalves];
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) {
+                    const int k = min(k0 + j, a.blocks_k - 1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = lane + 32 * i;
+                        rows[j][i] = r < t.y ? __ldg(a.scale_a + (int64_t)k * a.ranges.rows + t.x + r) : 0.f;
+                    }
+#pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h) {
+                        const int block = min(t.z / kSlice + h, a.blocks_n - 1);
+                        cols[j][h] = __ldg(a.scale_b + ((int64_t)t.w * a.blocks_n + block) * a.blocks_k + k);
+                    }
+                }
+                if (!bar_wait(scale_empty + 8 * slot.at(), slot.parity() ^ 1u, abort)) { give_up(10); break; }
+                float *to = scales + slot.at() * (kGroup * S::kScaleBytes / 4);
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j)
+#pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) to[(j * S::kHalves + h) * kBM + lane + 32 * i] = rows[j][i] * cols[j][h];
+                __syncwarp();
+                if (lane == 0) bar_arrive(scale_full + 8 * slot.at());
+                slot.next();
+            }
+        }
+    } else if (warp >= kFirstReader) {
+        // ---- epilogue warps: TMEM lanes 32 (warp % 4) .. + 31 are rows of the
+        // tile; the warps of a lane quarter share the columns out
+        constexpr int kOwn = S::kOwn, kRead = kReaders == 16 ? 8 : 32;   // its columns; read at a time
+        const int row0 = (warp & 3) * 32, first = (warp - kFirstReader) / 4 * kOwn;
+        const unsigned stage = base + S::kStageOff + (warp - kFirstReader) * S::kStaging;
+        const unsigned lanes = tmem + ((unsigned)row0 << 16) + first;
+        const float *const scales = reinterpret_cast<const float *>(smem + S::kScaleOff) + first / kSlice * kBM + row0 + lane;
+        const unsigned acc_empty_0 = PAIR ? in_block(acc_empty, 0) : 0;   // the first block's
+        Turn<kTiles> hand;
+        Turn<S::kAccs> acc;
+        Turn<kScales> slot;
+        while (ok) {
+            if (!bar_wait(tile_full + 8 * hand.at(), hand.parity(), abort)) { give_up(8); break; }
+            const int4 t = tiles[hand.at()];
+            __syncwarp();
+            if (lane == 0) bar_arrive(tile_empty + 8 * hand.at());
             hand.next();
             if (t.w == kEnd) break;
             const bool on = row0 + lane < t.y, any = row0 < t.y && t.z + first < a.n;
             float v[kOwn];
 #pragma unroll
             for (int i = 0; i < kOwn; ++i) v[i] = 0.f;
-            const float *sa = a.scale_a + t.x + row0 + lane;
-            const float *sb = a.scale_b;
-            if (t.w >= 0 && any) sb += ((int64_t)t.w * a.blocks_n + (t.z + first) / kSlice) * a.blocks_k;
-            // a slice's scales are read while the one before it is added
-            float row_scale = 0.f, col_scale = 0.f;
             const int n = t.w >= 0 ? a.blocks_k : 0;
-            if (n > 0 && on && any) {
-                row_scale = __ldg(sa);
-                col_scale = __ldg(sb);
-            }
             for (int k = 0; k < n; ++k) {
-                const float scale = row_scale * col_scale;
-                if (k + 1 < n && on && any) {
-                    row_scale = __ldg(sa += a.ranges.rows);
-                    col_scale = __ldg(++sb);
-                }
-                if (!bar_wait<PAIR>(acc_full + 8 * acc.at, acc.turn, abort)) { give_up(4); break; }
+                const int in_group = k % kGroup;
+                if (in_group == 0 && !bar_wait(scale_full + 8 * slot.at(), slot.parity(), abort)) { give_up(11); break; }
+                const float scale = scales[(slot.at() * kGroup + in_group) * (S::kScaleBytes / 4)];
+                if (!bar_wait(acc_full + 8 * acc.at(), acc.parity(), abort)) { give_up(4); break; }
                 fence_after();
                 if (any) {
-                    const unsigned from = lanes + acc.at * BN;
+                    const unsigned from = lanes + acc.at() * BN;
 #pragma unroll
                     for (int c = 0; c < kOwn; c += kRead) {
                         float w[kRead];
@@ -285,12 +338,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    // not a release to the cluster, which would wait for the next scales to arrive: what the first block
-                    // must not overtake are TMEM reads, complete here
-                    if (PAIR) bar_arrive_peer(in_block(acc_empty + 8 * acc.at, 0));
-                    else bar_arrive(acc_empty + 8 * acc.at);
+                    // not a release to the cluster, which would also order memory: what the first block must not overtake are
+                    // TMEM reads, complete here
+                    if (PAIR) bar_arrive_peer(acc_empty_0 + 8 * acc.at());
+                    else bar_arrive(acc_empty + 8 * acc.at());
                 }
                 acc.next();
+                if (in_group == kGroup - 1 || k + 1 == n) {
+                    if (lane == 0) bar_arrive(scale_empty + 8 * slot.at());
+                    slot.next();
+                }
             }
             if (!ok) break;
             if (!any) continue;
@@ -298,24 +355,37 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             // a group's last rows share the block with the next group's: no box for them
             const bool boxed = row0 + 32 <= t.y;
             const unsigned swz2 = (unsigned)(lane >> 1 & 3), swz4 = (unsigned)(lane & 7);
+            if (boxed && out_size == 2) {   // all of the warp's columns behind one fence
+                if (elect()) bulk_wait_read<0>();   // the staging's last stores have read it
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < kOwn; c += 32)
+#pragma unroll
+                    for (unsigned i = 0; i < 4; ++i)
+                        st_shared16(stage + c / 32 * 2048 + lane * 64 + ((i ^ swz2) << 4),
+                                    pack8(v + c + 8 * i, a.out_type == kOutBf16));
+                fence_async();
+                __syncwarp();
+                if (elect()) {
+#pragma unroll
+                    for (int c = 0; c < kOwn; c += 32)
+                        if (t.z + first + c < a.n) tma_store(&map_o, stage + c / 32 * 2048, t.z + first + c, t.x + row0, 0);
+                    bulk_commit();
+                }
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < kOwn; c += 32) {
                 const int x = t.z + first + c;
                 if (x >= a.n) break;
                 if (boxed) {
-                    if (elect()) bulk_wait_read<0>();   // the staging's last store has read it
+                    if (elect()) bulk_wait_read<0>();
                     __syncwarp();
-                    if (out_size == 4) {
 #pragma unroll
-                        for (unsigned i = 0; i < 8; ++i)
-                            st_shared16(stage + lane * 128 + ((i ^ swz4) << 4),
-                                        make_uint4(__float_as_uint(v[c + 4 * i]), __float_as_uint(v[c + 4 * i + 1]),
-                                                   __float_as_uint(v[c + 4 * i + 2]), __float_as_uint(v[c + 4 * i + 3])));
-                    } else {
-#pragma unroll
-                        for (unsigned i = 0; i < 4; ++i)
-                            st_shared16(stage + lane * 64 + ((i ^ swz2) << 4), pack8(v + c + 8 * i, a.out_type == kOutBf16));
-                    }
+                    for (unsigned i = 0; i < 8; ++i)
+                        st_shared16(stage + lane * 128 + ((i ^ swz4) << 4),
+                                    make_uint4(__float_as_uint(v[c + 4 * i]), __float_as_uint(v[c + 4 * i + 1]),
+                                               __float_as_uint(v[c + 4 * i + 2]), __float_as_uint(v[c + 4 * i + 3])));
                     fence_async();
                     __syncwarp();
                     if (elect()) {

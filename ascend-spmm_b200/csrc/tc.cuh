@@ -212,21 +212,9 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v)
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// 16 or 32 consecutive columns as above.
+// 8 or 32 consecutive columns as above.
+__device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[8]) { tmem_ld8(taddr, v); }
 __device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
-__device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[16])
-{
-    unsigned r[16];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, "
-                 "[%16];\n\ttcgen05.wait::ld.sync.aligned;\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-                   "=r"(r[15])
-                 : "r"(taddr)
-                 : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // ---- pairs of blocks (clusters of two) -------------------------------------
 __device__ __forceinline__ unsigned cluster_rank()
