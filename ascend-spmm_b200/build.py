@@ -36,7 +36,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-r
 CU_SOURCES = ["status.cu", "gather.cu", "gather_mma.cu", "window.cu", "window_warp.cu", "window_tc.cu", "rows.cu", "cube.cu", "preprocess.cu", "noalloc.cu", "l2plan.cu", "norm.cu", "gemm_tc.cu", "grouped.cu", "ortho.cu", "ortho_small.cu", "route.cu", "bucket.cu", "routed.cu", "embedding.cu", "fp8.cu", "capi_layers.cu", "capi.cu"]
 HEADERS = ["common.cuh", "engine.h"]
 LAYER_SOURCES = ["norm.cu", "gemm_tc.cu", "grouped.cu", "ortho.cu", "ortho_small.cu", "route.cu", "bucket.cu", "routed.cu", "embedding.cu", "fp8.cu", "capi_layers.cu"]
-LAYER_HEADERS = ["layer.cuh", "layer.h", "tc.cuh", "gemm_tc.cuh", "fp8_gemm.cuh", "ortho.cuh"]
+LAYER_HEADERS = ["layer.cuh", "vec.cuh", "layer.h", "tc.cuh", "gemm_tc.cuh", "fp8_gemm.cuh", "ortho.cuh"]
 
 
 def _newer(target: Path, deps) -> bool:

@@ -6,8 +6,11 @@
 // other's totals through distributed shared memory, so that a launch counts,
 // scans and places.  Places come from counts alone (the order of the shared
 // atomics that count does not show), so a result never depends on timing.
+// Further clusters of the launch, where a caller asks for them, write zeros
+// meanwhile: the sort leaves nearly all of the GPU to them.
 //
-// What bounds it: the latency of its phases.
+// What bounds it: the latency of its phases, and of a warp's turns (256 keys
+// each, whose loads are in flight together).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -25,7 +28,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kWarps = 32, kCluster = 8;
+constexpr int kWarps = 32, kBatch = 8;
 
 // Shared memory: counts [kWarps][buckets], then the block's totals [buckets]
 // and the scan's sums per warp.
@@ -36,6 +39,12 @@ __global__ void __launch_bounds__(kWarps * 32) bucket_kernel(const BucketSort a)
     extern __shared__ int smem[];
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
+    if ((int)blockIdx.x >= blocks) {   // not the first cluster
+        const int64_t threads = (int64_t)(gridDim.x - blocks) * blockDim.x;
+        for (int64_t i = (int64_t)(blockIdx.x - blocks) * blockDim.x + threadIdx.x; i < a.zero_vectors; i += threads)
+            __stcs(static_cast<uint4 *>(a.zero) + i, make_uint4(0, 0, 0, 0));
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, B = a.buckets;
     int *mine = smem + warp * B, *totals = smem + kWarps * B, *sums = totals + B;
     for (int i = threadIdx.x; i < kWarps * B; i += blockDim.x) smem[i] = 0;
@@ -45,30 +54,41 @@ __global__ void __launch_bounds__(kWarps * 32) bucket_kernel(const BucketSort a)
     const int64_t slices = (int64_t)blocks * kWarps;
     const int64_t each = ((a.n + slices - 1) / slices + 31) / 32 * 32;
     const int64_t begin = min(a.n, ((int64_t)block * kWarps + warp) * each), end = min(a.n, begin + each);
-    // The input at place i of this pass and its bucket, -1 where it is left out.
-    auto read = [&](int64_t i, int *input, bool raise) {
-        *input = -1;
-        if (i >= end) return -1;
-        const int at = a.order_in ? a.order_in[i] : (int)i;
-        if (at < 0) return -1;
-        *input = at;
-        const int64_t key = a.wide ? static_cast<const int64_t *>(a.keys)[at] : static_cast<const int *>(a.keys)[at];
-        if (key == a.skip) return -1;
-        if (key < 0 || key >= a.limit) {
-            if (raise) raise_status(a.status, SPMM_DEV_BAD_COLUMN, at);
-            return -1;
+    // kBatch x 32 keys from i on: each lane's input and key, and its bucket, -1 where it is left out.
+    int input[kBatch], bucket[kBatch];
+    int64_t key[kBatch];
+    auto read = [&](int64_t i, bool raise) {
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) {
+            const int64_t at = i + s * 32 + lane;
+            input[s] = -1;
+            key[s] = -1;
+            if (at < end) {
+                input[s] = a.order_in ? __ldg(a.order_in + at) : (int)at;
+                key[s] = a.wide ? ld_idx(static_cast<const int64_t *>(a.keys) + at) : ld_idx(static_cast<const int *>(a.keys) + at);
+            }
         }
-        return (int)(key >> a.shift) & a.mask;
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) {
+            bool in = input[s] >= 0 && key[s] != a.skip;
+            if (in && (key[s] < 0 || key[s] >= a.limit)) {
+                if (raise) raise_status(a.status, SPMM_DEV_BAD_COLUMN, input[s]);
+                in = false;
+            }
+            bucket[s] = in ? (int)(key[s] >> a.shift) & a.mask : -1;
+        }
     };
-    for (int64_t i = begin; i < end; i += 32) {
-        int input;
-        const int b = read(i + lane, &input, true);
-        if (b >= 0) atomicAdd(mine + b, 1);
+    for (int64_t i = begin; i < end; i += 32 * kBatch) {
+        read(i, true);
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s)
+            if (bucket[s] >= 0) atomicAdd(mine + bucket[s], 1);
     }
     __syncthreads();
     // per bucket: this warp's keys before each warp's, the block's total
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int sum = 0;
+#pragma unroll 8
         for (int w = 0; w < kWarps; ++w) {
             const int c = smem[w * B + b];
             smem[w * B + b] = sum;
@@ -81,6 +101,7 @@ __global__ void __launch_bounds__(kWarps * 32) bucket_kernel(const BucketSort a)
     const int b = threadIdx.x;
     int before = 0, all = 0;
     if (b < B)
+#pragma unroll 8
         for (int c = 0; c < blocks; ++c) {
             const int v = cluster.map_shared_rank(totals, c)[b];
             before += c < block ? v : 0;
@@ -111,51 +132,72 @@ __global__ void __launch_bounds__(kWarps * 32) bucket_kernel(const BucketSort a)
     }
     if (a.ptr && block == 0 && threadIdx.x == 0) a.ptr[B] = kept;
     __syncthreads();
-    for (int i = threadIdx.x; i < kWarps * B; i += blockDim.x) smem[i] += totals[i % B];
-    __syncthreads();
+    for (int i = lane; i < B; i += 32) mine[i] += totals[i];
+    __syncwarp();
 
-    for (int64_t i = begin; i < end; i += 32) {
-        int input;
-        const int bucket = read(i + lane, &input, false);
-        const unsigned peers = __match_any_sync(kFull, bucket);
-        const int rank = __popc(peers & ((1u << lane) - 1));
-        int place = -1;
-        if (bucket >= 0) place = mine[bucket] + rank;
-        __syncwarp();
-        if (bucket >= 0 && rank == 0) mine[bucket] += __popc(peers);
-        __syncwarp();
-        if (place >= 0) a.order[place] = input;
-        if (a.position && input >= 0) a.position[input] = place;
+    for (int64_t i = begin; i < end; i += 32 * kBatch) {
+        read(i, false);
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) {
+            const unsigned peers = __match_any_sync(kFull, bucket[s]);
+            const int rank = __popc(peers & ((1u << lane) - 1));
+            int place = -1;
+            if (bucket[s] >= 0) place = mine[bucket[s]] + rank;
+            __syncwarp();
+            if (bucket[s] >= 0 && rank == 0) mine[bucket[s]] += __popc(peers);
+            __syncwarp();
+            if (place >= 0) {
+                a.order[place] = input[s];
+                if (a.key_out) a.key_out[place] = (int)key[s];
+            }
+            if (a.position && input[s] >= 0) a.position[input[s]] = place;
+        }
     }
-    for (int64_t i = kept + (int64_t)block * blockDim.x + threadIdx.x; i < a.n; i += (int64_t)blocks * blockDim.x)
+    for (int64_t i = kept + (int64_t)block * blockDim.x + threadIdx.x; i < a.n; i += (int64_t)blocks * blockDim.x) {
         a.order[i] = -1;
+        if (a.key_out) a.key_out[i] = -1;
+    }
 }
 
 }  // namespace
 
 cudaError_t launch_bucket_sort(const BucketSort &a, cudaStream_t stream)
 {
-    const size_t smem = bucket_smem(a.buckets);
-    static PerDevice<bool> ready;   // the attribute outlasts the call
-    bool *done = ready.here();
-    if (!done || !*done) {
-        const cudaError_t e = cudaFuncSetAttribute(bucket_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)bucket_smem(kMostBuckets));
-        if (e != cudaSuccess) return e;
-        if (done) *done = true;
-    }
-    const unsigned blocks = a.n <= 4096 ? 1 : kCluster;
+    // Blocks of the cluster: one for few keys, 16 for many where the device can hold such a cluster.
+    static PerDevice<int> most;   // outlasts the call
+    int *known = most.here(), widest = known ? *known : 0;
     cudaLaunchConfig_t config{};
-    config.gridDim = blocks;
     config.blockDim = kWarps * 32;
-    config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = blocks;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
+    if (!widest) {
+        cudaError_t e = cudaFuncSetAttribute(bucket_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)bucket_smem(kMostBuckets));
+        if (e != cudaSuccess) return e;
+        int clusters = 0;
+        config.gridDim = attr.val.clusterDim.x = 16;
+        config.dynamicSmemBytes = bucket_smem(kMostBuckets);
+        if (cudaFuncSetAttribute(bucket_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&clusters, bucket_kernel, &config) != cudaSuccess)
+            clusters = 0;
+        (void)cudaGetLastError();
+        widest = clusters > 0 ? 16 : 8;
+        if (known) *known = widest;
+    }
+    const unsigned blocks = a.n <= 4096 ? 1 : a.n <= 32768 ? 8 : (unsigned)widest;
+    unsigned extra = 0;
+    if (a.zero_vectors > 0) {
+        const int64_t useful = (a.zero_vectors + kWarps * 32 - 1) / (kWarps * 32);
+        extra = (unsigned)std::min<int64_t>(useful, 2 * (int64_t)device_sm_count());
+        extra = (extra + blocks - 1) / blocks * blocks;   // whole clusters
+    }
+    config.gridDim = blocks + extra;
+    attr.val.clusterDim.x = blocks;
+    config.dynamicSmemBytes = bucket_smem(a.buckets);
     return cudaLaunchKernelEx(&config, bucket_kernel, a);
 }
 

@@ -99,7 +99,7 @@ cudaError_t launch_route_backward(const RouteLaunch &r, const float *grad, void 
 
 // ---- stable counting sort (bucket.cu) ---------------------------------------
 struct BucketSort {
-    const void *keys;       // [n] by input, int32 or int64
+    const void *keys;       // [n] in the order of order_in, int32 or int64
     bool wide;
     const int *order_in;    // the inputs in the order to keep (an earlier pass's), -1: none; null: as they are
     int64_t n;
@@ -110,6 +110,9 @@ struct BucketSort {
     int *ptr;               // [buckets + 1] first place of each bucket; may be null
     int *position;          // [n] place of each input, -1 where it is left out; may be null
     int *order;             // [n] input of each place, -1 past the last
+    int *key_out;           // [n] their keys, -1 past the last; may be null (then limit may pass 32 bits)
+    void *zero;             // 16-byte vectors to zero meanwhile
+    int64_t zero_vectors;
     DevStatus *status;
 };
 constexpr int kBucketBits = 10, kMostBuckets = 1 << kBucketBits;

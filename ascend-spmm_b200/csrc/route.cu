@@ -38,12 +38,6 @@ constexpr int kNanKey = INT32_MIN + 64;      // below every number's key, above 
 constexpr long long kNone64 = INT64_MIN;
 
 __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(kFull, v); }
-__device__ __forceinline__ float warp_max(float v)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-    return v;
-}
 template <typename F> __device__ __forceinline__ F warp_sum(F v)
 {
 #pragma unroll
@@ -62,6 +56,31 @@ __device__ __forceinline__ long long order_key(double d)
 {
     const long long b = __double_as_longlong(d + 0.0);
     return isnan(d) ? kNone64 + 1 : b ^ ((b >> 63) & INT64_MAX);
+}
+
+// Largest of the lanes' values; NaN only where all are.
+__device__ __forceinline__ float warp_max(float v)
+{
+    const int k = warp_max(order_key(v));
+    return k == kNanKey ? NAN : key_value(k);
+}
+
+// Descending order (a merge network of pairs: Batcher 1968).
+template <int N> __device__ __forceinline__ void sort_descending(int (&v)[N])
+{
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const int a = v[i + j], b = v[i + j + k];
+                        v[i + j] = max(a, b);
+                        v[i + j + k] = min(a, b);
+                    }
 }
 
 // The largest and the lowest lane that has it.
@@ -203,13 +222,23 @@ __device__ __forceinline__ bool too_close(float hi, float lo, float largest, flo
     return !(hi - lo > 0x1p-19f * largest + rel * fmaxf(fabsf(hi), fabsf(lo)));   // true for infinities, too
 }
 
-template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) route_kernel(const RouteArgs a)
+// Blocks of an SM: rows are handled in a long chain of dependent steps, so the
+// more warps take turns the better.
+constexpr int route_blocks(int vpl) { return vpl <= 2 ? 8 : vpl == 4 ? 6 : vpl == 8 ? 5 : vpl == 16 ? 4 : 2; }
+
+template <typename T, int VPL, bool VEC>
+__global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const RouteArgs a)
 {
+    __shared__ int chosen[8][kMostChosen + 1];
     constexpr int kLow = VPL - 1;   // bits of a key that hold the (reversed) place in the lane
     const int lane = threadIdx.x & 31, n = a.n;
     const int first = lane * VPL;
     const bool grouped = a.top_groups < a.groups;
     const bool by_logit = !a.bias && (!grouped || a.group_best == 1);
+    // groups that are whole lanes, a power of two of them
+    const int per = n / a.groups, lanes = per / VPL;
+    const bool by_lanes = per % VPL == 0 && (lanes & (lanes - 1)) == 0 && lanes <= 32;
+    int *const picks = chosen[threadIdx.x / 32];
     const int64_t step = (int64_t)gridDim.x * (blockDim.x / 32);
     for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; t < a.tokens; t += step) {
         const T *row = static_cast<const T *>(a.logits) + t * n;
@@ -252,24 +281,45 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
         const bool exact = by_logit && (sizeof(T) == 2 || VPL == 1);
         bool again = false;
         if (grouped) {
-            const int per = n / a.groups;
+            // lane g: the score of group g
             int mine = kNone;
-            for (int g = 0; g < a.groups; ++g) {
+            auto sum_of = [&](int top, int next) {   // of two keys without their low bits
+                return order_key((top == kNanKey ? NAN : key_value(top)) + (next == kNanKey ? NAN : key_value(next)));
+            };
+            if (by_lanes) {
                 int b1 = kNone, b2 = kNone;
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) {
-                    const int i = first + j, v = i >= g * per && i < (g + 1) * per ? key[j] : kNone;
-                    b2 = max(b2, min(b1, v));
-                    b1 = max(b1, v);
+                    b2 = max(b2, min(b1, key[j]));
+                    b1 = max(b1, key[j]);
                 }
-                const int top = warp_max(b1);
-                int score = top & ~kLow;
-                if (a.group_best == 2) {
-                    const int winner = __ffs(__ballot_sync(kFull, b1 == top)) - 1;
-                    const int next = warp_max(lane == winner ? b2 : b1) & ~kLow;
-                    score = order_key((score == kNanKey ? NAN : key_value(score)) + (next == kNanKey ? NAN : key_value(next)));
+                b1 &= ~kLow;
+                b2 &= ~kLow;
+                for (int o = 1; o < lanes; o <<= 1) {
+                    const int o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+                    b2 = max(min(b1, o1), max(b2, o2));
+                    b1 = max(b1, o1);
                 }
-                if (lane == g) mine = score;
+                const int score = a.group_best == 2 ? sum_of(b1, b2) : b1;
+                mine = __shfl_sync(kFull, score, min(lane, a.groups - 1) * lanes);
+                if (lane >= a.groups) mine = kNone;
+            } else {
+                for (int g = 0; g < a.groups; ++g) {
+                    int b1 = kNone, b2 = kNone;
+#pragma unroll
+                    for (int j = 0; j < VPL; ++j) {
+                        const int i = first + j, v = i >= g * per && i < (g + 1) * per ? key[j] : kNone;
+                        b2 = max(b2, min(b1, v));
+                        b1 = max(b1, v);
+                    }
+                    const int top = warp_max(b1);
+                    int score = top & ~kLow;
+                    if (a.group_best == 2) {
+                        const int winner = __ffs(__ballot_sync(kFull, b1 == top)) - 1;
+                        score = sum_of(score, warp_max(lane == winner ? b2 : b1) & ~kLow);
+                    }
+                    if (lane == g) mine = score;
+                }
             }
             int rank = 0;
             for (int h = 0; h < a.groups; ++h) {
@@ -281,28 +331,35 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
             const int last = __reduce_min_sync(kFull, stays ? mine : INT32_MAX);
             const int out = warp_max(stays ? kNone : mine);
             if (!exact) again = too_close(key_value(last), key_value(out), largest, 2 * rel);
+            if (by_lanes) {
+                if (first < n && !(kept >> (lane / lanes) & 1u)) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (first + j < n && !(kept >> ((first + j) / per) & 1u)) key[j] = kNone;
+                    for (int j = 0; j < VPL; ++j) key[j] = kNone;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VPL; ++j)
+                    if (first + j < n && !(kept >> ((first + j) / per) & 1u)) key[j] = kNone;
+            }
         }
-        int pick = 0, before = 0;
+        // each lane's keys in descending order: a pick is the largest of the lanes' first ones
+        sort_descending(key);
+        int before = 0;
         for (int p = 0; p <= a.k && !again; ++p) {
-            int m = kNone;
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) m = max(m, key[j]);
-            const int best = warp_max(m & ~kLow);   // the place in the lane only tells a lane's own values apart
+            const int best = warp_max(key[0] & ~kLow);   // the place in the lane only tells a lane's own values apart
             if (p > 0 && !exact && best != kNone)
                 again = too_close(key_value(before), key_value(best), largest, rel);
             before = best;
-            const int winner = __ffs(__ballot_sync(kFull, (m & ~kLow) == best)) - 1;
-            if (lane == winner) {
+            if (lane == __ffs(__ballot_sync(kFull, (key[0] & ~kLow) == best)) - 1) {
+                picks[p] = first + kLow - (key[0] & kLow);
 #pragma unroll
-                for (int j = 0; j < VPL; ++j)
-                    if (key[j] == m) key[j] = kNone;
+                for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
+                key[VPL - 1] = kNone;
             }
-            const int at = winner * VPL + kLow - (__shfl_sync(kFull, m, winner) & kLow);
-            if (lane == p) pick = at;
         }
+        __syncwarp();
+        int pick = lane < a.k ? picks[lane] : 0;
+        __syncwarp();
         if (again) pick = choose_exactly<T, VPL>(a, row, mx);
 
         const bool on = lane < a.k;
@@ -332,9 +389,13 @@ struct RouteBackwardArgs {
     DevStatus *status;
 };
 
+// Lane l has the vectors l, l + 32, ... of the row (without vectors: elements).
 template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) route_backward_kernel(const RouteBackwardArgs a)
 {
-    const int lane = threadIdx.x & 31, n = a.n, first = lane * VPL;
+    constexpr int kBytes = VEC ? (VPL * (int)sizeof(T) < 16 ? VPL * (int)sizeof(T) : 16) : (int)sizeof(T);
+    constexpr int kElems = kBytes / (int)sizeof(T), kVectors = VPL / kElems;
+    using V = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, std::conditional_t<kBytes == 4, unsigned, unsigned short>>>;
+    const int lane = threadIdx.x & 31, n = a.n;
     const int64_t step = (int64_t)gridDim.x * (blockDim.x / 32);
     for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; t < a.tokens; t += step) {
         const T *row = static_cast<const T *>(a.logits) + t * n;
@@ -343,8 +404,8 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
         int e = 0;
         float d = 0.f, xe = 0.f;
         if (on) {
-            e = a.experts[t * a.k + lane];
-            d = a.grad[t * a.k + lane] * a.scale;
+            e = __ldg(a.experts + t * a.k + lane);
+            d = __ldg(a.grad + t * a.k + lane) * a.scale;
             if (e < 0 || e >= n) {
                 raise_status(a.status, SPMM_DEV_BAD_COLUMN, t * a.k + lane);
                 on = false;
@@ -354,10 +415,19 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
         }
         float v[VPL], mx = 0.f, inv = 1.f;
         if (!a.sigmoid) {
-            load_lane<T, VPL, VEC>(row, first, n, -INFINITY, v);
             float m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) m = fmaxf(m, v[j]);
+            for (int c = 0; c < kVectors; ++c) {
+                const int at = (c * 32 + lane) * kElems;   // n is a multiple of kElems
+                V raw;
+                if (at < n) raw = __ldg(reinterpret_cast<const V *>(row + at));
+                const T *w = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+                for (int i = 0; i < kElems; ++i) {
+                    v[c * kElems + i] = at < n ? elem_f32<T>(w[i]) : -INFINITY;
+                    m = fmaxf(m, v[c * kElems + i]);
+                }
+            }
             mx = safe_max(warp_max(m));
             float z = 0.f;
 #pragma unroll
@@ -374,23 +444,14 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
         float along = 0.f;   // softmax: sum of d s
         if (!a.sigmoid) along = warp_sum(on ? d * s : 0.f);
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) v[j] = a.sigmoid ? 0.f : -v[j] * inv * along;
-        if constexpr (VEC) {
-            constexpr int kBytes = VPL * (int)sizeof(T) < 16 ? VPL * (int)sizeof(T) : 16, kElems = kBytes / (int)sizeof(T);
-            using V = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, std::conditional_t<kBytes == 4, unsigned, unsigned short>>>;
+        for (int c = 0; c < kVectors; ++c) {
+            const int at = (c * 32 + lane) * kElems;
+            if (at >= n) break;
+            V raw;
+            T *w = reinterpret_cast<T *>(&raw);
 #pragma unroll
-            for (int c = 0; c < VPL / kElems; ++c)
-                if (first + c * kElems < n) {
-                    V raw;
-                    T *w = reinterpret_cast<T *>(&raw);
-#pragma unroll
-                    for (int i = 0; i < kElems; ++i) w[i] = elem_of<T>(v[c * kElems + i]);
-                    reinterpret_cast<V *>(out + first)[c] = raw;
-                }
-        } else {
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (first + j < n) out[first + j] = elem_of<T>(v[j]);
+            for (int i = 0; i < kElems; ++i) w[i] = elem_of<T>(a.sigmoid ? 0.f : -v[c * kElems + i] * inv * along);
+            *reinterpret_cast<V *>(out + at) = raw;
         }
         __syncwarp();   // the chosen experts' values replace what the row got
         if (on) out[e] = elem_of<T>(a.sigmoid ? d * s * (1.f - s) : s * (d - along));

@@ -6,7 +6,10 @@
 //
 // position [tokens, k] and source [tokens * k] are each other's inverse (see
 // bucket.cu).  Dispatch and the unweighted combine are each other's gradient.
-// All are bound by memory.
+// All are bound by memory.  A warp owns a token: it reads the token's row once
+// and has the rows of all of its choices in flight.  Rows whose width is no
+// multiple of 16 bytes start anywhere; they are stored in whole vectors
+// between a few loose elements and read as pairs of vectors (vec.cuh).
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
@@ -14,34 +17,13 @@
 #include "engine.h"
 #include "layer.cuh"
 #include "layer.h"
+#include "vec.cuh"
 
 namespace spmmb {
 
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-
-// E consecutive elements as one access.
-template <typename T, int E> struct Piece {
-    static constexpr int kBytes = E * (int)sizeof(T);
-    using V = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 8, uint2, std::conditional_t<kBytes == 4, unsigned, unsigned short>>>;
-    V raw;
-    __device__ __forceinline__ void load(const T *p) { raw = __ldg(reinterpret_cast<const V *>(p)); }
-    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<V *>(p) = raw; }
-    __device__ __forceinline__ void zero() { raw = V{}; }
-    __device__ __forceinline__ void get(float *f) const
-    {
-        const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = elem_f32<T>(e[i]);
-    }
-    __device__ __forceinline__ void set(const float *f)
-    {
-        T *e = reinterpret_cast<T *>(&raw);
-#pragma unroll
-        for (int i = 0; i < E; ++i) e[i] = elem_of<T>(f[i]);
-    }
-};
 
 struct RowsArgs {
     const void *x;          // dispatch: [tokens, width]; combine: rows
@@ -56,7 +38,7 @@ struct RowsArgs {
 };
 
 // A valid position, -1 where there is none.
-__device__ __forceinline__ int64_t place_of(const RowsArgs &a, int64_t choice)
+__device__ __forceinline__ int place_of(const RowsArgs &a, int64_t choice)
 {
     const int p = __ldg(a.position + choice);
     if (p < -1 || p >= a.tokens * a.k) {
@@ -66,74 +48,128 @@ __device__ __forceinline__ int64_t place_of(const RowsArgs &a, int64_t choice)
     return p;
 }
 
+// Up to 32 of a token's choices, one per lane.
+struct Choices {
+    int place = -1;
+    float weight = 1.f;
+    int count;
+    __device__ __forceinline__ Choices(const RowsArgs &a, int64_t token, int first)
+    {
+        const int lane = threadIdx.x & 31;
+        count = min(32, a.k - first);
+        if (lane < count) {
+            place = place_of(a, token * a.k + first + lane);
+            if (a.weights) weight = __ldg(a.weights + token * a.k + first + lane);
+        }
+    }
+    __device__ __forceinline__ int place_at(int j) const { return __shfl_sync(kFull, place, j); }
+    __device__ __forceinline__ float weight_at(int j) const { return __shfl_sync(kFull, weight, j); }
+};
+
 // Zeros in the rows without a source: a warp per 32 rows.
-template <typename T, int E> __device__ __forceinline__ void zero_rows(const RowsArgs &a, int64_t warp, int64_t warps)
+template <bool ALIGNED, typename T> __device__ __forceinline__ void zero_rows(const RowsArgs &a, int64_t warp, int64_t warps)
 {
     const int lane = threadIdx.x & 31;
     const int64_t total = a.tokens * a.k;
     for (int64_t r = warp * 32; r < total; r += warps * 32) {
         unsigned empty = __ballot_sync(kFull, r + lane < total && __ldg(a.source + r + lane) < 0);
         while (empty) {
-            const int64_t row = r + __ffs(empty) - 1;
+            T *out = static_cast<T *>(a.out) + (r + __ffs(empty) - 1) * a.width;
             empty &= empty - 1;
-            Piece<T, E> z;
-            z.zero();
-            for (int64_t c = lane * E; c < a.width; c += 32 * E) z.store(static_cast<T *>(a.out) + row * a.width + c);
+            const RowSpan<ALIGNED, T> span(out, a.width);
+            for (int64_t c = lane; c < span.vectors; c += 32)
+                reinterpret_cast<uint4 *>(out + span.head)[c] = make_uint4(0, 0, 0, 0);
+            for (int64_t i = lane; i < span.loose(a.width); i += 32) out[span.loose_at(i)] = elem_of<T>(0.f);
         }
     }
 }
 
-template <typename T, int E> __global__ void __launch_bounds__(256) dispatch_kernel(const RowsArgs a)
+template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) dispatch_kernel(const RowsArgs a)
 {
+    constexpr int kElems = Pack16<T>::kElems;
     const int lane = threadIdx.x & 31;
     const int64_t warp = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
     for (int64_t t = warp; t < a.tokens; t += warps) {
         const T *x = static_cast<const T *>(a.x) + t * a.width;
-        for (int64_t c = lane * E; c < a.width; c += 32 * E) {
-            Piece<T, E> v;
-            v.load(x + c);
-            for (int j = 0; j < a.k; ++j) {
-                const int64_t p = place_of(a, t * a.k + j);
-                if (p >= 0) v.store(static_cast<T *>(a.out) + p * a.width + c);
+        for (int first = 0; first < a.k; first += 32) {
+            const Choices choice(a, t, first);
+            if constexpr (ALIGNED) {
+                for (int64_t c0 = 0; c0 < a.width; c0 += 32 * kElems) {
+                    const int64_t c = c0 + lane * kElems;
+                    Pack16<T> v;
+                    if (c < a.width) v = load16<true>(x + c);
+                    for (int j = 0; j < choice.count; ++j) {
+                        const int p = choice.place_at(j);
+                        if (p >= 0 && c < a.width)
+                            *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + p * a.width + c) = v.raw;
+                    }
+                }
+            } else {
+                for (int j = 0; j < choice.count; ++j) {
+                    const int p = choice.place_at(j);
+                    if (p < 0) continue;
+                    T *out = static_cast<T *>(a.out) + p * a.width;
+                    const RowSpan<false, T> span(out, a.width);
+                    for (int64_t c = lane; c < span.vectors; c += 32)
+                        reinterpret_cast<uint4 *>(out + span.head)[c] = load16<false>(x + span.head + c * kElems).raw;
+                    if (lane < span.loose(a.width)) out[span.loose_at(lane)] = x[span.loose_at(lane)];
+                }
             }
         }
     }
-    zero_rows<T, E>(a, warp, warps);
+    zero_rows<ALIGNED, T>(a, warp, warps);
 }
 
-template <typename T, int E> __global__ void __launch_bounds__(256) combine_kernel(const RowsArgs a)
+template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) combine_kernel(const RowsArgs a)
 {
+    constexpr int kElems = Pack16<T>::kElems;
     const int lane = threadIdx.x & 31;
-    const int64_t warp = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
-    for (int64_t t = warp; t < a.tokens; t += warps) {
-        for (int64_t c = lane * E; c < a.width; c += 32 * E) {
-            float sum[E];
+    for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; t < a.tokens; t += warps) {
+        const Choices choice(a, t, 0);
+        T *y = static_cast<T *>(a.out) + t * a.width;
+        const T *rows = static_cast<const T *>(a.x);
+        const RowSpan<ALIGNED, T> span(y, a.width);
+        for (int64_t c0 = 0; c0 < span.vectors; c0 += 32) {
+            const int64_t c = c0 + lane;
+            const bool on = c < span.vectors;
+            float sum[kElems];
 #pragma unroll
-            for (int i = 0; i < E; ++i) sum[i] = 0.f;
-#pragma unroll 4
+            for (int i = 0; i < kElems; ++i) sum[i] = 0.f;
+            auto add = [&](int p, float w) {
+                if (p < 0 || !on) return;
+                float f[kElems];
+                load16<ALIGNED>(rows + p * a.width + span.head + c * kElems).get(f);
+#pragma unroll
+                for (int i = 0; i < kElems; ++i) sum[i] = fmaf(w, f[i], sum[i]);
+            };
+#pragma unroll 8
+            for (int j = 0; j < choice.count; ++j) add(choice.place_at(j), choice.weight_at(j));
+            for (int j = 32; j < a.k; ++j)
+                add(place_of(a, t * a.k + j), a.weights ? __ldg(a.weights + t * a.k + j) : 1.f);
+            Pack16<T> v;
+            v.set(sum);
+            if (on) reinterpret_cast<uint4 *>(y + span.head)[c] = v.raw;
+        }
+        if constexpr (!ALIGNED) {
+            const bool on = lane < span.loose(a.width);
+            const int64_t c = span.loose_at(lane);
+            float sum = 0.f;
             for (int j = 0; j < a.k; ++j) {
-                const int64_t p = place_of(a, t * a.k + j);
-                if (p < 0) continue;
-                const float w = a.weights ? __ldg(a.weights + t * a.k + j) : 1.f;
-                Piece<T, E> v;
-                v.load(static_cast<const T *>(a.x) + p * a.width + c);
-                float f[E];
-                v.get(f);
-#pragma unroll
-                for (int i = 0; i < E; ++i) sum[i] = fmaf(w, f[i], sum[i]);
+                const int p = j < 32 ? choice.place_at(j) : place_of(a, t * a.k + j);
+                const float w = j < 32 ? choice.weight_at(j) : a.weights ? __ldg(a.weights + t * a.k + j) : 1.f;
+                if (p >= 0 && on) sum = fmaf(w, elem_f32<T>(rows[p * a.width + c]), sum);
             }
-            Piece<T, E> y;
-            y.set(sum);
-            y.store(static_cast<T *>(a.out) + t * a.width + c);
+            if (on) y[c] = elem_of<T>(sum);
         }
     }
 }
 
-// A warp per choice.
-template <typename T, int E> __global__ void __launch_bounds__(256) combine_backward_kernel(const RowsArgs a)
+// A warp per choice: the token's gradient is in L1 or L2 for the others.
+template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) combine_backward_kernel(const RowsArgs a)
 {
+    constexpr int kElems = Pack16<T>::kElems;
     const int lane = threadIdx.x & 31;
     const int64_t warp = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
@@ -144,25 +180,32 @@ template <typename T, int E> __global__ void __launch_bounds__(256) combine_back
             const float w = a.weights ? __ldg(a.weights + i) : 1.f;
             const T *dy = static_cast<const T *>(a.grad) + t * a.width;
             const T *row = static_cast<const T *>(a.x) + p * a.width;
-            T *out = static_cast<T *>(a.out) + p * a.width;
-            for (int64_t c = lane * E; c < a.width; c += 32 * E) {
-                Piece<T, E> v;
-                float g[E];
-                v.load(dy + c);
-                v.get(g);
+            T *out = static_cast<T *>(a.out) + p * a.width;   // where it is wanted; rows and drows are alike aligned
+            const RowSpan<ALIGNED, T> span(row, a.width);
+#pragma unroll 4
+            for (int64_t c = lane; c < span.vectors; c += 32) {
+                const int64_t at = span.head + c * kElems;
+                float g[kElems];
+                load16<ALIGNED>(dy + at).get(g);
                 if (a.dweights) {
-                    float f[E];
-                    v.load(row + c);
-                    v.get(f);
+                    float f[kElems];
+                    load16<true>(row + at).get(f);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) dot = fmaf(f[e], g[e], dot);
+                    for (int e = 0; e < kElems; ++e) dot = fmaf(f[e], g[e], dot);
                 }
                 if (a.out) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) g[e] *= w;
+                    for (int e = 0; e < kElems; ++e) g[e] *= w;
+                    Pack16<T> v;
                     v.set(g);
-                    v.store(out + c);
+                    *reinterpret_cast<uint4 *>(out + at) = v.raw;
                 }
+            }
+            if (lane < span.loose(a.width)) {
+                const int64_t at = span.loose_at(lane);
+                const float g = elem_f32<T>(dy[at]);
+                if (a.dweights) dot = fmaf(elem_f32<T>(row[at]), g, dot);
+                if (a.out) out[at] = elem_of<T>(g * w);
             }
         }
         if (a.dweights) {
@@ -171,19 +214,14 @@ template <typename T, int E> __global__ void __launch_bounds__(256) combine_back
             if (lane == 0) a.dweights[i] = dot;
         }
     }
-    if (a.out) zero_rows<T, E>(a, warp, warps);
+    if (a.out) zero_rows<ALIGNED, T>(a, warp, warps);
 }
 
-// Calls f with the type and the elements of the widest access that every row's start allows.
+// Calls f with whether every row starts on 16 bytes, and the type.
 template <typename F> cudaError_t by_rows(int dtype, int64_t width, F f)
 {
     auto run = [&](auto type) {
-        using T = decltype(type);
-        constexpr int kSize = (int)sizeof(T);
-        if (width * kSize % 16 == 0) return f(type, std::integral_constant<int, 16 / kSize>());
-        if (width * kSize % 8 == 0) return f(type, std::integral_constant<int, 8 / kSize>());
-        if (width * kSize % 4 == 0) return f(type, std::integral_constant<int, 4 / kSize>());
-        return f(type, std::integral_constant<int, 1>());
+        return width * (int)sizeof(type) % 16 == 0 ? f(std::true_type(), type) : f(std::false_type(), type);
     };
     switch (dtype) {
         case SPMM_F16: return run(__half());
@@ -206,24 +244,24 @@ RowsArgs args_of(const RoutedLaunch &r)
 
 cudaError_t launch_dispatch(const RoutedLaunch &r, cudaStream_t stream)
 {
-    return by_rows(r.dtype, r.width, [&](auto type, auto elems) {
-        dispatch_kernel<decltype(type), decltype(elems)::value><<<warp_blocks(r.tokens), 256, 0, stream>>>(args_of(r));
+    return by_rows(r.dtype, r.width, [&](auto aligned, auto type) {
+        dispatch_kernel<decltype(aligned)::value, decltype(type)><<<warp_blocks(r.tokens), 256, 0, stream>>>(args_of(r));
         return cudaGetLastError();
     });
 }
 
 cudaError_t launch_combine(const RoutedLaunch &r, cudaStream_t stream)
 {
-    return by_rows(r.dtype, r.width, [&](auto type, auto elems) {
-        combine_kernel<decltype(type), decltype(elems)::value><<<warp_blocks(r.tokens), 256, 0, stream>>>(args_of(r));
+    return by_rows(r.dtype, r.width, [&](auto aligned, auto type) {
+        combine_kernel<decltype(aligned)::value, decltype(type)><<<warp_blocks(r.tokens), 256, 0, stream>>>(args_of(r));
         return cudaGetLastError();
     });
 }
 
 cudaError_t launch_combine_backward(const RoutedLaunch &r, cudaStream_t stream)
 {
-    return by_rows(r.dtype, r.width, [&](auto type, auto elems) {
-        combine_backward_kernel<decltype(type), decltype(elems)::value>
+    return by_rows(r.dtype, r.width, [&](auto aligned, auto type) {
+        combine_backward_kernel<decltype(aligned)::value, decltype(type)>
             <<<warp_blocks(r.tokens * r.k), 256, 0, stream>>>(args_of(r));
         return cudaGetLastError();
     });
