@@ -1,18 +1,16 @@
 // Stable counting sort of keys: the places that rows of equal keys get when
 // the keys are put in order, each key's rows in their own order.
 //
-// One cluster of blocks.  A warp owns a contiguous slice of the keys; its
-// counts per bucket are kept in shared memory, and the blocks read each
-// other's totals through distributed shared memory, so that a launch counts,
-// scans and places.  Places come from counts alone (the order of the shared
-// atomics that count does not show), so a result never depends on timing.
-// Further clusters of the launch, where a caller asks for them, write zeros
-// meanwhile: the sort leaves nearly all of the GPU to them.
+// Each warp owns a contiguous slice of the keys and counts them per bucket in
+// shared memory; its keys' places are the keys of smaller buckets, those of
+// the same one in earlier slices, and their own rank among the slice's.  Places
+// come from counts alone (the order of the shared atomics that count does not
+// show), so a result never depends on timing.  One block does it all for few
+// keys; for many a first launch counts per block and a second one, whose
+// blocks add the counts of the others up, places.  Further blocks, where a
+// caller asks for them, write zeros beside the first phase: few SMs sort.
 //
-// What bounds it: the latency of its phases, and of a warp's turns (256 keys
-// each, whose loads are in flight together).
-#include <cooperative_groups.h>
-
+// What bounds it: the latency of its phases.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
@@ -25,180 +23,203 @@ namespace spmmb {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kWarps = 32, kBatch = 8;
+constexpr int kBatch = 8;             // keys of a lane in flight
+constexpr int kMostWarps = 32, kMostBlocks = 64;
 
-// Shared memory: counts [kWarps][buckets], then the block's totals [buckets]
+// Shared memory: counts [warps][buckets], then the block's totals [buckets]
 // and the scan's sums per warp.
-size_t bucket_smem(int buckets) { return (size_t)(kWarps + 1) * buckets * 4 + kWarps * 4; }
+size_t bucket_smem(int buckets, int warps) { return (size_t)(warps + 1) * buckets * 4 + warps * 4; }
 
-__global__ void __launch_bounds__(kWarps * 32) bucket_kernel(const BucketSort a)
+// COUNT: only the counts per block, [blocks][buckets] to a.counts.
+template <bool COUNT> __global__ void __launch_bounds__(kMostWarps * 32) bucket_kernel(const BucketSort a, const int blocks)
 {
     extern __shared__ int smem[];
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
-    if ((int)blockIdx.x >= blocks) {   // not the first cluster
+    const int block = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32, B = a.buckets;
+    if (block >= blocks) {
         const int64_t threads = (int64_t)(gridDim.x - blocks) * blockDim.x;
-        for (int64_t i = (int64_t)(blockIdx.x - blocks) * blockDim.x + threadIdx.x; i < a.zero_vectors; i += threads)
+        for (int64_t i = (int64_t)(block - blocks) * blockDim.x + threadIdx.x; i < a.zero_vectors; i += threads)
             __stcs(static_cast<uint4 *>(a.zero) + i, make_uint4(0, 0, 0, 0));
         return;
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, B = a.buckets;
-    int *mine = smem + warp * B, *totals = smem + kWarps * B, *sums = totals + B;
-    for (int i = threadIdx.x; i < kWarps * B; i += blockDim.x) smem[i] = 0;
+    const int bits = 32 - __clz(B - 1);   // of a bucket (none with a single one)
+    int *mine = smem + warp * B, *totals = smem + warps * B, *sums = totals + B;
+    for (int i = threadIdx.x; i < warps * B; i += blockDim.x) smem[i] = 0;
     __syncthreads();
 
     // this warp's keys: [begin, end), multiples of 32 apart
-    const int64_t slices = (int64_t)blocks * kWarps;
+    const int64_t slices = (int64_t)blocks * warps;
     const int64_t each = ((a.n + slices - 1) / slices + 31) / 32 * 32;
-    const int64_t begin = min(a.n, ((int64_t)block * kWarps + warp) * each), end = min(a.n, begin + each);
+    const int64_t begin = min(a.n, ((int64_t)block * warps + warp) * each), end = min(a.n, begin + each);
     // kBatch x 32 keys from i on: each lane's input and key, and its bucket, -1 where it is left out.
-    int input[kBatch], bucket[kBatch];
-    int64_t key[kBatch];
+    int input[kBatch], bucket[kBatch], key[kBatch];
     auto read = [&](int64_t i, bool raise) {
+        int64_t wide[kBatch];
 #pragma unroll
         for (int s = 0; s < kBatch; ++s) {
             const int64_t at = i + s * 32 + lane;
             input[s] = -1;
-            key[s] = -1;
+            wide[s] = -1;
             if (at < end) {
                 input[s] = a.order_in ? __ldg(a.order_in + at) : (int)at;
-                key[s] = a.wide ? ld_idx(static_cast<const int64_t *>(a.keys) + at) : ld_idx(static_cast<const int *>(a.keys) + at);
+                wide[s] = a.wide ? ld_idx(static_cast<const int64_t *>(a.keys) + at) : ld_idx(static_cast<const int *>(a.keys) + at);
             }
         }
 #pragma unroll
         for (int s = 0; s < kBatch; ++s) {
-            bool in = input[s] >= 0 && key[s] != a.skip;
-            if (in && (key[s] < 0 || key[s] >= a.limit)) {
+            bool in = input[s] >= 0 && wide[s] != a.skip;
+            if (in && (wide[s] < 0 || wide[s] >= a.limit)) {
                 if (raise) raise_status(a.status, SPMM_DEV_BAD_COLUMN, input[s]);
                 in = false;
             }
-            bucket[s] = in ? (int)(key[s] >> a.shift) & a.mask : -1;
+            key[s] = (int)wide[s];
+            bucket[s] = in ? key[s] >> a.shift & a.mask : -1;
         }
     };
+    const bool once = end - begin <= 32 * kBatch;   // they stay in registers
     for (int64_t i = begin; i < end; i += 32 * kBatch) {
-        read(i, true);
+        read(i, COUNT || blocks == 1);
 #pragma unroll
         for (int s = 0; s < kBatch; ++s)
             if (bucket[s] >= 0) atomicAdd(mine + bucket[s], 1);
     }
     __syncthreads();
-    // per bucket: this warp's keys before each warp's, the block's total
+    // per bucket: this block's keys before each warp's, their number
     for (int b = threadIdx.x; b < B; b += blockDim.x) {
         int sum = 0;
 #pragma unroll 8
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < warps; ++w) {
             const int c = smem[w * B + b];
             smem[w * B + b] = sum;
             sum += c;
         }
         totals[b] = sum;
+        if (COUNT) a.counts[block * B + b] = sum;
     }
-    cluster.sync();
-    // per bucket: the keys of smaller buckets, and of this one in earlier blocks
-    const int b = threadIdx.x;
-    int before = 0, all = 0;
-    if (b < B)
-#pragma unroll 8
-        for (int c = 0; c < blocks; ++c) {
-            const int v = cluster.map_shared_rank(totals, c)[b];
-            before += c < block ? v : 0;
-            all += v;
-        }
-    int scan = all;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(kFull, scan, o);
-        if (lane >= o) scan += u;
-    }
-    if (lane == 31) sums[warp] = scan;
-    cluster.sync();   // the other blocks have read this one's totals
-    if (warp == 0) {
-        int v = sums[lane];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(kFull, v, o);
-            if (lane >= o) v += u;
-        }
-        sums[lane] = v;
-    }
-    __syncthreads();
-    const int start = scan - all + (warp ? sums[warp - 1] : 0), kept = sums[kWarps - 1];
-    if (b < B) {
-        totals[b] = start + before;
-        if (a.ptr && block == 0) a.ptr[b] = start;
-    }
-    if (a.ptr && block == 0 && threadIdx.x == 0) a.ptr[B] = kept;
-    __syncthreads();
-    for (int i = lane; i < B; i += 32) mine[i] += totals[i];
-    __syncwarp();
-
-    for (int64_t i = begin; i < end; i += 32 * kBatch) {
-        read(i, false);
-#pragma unroll
-        for (int s = 0; s < kBatch; ++s) {
-            const unsigned peers = __match_any_sync(kFull, bucket[s]);
-            const int rank = __popc(peers & ((1u << lane) - 1));
-            int place = -1;
-            if (bucket[s] >= 0) place = mine[bucket[s]] + rank;
-            __syncwarp();
-            if (bucket[s] >= 0 && rank == 0) mine[bucket[s]] += __popc(peers);
-            __syncwarp();
-            if (place >= 0) {
-                a.order[place] = input[s];
-                if (a.key_out) a.key_out[place] = (int)key[s];
+    if constexpr (COUNT) {
+        return;
+    } else {
+        __syncthreads();
+        // per bucket: the keys of smaller buckets, and of this one in earlier blocks
+        int carry = 0;   // keys of the buckets before the current blockDim.x
+        for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+            const int b = b0 + threadIdx.x;
+            int before = 0, all = 0;
+            if (b < B) {
+                if (blocks == 1) {
+                    all = totals[b];
+                } else {
+#pragma unroll 16
+                    for (int c = 0; c < blocks; ++c) {
+                        const int v = __ldg(a.counts + c * B + b);
+                        before += c < block ? v : 0;
+                        all += v;
+                    }
+                }
             }
-            if (a.position && input[s] >= 0) a.position[input[s]] = place;
+            int scan = all;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(kFull, scan, o);
+                if (lane >= o) scan += u;
+            }
+            if (lane == 31) sums[warp] = scan;
+            __syncthreads();
+            if (warp == 0) {
+                int v = lane < warps ? sums[lane] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(kFull, v, o);
+                    if (lane >= o) v += u;
+                }
+                if (lane < warps) sums[lane] = v;
+            }
+            __syncthreads();
+            const int start = carry + scan - all + (warp ? sums[warp - 1] : 0);
+            if (b < B) {
+                totals[b] = start + before;
+                if (a.ptr && block == 0) a.ptr[b] = start;
+            }
+            carry += sums[warps - 1];
+            __syncthreads();
         }
-    }
-    for (int64_t i = kept + (int64_t)block * blockDim.x + threadIdx.x; i < a.n; i += (int64_t)blocks * blockDim.x) {
-        a.order[i] = -1;
-        if (a.key_out) a.key_out[i] = -1;
+        const int kept = carry;
+        if (block == 0 && threadIdx.x == 0) {
+            if (a.ptr) a.ptr[B] = kept;
+            if (a.count) *a.count = 0;
+        }
+        for (int i = lane; i < B; i += 32) mine[i] += totals[i];
+        __syncwarp();
+
+        for (int64_t i = begin; i < end; i += 32 * kBatch) {
+            if (!once) read(i, false);
+#pragma unroll
+            for (int s = 0; s < kBatch; ++s) {
+                if (i + s * 32 >= end) break;
+                // the lanes with this one's bucket, bit by bit (match_any takes a turn per distinct value)
+                unsigned peers = __ballot_sync(kFull, bucket[s] >= 0);
+                for (int bit = 0; bit < bits; ++bit) {
+                    const bool set = bucket[s] >> bit & 1;
+                    const unsigned ones = __ballot_sync(kFull, set);
+                    peers &= set ? ones : ~ones;
+                }
+                const int rank = __popc(peers & ((1u << lane) - 1));
+                int place = -1;
+                if (bucket[s] >= 0) place = mine[bucket[s]] + rank;
+                __syncwarp();
+                if (bucket[s] >= 0 && rank == 0) mine[bucket[s]] += __popc(peers);
+                __syncwarp();
+                if (place >= 0) {
+                    a.order[place] = input[s];
+                    if (a.key_out) a.key_out[place] = key[s];
+                }
+                if (a.position && input[s] >= 0) a.position[input[s]] = place;
+            }
+        }
+        for (int64_t i = kept + (int64_t)block * blockDim.x + threadIdx.x; i < a.n; i += (int64_t)blocks * blockDim.x) {
+            a.order[i] = -1;
+            if (a.key_out) a.key_out[i] = -1;
+        }
     }
 }
 
+// Blocks that sort: one for as many keys as its warps hold in two turns.
+int blocks_for(int64_t n) { return n <= 16384 ? 1 : (int)std::min<int64_t>(kMostBlocks, (n + 8191) / 8192); }
+
 }  // namespace
+
+size_t bucket_workspace(int64_t n, int buckets)
+{
+    const int blocks = blocks_for(n);
+    return blocks == 1 ? 0 : (size_t)blocks * buckets * sizeof(int);
+}
 
 cudaError_t launch_bucket_sort(const BucketSort &a, cudaStream_t stream)
 {
-    // Blocks of the cluster: one for few keys, 16 for many where the device can hold such a cluster.
-    static PerDevice<int> most;   // outlasts the call
-    int *known = most.here(), widest = known ? *known : 0;
-    cudaLaunchConfig_t config{};
-    config.blockDim = kWarps * 32;
-    config.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    if (!widest) {
-        cudaError_t e = cudaFuncSetAttribute(bucket_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)bucket_smem(kMostBuckets));
+    static PerDevice<bool> ready;   // the attributes outlast the call
+    bool *done = ready.here();
+    if (!done || !*done) {
+        for (auto kernel : {bucket_kernel<false>, bucket_kernel<true>}) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       (int)bucket_smem(kMostBuckets, kMostWarps));
+            if (e != cudaSuccess) return e;
+        }
+        if (done) *done = true;
+    }
+    const int blocks = blocks_for(a.n);
+    const int warps = a.n <= 2048 && a.buckets <= 256 ? 8 : kMostWarps;   // few keys: few warps, whose barriers are short
+    const size_t smem = bucket_smem(a.buckets, warps);
+    const int64_t useful = (a.zero_vectors + warps * 32 - 1) / (warps * 32);
+    const unsigned extra = (unsigned)std::min<int64_t>(useful, 2 * (int64_t)device_sm_count() * kMostWarps / warps);
+    if (blocks > 1) {
+        bucket_kernel<true><<<blocks + extra, warps * 32, smem, stream>>>(a, blocks);
+        const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
-        int clusters = 0;
-        config.gridDim = attr.val.clusterDim.x = 16;
-        config.dynamicSmemBytes = bucket_smem(kMostBuckets);
-        if (cudaFuncSetAttribute(bucket_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&clusters, bucket_kernel, &config) != cudaSuccess)
-            clusters = 0;
-        (void)cudaGetLastError();
-        widest = clusters > 0 ? 16 : 8;
-        if (known) *known = widest;
+        bucket_kernel<false><<<blocks, warps * 32, smem, stream>>>(a, blocks);
+    } else {
+        bucket_kernel<false><<<1 + extra, warps * 32, smem, stream>>>(a, 1);
     }
-    const unsigned blocks = a.n <= 4096 ? 1 : a.n <= 32768 ? 8 : (unsigned)widest;
-    unsigned extra = 0;
-    if (a.zero_vectors > 0) {
-        const int64_t useful = (a.zero_vectors + kWarps * 32 - 1) / (kWarps * 32);
-        extra = (unsigned)std::min<int64_t>(useful, 2 * (int64_t)device_sm_count());
-        extra = (extra + blocks - 1) / blocks * blocks;   // whole clusters
-    }
-    config.gridDim = blocks + extra;
-    attr.val.clusterDim.x = blocks;
-    config.dynamicSmemBytes = bucket_smem(a.buckets);
-    return cudaLaunchKernelEx(&config, bucket_kernel, a);
+    return cudaGetLastError();
 }
 
 }  // namespace spmmb

@@ -351,8 +351,14 @@ int spmm_route_experts_backward_launch(const void *logits, const int32_t *expert
     return e == cudaSuccess ? SPMM_OK : cuda_error(e, op);
 }
 
+size_t spmm_expert_plan_workspace_bytes(int64_t n, int64_t num_experts)
+{
+    if (n <= 0 || num_experts <= 0 || num_experts > spmmb::kMostBuckets) return 0;
+    return spmmb::bucket_workspace(n, (int)num_experts);
+}
+
 int spmm_expert_plan_launch(const void *experts, int32_t *group_ptr, int32_t *position, int32_t *source, int64_t n,
-                            int64_t num_experts, int itype, void *stream)
+                            int64_t num_experts, int itype, void *workspace, size_t workspace_bytes, void *stream)
 {
     const char *op = "expert_plan";
     if (itype != SPMM_I32 && itype != SPMM_I64)
@@ -363,12 +369,14 @@ int spmm_expert_plan_launch(const void *experts, int32_t *group_ptr, int32_t *po
     if (n > INT32_MAX) return capi_error(SPMM_ERR_ARG, "%s: size too large", op);
     if (!group_ptr || (n > 0 && (!experts || !position || !source)))
         return capi_error(SPMM_ERR_ARG, "%s: null array", op);
-    int rc;
+    int rc = check_workspace(workspace, workspace_bytes, spmm_expert_plan_workspace_bytes(n, num_experts), op);
+    if (rc) return rc;
     spmmb::BucketSort b{};
     b.status = status_or_error(op, &rc);
     if (rc) return rc;
     b.keys = experts; b.wide = itype == SPMM_I64; b.n = n; b.buckets = (int)num_experts; b.mask = -1;
     b.limit = num_experts; b.skip = -1; b.ptr = group_ptr; b.position = position; b.order = source;
+    b.counts = static_cast<int *>(workspace);
     const cudaError_t e = spmmb::launch_bucket_sort(b, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SPMM_OK : cuda_error(e, op);
 }

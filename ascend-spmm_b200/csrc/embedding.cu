@@ -7,10 +7,10 @@
 // bucket.cu) and adds each id's rows in their order, so it has no float
 // atomics and a result does not depend on timing.  The rows without an id are
 // zeroed beside the sort, which takes a few SMs.  The sorted ids are cut into
-// parts of kPart; an id's run that lies in one part is added and stored by
-// it, a run over several leaves one fp32 sum per part, which the part that
-// the run starts in adds up afterwards (a few ids of a power law hold
-// thousands of rows).  Both passes are bound by memory.
+// parts of kPart; an id's run of at most that many is added and stored by the
+// part that it starts in, a longer one leaves an fp32 sum in each of its parts,
+// which are added up afterwards (a few ids of a power law hold thousands of
+// rows).  Both passes are bound by memory.
 //
 // An id outside the table gives a row of zeros, no gradient, and the device status.
 #include <algorithm>
@@ -37,6 +37,7 @@ struct EmbedArgs {
     const int *order;       // backward: input indexes by id, -1 past the last
     const int *sorted;      // backward: their ids
     float *partial;         // backward: [2 * parts][width]
+    int *runs;              // backward: their number, then the parts in which runs over several start (in any order)
     int64_t n, rows, width;
     float scale;
     DevStatus *status;
@@ -93,44 +94,53 @@ template <bool ALIGNED, typename T, int E> __device__ __forceinline__ void store
     }
 }
 
-// The sorted ids `at` (input indexes) of a part, E columns from c on.
-// key: the id before the part, the part's, the id behind it.
+// The sorted ids of a part, as a block keeps them in shared memory: those
+// around it too, since a run of at most kPart rows over a border is added whole
+// by the part that it starts in.
+struct Part {
+    int key[3 * kPart + 2];   // key[kPart + 1 + i]: the id at place i of the part, -1 outside the ids
+    int at[2 * kPart];        // input indexes of the part and of kPart places behind it
+    int begin, end;           // the places that this part adds
+    bool more;                // the last run is longer and goes on: its sum is a partial one
+    bool before;              // the first run comes from before: its sum is a partial one
+};
+
+// E columns of the part's sums, from column c on.
 template <bool ALIGNED, typename T, int E>
-__device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const int *at, const int *key, int64_t c)
+__device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const Part &s, int64_t c)
 {
     const T *dy = static_cast<const T *>(a.in) + c;
+    const int *key = s.key + kPart + 1;
     float sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
-    bool first = true;   // the run is the part's first
+    bool before = s.before;
     constexpr int kAhead = 8;
-#pragma unroll
-    for (int i0 = 0; i0 < kPart; i0 += kAhead) {
-        if (at[i0] < 0) break;
+    for (int i0 = s.begin; i0 < s.end; i0 += kAhead) {
         float f[kAhead][E];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)   // past the last one: the row is read again and not added
-            load_columns<ALIGNED, T, E>(dy + (int64_t)max(at[i0 + j], 0) * a.width, f[j]);
+        for (int j = 0; j < kAhead; ++j)   // past the last one: a row is read again and not added
+            load_columns<ALIGNED, T, E>(dy + (int64_t)s.at[min(i0 + j, s.end - 1)] * a.width, f[j]);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int i = i0 + j;
-            if (at[i] < 0) break;
+            if (i >= s.end) break;
 #pragma unroll
             for (int e = 0; e < E; ++e) sum[e] += f[j][e];
-            const int k = key[i + 1];
-            if (i + 1 < kPart && key[i + 2] == k) continue;
-            // the run ends here, or with the part
-            const bool from_before = first && key[0] == k, goes_on = i + 1 == kPart && key[kPart + 1] == k;
-            if (from_before || goes_on) {
-                float *p = a.partial + (part * 2 + (from_before ? 0 : 1)) * a.width + c;
+            const int k = key[i];
+            if (i + 1 < s.end && key[i + 1] == k) continue;
+            const bool more = i + 1 == s.end && s.more;
+            if (before || more) {
+                float *p = a.partial + (part * 2 + (before ? 0 : 1)) * a.width + c;
 #pragma unroll
                 for (int e = 0; e < E; ++e) p[e] = sum[e];
+                if (!before && c == 0) a.runs[1 + atomicAdd(a.runs, 1)] = (int)part;
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) sum[e] *= a.scale;
                 store_columns<ALIGNED, T, E>(static_cast<T *>(a.out) + (int64_t)k * a.width + c, sum);
             }
-            first = false;
+            before = false;
 #pragma unroll
             for (int e = 0; e < E; ++e) sum[e] = 0.f;
         }
@@ -141,54 +151,71 @@ __device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const
 template <bool ALIGNED, typename T> __global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbedArgs a)
 {
     constexpr int kElems = Pack16<T>::kElems;
-    __shared__ int at[kPart], key[kPart + 2];
+    __shared__ Part s;
     const int64_t part = blockIdx.x, first = part * kPart;
-    for (int i = threadIdx.x; i < kPart + 2; i += blockDim.x) {
-        const int64_t p = first + i - 1;
-        const bool in = p >= 0 && p < a.n;
-        key[i] = in ? a.sorted[p] : -1;
-        if (i >= 1 && i <= kPart) at[i - 1] = in ? a.order[p] : -1;
+    for (int i = threadIdx.x; i < 3 * kPart + 2; i += blockDim.x) {
+        const int64_t p = first + i - (kPart + 1);
+        s.key[i] = p >= 0 && p < a.n ? a.sorted[p] : -1;
+    }
+    for (int i = threadIdx.x; i < 2 * kPart; i += blockDim.x) s.at[i] = first + i < a.n ? a.order[first + i] : -1;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, *key = s.key + kPart + 1;
+        static_assert(kPart == 32, "a lane per place");
+        // places of the first run where it comes from before, and places behind the part where the last one goes on
+        const unsigned valid = __ballot_sync(0xffffffffu, key[lane] >= 0);
+        const unsigned as_before = __ballot_sync(0xffffffffu, key[lane] >= 0 && key[lane] == key[-1]);
+        const unsigned as_last = __ballot_sync(0xffffffffu, key[lane] >= 0 && key[lane] == key[kPart - 1]);
+        const unsigned beyond = __ballot_sync(0xffffffffu, key[kPart + lane] >= 0 && key[kPart + lane] == key[kPart - 1]);
+        if (lane == 0) {
+            const int rest = as_before == ~0u ? kPart : __ffs(~as_before) - 1;
+            const int start = as_last == ~0u ? 0 : 32 - __clz(~as_last), over = beyond == ~0u ? kPart : __ffs(~beyond) - 1;
+            // a run is long if it has the place kPart before its last one, or behind its first one
+            const bool long_before = rest == kPart || (rest > 0 && key[rest - 1 - kPart] == key[rest - 1]);
+            const bool long_last = over > 0 && (rest == kPart || key[start + kPart] == key[kPart - 1]);
+            s.before = long_before;
+            s.begin = long_before ? 0 : rest;
+            s.more = long_last;
+            s.end = __popc(valid) + (long_last ? 0 : over);
+        }
     }
     __syncthreads();
+    if (s.begin >= s.end) return;
     const int64_t vectors = a.width / kElems, t = (int64_t)blockIdx.y * blockDim.x + threadIdx.x;
     if (t < vectors) {
-        sum_part<ALIGNED, T, kElems>(a, part, at, key, t * kElems);
+        sum_part<ALIGNED, T, kElems>(a, part, s, t * kElems);
     } else if (!ALIGNED && t - vectors < a.width - vectors * kElems) {   // the columns behind the last whole vector
-        sum_part<false, T, 1>(a, part, at, key, vectors * kElems + t - vectors);
+        sum_part<false, T, 1>(a, part, s, vectors * kElems + t - vectors);
     }
 }
 
-// Adds the sums of a run that starts in part blockIdx.x and goes on behind it:
-// 32 columns a block, kJoin warps with every kJoin-th part each, in a fixed order.
+// Adds the sums of each run over several parts: 32 columns at a time, kJoin
+// warps with every kJoin-th part each, in a fixed order.
 template <typename T> __global__ void __launch_bounds__(32 * kJoin) embedding_join_kernel(const EmbedArgs a)
 {
     __shared__ float sums[kJoin][32];
-    const int64_t part = blockIdx.x, last = (part + 1) * kPart - 1;
-    if (last + 1 >= a.n) return;
-    const int k = a.sorted[last];
-    if (k < 0 || a.sorted[last + 1] != k) return;
-    const int64_t first = part * kPart;
-    if (first > 0 && a.sorted[first] == k && a.sorted[first - 1] == k) return;   // it starts further up
-    // the parts that it goes on in: those whose first id is k
-    int64_t end = part + 1;
-    for (int more = blockDim.x; more == (int)blockDim.x; end += more) {
-        const int64_t p = (end + threadIdx.x) * kPart;
-        more = __syncthreads_count(p < a.n && a.sorted[p] == k);
-    }
-    const int group = threadIdx.x / 32;
-    for (int64_t c0 = (int64_t)blockIdx.y * 32; c0 < a.width; c0 += (int64_t)gridDim.y * 32) {
-        const int64_t c = c0 + threadIdx.x % 32;
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    const int64_t chunks = (a.width + 31) / 32, items = a.runs[0] * chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t part = a.runs[1 + item / chunks], c = item % chunks * 32 + lane;
+        const int k = a.sorted[(part + 1) * kPart - 1];
+        // the parts that it goes on in: those whose first id is k
+        int64_t end = part + 1;
+        for (int more = blockDim.x; more == (int)blockDim.x; end += more) {
+            const int64_t p = (end + threadIdx.x) * kPart;
+            more = __syncthreads_count(p < a.n && a.sorted[p] == k);
+        }
         float sum = 0.f;
         if (c < a.width) {
             if (group == 0) sum = a.partial[(part * 2 + 1) * a.width + c];
 #pragma unroll 8
             for (int64_t p = part + 1 + group; p < end; p += kJoin) sum += a.partial[p * 2 * a.width + c];
         }
-        sums[group][threadIdx.x % 32] = sum;
+        sums[group][lane] = sum;
         __syncthreads();
         if (group == 0 && c < a.width) {
 #pragma unroll
-            for (int g = 1; g < kJoin; ++g) sum += sums[g][threadIdx.x];
+            for (int g = 1; g < kJoin; ++g) sum += sums[g][lane];
             static_cast<T *>(a.out)[(int64_t)k * a.width + c] = elem_of<T>(sum * a.scale);
         }
         __syncthreads();
@@ -208,7 +235,25 @@ template <typename F> cudaError_t by_rows(int dtype, int64_t width, F f)
     }
 }
 
-size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
+// What the backward pass keeps in its workspace.
+struct Places {
+    size_t array[4], runs, counts, partial, bytes;   // array: the order and the ids of two sorting passes
+};
+Places places_of(int64_t n, int64_t width)
+{
+    const int64_t parts = (n + kPart - 1) / kPart;
+    Places p{};
+    auto take = [&](size_t bytes) {
+        const size_t at = p.bytes;
+        p.bytes += (bytes + 255) & ~size_t(255);
+        return at;
+    };
+    for (size_t &at : p.array) at = take((size_t)n * 4);
+    p.runs = take((size_t)(parts + 1) * 4);
+    p.counts = take(bucket_workspace(n, kMostBuckets));
+    p.partial = take((size_t)parts * 2 * width * sizeof(float));
+    return p;
+}
 
 }  // namespace
 
@@ -226,8 +271,7 @@ cudaError_t launch_embedding(const EmbeddingLaunch &l, cudaStream_t stream)
 
 size_t embedding_backward_workspace(int64_t n, int64_t width)
 {
-    const int64_t parts = (n + kPart - 1) / kPart;
-    return 4 * align256((size_t)n * 4) + (size_t)parts * 2 * width * sizeof(float);
+    return places_of(n, width).bytes;
 }
 
 cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, void *workspace, cudaStream_t stream)
@@ -238,8 +282,11 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
     if (bytes % 16)   // the sort writes whole vectors of zeros
         if ((e = cudaMemsetAsync(static_cast<char *>(l.out) + bytes / 16 * 16, 0, bytes % 16, stream)) != cudaSuccess) return e;
     char *ws = static_cast<char *>(workspace);
+    const Places places = places_of(l.n, l.width);
+    auto ints = [&](size_t at) { return reinterpret_cast<int *>(ws + at); };
     int *array[4];   // order and ids of two passes
-    for (int i = 0; i < 4; ++i) array[i] = reinterpret_cast<int *>(ws + i * align256((size_t)l.n * 4));
+    for (int i = 0; i < 4; ++i) array[i] = ints(places.array[i]);
+    const unsigned parts = (unsigned)((l.n + kPart - 1) / kPart);
     int bits = 1;
     while (bits < 31 && (int64_t(1) << bits) < l.rows) ++bits;
     const int passes = (bits + kBucketBits - 1) / kBucketBits, each = (bits + passes - 1) / passes;
@@ -257,6 +304,8 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
         s.skip = skip;
         s.order = array[p % 2];
         s.key_out = array[2 + p % 2];
+        s.counts = ints(places.counts);
+        s.count = ints(places.runs);
         s.zero = static_cast<uint4 *>(l.out) + vectors * p / passes;   // a share of the zeros beside each pass
         s.zero_vectors = vectors * (p + 1) / passes - vectors * p / passes;
         s.status = l.status;
@@ -264,9 +313,9 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
     }
     EmbedArgs a{};
     a.in = l.in; a.out = l.out; a.order = array[(passes - 1) % 2]; a.sorted = array[2 + (passes - 1) % 2];
-    a.partial = reinterpret_cast<float *>(ws + 4 * align256((size_t)l.n * 4));
+    a.runs = ints(places.runs);
+    a.partial = reinterpret_cast<float *>(ws + places.partial);
     a.n = l.n; a.rows = l.rows; a.width = l.width; a.scale = l.scale; a.status = l.status;
-    const unsigned parts = (unsigned)((l.n + kPart - 1) / kPart);
     return by_rows(l.dtype, l.width, [&](auto aligned, auto type) {
         using T = decltype(type);
         constexpr bool kAligned = decltype(aligned)::value;
@@ -274,7 +323,8 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
         const int64_t threads = l.width / kElems + l.width % kElems;
         embedding_sum_kernel<kAligned, T><<<dim3(parts, (unsigned)((threads + 127) / 128)), 128, 0, stream>>>(a);
         if (parts > 1)
-            embedding_join_kernel<T><<<dim3(parts, (unsigned)std::min<int64_t>((l.width + 31) / 32, 64)), 32 * kJoin, 0, stream>>>(a);
+            embedding_join_kernel<T><<<(unsigned)std::min<int64_t>(parts * ((l.width + 31) / 32), 4 * (int64_t)device_sm_count()),
+                                       32 * kJoin, 0, stream>>>(a);
         return cudaGetLastError();
     });
 }

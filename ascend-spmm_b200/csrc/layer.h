@@ -111,11 +111,14 @@ struct BucketSort {
     int *position;          // [n] place of each input, -1 where it is left out; may be null
     int *order;             // [n] input of each place, -1 past the last
     int *key_out;           // [n] their keys, -1 past the last; may be null (then limit may pass 32 bits)
+    int *counts;            // workspace: bucket_workspace bytes
+    int *count;             // set to 0; may be null
     void *zero;             // 16-byte vectors to zero meanwhile
     int64_t zero_vectors;
     DevStatus *status;
 };
 constexpr int kBucketBits = 10, kMostBuckets = 1 << kBucketBits;
+size_t bucket_workspace(int64_t n, int buckets);
 cudaError_t launch_bucket_sort(const BucketSort &a, cudaStream_t stream);
 
 // ---- rows to their experts and back (routed.cu) -------------------------------

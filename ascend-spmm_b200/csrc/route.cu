@@ -10,7 +10,9 @@
 //           d = renormalized ? (g - sum(g s) / S) / S : g        (chosen ones)
 //           dx = s (d - sum(d s)) (softmax),  d s (1 - s) (sigmoid)
 //
-// A warp owns a row, lane l the experts l * VPL .. + VPL - 1 in registers.
+// A team of LANES lanes owns a row (a warp where it has more than 128
+// experts), lane l the experts l * VPL .. + VPL - 1 in registers, each sorted
+// by a network; a pick is then the largest of the lanes' first ones.
 //
 // The choice is what 64-bit scores give, from 32-bit ones: where two values
 // that the choice tells apart (a pick and the next one, the last group kept
@@ -20,6 +22,9 @@
 //
 // NaN counts as the lowest value in every choice; a row whose logits are all
 // -infinity gets zero weights.
+//
+// What bounds it: instructions (about 17 for each expert's score and its
+// place in the order, 20 for each pick), not the 4 bytes of a logit.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
@@ -38,10 +43,27 @@ constexpr int kNanKey = INT32_MIN + 64;      // below every number's key, above 
 constexpr long long kNone64 = INT64_MIN;
 
 __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(kFull, v); }
-template <typename F> __device__ __forceinline__ F warp_sum(F v)
+// Over the teams of LANES lanes, each by itself.
+template <int LANES = 32, typename F> __device__ __forceinline__ F warp_sum(F v)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+template <int LANES> __device__ __forceinline__ int team_max(int v)
+{
+    if constexpr (LANES == 32) {
+        return warp_max(v);
+    } else {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
+        return v;
+    }
+}
+template <int LANES> __device__ __forceinline__ float team_max(float v)
+{
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
 }
 
@@ -51,12 +73,20 @@ __device__ __forceinline__ int order_key(float f)
     const int b = __float_as_int(f + 0.f);
     return isnan(f) ? kNanKey : b ^ ((b >> 31) & 0x7fffffff);
 }
+// The same without a look at NaN and -0: positive NaNs above infinity, others below -infinity.
+__device__ __forceinline__ int raw_key(float f)
+{
+    const int b = __float_as_int(f);
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+constexpr int kInfKey = 0x7f800000, kMinusInfKey = (int)0x807fffff;
 __device__ __forceinline__ float key_value(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 __device__ __forceinline__ long long order_key(double d)
 {
     const long long b = __double_as_longlong(d + 0.0);
     return isnan(d) ? kNone64 + 1 : b ^ ((b >> 63) & INT64_MAX);
 }
+__device__ __forceinline__ double key_value(long long k) { return __longlong_as_double(k ^ ((k >> 63) & INT64_MAX)); }
 
 // Largest of the lanes' values; NaN only where all are.
 __device__ __forceinline__ float warp_max(float v)
@@ -83,15 +113,12 @@ template <int N> __device__ __forceinline__ void sort_descending(int (&v)[N])
                     }
 }
 
-// The largest and the lowest lane that has it.
+// The largest of 64-bit keys and the lowest lane that has it.
 __device__ __forceinline__ long long warp_best(long long v, int *lane)
 {
-    long long best = v;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const long long u = __shfl_xor_sync(kFull, best, o);
-        best = u > best ? u : best;
-    }
+    const int hi = warp_max((int)(v >> 32));
+    const unsigned lo = __reduce_max_sync(kFull, (int)(v >> 32) == hi ? (unsigned)v : 0u);
+    const long long best = (long long)hi << 32 | lo;
     *lane = __ffs(__ballot_sync(kFull, v == best)) - 1;
     return best;
 }
@@ -137,78 +164,92 @@ __device__ __forceinline__ void load_lane(const T *row, int at, int n, float fil
 __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f : m; }
 
 // ---- the row in 64 bits ------------------------------------------------------
-// Returns lane p's pick (p < k).
+// The whole warp; returns lane p's pick (p < k).  Few rows need it, but a
+// kernel ends with its slowest warp: as short a chain as it can be.
 template <typename T, int VPL> __device__ __noinline__ int choose_exactly(const RouteArgs &a, const T *row, float mx)
 {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, first = lane * VPL;
     const bool by_logit = !a.bias && (a.groups == a.top_groups || a.group_best == 1);
-    double c[VPL];
-    double z = 0;
-    for (int j = 0; j < VPL; ++j) {
-        const int i = lane * VPL + j;
-        const double x = i < a.n ? (double)elem_f32<T>(row[i]) : -INFINITY;
-        if (by_logit) c[j] = x;
-        else if (a.sigmoid) c[j] = 1 / (1 + exp(-x));
-        else z += c[j] = exp(x - (double)mx);
-    }
-    if (!by_logit && !a.sigmoid) {
+    double c[VPL], z = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) c[j] = first + j < a.n ? (double)elem_f32<T>(row[first + j]) : -INFINITY;
+    if (!by_logit && a.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) c[j] = 1 / (1 + exp(-c[j]));
+    } else if (!by_logit) {
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) z += c[j] = exp(c[j] - (double)mx);
         z = warp_sum(z);
+#pragma unroll
         for (int j = 0; j < VPL; ++j) c[j] = z == 0 ? 0 : c[j] / z;
     }
-    if (a.bias)
-        for (int j = 0; j < VPL; ++j)
-            if (lane * VPL + j < a.n) c[j] += (double)a.bias[lane * VPL + j];
     long long key[VPL];
-    for (int j = 0; j < VPL; ++j) key[j] = lane * VPL + j < a.n ? order_key(c[j]) : kNone64;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+        if (a.bias && first + j < a.n) c[j] += (double)__ldg(a.bias + first + j);
+        key[j] = first + j < a.n ? order_key(c[j]) : kNone64;
+    }
     if (a.top_groups < a.groups) {
-        const int per = a.n / a.groups;
-        long long mine = kNone64;
-        for (int g = 0; g < a.groups; ++g) {
-            double sum = 0;
-            long long above = INT64_MAX;   // the group's picks so far are those above (above, first)
-            int first = -1;
-            for (int b = 0; b < a.group_best; ++b) {
-                long long best = kNone64;
-                int at = -1;
-                for (int j = 0; j < VPL; ++j) {
-                    const int i = lane * VPL + j;
-                    if (i < g * per || i >= (g + 1) * per || key[j] > above || (key[j] == above && i <= first)) continue;
-                    if (key[j] > best) {
-                        best = key[j];
-                        at = j;
-                    }
-                }
-                int winner;
-                above = warp_best(best, &winner);
-                const double v = __shfl_sync(kFull, at >= 0 ? c[at] : 0.0, winner);
-                first = __shfl_sync(kFull, lane * VPL + at, winner);
-                sum += v;
+        const int per = a.n / a.groups, lanes = per / VPL;
+        auto sum_of = [&](long long top, long long next) {
+            return a.group_best == 2 ? order_key(key_value(top) + key_value(next)) : top;
+        };
+        auto join = [](long long &b1, long long &b2, int o) {
+            const long long o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+            b2 = max(min(b1, o1), max(b2, o2));
+            b1 = max(b1, o1);
+        };
+        long long mine = kNone64;   // lane g: the score of group g
+        if (per % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+            long long b1 = kNone64, b2 = kNone64;
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) {
+                b2 = max(b2, min(b1, key[j]));
+                b1 = max(b1, key[j]);
             }
-            if (lane == g) mine = order_key(sum);
+            for (int o = 1; o < lanes; o <<= 1) join(b1, b2, o);
+            mine = __shfl_sync(kFull, sum_of(b1, b2), min(lane, a.groups - 1) * lanes);
+        } else {
+            for (int g = 0; g < a.groups; ++g) {
+                long long b1 = kNone64, b2 = kNone64;
+#pragma unroll
+                for (int j = 0; j < VPL; ++j) {
+                    const long long v = first + j >= g * per && first + j < (g + 1) * per ? key[j] : kNone64;
+                    b2 = max(b2, min(b1, v));
+                    b1 = max(b1, v);
+                }
+                for (int o = 1; o < 32; o <<= 1) join(b1, b2, o);
+                if (lane == g) mine = sum_of(b1, b2);
+            }
         }
         int rank = 0;
+#pragma unroll 4
         for (int h = 0; h < a.groups; ++h) {
             const long long other = __shfl_sync(kFull, mine, h);
             rank += other > mine || (other == mine && h < lane);
         }
         const unsigned kept = __ballot_sync(kFull, lane < a.groups && rank < a.top_groups);
+#pragma unroll
         for (int j = 0; j < VPL; ++j)
-            if (lane * VPL + j < a.n && !(kept >> ((lane * VPL + j) / per) & 1u)) key[j] = kNone64;
+            if (first + j < a.n && !(kept >> ((first + j) / per) & 1u)) key[j] = kNone64;
     }
     int pick = 0;
     for (int p = 0; p < a.k; ++p) {
-        long long best = kNone64;
+        long long best = key[0];
         int at = 0;
-        for (int j = 0; j < VPL; ++j)
+#pragma unroll
+        for (int j = 1; j < VPL; ++j)
             if (key[j] > best) {
                 best = key[j];
                 at = j;
             }
         int winner;
         warp_best(best, &winner);
-        if (lane == winner) key[at] = kNone64;
-        at = __shfl_sync(kFull, at, winner);
-        if (lane == p) pick = winner * VPL + at;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+            if (lane == winner && j == at) key[j] = kNone64;
+        at = __shfl_sync(kFull, first + at, winner);
+        if (lane == p) pick = at;
     }
     return pick;
 }
@@ -222,70 +263,71 @@ __device__ __forceinline__ bool too_close(float hi, float lo, float largest, flo
     return !(hi - lo > 0x1p-19f * largest + rel * fmaxf(fabsf(hi), fabsf(lo)));   // true for infinities, too
 }
 
-// Blocks of an SM: rows are handled in a long chain of dependent steps, so the
-// more warps take turns the better.
-constexpr int route_blocks(int vpl) { return vpl <= 2 ? 8 : vpl == 4 ? 6 : vpl == 8 ? 5 : vpl == 16 ? 4 : 2; }
+__device__ __forceinline__ float reciprocal(float x)   // within 2^-23 of itself
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
-template <typename T, int VPL, bool VEC>
+// Blocks of an SM: a row is a long chain of dependent steps, so the more warps take turns the better.
+constexpr int route_blocks(int vpl) { return vpl == 8 ? 5 : vpl == 16 ? 4 : 2; }
+
+template <typename T, int LANES, int VPL, bool VEC>
 __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const RouteArgs a)
 {
-    __shared__ int chosen[8][kMostChosen + 1];
     constexpr int kLow = VPL - 1;   // bits of a key that hold the (reversed) place in the lane
-    const int lane = threadIdx.x & 31, n = a.n;
+    constexpr int kTeams = 32 / LANES;
+    constexpr unsigned kTeam = LANES == 32 ? kFull : (1u << LANES) - 1;
+    __shared__ int s_pick[8][kTeams][kMostChosen + 1], s_key[8][kTeams][kMostChosen + 1], s_score[8][kTeams][kMostGroups];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % LANES, team = threadIdx.x % 32 / LANES, n = a.n;
     const int first = lane * VPL;
     const bool grouped = a.top_groups < a.groups;
     const bool by_logit = !a.bias && (!grouped || a.group_best == 1);
     // groups that are whole lanes, a power of two of them
     const int per = n / a.groups, lanes = per / VPL;
-    const bool by_lanes = per % VPL == 0 && (lanes & (lanes - 1)) == 0 && lanes <= 32;
-    int *const picks = chosen[threadIdx.x / 32];
-    const int64_t step = (int64_t)gridDim.x * (blockDim.x / 32);
-    for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; t < a.tokens; t += step) {
+    const bool by_lanes = per % VPL == 0 && (lanes & (lanes - 1)) == 0;
+    // by logits: 16-bit ones are compared exactly, 32-bit ones where their keys differ above the low bits
+    const float rel = by_logit ? VPL * 0x1p-23f : 0x1p-21f + VPL * 0x1p-22f;
+    const bool exact = by_logit && sizeof(T) == 2;
+    float bias[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) bias[j] = a.bias && first + j < n ? __ldg(a.bias + first + j) : 0.f;
+    int *const picks = s_pick[warp][team], *const keys = s_key[warp][team], *const scores = s_score[warp][team];
+    const int64_t step = (int64_t)gridDim.x * 8 * kTeams;
+    for (int64_t t0 = ((int64_t)blockIdx.x * 8 + warp) * kTeams; t0 < a.tokens; t0 += step) {
+        const int64_t t = min(t0 + team, a.tokens - 1);   // a team past the last row does it again and stores nothing
         const T *row = static_cast<const T *>(a.logits) + t * n;
-        float x[VPL];
-        load_lane<T, VPL, VEC>(row, first, n, -INFINITY, x);
-        float mx = 0.f, inv = 1.f;
         float c[VPL];   // the values to choose by
+        load_lane<T, VPL, VEC>(row, first, n, -INFINITY, c);
+        float mx = 0.f, inv = 1.f;
         if (!a.sigmoid) {
             float m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) m = fmaxf(m, x[j]);
-            mx = safe_max(warp_max(m));
-            float z = 0.f;
+            for (int j = 0; j < VPL; ++j) m = fmaxf(m, c[j]);
+            mx = safe_max(team_max<LANES>(m));
+            float e[VPL], z = 0.f;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) z += c[j] = __expf(x[j] - mx);
-            z = warp_sum(z);
+            for (int j = 0; j < VPL; ++j) z += e[j] = __expf(c[j] - mx);
+            z = warp_sum<LANES>(z);
             inv = z == 0.f ? 0.f : 1.f / z;
+            if (!by_logit) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) c[j] *= inv;
+                for (int j = 0; j < VPL; ++j) c[j] = e[j] * inv;
+            }
         } else if (!by_logit) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) c[j] = __fdividef(1.f, 1.f + __expf(-x[j]));
-        }
-        if (by_logit) {
-#pragma unroll
-            for (int j = 0; j < VPL; ++j) c[j] = x[j];
-        } else if (a.bias) {
-#pragma unroll
-            for (int j = 0; j < VPL; ++j)
-                if (first + j < n) c[j] += __ldg(a.bias + first + j);
+            for (int j = 0; j < VPL; ++j) c[j] = reciprocal(1.f + __expf(-c[j]));
         }
         int key[VPL];
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)
-            key[j] = first + j < n ? (order_key(c[j]) & ~kLow) | (kLow - j) : kNone;
+        for (int j = 0; j < VPL; ++j)   // the sum with 0 makes -0 one
+            key[j] = first + j < n ? (raw_key(c[j] + bias[j]) & ~kLow) | (kLow - j) : kNone;
 
-        // by logits: 16-bit ones are compared exactly, 32-bit ones where their keys differ above the low bits
         const float largest = by_logit ? 0.f : a.sigmoid ? 1.f : inv;
-        const float rel = by_logit ? VPL * 0x1p-23f : 0x1p-21f + VPL * 0x1p-22f;
-        const bool exact = by_logit && (sizeof(T) == 2 || VPL == 1);
         bool again = false;
         if (grouped) {
-            // lane g: the score of group g
-            int mine = kNone;
-            auto sum_of = [&](int top, int next) {   // of two keys without their low bits
-                return order_key((top == kNanKey ? NAN : key_value(top)) + (next == kNanKey ? NAN : key_value(next)));
-            };
+            auto sum_of = [&](int top, int next) { return raw_key(key_value(top) + key_value(next)); };
             if (by_lanes) {
                 int b1 = kNone, b2 = kNone;
 #pragma unroll
@@ -300,39 +342,52 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                     b2 = max(min(b1, o1), max(b2, o2));
                     b1 = max(b1, o1);
                 }
-                const int score = a.group_best == 2 ? sum_of(b1, b2) : b1;
-                mine = __shfl_sync(kFull, score, min(lane, a.groups - 1) * lanes);
-                if (lane >= a.groups) mine = kNone;
+                if (lane % lanes == 0 && lane / lanes < a.groups) scores[lane / lanes] = a.group_best == 2 ? sum_of(b1, b2) : b1;
             } else {
                 for (int g = 0; g < a.groups; ++g) {
                     int b1 = kNone, b2 = kNone;
 #pragma unroll
                     for (int j = 0; j < VPL; ++j) {
-                        const int i = first + j, v = i >= g * per && i < (g + 1) * per ? key[j] : kNone;
+                        const int i = first + j, v = i >= g * per && i < (g + 1) * per ? key[j] & ~kLow : kNone;
                         b2 = max(b2, min(b1, v));
                         b1 = max(b1, v);
                     }
-                    const int top = warp_max(b1);
-                    int score = top & ~kLow;
-                    if (a.group_best == 2) {
-                        const int winner = __ffs(__ballot_sync(kFull, b1 == top)) - 1;
-                        score = sum_of(score, warp_max(lane == winner ? b2 : b1) & ~kLow);
+#pragma unroll
+                    for (int o = 1; o < LANES; o <<= 1) {
+                        const int o1 = __shfl_xor_sync(kFull, b1, o), o2 = __shfl_xor_sync(kFull, b2, o);
+                        b2 = max(min(b1, o1), max(b2, o2));
+                        b1 = max(b1, o1);
                     }
-                    if (lane == g) mine = score;
+                    if (lane == 0) scores[g] = a.group_best == 2 ? sum_of(b1, b2) : b1;
                 }
             }
-            int rank = 0;
-            for (int h = 0; h < a.groups; ++h) {
-                const int other = __shfl_sync(kFull, mine, h);
-                rank += other > mine || (other == mine && h < lane);
+            __syncwarp();
+            unsigned kept = 0;
+            int last = INT32_MAX, out = INT32_MIN;   // the lowest score kept, the highest left out
+            for (int g = lane; g < a.groups; g += LANES) {
+                const int mine = scores[g];
+                int rank = 0;
+                for (int h = 0; h < a.groups; ++h) {
+                    const int other = scores[h];
+                    rank += other > mine || (other == mine && h < g);
+                }
+                if (rank < a.top_groups) {
+                    kept |= 1u << g;
+                    last = min(last, mine);
+                } else {
+                    out = max(out, mine);
+                }
+                again |= mine > kInfKey || mine < (kMinusInfKey & ~kLow);   // NaN
             }
-            const bool stays = lane < a.groups && rank < a.top_groups;
-            const unsigned kept = __ballot_sync(kFull, stays);
-            const int last = __reduce_min_sync(kFull, stays ? mine : INT32_MAX);
-            const int out = warp_max(stays ? kNone : mine);
-            if (!exact) again = too_close(key_value(last), key_value(out), largest, 2 * rel);
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) {
+                kept |= __shfl_xor_sync(kFull, kept, o);
+                last = min(last, __shfl_xor_sync(kFull, last, o));
+                out = max(out, __shfl_xor_sync(kFull, out, o));
+            }
+            if (!exact) again |= too_close(key_value(last), key_value(out), largest, 2 * rel);
             if (by_lanes) {
-                if (first < n && !(kept >> (lane / lanes) & 1u)) {
+                if (!(kept >> (lane / lanes) & 1u)) {
 #pragma unroll
                     for (int j = 0; j < VPL; ++j) key[j] = kNone;
                 }
@@ -342,38 +397,52 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                     if (first + j < n && !(kept >> ((first + j) / per) & 1u)) key[j] = kNone;
             }
         }
-        // each lane's keys in descending order: a pick is the largest of the lanes' first ones
         sort_descending(key);
-        int before = 0;
-        for (int p = 0; p <= a.k && !again; ++p) {
-            const int best = warp_max(key[0] & ~kLow);   // the place in the lane only tells a lane's own values apart
-            if (p > 0 && !exact && best != kNone)
-                again = too_close(key_value(before), key_value(best), largest, rel);
-            before = best;
-            if (lane == __ffs(__ballot_sync(kFull, (key[0] & ~kLow) == best)) - 1) {
+        for (int p = 0; p <= a.k; ++p) {
+            const int best = team_max<LANES>(key[0] & ~kLow);   // the place in the lane only tells a lane's own values apart
+            const unsigned has = __ballot_sync(kFull, (key[0] & ~kLow) == best) >> (team * LANES) & kTeam;
+            const bool winner = lane == __ffs(has) - 1;
+            if (winner) {
                 picks[p] = first + kLow - (key[0] & kLow);
-#pragma unroll
-                for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
-                key[VPL - 1] = kNone;
+                keys[p] = best;
             }
+#pragma unroll
+            for (int j = 0; j + 1 < VPL; ++j) key[j] = winner ? key[j + 1] : key[j];
+            key[VPL - 1] = winner ? kNone : key[VPL - 1];
         }
         __syncwarp();
-        int pick = lane < a.k ? picks[lane] : 0;
+        // the row is decided in 64 bits where a pick and the next one are too close, and where a NaN was met
+        for (int p = lane; p < a.k; p += LANES) {
+            const int mine = keys[p], next = keys[p + 1];
+            again |= mine > kInfKey || mine < (kMinusInfKey & ~kLow);
+            if (!exact && next != kNone) again |= too_close(key_value(mine), key_value(next), largest, rel);
+        }
+        unsigned unsure = __ballot_sync(kFull, again);
+        while (unsure) {
+            const int who = (__ffs(unsure) - 1) / LANES;
+            unsure &= ~(kTeam << (who * LANES));
+            const T *its_row = static_cast<const T *>(a.logits) + min(t0 + who, a.tokens - 1) * n;
+            const float its_mx = __shfl_sync(kFull, mx, who * LANES);
+            const int pick = choose_exactly<T, (LANES * VPL + 31) / 32>(a, its_row, its_mx);
+            if ((int)threadIdx.x % 32 < a.k) s_pick[warp][who][threadIdx.x % 32] = pick;
+        }
         __syncwarp();
-        if (again) pick = choose_exactly<T, VPL>(a, row, mx);
-
-        const bool on = lane < a.k;
-        float s = 0.f;
-        if (on) {
-            const float v = elem_f32<T>(row[pick]);
-            s = a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - mx) * inv;
+        auto score = [&](int p) {
+            const float v = elem_f32<T>(row[picks[p]]);
+            return a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - mx) * inv;
+        };
+        float total = 1.f;
+        if (a.renormalize) {
+            float sum = 0.f;
+            for (int p = lane; p < a.k; p += LANES) sum += score(p);
+            total = warp_sum<LANES>(sum) + 1e-20f;
         }
-        float w = s;
-        if (a.renormalize) w = s / (warp_sum(s) + 1e-20f);
-        if (on) {
-            a.weights[t * a.k + lane] = w * a.scale;
-            a.experts[t * a.k + lane] = pick;
-        }
+        if (t0 + team < a.tokens)
+            for (int p = lane; p < a.k; p += LANES) {
+                a.weights[t * a.k + p] = (a.renormalize ? score(p) / total : score(p)) * a.scale;
+                a.experts[t * a.k + p] = picks[p];
+            }
+        __syncwarp();   // the picks have been read
     }
 }
 
@@ -458,20 +527,27 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
     }
 }
 
-// Calls f with the values per lane (a power of two) and whether rows are read in vectors.
-template <typename T, typename F> cudaError_t by_width(int n, F f)
+// Calls f with a row's lanes and the values per lane (powers of two), and whether rows are read in vectors.
+template <typename T, bool TEAMS, typename F> cudaError_t by_width(int n, F f)
 {
-    auto run = [&](auto vpl) {
-        constexpr int kVpl = decltype(vpl)::value;
-        constexpr int kBytes = std::min(16, kVpl * (int)sizeof(T));
-        return n * (int)sizeof(T) % kBytes == 0 ? f(vpl, std::true_type()) : f(vpl, std::false_type());
+    auto run = [&](auto lanes, auto vpl) {
+        constexpr int kBytes = std::min(16, decltype(vpl)::value * (int)sizeof(T));
+        return n * (int)sizeof(T) % kBytes == 0 ? f(lanes, vpl, std::true_type()) : f(lanes, vpl, std::false_type());
     };
-    if (n <= 32) return run(std::integral_constant<int, 1>());
-    if (n <= 64) return run(std::integral_constant<int, 2>());
-    if (n <= 128) return run(std::integral_constant<int, 4>());
-    if (n <= 256) return run(std::integral_constant<int, 8>());
-    if (n <= 512) return run(std::integral_constant<int, 16>());
-    return run(std::integral_constant<int, 32>());
+#define SPMM_ROUTE(LANES, VPL) run(std::integral_constant<int, LANES>(), std::integral_constant<int, VPL>())
+    if constexpr (TEAMS) {
+        if (n <= 32) return SPMM_ROUTE(4, 8);
+        if (n <= 64) return SPMM_ROUTE(8, 8);
+        if (n <= 128) return SPMM_ROUTE(16, 8);
+    } else {
+        if (n <= 32) return SPMM_ROUTE(32, 1);
+        if (n <= 64) return SPMM_ROUTE(32, 2);
+        if (n <= 128) return SPMM_ROUTE(32, 4);
+    }
+    if (n <= 256) return SPMM_ROUTE(32, 8);
+    if (n <= 512) return SPMM_ROUTE(32, 16);
+    return SPMM_ROUTE(32, 32);
+#undef SPMM_ROUTE
 }
 
 template <typename F> cudaError_t by_type(int dtype, F f)
@@ -496,8 +572,11 @@ cudaError_t launch_route(const RouteLaunch &r, cudaStream_t stream)
                 r.sigmoid, r.renormalize, r.scale};
     return by_type(r.dtype, [&](auto type) {
         using T = decltype(type);
-        return by_width<T>(r.n, [&](auto vpl, auto vec) {
-            route_kernel<T, decltype(vpl)::value, decltype(vec)::value><<<row_blocks(r.tokens), 256, 0, stream>>>(a);
+        return by_width<T, true>(r.n, [&](auto lanes, auto vpl, auto vec) {
+            constexpr int kLanes = decltype(lanes)::value, kVpl = decltype(vpl)::value;
+            const int64_t warps = (r.tokens + 32 / kLanes - 1) / (32 / kLanes);
+            const unsigned blocks = (unsigned)std::min<int64_t>((warps + 7) / 8, route_blocks(kVpl) * (int64_t)device_sm_count());
+            route_kernel<T, kLanes, kVpl, decltype(vec)::value><<<blocks, 256, 0, stream>>>(a);
             return cudaGetLastError();
         });
     });
@@ -510,7 +589,7 @@ cudaError_t launch_route_backward(const RouteLaunch &r, const float *grad, void 
                         status};
     return by_type(r.dtype, [&](auto type) {
         using T = decltype(type);
-        return by_width<T>(r.n, [&](auto vpl, auto vec) {
+        return by_width<T, false>(r.n, [&](auto, auto vpl, auto vec) {
             route_backward_kernel<T, decltype(vpl)::value, decltype(vec)::value>
                 <<<row_blocks(r.tokens), 256, 0, stream>>>(a);
             return cudaGetLastError();

@@ -84,6 +84,8 @@ template <bool ALIGNED, typename T> __device__ __forceinline__ void zero_rows(co
     }
 }
 
+constexpr int kAtOnce = 4;   // vectors of a row that a lane has in flight
+
 template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) dispatch_kernel(const RowsArgs a)
 {
     constexpr int kElems = Pack16<T>::kElems;
@@ -94,27 +96,41 @@ template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) dispa
         const T *x = static_cast<const T *>(a.x) + t * a.width;
         for (int first = 0; first < a.k; first += 32) {
             const Choices choice(a, t, first);
-            if constexpr (ALIGNED) {
-                for (int64_t c0 = 0; c0 < a.width; c0 += 32 * kElems) {
-                    const int64_t c = c0 + lane * kElems;
-                    Pack16<T> v;
-                    if (c < a.width) v = load16<true>(x + c);
-                    for (int j = 0; j < choice.count; ++j) {
-                        const int p = choice.place_at(j);
-                        if (p >= 0 && c < a.width)
-                            *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + p * a.width + c) = v.raw;
-                    }
+            // the token's row, kAtOnce vectors a lane at a time; whole vectors of a result start at another place in each
+            // row where rows are not aligned, so that there a row is read again for each choice (from L1)
+            for (int64_t c0 = 0; ALIGNED && c0 < a.width; c0 += 32 * kElems * kAtOnce) {
+                Pack16<T> v[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int64_t c = c0 + (32 * i + lane) * kElems;
+                    if (c < a.width) v[i].raw = __ldcs(reinterpret_cast<const uint4 *>(x + c));
                 }
-            } else {
                 for (int j = 0; j < choice.count; ++j) {
                     const int p = choice.place_at(j);
                     if (p < 0) continue;
                     T *out = static_cast<T *>(a.out) + p * a.width;
-                    const RowSpan<false, T> span(out, a.width);
-                    for (int64_t c = lane; c < span.vectors; c += 32)
-                        reinterpret_cast<uint4 *>(out + span.head)[c] = load16<false>(x + span.head + c * kElems).raw;
-                    if (lane < span.loose(a.width)) out[span.loose_at(lane)] = x[span.loose_at(lane)];
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        const int64_t c = c0 + (32 * i + lane) * kElems;
+                        if (c < a.width) __stcs(reinterpret_cast<uint4 *>(out + c), v[i].raw);
+                    }
                 }
+            }
+            for (int j = 0; !ALIGNED && j < choice.count; ++j) {
+                const int p = choice.place_at(j);
+                if (p < 0) continue;
+                T *out = static_cast<T *>(a.out) + p * a.width;
+                const RowSpan<false, T> span(out, a.width);
+                for (int64_t c0 = lane; c0 < span.vectors; c0 += 32 * kAtOnce) {
+                    Pack16<T> v[kAtOnce];
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)   // past the last one: it is read again
+                        v[i] = load16<false>(x + span.head + min(c0 + 32 * i, span.vectors - 1) * kElems);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)
+                        if (c0 + 32 * i < span.vectors) __stcs(reinterpret_cast<uint4 *>(out + span.head) + c0 + 32 * i, v[i].raw);
+                }
+                if (lane < span.loose(a.width)) out[span.loose_at(lane)] = x[span.loose_at(lane)];
             }
         }
     }
@@ -127,39 +143,56 @@ template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) combi
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
     for (int64_t t = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; t < a.tokens; t += warps) {
-        const Choices choice(a, t, 0);
         T *y = static_cast<T *>(a.out) + t * a.width;
         const T *rows = static_cast<const T *>(a.x);
         const RowSpan<ALIGNED, T> span(y, a.width);
-        for (int64_t c0 = 0; c0 < span.vectors; c0 += 32) {
-            const int64_t c = c0 + lane;
-            const bool on = c < span.vectors;
-            float sum[kElems];
+        // kAtOnce vectors a lane of each row: a warp reads 2 KB of it in one go
+        for (int64_t c0 = lane; c0 - lane < span.vectors; c0 += 32 * kAtOnce) {
+            float sum[kAtOnce][kElems];
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) sum[i] = 0.f;
-            auto add = [&](int p, float w) {
-                if (p < 0 || !on) return;
-                float f[kElems];
-                load16<ALIGNED>(rows + p * a.width + span.head + c * kElems).get(f);
+            for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) sum[i] = fmaf(w, f[i], sum[i]);
-            };
-#pragma unroll 8
-            for (int j = 0; j < choice.count; ++j) add(choice.place_at(j), choice.weight_at(j));
-            for (int j = 32; j < a.k; ++j)
-                add(place_of(a, t * a.k + j), a.weights ? __ldg(a.weights + t * a.k + j) : 1.f);
-            Pack16<T> v;
-            v.set(sum);
-            if (on) reinterpret_cast<uint4 *>(y + span.head)[c] = v.raw;
+                for (int e = 0; e < kElems; ++e) sum[i][e] = 0.f;
+            for (int first = 0; first < a.k; first += 32) {
+                const Choices choice(a, t, first);
+#pragma unroll 2
+                for (int j = 0; j < choice.count; ++j) {
+                    const int p = choice.place_at(j);
+                    const float w = choice.weight_at(j);
+                    if (p < 0) continue;
+                    const T *row = rows + p * a.width + span.head;
+                    Pack16<T> v[kAtOnce];
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)   // past the last one: read again and not stored
+                        v[i] = load16<ALIGNED>(row + min(c0 + 32 * i, span.vectors - 1) * kElems);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        float f[kElems];
+                        v[i].get(f);
+#pragma unroll
+                        for (int e = 0; e < kElems; ++e) sum[i][e] = fmaf(w, f[e], sum[i][e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (c0 + 32 * i < span.vectors) {
+                    Pack16<T> v;
+                    v.set(sum[i]);
+                    __stcs(reinterpret_cast<uint4 *>(y + span.head) + c0 + 32 * i, v.raw);
+                }
         }
         if constexpr (!ALIGNED) {
             const bool on = lane < span.loose(a.width);
-            const int64_t c = span.loose_at(lane);
+            const int64_t c = on ? span.loose_at(lane) : 0;
             float sum = 0.f;
-            for (int j = 0; j < a.k; ++j) {
-                const int p = j < 32 ? choice.place_at(j) : place_of(a, t * a.k + j);
-                const float w = j < 32 ? choice.weight_at(j) : a.weights ? __ldg(a.weights + t * a.k + j) : 1.f;
-                if (p >= 0 && on) sum = fmaf(w, elem_f32<T>(rows[p * a.width + c]), sum);
+            for (int first = 0; first < a.k; first += 32) {
+                const Choices choice(a, t, first);
+                for (int j = 0; j < choice.count; ++j) {
+                    const int p = choice.place_at(j);
+                    const float w = choice.weight_at(j);
+                    if (p >= 0 && on) sum = fmaf(w, elem_f32<T>(rows[p * a.width + c]), sum);
+                }
             }
             if (on) y[c] = elem_of<T>(sum);
         }
@@ -182,23 +215,29 @@ template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) combi
             const T *row = static_cast<const T *>(a.x) + p * a.width;
             T *out = static_cast<T *>(a.out) + p * a.width;   // where it is wanted; rows and drows are alike aligned
             const RowSpan<ALIGNED, T> span(row, a.width);
-#pragma unroll 4
-            for (int64_t c = lane; c < span.vectors; c += 32) {
-                const int64_t at = span.head + c * kElems;
-                float g[kElems];
-                load16<ALIGNED>(dy + at).get(g);
-                if (a.dweights) {
-                    float f[kElems];
-                    load16<true>(row + at).get(f);
+            for (int64_t c0 = lane; c0 < span.vectors; c0 += 32 * kAtOnce) {
+                Pack16<T> gv[kAtOnce], fv[kAtOnce];
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const int64_t c = c0 + 32 * j;
+                    gv[j].raw = fv[j].raw = make_uint4(0, 0, 0, 0);
+                    if (c < span.vectors) {
+                        gv[j] = load16<ALIGNED>(dy + span.head + c * kElems);
+                        if (a.dweights) fv[j].raw = __ldcs(reinterpret_cast<const uint4 *>(row + span.head) + c);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const int64_t c = c0 + 32 * j;
+                    float g[kElems], f[kElems];
+                    gv[j].get(g);
+                    fv[j].get(f);
 #pragma unroll
                     for (int e = 0; e < kElems; ++e) dot = fmaf(f[e], g[e], dot);
-                }
-                if (a.out) {
 #pragma unroll
                     for (int e = 0; e < kElems; ++e) g[e] *= w;
-                    Pack16<T> v;
-                    v.set(g);
-                    *reinterpret_cast<uint4 *>(out + at) = v.raw;
+                    gv[j].set(g);
+                    if (a.out && c < span.vectors) __stcs(reinterpret_cast<uint4 *>(out + span.head) + c, gv[j].raw);
                 }
             }
             if (lane < span.loose(a.width)) {

@@ -986,6 +986,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
         auto [w, e] = route_experts_forward(logits, bias, o);
         ctx->save_for_backward({logits, e});
         ctx->mark_non_differentiable({e});
+        ctx->set_materialize_grads(false);   // no zeros for e
         ctx->saved_data["scoring"] = (int64_t)o.scoring;
         ctx->saved_data["renormalize"] = o.renormalize;
         ctx->saved_data["scale"] = o.scale;
@@ -1034,9 +1035,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(const at::Tensor &exp
     const auto opt = e.options().dtype(at::kInt);
     at::Tensor ptr = at::empty({num_experts + 1}, opt), position = at::empty(e.sizes(), opt),
                source = at::empty({e.numel()}, opt);
+    const size_t wbytes = spmm_expert_plan_workspace_bytes(e.numel(), num_experts);
+    at::Tensor ws = wbytes ? workspace(wbytes, e) : at::Tensor();
     check_rc(spmm_expert_plan_launch(e.data_ptr(), ptr.data_ptr<int>(), position.data_ptr<int>(), source.data_ptr<int>(),
                                      e.numel(), num_experts, e.scalar_type() == at::kLong ? SPMM_I64 : SPMM_I32,
-                                     stream_of(e)));
+                                     wbytes ? ws.data_ptr() : nullptr, wbytes, stream_of(e)));
     return {ptr, position, source};
 }
 

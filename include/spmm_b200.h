@@ -415,8 +415,9 @@ int spmm_route_experts_backward_launch(const void *logits, const int32_t *expert
  *   source    [n]                choice of each row, -1 behind the last row
  * An expert outside [-1, num_experts) counts as -1 and raises
  * SPMM_DEV_BAD_COLUMN.  At most 1024 experts. */
+size_t spmm_expert_plan_workspace_bytes(int64_t n, int64_t num_experts);
 int spmm_expert_plan_launch(const void *experts, int32_t *group_ptr, int32_t *position, int32_t *source, int64_t n,
-                            int64_t num_experts, int itype, void *stream);
+                            int64_t num_experts, int itype, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Rows to their experts and back, k choices per row of x [tokens, width]:
  *   dispatch  rows[r] = x[source[r] / k], rows without a source are zero

@@ -21,7 +21,9 @@ def lib():
     L.spmm_last_error.restype = ctypes.c_char_p
     L.spmm_route_experts_launch.argtypes = [V] * 4 + [I64] * 3 + [INT] + [I64] * 2 + [INT] * 2 + [F64, INT, V]
     L.spmm_route_experts_backward_launch.argtypes = [V] * 4 + [I64] * 3 + [INT] * 2 + [F64, INT, V]
-    L.spmm_expert_plan_launch.argtypes = [V] * 4 + [I64] * 2 + [INT, V]
+    L.spmm_expert_plan_workspace_bytes.restype = SZ
+    L.spmm_expert_plan_workspace_bytes.argtypes = [I64] * 2
+    L.spmm_expert_plan_launch.argtypes = [V] * 4 + [I64] * 2 + [INT, V, SZ, V]
     L.spmm_dispatch_rows_launch.argtypes = [V] * 4 + [I64] * 3 + [INT, V]
     L.spmm_combine_rows_launch.argtypes = [V] * 4 + [I64] * 3 + [INT, V]
     L.spmm_combine_rows_backward_launch.argtypes = [V] * 7 + [I64] * 3 + [INT, V]
@@ -79,7 +81,7 @@ def test_route_experts(lib):
 
 def test_expert_plan(lib):
     f = lambda **k: lib.spmm_expert_plan_launch(  # noqa: E731
-        k.get("e", PTR), k.get("ptr", PTR), PTR, k.get("s", PTR), k.get("n", 8), k.get("num", 4), k.get("itype", 0), None)
+        k.get("e", PTR), k.get("ptr", PTR), PTR, k.get("s", PTR), k.get("n", 8), k.get("num", 4), k.get("itype", 0), k.get("ws"), k.get("bytes", 0), None)
     refused(lib, f(itype=2), "int32 or int64")
     refused(lib, f(num=0), "number of experts must be in [1, 1024]")
     refused(lib, f(num=1025), "number of experts must be in [1, 1024]")
@@ -88,6 +90,10 @@ def test_expert_plan(lib):
     refused(lib, f(e=None), "null array")
     refused(lib, f(s=None), "null array")
     refused(lib, f(ptr=None, n=0), "null array")
+    assert lib.spmm_expert_plan_workspace_bytes(0, 4) == 0
+    need = lib.spmm_expert_plan_workspace_bytes(1 << 20, 64)
+    assert need > 0 and f(n=1 << 20, num=64, ws=PTR, bytes=need - 1) == 6 and f(n=1 << 20, num=64, bytes=need) == 6
+    refused(lib, f(n=1 << 20, num=64, ws=PTR + 8, bytes=need), "16-byte aligned")
 
 
 def test_rows(lib):
