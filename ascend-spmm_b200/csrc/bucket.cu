@@ -25,7 +25,7 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kBatch = 8;             // keys of a lane in flight
-constexpr int kMostWarps = 32, kMostBlocks = 64;
+constexpr int kMostWarps = 32, kMostBlocks = 128;
 
 // Shared memory: counts [warps][buckets], then the block's totals [buckets]
 // and the scan's sums per warp.
@@ -60,8 +60,12 @@ template <bool COUNT> __global__ void __launch_bounds__(kMostWarps * 32) bucket_
             const int64_t at = i + s * 32 + lane;
             input[s] = -1;
             wide[s] = -1;
-            if (at < end) {
-                input[s] = a.order_in ? __ldg(a.order_in + at) : (int)at;
+            if (at < end && a.pairs_in) {
+                const int2 v = __ldg(a.pairs_in + at);
+                input[s] = v.x;
+                wide[s] = v.y;
+            } else if (at < end) {
+                input[s] = (int)at;
                 wide[s] = a.wide ? ld_idx(static_cast<const int64_t *>(a.keys) + at) : ld_idx(static_cast<const int *>(a.keys) + at);
             }
         }
@@ -146,7 +150,7 @@ template <bool COUNT> __global__ void __launch_bounds__(kMostWarps * 32) bucket_
         const int kept = carry;
         if (block == 0 && threadIdx.x == 0) {
             if (a.ptr) a.ptr[B] = kept;
-            if (a.count) *a.count = 0;
+            if (a.clear) a.clear[0] = a.clear[1] = 0;
         }
         for (int i = lane; i < B; i += 32) mine[i] += totals[i];
         __syncwarp();
@@ -170,21 +174,21 @@ template <bool COUNT> __global__ void __launch_bounds__(kMostWarps * 32) bucket_
                 if (bucket[s] >= 0 && rank == 0) mine[bucket[s]] += __popc(peers);
                 __syncwarp();
                 if (place >= 0) {
-                    a.order[place] = input[s];
-                    if (a.key_out) a.key_out[place] = key[s];
+                    if (a.pairs) a.pairs[place] = make_int2(input[s], key[s]);
+                    else a.order[place] = input[s];
                 }
                 if (a.position && input[s] >= 0) a.position[input[s]] = place;
             }
         }
         for (int64_t i = kept + (int64_t)block * blockDim.x + threadIdx.x; i < a.n; i += (int64_t)blocks * blockDim.x) {
-            a.order[i] = -1;
-            if (a.key_out) a.key_out[i] = -1;
+            if (a.pairs) a.pairs[i] = make_int2(-1, -1);
+            else a.order[i] = -1;
         }
     }
 }
 
-// Blocks that sort: one for as many keys as its warps hold in two turns.
-int blocks_for(int64_t n) { return n <= 16384 ? 1 : (int)std::min<int64_t>(kMostBlocks, (n + 8191) / 8192); }
+// Blocks that sort: one for few keys, else one for every 4096.
+int blocks_for(int64_t n) { return n <= 6144 ? 1 : (int)std::min<int64_t>(kMostBlocks, (n + 4095) / 4096); }
 
 }  // namespace
 

@@ -27,17 +27,19 @@ namespace spmmb {
 namespace {
 
 constexpr int kPart = 32;      // sorted ids of a part
-constexpr int kJoin = 8;       // groups of threads that add a run's parts side by side
+constexpr int kFew = 8;        // a run over at most so many parts is added up by a warp, a longer one by a block
+constexpr int kJoin = 16;      // of so many warps
 
 struct EmbedArgs {
     const void *ids;        // forward
     bool wide;
     const void *in;         // the table; backward: dy
     void *out;              // y; backward: dtable
-    const int *order;       // backward: input indexes by id, -1 past the last
-    const int *sorted;      // backward: their ids
+    const int2 *sorted;     // backward: input indexes and their ids, by id; -1 past the last
     float *partial;         // backward: [2 * parts][width]
-    int *runs;              // backward: their number, then the parts in which runs over several start (in any order)
+    // backward: the numbers of long runs of few parts and of many, then the parts that they start in (in any order), the
+    // former from the front and the latter from the back
+    int *runs;
     int64_t n, rows, width;
     float scale;
     DevStatus *status;
@@ -134,7 +136,12 @@ __device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const
                 float *p = a.partial + (part * 2 + (before ? 0 : 1)) * a.width + c;
 #pragma unroll
                 for (int e = 0; e < E; ++e) p[e] = sum[e];
-                if (!before && c == 0) a.runs[1 + atomicAdd(a.runs, 1)] = (int)part;
+                if (!before && c == 0) {
+                    const int64_t far = (part + kFew) * kPart, parts = (a.n + kPart - 1) / kPart;
+                    const bool many = far < a.n && a.sorted[far].y == k;
+                    const int i = atomicAdd(a.runs + many, 1);
+                    a.runs[many ? parts + 1 - i : 2 + i] = (int)part;
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e) sum[e] *= a.scale;
@@ -155,9 +162,10 @@ template <bool ALIGNED, typename T> __global__ void __launch_bounds__(128) embed
     const int64_t part = blockIdx.x, first = part * kPart;
     for (int i = threadIdx.x; i < 3 * kPart + 2; i += blockDim.x) {
         const int64_t p = first + i - (kPart + 1);
-        s.key[i] = p >= 0 && p < a.n ? a.sorted[p] : -1;
+        const int2 v = p >= 0 && p < a.n ? __ldg(a.sorted + p) : make_int2(-1, -1);
+        s.key[i] = v.y;
+        if (i > kPart && i <= 3 * kPart) s.at[i - (kPart + 1)] = v.x;
     }
-    for (int i = threadIdx.x; i < 2 * kPart; i += blockDim.x) s.at[i] = first + i < a.n ? a.order[first + i] : -1;
     __syncthreads();
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x, *key = s.key + kPart + 1;
@@ -189,34 +197,57 @@ template <bool ALIGNED, typename T> __global__ void __launch_bounds__(128) embed
     }
 }
 
-// Adds the sums of each run over several parts: 32 columns at a time, kJoin
-// warps with every kJoin-th part each, in a fixed order.
+// Adds the sums of each long run, kOwn columns a lane (32 apart): those over
+// few parts a warp each, then those over many a block each, whose warps have
+// every kJoin-th part; both in a fixed order.
 template <typename T> __global__ void __launch_bounds__(32 * kJoin) embedding_join_kernel(const EmbedArgs a)
 {
-    __shared__ float sums[kJoin][32];
-    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-    const int64_t chunks = (a.width + 31) / 32, items = a.runs[0] * chunks;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t part = a.runs[1 + item / chunks], c = item % chunks * 32 + lane;
-        const int k = a.sorted[(part + 1) * kPart - 1];
+    constexpr int kOwn = 4, kColumns = 32 * kOwn;
+    __shared__ float sums[kJoin][kColumns];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int64_t chunks = (a.width + kColumns - 1) / kColumns, parts = (a.n + kPart - 1) / kPart;
+    auto add = [&](float (&sum)[kOwn], int64_t row, int64_t c) {   // row of the partial sums
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (c + 32 * i < a.width) sum[i] += __ldcs(a.partial + row * a.width + c + 32 * i);
+    };
+    for (int64_t item = (int64_t)blockIdx.x * kJoin + warp; item < a.runs[0] * chunks; item += (int64_t)gridDim.x * kJoin) {
+        const int64_t part = a.runs[2 + item / chunks], c = item % chunks * kColumns + lane;
+        const int k = a.sorted[(part + 1) * kPart - 1].y;
         // the parts that it goes on in: those whose first id is k
+        const int64_t p = (part + 1 + lane) * kPart;
+        const unsigned in = __ballot_sync(0xffffffffu, lane < kFew && p < a.n && a.sorted[p].y == k);
+        const int more = __ffs(~in) - 1;
+        float sum[kOwn] = {};
+        add(sum, part * 2 + 1, c);
+#pragma unroll
+        for (int i = 1; i <= kFew; ++i)
+            if (i <= more) add(sum, (part + i) * 2, c);
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            if (c + 32 * i < a.width) static_cast<T *>(a.out)[(int64_t)k * a.width + c + 32 * i] = elem_of<T>(sum[i] * a.scale);
+    }
+    for (int64_t item = blockIdx.x; item < a.runs[1] * chunks; item += gridDim.x) {
+        const int64_t part = a.runs[parts + 1 - item / chunks], c = item % chunks * kColumns + lane;
+        const int k = a.sorted[(part + 1) * kPart - 1].y;
         int64_t end = part + 1;
         for (int more = blockDim.x; more == (int)blockDim.x; end += more) {
             const int64_t p = (end + threadIdx.x) * kPart;
-            more = __syncthreads_count(p < a.n && a.sorted[p] == k);
+            more = __syncthreads_count(p < a.n && a.sorted[p].y == k);
         }
-        float sum = 0.f;
-        if (c < a.width) {
-            if (group == 0) sum = a.partial[(part * 2 + 1) * a.width + c];
+        float sum[kOwn] = {};
+        if (warp == 0) add(sum, part * 2 + 1, c);
 #pragma unroll 8
-            for (int64_t p = part + 1 + group; p < end; p += kJoin) sum += a.partial[p * 2 * a.width + c];
-        }
-        sums[group][lane] = sum;
-        __syncthreads();
-        if (group == 0 && c < a.width) {
+        for (int64_t p = part + 1 + warp; p < end; p += kJoin) add(sum, p * 2, c);
 #pragma unroll
-            for (int g = 1; g < kJoin; ++g) sum += sums[g][lane];
-            static_cast<T *>(a.out)[(int64_t)k * a.width + c] = elem_of<T>(sum * a.scale);
+        for (int i = 0; i < kOwn; ++i) sums[warp][lane + 32 * i] = sum[i];
+        __syncthreads();
+        if (threadIdx.x < kColumns) {
+            const int64_t at = item % chunks * kColumns + threadIdx.x;
+            float all = 0.f;
+#pragma unroll
+            for (int g = 0; g < kJoin; ++g) all += sums[g][threadIdx.x];
+            if (at < a.width) static_cast<T *>(a.out)[(int64_t)k * a.width + at] = elem_of<T>(all * a.scale);
         }
         __syncthreads();
     }
@@ -237,7 +268,7 @@ template <typename F> cudaError_t by_rows(int dtype, int64_t width, F f)
 
 // What the backward pass keeps in its workspace.
 struct Places {
-    size_t array[4], runs, counts, partial, bytes;   // array: the order and the ids of two sorting passes
+    size_t sorted[2], runs, counts, partial, bytes;   // sorted: of two sorting passes in turn
 };
 Places places_of(int64_t n, int64_t width)
 {
@@ -248,8 +279,8 @@ Places places_of(int64_t n, int64_t width)
         p.bytes += (bytes + 255) & ~size_t(255);
         return at;
     };
-    for (size_t &at : p.array) at = take((size_t)n * 4);
-    p.runs = take((size_t)(parts + 1) * 4);
+    for (size_t &at : p.sorted) at = take((size_t)n * sizeof(int2));
+    p.runs = take((size_t)(parts + 2) * 4);
     p.counts = take(bucket_workspace(n, kMostBuckets));
     p.partial = take((size_t)parts * 2 * width * sizeof(float));
     return p;
@@ -283,9 +314,8 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
         if ((e = cudaMemsetAsync(static_cast<char *>(l.out) + bytes / 16 * 16, 0, bytes % 16, stream)) != cudaSuccess) return e;
     char *ws = static_cast<char *>(workspace);
     const Places places = places_of(l.n, l.width);
-    auto ints = [&](size_t at) { return reinterpret_cast<int *>(ws + at); };
-    int *array[4];   // order and ids of two passes
-    for (int i = 0; i < 4; ++i) array[i] = ints(places.array[i]);
+    int2 *const sorted[2] = {reinterpret_cast<int2 *>(ws + places.sorted[0]), reinterpret_cast<int2 *>(ws + places.sorted[1])};
+    int *const runs = reinterpret_cast<int *>(ws + places.runs);
     const unsigned parts = (unsigned)((l.n + kPart - 1) / kPart);
     int bits = 1;
     while (bits < 31 && (int64_t(1) << bits) < l.rows) ++bits;
@@ -293,27 +323,26 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
     const int64_t vectors = (int64_t)(bytes / 16);
     for (int p = 0; p < passes; ++p) {
         BucketSort s{};
-        s.keys = p ? static_cast<const void *>(array[2 + (p - 1) % 2]) : l.ids;
-        s.wide = p == 0 && l.itype == SPMM_I64;
-        s.order_in = p ? array[(p - 1) % 2] : nullptr;
+        if (p == 0) s.keys = l.ids;
+        else s.pairs_in = sorted[(p - 1) % 2];
+        s.wide = l.itype == SPMM_I64;
         s.n = l.n;
         s.buckets = 1 << each;
         s.shift = p * each;
         s.mask = (1 << each) - 1;
         s.limit = l.rows;
         s.skip = skip;
-        s.order = array[p % 2];
-        s.key_out = array[2 + p % 2];
-        s.counts = ints(places.counts);
-        s.count = ints(places.runs);
+        s.pairs = sorted[p % 2];
+        s.counts = reinterpret_cast<int *>(ws + places.counts);
+        s.clear = runs;
         s.zero = static_cast<uint4 *>(l.out) + vectors * p / passes;   // a share of the zeros beside each pass
         s.zero_vectors = vectors * (p + 1) / passes - vectors * p / passes;
         s.status = l.status;
         if ((e = launch_bucket_sort(s, stream)) != cudaSuccess) return e;
     }
     EmbedArgs a{};
-    a.in = l.in; a.out = l.out; a.order = array[(passes - 1) % 2]; a.sorted = array[2 + (passes - 1) % 2];
-    a.runs = ints(places.runs);
+    a.in = l.in; a.out = l.out; a.sorted = sorted[(passes - 1) % 2];
+    a.runs = runs;
     a.partial = reinterpret_cast<float *>(ws + places.partial);
     a.n = l.n; a.rows = l.rows; a.width = l.width; a.scale = l.scale; a.status = l.status;
     return by_rows(l.dtype, l.width, [&](auto aligned, auto type) {
@@ -323,7 +352,7 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
         const int64_t threads = l.width / kElems + l.width % kElems;
         embedding_sum_kernel<kAligned, T><<<dim3(parts, (unsigned)((threads + 127) / 128)), 128, 0, stream>>>(a);
         if (parts > 1)
-            embedding_join_kernel<T><<<(unsigned)std::min<int64_t>(parts * ((l.width + 31) / 32), 4 * (int64_t)device_sm_count()),
+            embedding_join_kernel<T><<<(unsigned)std::min<int64_t>(parts * ((l.width + 127) / 128), 4 * (int64_t)device_sm_count()),
                                        32 * kJoin, 0, stream>>>(a);
         return cudaGetLastError();
     });

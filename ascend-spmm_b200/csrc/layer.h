@@ -99,9 +99,9 @@ cudaError_t launch_route_backward(const RouteLaunch &r, const float *grad, void 
 
 // ---- stable counting sort (bucket.cu) ---------------------------------------
 struct BucketSort {
-    const void *keys;       // [n] in the order of order_in, int32 or int64
+    const void *keys;       // [n] int32 or int64, or instead of them
     bool wide;
-    const int *order_in;    // the inputs in the order to keep (an earlier pass's), -1: none; null: as they are
+    const int2 *pairs_in;   // [n] inputs and their keys in the order to keep (an earlier pass's), -1: none
     int64_t n;
     int buckets;            // at most kMostBuckets; a key's bucket is (key >> shift) & mask
     int shift, mask;
@@ -109,10 +109,10 @@ struct BucketSort {
     int64_t skip;           // this key is left out
     int *ptr;               // [buckets + 1] first place of each bucket; may be null
     int *position;          // [n] place of each input, -1 where it is left out; may be null
-    int *order;             // [n] input of each place, -1 past the last
-    int *key_out;           // [n] their keys, -1 past the last; may be null (then limit may pass 32 bits)
+    int *order;             // [n] input of each place, -1 past the last, or instead of it
+    int2 *pairs;            // [n] input and key of each place
     int *counts;            // workspace: bucket_workspace bytes
-    int *count;             // set to 0; may be null
+    int *clear;             // two integers to set to 0; may be null
     void *zero;             // 16-byte vectors to zero meanwhile
     int64_t zero_vectors;
     DevStatus *status;

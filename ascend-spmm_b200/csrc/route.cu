@@ -136,7 +136,7 @@ struct RouteArgs {
 };
 
 // VPL values of a lane from `at` on; those past the row's end are `fill`.
-template <typename T, int VPL, bool VEC>
+template <typename T, int VPL, bool VEC, bool SHARED = false>
 __device__ __forceinline__ void load_lane(const T *row, int at, int n, float fill, float (&v)[VPL])
 {
     if constexpr (VEC) {
@@ -145,7 +145,8 @@ __device__ __forceinline__ void load_lane(const T *row, int at, int n, float fil
 #pragma unroll
         for (int c = 0; c < VPL / kElems; ++c) {
             if (at + c * kElems < n) {   // n is a multiple of kElems
-                const V raw = __ldg(reinterpret_cast<const V *>(row + at) + c);
+                const V *from = reinterpret_cast<const V *>(row + at) + c;
+                const V raw = SHARED ? *from : __ldg(from);
                 const T *e = reinterpret_cast<const T *>(&raw);
 #pragma unroll
                 for (int i = 0; i < kElems; ++i) v[c * kElems + i] = elem_f32<T>(e[i]);
@@ -270,12 +271,32 @@ __device__ __forceinline__ float reciprocal(float x)   // within 2^-23 of itself
     return y;
 }
 
+// exp(x) within 2^-21 of itself (|x| log2(e) rounds by 2^-24 of it; where x is far from 0, exp(x) or, of a sigmoid, 1 is
+// all that is left), 0 below 2^-126.
+__device__ __forceinline__ float fast_exp(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
 // Blocks of an SM: a row is a long chain of dependent steps, so the more warps take turns the better.
-constexpr int route_blocks(int vpl) { return vpl == 8 ? 5 : vpl == 16 ? 4 : 2; }
+constexpr int route_blocks(int vpl) { return vpl == 8 ? 4 : vpl == 16 ? 3 : 2; }
+
+// Calls f with this lane's share of the k choices.
+template <int LANES, typename F> __device__ __forceinline__ void each_choice(int lane, int k, F f)
+{
+    if constexpr (LANES >= kMostChosen) {
+        if (lane < k) f(lane);
+    } else {
+        for (int p = lane; p < k; p += LANES) f(p);
+    }
+}
 
 template <typename T, int LANES, int VPL, bool VEC>
 __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const RouteArgs a)
 {
+    extern __shared__ __align__(16) unsigned char staged[];   // VEC: two turns' rows of each warp
     constexpr int kLow = VPL - 1;   // bits of a key that hold the (reversed) place in the lane
     constexpr int kTeams = 32 / LANES;
     constexpr unsigned kTeam = LANES == 32 ? kFull : (1u << LANES) - 1;
@@ -290,16 +311,37 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
     // by logits: 16-bit ones are compared exactly, 32-bit ones where their keys differ above the low bits
     const float rel = by_logit ? VPL * 0x1p-23f : 0x1p-21f + VPL * 0x1p-22f;
     const bool exact = by_logit && sizeof(T) == 2;
-    float bias[VPL];
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) bias[j] = a.bias && first + j < n ? __ldg(a.bias + first + j) : 0.f;
+    // a warp's turn is kTeams rows, which lie together: the next turn's are on their way while this one's are worked on
+    const int turn_bytes = kTeams * n * (int)sizeof(T);
+    unsigned char *const buffers = staged + warp * 2 * turn_bytes;
+    auto fetch = [&](int64_t t0, int buffer) {
+        if constexpr (VEC) {
+            const int64_t at = t0 * n * (int64_t)sizeof(T), end = a.tokens * n * (int64_t)sizeof(T);
+            const unsigned to = (unsigned)__cvta_generic_to_shared(buffers + buffer * turn_bytes);
+            for (int i = (threadIdx.x & 31) * 16; i < turn_bytes; i += 512)
+                if (at + i < end)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + i),
+                                 "l"(static_cast<const unsigned char *>(a.logits) + at + i)
+                                 : "memory");
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        }
+    };
     int *const picks = s_pick[warp][team], *const keys = s_key[warp][team], *const scores = s_score[warp][team];
     const int64_t step = (int64_t)gridDim.x * 8 * kTeams;
-    for (int64_t t0 = ((int64_t)blockIdx.x * 8 + warp) * kTeams; t0 < a.tokens; t0 += step) {
+    const int64_t start = ((int64_t)blockIdx.x * 8 + warp) * kTeams;
+    if (start < a.tokens) fetch(start, 0);
+    int buffer = 0;
+    for (int64_t t0 = start; t0 < a.tokens; t0 += step, buffer ^= 1) {
         const int64_t t = min(t0 + team, a.tokens - 1);   // a team past the last row does it again and stores nothing
         const T *row = static_cast<const T *>(a.logits) + t * n;
+        if constexpr (VEC) {
+            fetch(t0 + step, buffer ^ 1);
+            asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+            __syncwarp();
+            row = reinterpret_cast<const T *>(buffers + buffer * turn_bytes) + (int)(t - t0) * n;
+        }
         float c[VPL];   // the values to choose by
-        load_lane<T, VPL, VEC>(row, first, n, -INFINITY, c);
+        load_lane<T, VPL, VEC, VEC>(row, first, n, -INFINITY, c);
         float mx = 0.f, inv = 1.f;
         if (!a.sigmoid) {
             float m = -INFINITY;
@@ -308,21 +350,31 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
             mx = safe_max(team_max<LANES>(m));
             float e[VPL], z = 0.f;
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) z += e[j] = __expf(c[j] - mx);
+            for (int j = 0; j < VPL; ++j) z += e[j] = fast_exp(c[j] - mx);
             z = warp_sum<LANES>(z);
-            inv = z == 0.f ? 0.f : 1.f / z;
+            inv = z == 0.f ? 0.f : reciprocal(z);
             if (!by_logit) {
 #pragma unroll
                 for (int j = 0; j < VPL; ++j) c[j] = e[j] * inv;
             }
         } else if (!by_logit) {
 #pragma unroll
-            for (int j = 0; j < VPL; ++j) c[j] = reciprocal(1.f + __expf(-c[j]));
+            for (int j = 0; j < VPL; ++j) c[j] = reciprocal(1.f + fast_exp(-c[j]));
+        }
+        if (a.bias) {
+            float b[VPL];
+            load_lane<float, VPL, VEC>(a.bias, first, n, 0.f, b);
+#pragma unroll
+            for (int j = 0; j < VPL; ++j) c[j] += b[j];
         }
         int key[VPL];
 #pragma unroll
-        for (int j = 0; j < VPL; ++j)   // the sum with 0 makes -0 one
-            key[j] = first + j < n ? (raw_key(c[j] + bias[j]) & ~kLow) | (kLow - j) : kNone;
+        for (int j = 0; j < VPL; ++j) key[j] = (raw_key(c[j] + 0.f) & ~kLow) | (kLow - j);   // the sum makes -0 a 0
+        if (first + VPL > n) {
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+                if (first + j >= n) key[j] = kNone;
+        }
 
         const float largest = by_logit ? 0.f : a.sigmoid ? 1.f : inv;
         bool again = false;
@@ -379,11 +431,17 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                 }
                 again |= mine > kInfKey || mine < (kMinusInfKey & ~kLow);   // NaN
             }
+            if constexpr (LANES == 32) {
+                kept = __reduce_or_sync(kFull, kept);
+                last = __reduce_min_sync(kFull, last);
+                out = warp_max(out);
+            } else {
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) {
-                kept |= __shfl_xor_sync(kFull, kept, o);
-                last = min(last, __shfl_xor_sync(kFull, last, o));
-                out = max(out, __shfl_xor_sync(kFull, out, o));
+                for (int o = LANES / 2; o > 0; o >>= 1) {
+                    kept |= __shfl_xor_sync(kFull, kept, o);
+                    last = min(last, __shfl_xor_sync(kFull, last, o));
+                    out = max(out, __shfl_xor_sync(kFull, out, o));
+                }
             }
             if (!exact) again |= too_close(key_value(last), key_value(out), largest, 2 * rel);
             if (by_lanes) {
@@ -412,11 +470,11 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
         }
         __syncwarp();
         // the row is decided in 64 bits where a pick and the next one are too close, and where a NaN was met
-        for (int p = lane; p < a.k; p += LANES) {
+        each_choice<LANES>(lane, a.k, [&](int p) {
             const int mine = keys[p], next = keys[p + 1];
             again |= mine > kInfKey || mine < (kMinusInfKey & ~kLow);
             if (!exact && next != kNone) again |= too_close(key_value(mine), key_value(next), largest, rel);
-        }
+        });
         unsigned unsure = __ballot_sync(kFull, again);
         while (unsure) {
             const int who = (__ffs(unsure) - 1) / LANES;
@@ -429,19 +487,21 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
         __syncwarp();
         auto score = [&](int p) {
             const float v = elem_f32<T>(row[picks[p]]);
-            return a.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - mx) * inv;
+            return a.sigmoid ? reciprocal(1.f + expf(-v)) : expf(v - mx) * inv;
         };
-        float total = 1.f;
+        const float own = lane < a.k ? score(lane) : 0.f;   // a row of few lanes has more of them: worked out again
+        float factor = a.scale;
         if (a.renormalize) {
-            float sum = 0.f;
-            for (int p = lane; p < a.k; p += LANES) sum += score(p);
-            total = warp_sum<LANES>(sum) + 1e-20f;
+            float sum = own;
+            if constexpr (LANES < kMostChosen)
+                for (int p = lane + LANES; p < a.k; p += LANES) sum += score(p);
+            factor *= reciprocal(warp_sum<LANES>(sum) + 1e-20f);
         }
         if (t0 + team < a.tokens)
-            for (int p = lane; p < a.k; p += LANES) {
-                a.weights[t * a.k + p] = (a.renormalize ? score(p) / total : score(p)) * a.scale;
+            each_choice<LANES>(lane, a.k, [&](int p) {
+                a.weights[t * a.k + p] = (p == lane ? own : score(p)) * factor;
                 a.experts[t * a.k + p] = picks[p];
-            }
+            });
         __syncwarp();   // the picks have been read
     }
 }
@@ -576,7 +636,18 @@ cudaError_t launch_route(const RouteLaunch &r, cudaStream_t stream)
             constexpr int kLanes = decltype(lanes)::value, kVpl = decltype(vpl)::value;
             const int64_t warps = (r.tokens + 32 / kLanes - 1) / (32 / kLanes);
             const unsigned blocks = (unsigned)std::min<int64_t>((warps + 7) / 8, route_blocks(kVpl) * (int64_t)device_sm_count());
-            route_kernel<T, kLanes, kVpl, decltype(vec)::value><<<blocks, 256, 0, stream>>>(a);
+            auto kernel = route_kernel<T, kLanes, kVpl, decltype(vec)::value>;
+            const int smem = decltype(vec)::value ? 8 * 2 * (32 / kLanes) * r.n * (int)sizeof(T) : 0;
+            if (smem > 16384) {   // with what the kernel has of its own, more than a block gets unasked
+                static PerDevice<bool> ready;   // the attribute outlasts the call
+                bool *done = ready.here();
+                if (!done || !*done) {
+                    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+                    if (e != cudaSuccess) return e;
+                    if (done) *done = true;
+                }
+            }
+            kernel<<<blocks, 256, smem, stream>>>(a);
             return cudaGetLastError();
         });
     });
