@@ -41,58 +41,46 @@ struct EmbedArgs {
     // former from the front and the latter from the back
     int *runs;
     int64_t n, rows, width;
+    int lanes;              // forward: of a row's team
     float scale;
     DevStatus *status;
 };
 
-// A warp per row.
+// A team of a.lanes lanes per row, kAtOnce vectors a lane in flight.
+constexpr int kAtOnce = 4;
 template <bool ALIGNED, typename T> __global__ void __launch_bounds__(256) embedding_kernel(const EmbedArgs a)
 {
     constexpr int kElems = Pack16<T>::kElems;
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = (int64_t)gridDim.x * (blockDim.x / 32);
-    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; i < a.n; i += warps) {
+    const int lane = threadIdx.x & (a.lanes - 1);
+    const int64_t teams = (int64_t)gridDim.x * blockDim.x / a.lanes;
+    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / a.lanes; i < a.n; i += teams) {
         const int64_t id = a.wide ? ld_idx(static_cast<const int64_t *>(a.ids) + i) : ld_idx(static_cast<const int *>(a.ids) + i);
         const bool found = id >= 0 && id < a.rows;
         if (!found && lane == 0) raise_status(a.status, SPMM_DEV_BAD_COLUMN, i);
         const T *row = static_cast<const T *>(a.in) + (found ? id : 0) * a.width;
         T *out = static_cast<T *>(a.out) + i * a.width;
         const RowSpan<ALIGNED, T> span(out, a.width);
-#pragma unroll 4
-        for (int64_t c = lane; c < span.vectors; c += 32) {
-            Pack16<T> v;
-            v.raw = make_uint4(0, 0, 0, 0);
-            if (found) {
+        for (int64_t c0 = lane; c0 < span.vectors; c0 += a.lanes * kAtOnce) {
+            Pack16<T> v[kAtOnce];
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n) {
+                v[n].raw = make_uint4(0, 0, 0, 0);
+                if (found && c0 + n * a.lanes < span.vectors) v[n] = load16<ALIGNED>(row + span.head + (c0 + n * a.lanes) * kElems);
+            }
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n) {
                 float f[kElems];
-                load16<ALIGNED>(row + span.head + c * kElems).get(f);
+                v[n].get(f);
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) f[e] *= a.scale;
-                v.set(f);
+                if (found) v[n].set(f);   // else zeros, whatever the scale's sign
+                if (c0 + n * a.lanes < span.vectors) __stcs(reinterpret_cast<uint4 *>(out + span.head) + c0 + n * a.lanes, v[n].raw);
             }
-            __stcs(reinterpret_cast<uint4 *>(out + span.head) + c, v.raw);
         }
-        if (lane < span.loose(a.width)) {
-            const int64_t c = span.loose_at(lane);
+        for (int64_t n = lane; n < span.loose(a.width); n += a.lanes) {
+            const int64_t c = span.loose_at(n);
             out[c] = elem_of<T>(found ? elem_f32<T>(row[c]) * a.scale : 0.f);
         }
-    }
-}
-
-// E columns of a row from column c on.
-template <bool ALIGNED, typename T, int E> __device__ __forceinline__ void load_columns(const T *p, float (&f)[E])
-{
-    if constexpr (E == 1) f[0] = elem_f32<T>(*p);
-    else load16<ALIGNED>(p).get(f);
-}
-template <bool ALIGNED, typename T, int E> __device__ __forceinline__ void store_columns(T *p, const float (&f)[E])
-{
-    if constexpr (ALIGNED) {
-        Pack16<T> v;
-        v.set(f);
-        *reinterpret_cast<uint4 *>(p) = v.raw;
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) p[e] = elem_of<T>(f[e]);
     }
 }
 
@@ -102,50 +90,75 @@ template <bool ALIGNED, typename T, int E> __device__ __forceinline__ void store
 struct Part {
     int key[3 * kPart + 2];   // key[kPart + 1 + i]: the id at place i of the part, -1 outside the ids
     int at[2 * kPart];        // input indexes of the part and of kPart places behind it
+    int head[2 * kPart];      // elements before the first whole vector of their ids' rows of dtable
     int begin, end;           // the places that this part adds
     bool more;                // the last run is longer and goes on: its sum is a partial one
     bool before;              // the first run comes from before: its sum is a partial one
 };
 
-// E columns of the part's sums, from column c on.
+// The part's sums, of E columns: the `slot`-th whole vector of an id's row of
+// dtable or, with E == 1, its `slot`-th loose element.  Where they lie in the
+// row goes by the id, so that a result is stored in whole vectors.
 template <bool ALIGNED, typename T, int E>
-__device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const Part &s, int64_t c)
+__device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const Part &s, int64_t slot)
 {
-    const T *dy = static_cast<const T *>(a.in) + c;
+    constexpr int kElems = Pack16<T>::kElems;
     const int *key = s.key + kPart + 1;
+    // the column of the slot in the row of the id at place i, -1 where the row has no such one
+    const int width = (int)a.width;
+    auto column = [&](int i) -> int {
+        if constexpr (ALIGNED) return (int)slot * kElems;
+        const int head = s.head[i], vectors = (width - head) / kElems;
+        if constexpr (E == 1) {
+            const int c = slot < head ? (int)slot : (int)slot + vectors * kElems;
+            return c < width ? c : -1;
+        }
+        return slot < vectors ? head + (int)slot * kElems : -1;
+    };
     float sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.f;
     bool before = s.before;
     constexpr int kAhead = 8;
+    using Raw = std::conditional_t<E == 1, T, Pack16<T>>;
     for (int i0 = s.begin; i0 < s.end; i0 += kAhead) {
-        float f[kAhead][E];
+        Raw raw[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)   // past the last one: a row is read again and not added
-            load_columns<ALIGNED, T, E>(dy + (int64_t)s.at[min(i0 + j, s.end - 1)] * a.width, f[j]);
+        for (int j = 0; j < kAhead; ++j) {   // past the last one: a row is read again and not added
+            const int i = min(i0 + j, s.end - 1), c = max(column(i), 0);
+            const T *p = static_cast<const T *>(a.in) + (int64_t)s.at[i] * a.width + c;
+            if constexpr (E == 1) raw[j] = *p;
+            else raw[j] = load16<ALIGNED>(p);
+        }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int i = i0 + j;
             if (i >= s.end) break;
+            float f[E];
+            if constexpr (E == 1) f[0] = elem_f32<T>(raw[j]);
+            else raw[j].get(f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum[e] += f[j][e];
+            for (int e = 0; e < E; ++e) sum[e] += f[e];
             const int k = key[i];
             if (i + 1 < s.end && key[i + 1] == k) continue;
             const bool more = i + 1 == s.end && s.more;
+            const int c = column(i);
             if (before || more) {
                 float *p = a.partial + (part * 2 + (before ? 0 : 1)) * a.width + c;
 #pragma unroll
-                for (int e = 0; e < E; ++e) p[e] = sum[e];
-                if (!before && c == 0) {
-                    const int64_t far = (part + kFew) * kPart, parts = (a.n + kPart - 1) / kPart;
-                    const bool many = far < a.n && a.sorted[far].y == k;
-                    const int i = atomicAdd(a.runs + many, 1);
-                    a.runs[many ? parts + 1 - i : 2 + i] = (int)part;
-                }
-            } else {
+                for (int e = 0; e < E; ++e)
+                    if (c >= 0) p[e] = sum[e];
+            } else if (c >= 0) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) sum[e] *= a.scale;
-                store_columns<ALIGNED, T, E>(static_cast<T *>(a.out) + (int64_t)k * a.width + c, sum);
+                T *p = static_cast<T *>(a.out) + (int64_t)k * a.width + c;
+                if constexpr (E == 1) {
+                    *p = elem_of<T>(sum[0]);
+                } else {
+                    Pack16<T> v;
+                    v.set(sum);
+                    *reinterpret_cast<uint4 *>(p) = v.raw;
+                }
             }
             before = false;
 #pragma unroll
@@ -154,22 +167,38 @@ __device__ __forceinline__ void sum_part(const EmbedArgs &a, int64_t part, const
     }
 }
 
-// A block per part (and a slice of the columns: blockIdx.y).
-template <bool ALIGNED, typename T> __global__ void __launch_bounds__(128) embedding_sum_kernel(const EmbedArgs a)
+// Threads that a part needs: one for each whole vector of a row, and one for
+// each element that can lie outside them.
+template <typename T> int64_t part_threads(int64_t width)
+{
+    constexpr int64_t kElems = Pack16<T>::kElems;
+    return width % kElems == 0 ? width / kElems : width / kElems + 2 * (kElems - 1);
+}
+
+// blockDim.x threads of blockDim.y parts (and of a slice of the columns: blockIdx.y).
+constexpr int kSumThreads = 128, kMostParts = 16;
+template <bool ALIGNED, typename T> __global__ void __launch_bounds__(kSumThreads, 8) embedding_sum_kernel(const EmbedArgs a)
 {
     constexpr int kElems = Pack16<T>::kElems;
-    __shared__ Part s;
-    const int64_t part = blockIdx.x, first = part * kPart;
-    for (int i = threadIdx.x; i < 3 * kPart + 2; i += blockDim.x) {
-        const int64_t p = first + i - (kPart + 1);
-        const int2 v = p >= 0 && p < a.n ? __ldg(a.sorted + p) : make_int2(-1, -1);
-        s.key[i] = v.y;
-        if (i > kPart && i <= 3 * kPart) s.at[i - (kPart + 1)] = v.x;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x, *key = s.key + kPart + 1;
-        static_assert(kPart == 32, "a lane per place");
+    static_assert(kPart == 32, "a lane per place");
+    __shared__ Part shared[kMostParts];
+    const int warp = (threadIdx.y * blockDim.x + threadIdx.x) / 32, lane = (threadIdx.y * blockDim.x + threadIdx.x) % 32;
+    const int64_t parts = (a.n + kPart - 1) / kPart, part0 = (int64_t)blockIdx.x * blockDim.y;
+    for (int n = warp; n < (int)blockDim.y; n += kSumThreads / 32) {   // a warp lays out a part
+        Part &s = shared[n];
+        const int64_t first = (part0 + n) * kPart;
+        for (int i = lane; i < 3 * kPart + 2; i += 32) {
+            const int64_t p = first + i - (kPart + 1);
+            const int2 v = p >= 0 && p < a.n ? __ldg(a.sorted + p) : make_int2(-1, -1);
+            s.key[i] = v.y;
+            if (i > kPart && i <= 3 * kPart) {
+                s.at[i - (kPart + 1)] = v.x;
+                if (!ALIGNED)
+                    s.head[i - (kPart + 1)] = RowSpan<false, T>(static_cast<T *>(a.out) + (int64_t)max(v.y, 0) * a.width, a.width).head;
+            }
+        }
+        __syncwarp();
+        const int *key = s.key + kPart + 1;
         // places of the first run where it comes from before, and places behind the part where the last one goes on
         const unsigned valid = __ballot_sync(0xffffffffu, key[lane] >= 0);
         const unsigned as_before = __ballot_sync(0xffffffffu, key[lane] >= 0 && key[lane] == key[-1]);
@@ -185,16 +214,22 @@ template <bool ALIGNED, typename T> __global__ void __launch_bounds__(128) embed
             s.begin = long_before ? 0 : rest;
             s.more = long_last;
             s.end = __popc(valid) + (long_last ? 0 : over);
+            // a long run that starts here: for the join, beside those of few parts or of many
+            if (blockIdx.y == 0 && long_last && rest < kPart) {
+                const int64_t far = first + kFew * kPart;
+                const bool many = far < a.n && a.sorted[far].y == key[kPart - 1];
+                const int i = atomicAdd(a.runs + many, 1);
+                a.runs[many ? parts + 1 - i : 2 + i] = (int)(part0 + n);
+            }
         }
     }
     __syncthreads();
-    if (s.begin >= s.end) return;
+    const Part &s = shared[threadIdx.y];
+    const int64_t part = part0 + threadIdx.y;
+    if (part >= parts || s.begin >= s.end) return;
     const int64_t vectors = a.width / kElems, t = (int64_t)blockIdx.y * blockDim.x + threadIdx.x;
-    if (t < vectors) {
-        sum_part<ALIGNED, T, kElems>(a, part, s, t * kElems);
-    } else if (!ALIGNED && t - vectors < a.width - vectors * kElems) {   // the columns behind the last whole vector
-        sum_part<false, T, 1>(a, part, s, vectors * kElems + t - vectors);
-    }
+    if (t < vectors) sum_part<ALIGNED, T, kElems>(a, part, s, t);
+    else if (!ALIGNED && t - vectors < 2 * (kElems - 1)) sum_part<false, T, 1>(a, part, s, t - vectors);
 }
 
 // Adds the sums of each long run, kOwn columns a lane (32 apart): those over
@@ -206,11 +241,23 @@ template <typename T> __global__ void __launch_bounds__(32 * kJoin) embedding_jo
     __shared__ float sums[kJoin][kColumns];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int64_t chunks = (a.width + kColumns - 1) / kColumns, parts = (a.n + kPart - 1) / kPart;
-    auto add = [&](float (&sum)[kOwn], int64_t row, int64_t c) {   // row of the partial sums
+    // N rows of the partial sums, 2 * stride apart, all of their loads in flight; `count` of them are there
+    auto add = [&](float (&sum)[kOwn], auto rows, int64_t row, int64_t stride, int count, int64_t c) {
+        constexpr int N = decltype(rows)::value;
+        float f[N][kOwn];
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-            if (c + 32 * i < a.width) sum[i] += __ldcs(a.partial + row * a.width + c + 32 * i);
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i)   // what is not there: the last one again, not added
+                f[n][i] = __ldcs(a.partial + (row + 2 * stride * min(n, count - 1)) * a.width + min(c + 32 * i, a.width - 1));
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i)
+                if (n < count) sum[i] += f[n][i];
     };
+    std::integral_constant<int, 1> one;
+    std::integral_constant<int, kFew> several;
     for (int64_t item = (int64_t)blockIdx.x * kJoin + warp; item < a.runs[0] * chunks; item += (int64_t)gridDim.x * kJoin) {
         const int64_t part = a.runs[2 + item / chunks], c = item % chunks * kColumns + lane;
         const int k = a.sorted[(part + 1) * kPart - 1].y;
@@ -219,10 +266,8 @@ template <typename T> __global__ void __launch_bounds__(32 * kJoin) embedding_jo
         const unsigned in = __ballot_sync(0xffffffffu, lane < kFew && p < a.n && a.sorted[p].y == k);
         const int more = __ffs(~in) - 1;
         float sum[kOwn] = {};
-        add(sum, part * 2 + 1, c);
-#pragma unroll
-        for (int i = 1; i <= kFew; ++i)
-            if (i <= more) add(sum, (part + i) * 2, c);
+        add(sum, one, part * 2 + 1, 0, 1, c);
+        if (more > 0) add(sum, several, (part + 1) * 2, 1, more, c);
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
             if (c + 32 * i < a.width) static_cast<T *>(a.out)[(int64_t)k * a.width + c + 32 * i] = elem_of<T>(sum[i] * a.scale);
@@ -236,9 +281,9 @@ template <typename T> __global__ void __launch_bounds__(32 * kJoin) embedding_jo
             more = __syncthreads_count(p < a.n && a.sorted[p].y == k);
         }
         float sum[kOwn] = {};
-        if (warp == 0) add(sum, part * 2 + 1, c);
-#pragma unroll 8
-        for (int64_t p = part + 1 + warp; p < end; p += kJoin) add(sum, p * 2, c);
+        if (warp == 0) add(sum, one, part * 2 + 1, 0, 1, c);
+        for (int64_t p = part + 1 + warp; p < end; p += kJoin * kFew)
+            add(sum, several, p * 2, kJoin, (int)min((int64_t)kFew, (end - p + kJoin - 1) / kJoin), c);
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) sums[warp][lane + 32 * i] = sum[i];
         __syncthreads();
@@ -293,7 +338,10 @@ cudaError_t launch_embedding(const EmbeddingLaunch &l, cudaStream_t stream)
     EmbedArgs a{};
     a.ids = l.ids; a.wide = l.itype == SPMM_I64; a.in = l.in; a.out = l.out; a.n = l.n; a.rows = l.rows;
     a.width = l.width; a.scale = l.scale; a.status = l.status;
-    const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>((l.n + 7) / 8, 32 * (int64_t)device_sm_count()));
+    const int64_t vectors = l.width * (l.dtype == SPMM_F32 ? 4 : 2) / 16;
+    for (a.lanes = 2; a.lanes < 32 && a.lanes * kAtOnce < vectors;) a.lanes *= 2;
+    const unsigned blocks = (unsigned)std::max<int64_t>(
+        1, std::min<int64_t>((l.n * a.lanes + 255) / 256, 32 * (int64_t)device_sm_count()));
     return by_rows(l.dtype, l.width, [&](auto aligned, auto type) {
         embedding_kernel<decltype(aligned)::value, decltype(type)><<<blocks, 256, 0, stream>>>(a);
         return cudaGetLastError();
@@ -348,9 +396,12 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
     return by_rows(l.dtype, l.width, [&](auto aligned, auto type) {
         using T = decltype(type);
         constexpr bool kAligned = decltype(aligned)::value;
-        constexpr int kElems = Pack16<T>::kElems;
-        const int64_t threads = l.width / kElems + l.width % kElems;
-        embedding_sum_kernel<kAligned, T><<<dim3(parts, (unsigned)((threads + 127) / 128)), 128, 0, stream>>>(a);
+        const int64_t threads = part_threads<T>(l.width);
+        int each = kSumThreads;   // threads of a part
+        while (each > kSumThreads / kMostParts && each / 2 >= threads) each /= 2;
+        const dim3 block(each, kSumThreads / each);
+        const dim3 grid((parts + block.y - 1) / block.y, (unsigned)((threads + each - 1) / each));
+        embedding_sum_kernel<kAligned, T><<<grid, block, 0, stream>>>(a);
         if (parts > 1)
             embedding_join_kernel<T><<<(unsigned)std::min<int64_t>(parts * ((l.width + 127) / 128), 4 * (int64_t)device_sm_count()),
                                        32 * kJoin, 0, stream>>>(a);

@@ -6,9 +6,9 @@
 //   experts: the k largest c, in descending order, the lowest index first
 //           among equal ones;  weights: w = s[chosen], divided by their sum
 //           + 1e-20 with `renormalize`, times `scale`
-//   backward, with g = scale * dw and S the sum:
-//           d = renormalized ? (g - sum(g s) / S) / S : g        (chosen ones)
-//           dx = s (d - sum(d s)) (softmax),  d s (1 - s) (sigmoid)
+//   backward, with g = scale * dw, S the sum and r = s / S:
+//           u = renormalized ? r (g - sum(g r)) : g s           (chosen ones)
+//           dx = u - s sum(u) (softmax),  u (1 - s) (sigmoid)
 //
 // A team of LANES lanes owns a row (a warp where it has more than 128
 // experts), lane l the experts l * VPL .. + VPL - 1 in registers, each sorted
@@ -564,14 +564,17 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
             z = warp_sum(z);
             inv = z == 0.f ? 0.f : 1.f / z;
         }
+        // u: the gradient of log s; with renormalize its sum is g w' times what 1e-20 takes of the sum of the weights, which
+        // as a difference would be rounding alone
         const float s = !on ? 0.f : a.sigmoid ? 1.f / (1.f + expf(-xe)) : expf(xe - mx) * inv;
-        if (!on) d = 0.f;
+        float u = on ? d * s : 0.f, along;
         if (a.renormalize) {
-            const float total = warp_sum(s) + 1e-20f;
-            d = (d - warp_sum(d * s) / total) / total;
+            const float total = warp_sum(s) + 1e-20f, w = s / total, mean = warp_sum(on ? d * w : 0.f);
+            u = on ? w * (d - mean) : 0.f;
+            along = mean * (1e-20f / total);
+        } else {
+            along = warp_sum(u);
         }
-        float along = 0.f;   // softmax: sum of d s
-        if (!a.sigmoid) along = warp_sum(on ? d * s : 0.f);
 #pragma unroll
         for (int c = 0; c < kVectors; ++c) {
             const int at = (c * 32 + lane) * kElems;
@@ -583,7 +586,7 @@ template <typename T, int VPL, bool VEC> __global__ void __launch_bounds__(256) 
             *reinterpret_cast<V *>(out + at) = raw;
         }
         __syncwarp();   // the chosen experts' values replace what the row got
-        if (on) out[e] = elem_of<T>(a.sigmoid ? d * s * (1.f - s) : s * (d - along));
+        if (on) out[e] = elem_of<T>(a.sigmoid ? u / (1.f + expf(xe)) : u - s * along);
     }
 }
 
