@@ -128,7 +128,7 @@ int check_embedding(const void *ids, const void *in, const void *out, int64_t n,
         return capi_error(SPMM_ERR_ARG, "%s: index arrays must be int32 or int64", op);
     if ((rc = check_size(n, width, 1, op)) || (rc = check_size(rows, width, 1, op))) return rc;
     if (width < 1) return capi_error(SPMM_ERR_ARG, "%s requires a feature width of at least 1", op);
-    if (n > INT32_MAX || rows > INT32_MAX || width > INT32_MAX)
+    if (n > INT32_MAX || rows > INT32_MAX || width > (1 << 24))
         return capi_error(SPMM_ERR_ARG, "%s: size too large", op);
     if (!std::isfinite((float)scale)) return capi_error(SPMM_ERR_ARG, "%s: scale must be finite", op);
     if (n > 0 && (!ids || !in)) return capi_error(SPMM_ERR_ARG, "%s: null array", op);

@@ -255,13 +255,15 @@ template <typename T, int VPL> __device__ __noinline__ int choose_exactly(const 
     return pick;
 }
 
-// Whether two values that the choice tells apart are closer than their
-// errors.  A 32-bit score is off by less than 2^-21 of the row's largest, its
-// sum with a bias (or of two) by 2^-23 of itself, and its key has lost
-// `lost` bits.
-__device__ __forceinline__ bool too_close(float hi, float lo, float largest, float rel)
+// Whether two values that the choice tells apart may be closer than their
+// errors.  A 32-bit score is off by at most 2^-21 of the row's largest one (of
+// 1 for a sigmoid) for its exponential and the reciprocal, and, with a
+// softmax, by its share of the sum's error, (VPL + 5) 2^-24; `score` is more
+// than twice that.  A sum of two rounds by 2^-24 of itself, and a key has lost
+// the bits that hold the place: `rel`.
+__device__ __forceinline__ bool too_close(float hi, float lo, float score, float rel)
 {
-    return !(hi - lo > 0x1p-19f * largest + rel * fmaxf(fabsf(hi), fabsf(lo)));   // true for infinities, too
+    return !(hi - lo > score + rel * fmaxf(fabsf(hi), fabsf(lo)));   // true for infinities, too
 }
 
 __device__ __forceinline__ float reciprocal(float x)   // within 2^-23 of itself
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                 if (first + j >= n) key[j] = kNone;
         }
 
-        const float largest = by_logit ? 0.f : a.sigmoid ? 1.f : inv;
+        const float unsure_by = by_logit ? 0.f : (0x1p-19f + VPL * 0x1p-22f) * (a.sigmoid ? 1.f : inv);
         bool again = false;
         if (grouped) {
             auto sum_of = [&](int top, int next) { return raw_key(key_value(top) + key_value(next)); };
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                     out = max(out, __shfl_xor_sync(kFull, out, o));
                 }
             }
-            if (!exact) again |= too_close(key_value(last), key_value(out), largest, 2 * rel);
+            if (!exact) again |= too_close(key_value(last), key_value(out), 2 * unsure_by, 2 * rel);
             if (by_lanes) {
                 if (!(kept >> (lane / lanes) & 1u)) {
 #pragma unroll
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
         each_choice<LANES>(lane, a.k, [&](int p) {
             const int mine = keys[p], next = keys[p + 1];
             again |= mine > kInfKey || mine < (kMinusInfKey & ~kLow);
-            if (!exact && next != kNone) again |= too_close(key_value(mine), key_value(next), largest, rel);
+            if (!exact && next != kNone) again |= too_close(key_value(mine), key_value(next), unsure_by, rel);
         });
         unsigned unsure = __ballot_sync(kFull, again);
         while (unsure) {
