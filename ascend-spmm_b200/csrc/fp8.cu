@@ -173,7 +173,10 @@ template <int BN, bool PAIR = false> cudaError_t launch_tiles(const Fp8Launch &l
     if (!tc::make_byte_map(&x, l.x, l.K, l.rows, 1, tc::kBM) ||
         !tc::make_byte_map(&w, l.groups > 0 ? l.w : l.x, l.K, l.groups > 0 ? l.N : 1, std::max<int64_t>(l.groups, 1),
                            PAIR ? BN / 2 : BN) ||
-        !tc::make_out_map(&out, l.out, l.N, l.rows, 1, l.N, 0, a.out_type))
+        // 16-bit results are stored 64 columns at a time, those of 32-column warps and fp32 ones 32
+        !(S::kOwn == 64 && a.out_type != tc::kOutF32
+              ? tc::make_map(&out, l.out, l.N, l.rows, 1, l.N, 0, 32, a.out_type == tc::kOutBf16)
+              : tc::make_out_map(&out, l.out, l.N, l.rows, 1, l.N, 0, a.out_type)))
         return cudaErrorInvalidValue;
     constexpr int kBlocks = PAIR ? 2 : 1;   // per tile
     const int64_t tiles = row_tiles_of(l, kBlocks * tc::kBM) * ((l.N + BN - 1) / BN);

@@ -48,7 +48,7 @@ template <int BN, bool PAIR> struct Fp8Shape {
     static constexpr int kReaders = BN == 256 ? 16 : 8, kOwn = BN / (kReaders / 4);
     static constexpr int kFirstReader = 4, kThreads = 32 * (kFirstReader + kReaders);   // warp 3 has no work
     static constexpr int kA = kBM * kSlice, kB = (PAIR ? BN / 2 : BN) * kSlice;
-    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 5 : 6, kStaging = 4096;             // of an epilogue warp, twice 32 x 32 16-bit values
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 5 : 6, kStaging = 4096;             // of an epilogue warp: 32 rows x 128 bytes
     static constexpr int kAccs = BN == 256 ? 2 : 4, kCols = kAccs * BN;
     static constexpr int kHalves = BN == 256 ? 2 : 1, kScaleBytes = kHalves * kBM * 4;   // of a slice, per block of 128 columns
     static constexpr int kStageOff = kStages * (kA + kB), kScaleOff = kStageOff + kReaders * kStaging;
@@ -355,21 +355,21 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             // a group's last rows share the block with the next group's: no box for them
             const bool boxed = row0 + 32 <= t.y;
             const unsigned swz2 = (unsigned)(lane >> 1 & 3), swz4 = (unsigned)(lane & 7);
-            if (boxed && out_size == 2) {   // all of the warp's columns behind one fence
-                if (elect()) bulk_wait_read<0>();   // the staging's last stores have read it
+            if (boxed && out_size == 2) {   // all of the warp's columns in one box
+                if (elect()) bulk_wait_read<0>();   // the staging's last store has read it
                 __syncwarp();
+                auto stage_row = [&](auto bf16) {
 #pragma unroll
-                for (int c = 0; c < kOwn; c += 32)
-#pragma unroll
-                    for (unsigned i = 0; i < 4; ++i)
-                        st_shared16(stage + c / 32 * 2048 + lane * 64 + ((i ^ swz2) << 4),
-                                    pack8(v + c + 8 * i, a.out_type == kOutBf16));
+                    for (unsigned i = 0; i < kOwn / 8; ++i)
+                        st_shared16(kOwn == 64 ? stage + lane * 128 + ((i ^ swz4) << 4) : stage + lane * 64 + ((i ^ swz2) << 4),
+                                    pack8(v + 8 * i, decltype(bf16)::value));
+                };
+                if (a.out_type == kOutBf16) stage_row(std::true_type());
+                else stage_row(std::false_type());
                 fence_async();
                 __syncwarp();
                 if (elect()) {
-#pragma unroll
-                    for (int c = 0; c < kOwn; c += 32)
-                        if (t.z + first + c < a.n) tma_store(&map_o, stage + c / 32 * 2048, t.z + first + c, t.x + row0, 0);
+                    tma_store(&map_o, stage, t.z + first, t.x + row0, 0);
                     bulk_commit();
                 }
                 continue;
