@@ -10,7 +10,10 @@
 // blocks add the counts of the others up, places.  Further blocks, where a
 // caller asks for them, write zeros beside the first phase: few SMs sort.
 //
-// What bounds it: the latency of its phases.
+// What bounds it: the latency of its phases, and with many keys the scattered
+// stores.  36 keys 3.7 us; 262144 keys, 64 buckets, 6 and 12 us; 524287, 512
+// buckets, 18 us for the second launch.  One cluster of 16 blocks with all
+// phases in a launch took 36 and 58 us.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"

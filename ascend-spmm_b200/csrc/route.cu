@@ -23,8 +23,12 @@
 // NaN counts as the lowest value in every choice; a row whose logits are all
 // -infinity gets zero weights.
 //
-// What bounds it: instructions (about 17 for each expert's score and its
-// place in the order, 20 for each pick), not the 4 bytes of a logit.
+// What bounds it: instructions (some 1000 a warp for a row of 256 experts in
+// eight groups, eight picks), not the 4 bytes of a logit.  65537 such rows, fp32,
+// sigmoid and bias: 82 us forward (11 us of memory; about 25 are scores, groups and
+// bias, 20 the picks, 6 the 0.5 % of rows that are decided in 64 bits), 26 us
+// backward (21 us of memory); 16411 rows of 64 experts, bf16, six picks: 6.5 and
+// 6.3 us.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"
