@@ -371,13 +371,15 @@ int spmm_expert_plan_launch(const void *experts, int32_t *group_ptr, int32_t *po
         return capi_error(SPMM_ERR_ARG, "%s: null array", op);
     int rc = check_workspace(workspace, workspace_bytes, spmm_expert_plan_workspace_bytes(n, num_experts), op);
     if (rc) return rc;
-    spmmb::BucketSort b{};
+    spmmb::BucketPasses sort{};
+    sort.passes = 1;
+    spmmb::BucketSort &b = sort.pass[0];
     b.status = status_or_error(op, &rc);
     if (rc) return rc;
     b.keys = experts; b.wide = itype == SPMM_I64; b.n = n; b.buckets = (int)num_experts; b.mask = -1;
     b.limit = num_experts; b.skip = -1; b.ptr = group_ptr; b.position = position; b.order = source;
     b.counts = static_cast<int *>(workspace);
-    const cudaError_t e = spmmb::launch_bucket_sort(b, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = spmmb::launch_bucket_sort(sort, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SPMM_OK : cuda_error(e, op);
 }
 

@@ -372,8 +372,11 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
     while (bits < 31 && (int64_t(1) << bits) < l.rows) ++bits;
     const int passes = (bits + kBucketBits - 1) / kBucketBits, each = (bits + passes - 1) / passes;
     const int64_t vectors = (int64_t)(bytes / 16);
+    BucketPasses sort{};
+    static_assert(4 * kBucketBits >= 31, "passes for every id");
+    sort.passes = passes;
     for (int p = 0; p < passes; ++p) {
-        BucketSort s{};
+        BucketSort &s = sort.pass[p];
         if (p == 0) s.keys = l.ids;
         else s.pairs_in = sorted[(p - 1) % 2];
         s.wide = l.itype == SPMM_I64;
@@ -389,8 +392,8 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
         s.zero = static_cast<uint4 *>(l.out) + vectors * p / passes;   // a share of the zeros beside each pass
         s.zero_vectors = vectors * (p + 1) / passes - vectors * p / passes;
         s.status = l.status;
-        if ((e = launch_bucket_sort(s, stream)) != cudaSuccess) return e;
     }
+    if ((e = launch_bucket_sort(sort, stream)) != cudaSuccess) return e;
     EmbedArgs a{};
     a.in = l.in; a.out = l.out; a.sorted = sorted[(passes - 1) % 2];
     a.runs = runs;

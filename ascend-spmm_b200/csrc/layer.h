@@ -118,8 +118,13 @@ struct BucketSort {
     DevStatus *status;
 };
 constexpr int kBucketBits = 10, kMostBuckets = 1 << kBucketBits;
+// Passes of a sort by more bits, the lowest first; of the same n and numbers of buckets.
+struct BucketPasses {
+    BucketSort pass[4];
+    int passes;
+};
 size_t bucket_workspace(int64_t n, int buckets);
-cudaError_t launch_bucket_sort(const BucketSort &a, cudaStream_t stream);
+cudaError_t launch_bucket_sort(const BucketPasses &a, cudaStream_t stream);
 
 // ---- rows to their experts and back (routed.cu) -------------------------------
 struct RoutedLaunch {
