@@ -14,8 +14,8 @@
 // What bounds it: the latency of its phases, and with many keys the scattered
 // stores.  36 keys 3.7 us; 262144 keys, 64 buckets, 6 and 12 us; 524287, 512
 // buckets, 18 us for the second launch; both passes of 6144 ids of 131071 rows in
-// one launch 1.8 us less than in two, and 2.5 us less of the host's time.  One cluster of 16 blocks with all
-// phases in a launch took 36 and 58 us.
+// one launch 1.8 us less than in two, and 2.5 us less of the host's time.  One
+// cluster of 16 blocks with all phases in a launch took 36 and 58 us.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"

@@ -37,8 +37,8 @@ __device__ __forceinline__ float scale_of(float amax) { return __fdiv_rn(fmaxf(a
 
 // x / s correctly rounded, from the correctly rounded reciprocal of s
 // (Markstein 1990: one residual and one correction of x * (1 / s)).  The scale
-// keeps all of it in fp32's normal range, but for quotients that round to zero in e4m3.  Not
-// finite: NaN (the residual of an infinity is).
+// keeps all of it in fp32's normal range, but for quotients that round to zero
+// in e4m3.  Not finite: NaN (the residual of an infinity is).
 __device__ __forceinline__ float quotient(float x, float s, float inverse)
 {
     const float q = x * inverse;
@@ -186,7 +186,6 @@ template <int BN, bool PAIR = false> cudaError_t launch_tiles(const Fp8Launch &l
     const unsigned grid = kBlocks * (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, device_sm_count() / kBlocks));
     return tc::launch_overlapped(kernel, grid, kBlocks, S::kThreads, S::kBytes, stream, x, w, out, a);
 }
-
 
 }  // namespace
 

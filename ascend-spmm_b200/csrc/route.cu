@@ -28,7 +28,8 @@
 // sigmoid and bias: 82 us forward (11 us of memory; about 25 are scores, groups and
 // bias, 20 the picks, 6 the 0.5 % of rows that are decided in 64 bits), 26 us
 // backward (21 us of memory); 16411 rows of 64 experts, bf16, six picks: 6.5 and
-// 6.3 us.
+// 6.3 us.  Rows all of whose logits are equal, which 64 bits decide one by one,
+// are the worst: 65537 of 256 experts by softmax 144 us, where random ones take 56.
 #include <algorithm>
 
 #include "../../include/spmm_b200.h"

@@ -6,10 +6,10 @@
 //
 // position [tokens, k] and source [tokens * k] are each other's inverse (see
 // bucket.cu).  Dispatch and the unweighted combine are each other's gradient.
-// All are bound by memory.  A team of lanes owns a token and has four vectors a
-// lane of each row in flight.  Rows whose width is no
-// multiple of 16 bytes start anywhere; they are stored in whole vectors
-// between a few loose elements and read as pairs of vectors (vec.cuh).
+// All are bound by memory.  A team of lanes owns a token and has up to four
+// vectors a lane of each row in flight.  Rows whose width is no multiple of 16
+// bytes start anywhere; they are stored in whole vectors between a few loose
+// elements and read as pairs of vectors (vec.cuh).
 //
 // Measured (TB/s of the bytes above; a plain copy reaches 6.5): 32771 rows of
 // 1024 bf16, eight choices, dispatch 93 us 6.4, combine 110 us 5.5, backward

@@ -38,8 +38,8 @@ class _Router(torch.nn.Module):
 
     def forward(self, x, products):
         """x [rows, in] -> [rows, out]; ``products(rows, group_ptr)`` are the experts'."""
-        logits = x.float() @ self.gate
-        weights, experts = spmm_npu.route_experts(logits, bias=self.bias, **self.options)
+        logits = x.float() @ self.gate.float()   # scores are fp32, also in a module that was cast to 16 bits
+        weights, experts = spmm_npu.route_experts(logits, bias=self.bias.float(), **self.options)
         group_ptr, position, source = spmm_npu.expert_plan(experts, self.gate.size(1))
         self.group_ptr = group_ptr
         rows = spmm_npu.dispatch_rows(x, position, source)

@@ -93,6 +93,41 @@ def test_served_in_8_bits(experts):
     assert {"up", "up_scale", "down", "down_scale", "router.bias"} <= set(state)
 
 
+def test_a_layer_cast_to_16_bits(experts):
+    """Its scores stay fp32: those of the rounded gate and bias, so the same experts as the uncast layer that holds them."""
+    torch.manual_seed(5)
+    layer = experts.ExpertLayer(32, 48, 8, 2, scoring="sigmoid").cuda()
+    layer.router.bias.normal_()
+    layer.bfloat16()
+    x = torch.randn(60, 32, device="cuda").bfloat16()
+    y = layer(x)
+    assert y.dtype == torch.bfloat16
+    twin = experts.ExpertLayer(32, 48, 8, 2, dtype=torch.bfloat16, scoring="sigmoid").cuda()
+    with torch.no_grad():
+        for name in ("up", "down"):
+            getattr(twin, name).copy_(getattr(layer, name))
+        twin.router.gate.copy_(layer.router.gate)
+        twin.router.bias.copy_(layer.router.bias)
+    assert torch.equal(twin(x), y) and torch.equal(layer.router.group_ptr, twin.router.group_ptr)
+    y.float().sum().backward()
+    assert all(p.grad.dtype == torch.bfloat16 and bool(torch.isfinite(p.grad).all()) for p in layer.parameters())
+
+
+def test_no_rows(experts):
+    layer = experts.ExpertLayer(32, 48, 8, 2).cuda()
+    x = torch.empty(0, 32, device="cuda", requires_grad=True)
+    y = layer(x)
+    assert y.shape == (0, 32) and layer.router.group_ptr.tolist() == [0] * 9
+    y.sum().backward()
+    assert x.grad.shape == x.shape and all(bool((p.grad == 0).all()) for p in layer.parameters())
+    layer.balance()
+    assert layer.quantized()(x.detach()).shape == (0, 32)
+    ids = torch.empty(0, dtype=torch.int64, device="cuda")
+    features = experts.NodeFeatures(10, 32).cuda()
+    features(ids).sum().backward()
+    assert bool((features.table.grad == 0).all())
+
+
 def test_a_training_step_of_them_together(experts, relational):  # noqa: F811
     torch.manual_seed(3)
     n, relations = 80, 3

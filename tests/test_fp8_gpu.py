@@ -112,6 +112,16 @@ def test_sizes_of_use(lib, rows, groups, K, N):  # noqa: F811
     check(lib, *make(lib, sizes, K, N, BF16, seed=1))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("sizes,N", [([6000, 0, 9003, 4097], 256), ([257, 255, 256, 1, 5000, 4, 0, 4000], 512),
+                                     ([3] * 30 + [5000, 4700], 512), ([0, 0, 19500, 0], 256)])
+def test_many_rows(lib, sizes, N, dtype):  # noqa: F811
+    """Groups that end inside a pair's tile of 256 rows, rows before the first one and behind the last."""
+    x, w, ptr = make(lib, sizes, 144, N, dtype, seed=2, before=77, after=133)
+    y = check(lib, x, w, ptr)
+    assert bool((y[:77] == 0).all()) and bool((y[len(y) - 133:] == 0).all())
+
+
 def test_rows_outside_every_group_and_index_types(lib):  # noqa: F811
     for idt in (torch.int32, torch.int64):
         x, w, ptr = make(lib, [40, 3], 64, 32, BF16, before=5, after=9, idt=idt)
