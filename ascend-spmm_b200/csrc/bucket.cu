@@ -12,7 +12,7 @@
 // them, write zeros beside the first phase: few SMs sort.
 //
 // What bounds it: the latency of its phases, and with many keys the scattered
-// stores.  36 keys 3.7 us; 262144 keys, 64 buckets, 6 and 12 us; 524287, 512
+// stores.  36 keys 3.6 us; 262144 keys, 64 buckets, 6 and 12 us; 524287, 512
 // buckets, 18 us for the second launch; both passes of 6144 ids of 131071 rows in
 // one launch 1.8 us less than in two, and 2.5 us less of the host's time.  One
 // cluster of 16 blocks with all phases in a launch took 36 and 58 us.
@@ -213,14 +213,27 @@ __global__ void __launch_bounds__(kMostWarps * 32) bucket_passes_kernel(const Bu
     }
 }
 
-// Blocks that sort: one for few keys, else one for every 4096.
-int blocks_for(int64_t n) { return n <= 6144 ? 1 : (int)std::min<int64_t>(kMostBlocks, (n + 4095) / 4096); }
+// Blocks that sort, and their warps.  One block for as many keys as stay in
+// its registers (8192; 7000 ids of 50021 rows, width 64: 36 us, of two blocks
+// 40).  Else one for every 2048 keys, of 16 warps (16384 ids 39 us; 4096 keys
+// and 32 warps 44), as long as there are few of them, since each adds up the
+// counts of all (262144 ids: 56 us; 4096 keys and 32 warps 53).
+struct Blocks {
+    int count, warps;
+};
+Blocks blocks_for(int64_t n, int buckets)
+{
+    if (n <= 2048 && buckets <= 256) return {1, 8};   // few warps, whose barriers are short
+    if (n <= kMostWarps * 32 * kBatch) return {1, kMostWarps};
+    if (n <= 131072) return {(int)((n + 2047) / 2048), 16};
+    return {(int)std::min<int64_t>(kMostBlocks, (n + 4095) / 4096), kMostWarps};
+}
 
 }  // namespace
 
 size_t bucket_workspace(int64_t n, int buckets)
 {
-    const int blocks = blocks_for(n);
+    const int blocks = blocks_for(n, buckets).count;
     return blocks == 1 ? 0 : (size_t)blocks * buckets * sizeof(int);
 }
 
@@ -240,8 +253,8 @@ cudaError_t launch_bucket_sort(const BucketPasses &all, cudaStream_t stream)
         if (e != cudaSuccess) return e;
         if (done) *done = true;
     }
-    const int blocks = blocks_for(a.n);
-    const int warps = a.n <= 2048 && a.buckets <= 256 ? 8 : kMostWarps;   // few keys: few warps, whose barriers are short
+    const Blocks sorting = blocks_for(a.n, a.buckets);
+    const int blocks = sorting.count, warps = sorting.warps;
     const size_t smem = bucket_smem(a.buckets, warps);
     auto zeroing = [&](int64_t vectors) {
         return (unsigned)std::min<int64_t>((vectors + warps * 32 - 1) / (warps * 32),

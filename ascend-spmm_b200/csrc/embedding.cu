@@ -11,9 +11,9 @@
 // part that it starts in, a longer one leaves an fp32 sum in each of its parts,
 // which are added up afterwards (a few ids of a power law hold thousands of
 // rows).  Both passes are bound by memory: 524287 ids of 131071 rows of 512
-// fp32, density 1 / rank, forward 215 us (1.25 GB, 5.8 TB/s), backward 320 us
-// (sorting and zeros 86, sums 196, long runs 39); 16411 ids of 50021 rows of 1024
-// bf16 10 us and 63 us (sorting and zeros 39, sums 18, long runs 6).
+// fp32, density 1 / rank, forward 215 us (1.25 GB, 5.8 TB/s), backward 325 us
+// (sorting and zeros 90, sums 196, long runs 39); 16411 ids of 50021 rows of 1024
+// bf16 10 us and 58 us (sorting and zeros 34, sums 18, long runs 6).
 //
 // An id outside the table gives a row of zeros, no gradient, and the device status.
 #include <algorithm>
