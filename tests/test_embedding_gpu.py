@@ -117,6 +117,29 @@ def test_gradient_against_differences(lib):  # noqa: F811
     assert abs(float((d.double() * v.double()).sum() - want)) < float(slack)
 
 
+def test_the_graph_of_the_gradient(lib):  # noqa: F811
+    """Kept, used twice, freed, of a table that is no leaf; ids that were changed in between are refused."""
+    ids, table, dy = ids_of(300, 60), normal(60, 24).requires_grad_(True), normal(300, 24)
+    want = lib.embedding_grad(ids, dy, 60, 3.0)
+    y = lib.embedding(ids, table * 2, 1.5)
+    (first,) = torch.autograd.grad(y, table, dy, retain_graph=True)
+    (second,) = torch.autograd.grad(y, table, dy)
+    assert torch.equal(first, want) and torch.equal(second, want)   # twice is exact
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, table, dy)
+    y = lib.embedding(ids, table)
+    ids[0] = 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.no_grad():
+        assert not lib.embedding(ids, table).requires_grad
+    with torch.inference_mode():
+        assert not lib.embedding(ids, table).requires_grad
+    y = lib.embedding(ids, table)
+    y.add_(1).sum().backward()   # the result may be changed in place
+    assert torch.equal(table.grad, lib.embedding_grad(ids, torch.ones(300, 24, device="cuda"), 60))
+
+
 def test_captured_and_replayed(lib):  # noqa: F811
     ids, table, dy = ids_of(5000, 2000), normal(2000, 40, dtype=F16), normal(5000, 40, dtype=F16)
     lib.embedding_grad(ids, dy, 2000)
