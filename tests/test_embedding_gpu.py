@@ -47,6 +47,12 @@ def test_numbers_of_ids_and_rows(lib, n, rows):  # noqa: F811
     check(lib, ids_of(n, rows, seed=n), rows, 16, F32, scale=0.5)
 
 
+@pytest.mark.parametrize("n", [2048, 2049, 8191, 8192, 8193, 131072, 131073])
+@pytest.mark.parametrize("rows", [200, 1025, (1 << 20) + 1])
+def test_where_the_sort_s_blocks_change(lib, n, rows):  # noqa: F811
+    check(lib, ids_of(n, rows, seed=n, power=3.0), rows, 8, F32)
+
+
 @pytest.mark.parametrize("power", [1.0, 4.0, 40.0])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_repeated_ids(lib, power, dtype):  # noqa: F811

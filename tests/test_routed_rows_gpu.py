@@ -41,6 +41,12 @@ def test_plan(lib, tokens, k, num, dtype):  # noqa: F811
     check_plan(lib, experts_of(tokens, k, num, seed=tokens, dtype=dtype), num)
 
 
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 8191, 8192, 8193, 10240, 10241, 131072, 131073, 524288, 524289])
+@pytest.mark.parametrize("num", [64, 257, 1024])
+def test_plan_where_its_blocks_change(lib, n, num):  # noqa: F811
+    check_plan(lib, experts_of(n, 1, num, seed=n), num)
+
+
 @pytest.mark.parametrize("tokens", [50, 6000])
 def test_plan_of_unequal_loads(lib, tokens):  # noqa: F811
     """One expert has every row; none has any; experts without rows between others."""
