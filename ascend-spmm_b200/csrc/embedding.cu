@@ -11,9 +11,9 @@
 // part that it starts in, a longer one leaves an fp32 sum in each of its parts,
 // which are added up afterwards (a few ids of a power law hold thousands of
 // rows).  Both passes are bound by memory: 524287 ids of 131071 rows of 512
-// fp32, density 1 / rank, forward 215 us (1.25 GB, 5.8 TB/s), backward 325 us
-// (sorting and zeros 90, sums 196, long runs 39); 16411 ids of 50021 rows of 1024
-// bf16 10 us and 58 us (sorting and zeros 34, sums 18, long runs 6).
+// fp32, density 1 / rank, forward 215 us (1.25 GB, 5.8 TB/s), backward 316 us
+// (sorting and zeros 90, sums 196, long runs 30); 16411 ids of 50021 rows of 1024
+// bf16 10 us and 59 us (sorting and zeros 34, sums 18, long runs 7).
 //
 // An id outside the table gives a row of zeros, no gradient, and the device status.
 #include <algorithm>
@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kPart = 32;      // sorted ids of a part
 constexpr int kFew = 8;        // a run over at most so many parts is added up by a warp, a longer one by a block
-constexpr int kJoin = 16;      // of so many warps
+constexpr int kJoin = 32;      // of so many warps (16: 39 us for the 30 below, 6 for the 7)
 
 struct EmbedArgs {
     const void *ids;        // forward
@@ -409,7 +409,7 @@ cudaError_t launch_embedding_backward(const EmbeddingLaunch &l, int64_t skip, vo
         const dim3 grid((parts + block.y - 1) / block.y, (unsigned)((threads + each - 1) / each));
         embedding_sum_kernel<kAligned, T><<<grid, block, 0, stream>>>(a);
         if (parts > 1)
-            embedding_join_kernel<T><<<(unsigned)std::min<int64_t>(parts * ((l.width + 127) / 128), 4 * (int64_t)device_sm_count()),
+            embedding_join_kernel<T><<<(unsigned)std::min<int64_t>(parts * ((l.width + 127) / 128), 2 * (int64_t)device_sm_count()),
                                        32 * kJoin, 0, stream>>>(a);
         return cudaGetLastError();
     });
