@@ -15,7 +15,6 @@ operators where ``own`` is set), ``work()`` the bytes and operations a pass
 cannot do without and ``exact()`` the definition in 64 bits.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -189,9 +188,7 @@ def prepare(case, seed):
 # one pass
 # --------------------------------------------------------------------------
 
-@functools.lru_cache(maxsize=None)
 def _operators():
-    """This repository's operators, imported once as a program does."""
     at = str(Path(__file__).resolve().parents[1] / "ascend-spmm_b200")
     if at not in sys.path:
         sys.path.insert(0, at)
