@@ -264,8 +264,8 @@ template <typename T, int VPL> __device__ __noinline__ int choose_exactly(const 
 // errors.  A 32-bit score is off by at most 2^-21 of the row's largest one (of
 // 1 for a sigmoid) for its exponential and the reciprocal, and, with a
 // softmax, by its share of the sum's error, (VPL + 5) 2^-24; `score` is more
-// than twice that.  A sum of two rounds by 2^-24 of itself, and a key has lost
-// the bits that hold the place: `rel`.
+// than twice that.  A sum with the bias rounds by 2^-24 of itself, and a key has
+// lost the bits that hold the place: `rel`.
 __device__ __forceinline__ bool too_close(float hi, float lo, float score, float rel)
 {
     return !(hi - lo > score + rel * fmaxf(fabsf(hi), fabsf(lo)));   // true for infinities, too
@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
     constexpr int kTeams = 32 / LANES;
     constexpr unsigned kTeam = LANES == 32 ? kFull : (1u << LANES) - 1;
     __shared__ int s_pick[8][kTeams][kMostChosen + 1], s_key[8][kTeams][kMostChosen + 1], s_score[8][kTeams][kMostGroups];
+    __shared__ float s_slack[8][kTeams][kMostGroups];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % LANES, team = threadIdx.x % 32 / LANES, n = a.n;
     const int first = lane * VPL;
     const bool grouped = a.top_groups < a.groups;
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
         }
     };
     int *const picks = s_pick[warp][team], *const keys = s_key[warp][team], *const scores = s_score[warp][team];
+    float *const slacks = s_slack[warp][team];
     const int64_t step = (int64_t)gridDim.x * 8 * kTeams;
     const int64_t start = ((int64_t)blockIdx.x * 8 + warp) * kTeams;
     if (start < a.tokens) fetch(start, 0);
@@ -386,7 +388,14 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
         const float unsure_by = by_logit ? 0.f : (0x1p-19f + VPL * 0x1p-22f) * (a.sigmoid ? 1.f : inv);
         bool again = false;
         if (grouped) {
-            auto sum_of = [&](int top, int next) { return raw_key(key_value(top) + key_value(next)); };
+            // A group's score, and how far it may be off.  That goes by its terms, which can nearly cancel: each is off by at
+            // most half of `unsure_by` and half of `rel` of itself, the sum's own rounding by 2^-24 of them.
+            auto put = [&](int g, int top, int next) {
+                const bool two = a.group_best == 2;
+                const float v = key_value(top), w = two ? key_value(next) : 0.f;
+                scores[g] = two ? raw_key(v + w) : top;
+                slacks[g] = unsure_by + rel * (fabsf(v) + fabsf(w));
+            };
             if (by_lanes) {
                 int b1 = kNone, b2 = kNone;
 #pragma unroll
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                     b2 = max(min(b1, o1), max(b2, o2));
                     b1 = max(b1, o1);
                 }
-                if (lane % lanes == 0 && lane / lanes < a.groups) scores[lane / lanes] = a.group_best == 2 ? sum_of(b1, b2) : b1;
+                if (lane % lanes == 0 && lane / lanes < a.groups) put(lane / lanes, b1, b2);
             } else {
                 for (int g = 0; g < a.groups; ++g) {
                     int b1 = kNone, b2 = kNone;
@@ -417,14 +426,15 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                         b2 = max(min(b1, o1), max(b2, o2));
                         b1 = max(b1, o1);
                     }
-                    if (lane == 0) scores[g] = a.group_best == 2 ? sum_of(b1, b2) : b1;
+                    if (lane == 0) put(g, b1, b2);
                 }
             }
             __syncwarp();
             unsigned kept = 0;
-            int last = INT32_MAX, out = INT32_MIN;   // the lowest score kept, the highest left out
+            float low = INFINITY, high = -INFINITY;   // what the groups kept have at least, those left out at most
             for (int g = lane; g < a.groups; g += LANES) {
                 const int mine = scores[g];
+                const float score = key_value(mine), slack = slacks[g];
                 int rank = 0;
                 for (int h = 0; h < a.groups; ++h) {
                     const int other = scores[h];
@@ -432,25 +442,26 @@ __global__ void __launch_bounds__(256, route_blocks(VPL)) route_kernel(const Rou
                 }
                 if (rank < a.top_groups) {
                     kept |= 1u << g;
-                    last = min(last, mine);
+                    low = fminf(low, score - slack);
+                    again |= !exact && !(slack < INFINITY);   // its terms are not finite: nothing is known of its order
                 } else {
-                    out = max(out, mine);
+                    high = fmaxf(high, score + slack);   // a cut -infinity is a NaN, which is the smaller one
                 }
                 again |= mine > kInfKey || mine < (kMinusInfKey & ~kLow);   // NaN
             }
             if constexpr (LANES == 32) {
                 kept = __reduce_or_sync(kFull, kept);
-                last = __reduce_min_sync(kFull, last);
-                out = warp_max(out);
+                low = key_value(__reduce_min_sync(kFull, raw_key(low)));
+                high = key_value(warp_max(raw_key(high)));
             } else {
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) {
                     kept |= __shfl_xor_sync(kFull, kept, o);
-                    last = min(last, __shfl_xor_sync(kFull, last, o));
-                    out = max(out, __shfl_xor_sync(kFull, out, o));
+                    low = fminf(low, __shfl_xor_sync(kFull, low, o));
+                    high = fmaxf(high, __shfl_xor_sync(kFull, high, o));
                 }
             }
-            if (!exact) again |= too_close(key_value(last), key_value(out), 2 * unsure_by, 2 * rel);
+            again |= !exact && !(low > high);
             if (by_lanes) {
                 if (!(kept >> (lane / lanes) & 1u)) {
 #pragma unroll
@@ -648,7 +659,7 @@ cudaError_t launch_route(const RouteLaunch &r, cudaStream_t stream)
             const unsigned blocks = (unsigned)std::min<int64_t>((warps + 7) / 8, route_blocks(kVpl) * (int64_t)device_sm_count());
             auto kernel = route_kernel<T, kLanes, kVpl, decltype(vec)::value>;
             const int smem = decltype(vec)::value ? 8 * 2 * (32 / kLanes) * r.n * (int)sizeof(T) : 0;
-            if (smem > 16384) {   // with what the kernel has of its own, more than a block gets unasked
+            if (smem >= 16384) {   // with what the kernel has of its own, more than a block gets unasked
                 static PerDevice<bool> ready;   // the attribute outlasts the call
                 bool *done = ready.here();
                 if (!done || !*done) {
