@@ -234,10 +234,11 @@ __device__ __forceinline__ void bar_arrive_cluster(unsigned remote)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
 }
-// As bar_arrive_cluster, ordering this block's accesses only.
-__device__ __forceinline__ void bar_arrive_peer(unsigned remote)
+// The same where TMEM alone is handed over, whose order is that of the fences around it (fence_before here, fence_after
+// behind the wait): memory is not ordered, which for a warp in the middle of its work is slow.
+__device__ __forceinline__ void bar_arrive_tmem(unsigned remote)
 {
-    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(remote) : "memory");
 }
 __device__ __forceinline__ void cluster_sync()
 {
