@@ -212,7 +212,17 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float *v)
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// 8 or 32 consecutive columns as above.
+// 2, 8 or 32 consecutive columns as above.
+__device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[2])
+{
+    unsigned r[2];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];\n\ttcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(r[0]), "=r"(r[1])
+                 : "r"(taddr)
+                 : "memory");
+    v[0] = __uint_as_float(r[0]);
+    v[1] = __uint_as_float(r[1]);
+}
 __device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[8]) { tmem_ld8(taddr, v); }
 __device__ __forceinline__ void tmem_ld(unsigned taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
 
