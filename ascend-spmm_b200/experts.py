@@ -31,7 +31,10 @@ class _Router(torch.nn.Module):
 
     def __init__(self, gate, bias, options):
         super().__init__()
-        self.gate = gate
+        if isinstance(gate, torch.nn.Parameter):
+            self.gate = gate
+        else:   # of a layer that does not train
+            self.register_buffer("gate", gate)
         self.register_buffer("bias", bias)
         self.options = dict(options)
         self.group_ptr = None   # of the last call: group_ptr[e + 1] - group_ptr[e] rows went to expert e

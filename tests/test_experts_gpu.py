@@ -93,6 +93,22 @@ def test_served_in_8_bits(experts):
     assert {"up", "up_scale", "down", "down_scale", "router.bias"} <= set(state)
 
 
+def test_the_state_of_a_served_layer(experts):
+    """All of it: another served layer that loads it answers alike; the gate moves with the rest."""
+    torch.manual_seed(7)
+    served = experts.ExpertLayer(32, 48, 8, 2, scoring="sigmoid", dtype=torch.bfloat16).cuda().quantized()
+    other = experts.ExpertLayer(32, 48, 8, 2, scoring="sigmoid", dtype=torch.bfloat16).cuda().quantized()
+    x = torch.randn(40, 32, device="cuda").bfloat16()
+    want = served(x)
+    assert not torch.equal(other(x), want)
+    other.load_state_dict(served.state_dict())
+    assert torch.equal(other(x), want)
+    assert not any(p.requires_grad for p in served.parameters())
+    served.cpu()
+    assert all(t.device.type == "cpu" for t in (served.router.gate, *served.state_dict().values()))
+    assert torch.equal(served.cuda()(x), want)
+
+
 def test_a_layer_cast_to_16_bits(experts):
     """Its scores stay fp32: those of the rounded gate and bias, so the same experts as the uncast layer that holds them."""
     torch.manual_seed(5)
