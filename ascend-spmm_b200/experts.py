@@ -26,6 +26,24 @@ import torch
 import spmm_npu
 
 
+class _KeepsTypes(torch.nn.Module):
+    """A module whose buffers named in ``kept`` go where it goes, and keep their types when it is cast."""
+
+    kept = ()
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: self._buffers[name] for name in self.kept}
+        self._buffers.update(dict.fromkeys(kept))
+        try:
+            super()._apply(fn, recurse)
+        finally:
+            self._buffers.update(kept)
+        for name, buffer in kept.items():
+            as_cast = fn(buffer.new_empty(0))
+            self._buffers[name] = fn(buffer) if as_cast.dtype == buffer.dtype else buffer.to(as_cast.device)
+        return self
+
+
 class _Router(torch.nn.Module):
     """Scores of the experts, their choice, and the way of the rows to the experts and back."""
 
@@ -82,8 +100,11 @@ class ExpertLayer(torch.nn.Module):
         return QuantizedExpertLayer(self)
 
 
-class QuantizedExpertLayer(torch.nn.Module):
-    """An ``ExpertLayer`` whose products run in 8-bit floating point (not differentiable)."""
+class QuantizedExpertLayer(_KeepsTypes):
+    """An ``ExpertLayer`` whose products run in 8-bit floating point (not differentiable).  Cast to another type, it keeps
+    its 8-bit weights and their fp32 scales."""
+
+    kept = ("up", "up_scale", "down", "down_scale")
 
     @torch.no_grad()
     def __init__(self, layer: ExpertLayer):

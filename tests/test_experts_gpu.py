@@ -129,6 +129,27 @@ def test_a_layer_cast_to_16_bits(experts):
     assert all(p.grad.dtype == torch.bfloat16 and bool(torch.isfinite(p.grad).all()) for p in layer.parameters())
 
 
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.to(torch.bfloat16),
+                                  lambda m: m.to("cpu", torch.float16).cuda(), lambda m: torch.nn.Sequential(m).half()[0]])
+def test_a_served_layer_cast_to_16_bits(experts, cast):
+    """Its 8-bit weights and their scales stay as they are; it answers as the layer of the cast gate."""
+    torch.manual_seed(6)
+    layer = experts.ExpertLayer(32, 48, 8, 2, dtype=torch.bfloat16).cuda()
+    served, twin = layer.quantized(), layer.quantized()
+    names = ["up", "up_scale", "down", "down_scale"]
+    before = {name: served.state_dict()[name].clone() for name in names}
+    order = list(served.state_dict())
+    served = cast(served)
+    assert list(served.state_dict()) == order
+    for name in names:
+        now = served.state_dict()[name]
+        assert now.dtype == before[name].dtype and now.is_cuda and torch.equal(now.float(), before[name].float()), name
+    assert served.router.gate.dtype in (torch.float16, torch.bfloat16)
+    twin.router.gate.copy_(served.router.gate)
+    x = torch.randn(40, 32, device="cuda").bfloat16()
+    assert torch.equal(served(x), twin(x))
+
+
 def test_no_rows(experts):
     layer = experts.ExpertLayer(32, 48, 8, 2).cuda()
     x = torch.empty(0, 32, device="cuda", requires_grad=True)
