@@ -44,8 +44,11 @@ class _KeepsTypes(torch.nn.Module):
         return self
 
 
-class _Router(torch.nn.Module):
-    """Scores of the experts, their choice, and the way of the rows to the experts and back."""
+class _Router(_KeepsTypes):
+    """Scores of the experts, their choice, and the way of the rows to the experts and back.  The bias stays fp32 in a module
+    that is cast to 16 bits, where the steps of ``balance`` would be rounded away."""
+
+    kept = ("bias",)
 
     def __init__(self, gate, bias, options):
         super().__init__()
@@ -60,7 +63,7 @@ class _Router(torch.nn.Module):
     def forward(self, x, products):
         """x [rows, in] -> [rows, out]; ``products(rows, group_ptr)`` are the experts'."""
         logits = x.float() @ self.gate.float()   # scores are fp32, also in a module that was cast to 16 bits
-        weights, experts = spmm_npu.route_experts(logits, bias=self.bias.float(), **self.options)
+        weights, experts = spmm_npu.route_experts(logits, bias=self.bias, **self.options)
         group_ptr, position, source = spmm_npu.expert_plan(experts, self.gate.size(1))
         self.group_ptr = group_ptr
         rows = spmm_npu.dispatch_rows(x, position, source)

@@ -150,6 +150,23 @@ def test_a_served_layer_cast_to_16_bits(experts, cast):
     assert torch.equal(served(x), twin(x))
 
 
+def test_balance_of_a_layer_cast_to_16_bits(experts):
+    """The bias stays fp32: small steps add up at any size of it."""
+    torch.manual_seed(8)
+    layer = experts.ExpertLayer(32, 48, 8, 2, scoring="sigmoid").cuda().bfloat16()
+    layer.router.bias.copy_(torch.linspace(-3, 3, 8, device="cuda"))
+    x = torch.randn(60, 32, device="cuda").bfloat16()
+    want = layer.router.bias.double()
+    for _ in range(5):
+        layer(x)
+        load = layer.router.group_ptr.diff().double()
+        want = want + 1e-3 * torch.sign(load.mean() - load)
+        layer.balance(1e-3)
+    # five sums and their step, each off by at most 2^-24 of 4
+    assert float((layer.router.bias.double() - want).abs().max()) <= 6 * 2.0 ** -22
+    assert layer.router.bias.dtype == torch.float32 and layer.half().quantized().bfloat16().router.bias.dtype == torch.float32
+
+
 def test_no_rows(experts):
     layer = experts.ExpertLayer(32, 48, 8, 2).cuda()
     x = torch.empty(0, 32, device="cuda", requires_grad=True)
