@@ -167,6 +167,25 @@ def test_balance_of_a_layer_cast_to_16_bits(experts):
     assert layer.router.bias.dtype == torch.float32 and layer.half().quantized().bfloat16().router.bias.dtype == torch.float32
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_under_autocast(experts, dtype):
+    """The scores stay fp32: the same experts, results and gradients as without it."""
+    torch.manual_seed(9)
+    layer = experts.ExpertLayer(64, 48, 32, 4, scoring="sigmoid").cuda()
+    x = torch.randn(300, 64, device="cuda", requires_grad=True)
+    dy = torch.randn(300, 64, device="cuda")
+    want = layer(x)
+    want_ptr = layer.router.group_ptr
+    want_grads = torch.autograd.grad(want, [x, *layer.parameters()], dy)
+    with torch.autocast("cuda", dtype=dtype):
+        got = layer(x)
+        served = layer.quantized()(x.detach())
+    assert torch.equal(got, want) and torch.equal(layer.router.group_ptr, want_ptr)
+    for a, b in zip(torch.autograd.grad(got, [x, *layer.parameters()], dy), want_grads):
+        assert torch.equal(a, b)
+    assert torch.equal(served, layer.quantized()(x.detach()))
+
+
 def test_no_rows(experts):
     layer = experts.ExpertLayer(32, 48, 8, 2).cuda()
     x = torch.empty(0, 32, device="cuda", requires_grad=True)
