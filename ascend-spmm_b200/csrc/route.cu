@@ -17,8 +17,9 @@
 // The choice is what 64-bit scores give, from 32-bit ones: where two values
 // that the choice tells apart (a pick and the next one, the last group kept
 // and the best one left out) are closer than their error bounds, the warp
-// decides the row again in 64 bits.  Without a bias the scores grow with the
-// logits, which are then compared as they are (exactly).
+// decides the row again in 64 bits.  Where nothing is added to a score (no bias,
+// no groups by sums of two) the logits are compared as they are, which is exact:
+// the scores grow with them, also where 64 bits round two of them alike.
 //
 // NaN counts as the lowest value in every choice; a row whose logits are all
 // -infinity gets zero weights.

@@ -183,10 +183,14 @@ def route_experts(logits, top_k, bias=None, scoring="softmax", groups=1, top_gro
     [num_experts], for balance) is added to them for the choice alone.  With
     ``groups`` > ``top_groups`` the experts are that many ranges of equal size,
     and only those of the ``top_groups`` ranges with the largest sums of their
-    ``group_best`` (1 or 2) largest values can be chosen.  Equal values go to
-    the lowest index, NaN below all.  ``renormalize`` divides the chosen scores
-    by their sum + 1e-20; ``scale`` multiplies them.  At most 1024 experts, 32
-    chosen ones, 32 groups.
+    ``group_best`` (1 or 2) largest values can be chosen.  Values are compared
+    as 64-bit scores, or, where nothing is added to a score (no ``bias``, and no
+    sums of two by ``groups``), as the logits, in whose order the scores are:
+    scores that round to the same number, as of sigmoid 1 above 37, tie with a
+    bias of zeros and not with None.  Equal values go to the lowest index, NaN
+    below all.  ``renormalize`` divides the chosen scores by their sum + 1e-20;
+    ``scale`` multiplies them; sigmoids below 2^-126 count as 0 in the weights.
+    At most 1024 experts, 32 chosen ones, 32 groups.
 
     The weights are differentiable in the logits; the choice is a constant.
     """

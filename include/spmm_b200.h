@@ -394,10 +394,12 @@ int spmm_orthogonalize_launch(const void *update, void *out, int64_t batch, int6
  *            descending order, the lowest index first among equal ones
  *   weights  [tokens, top_k] s of these, divided by their sum + 1e-20 with
  *            renormalize, times scale
- * The choice is that of 64-bit scores (without a bias, of the logits
- * themselves).  NaN counts as the lowest value in it; a row whose logits are
- * all -infinity has weights of zero.  At most 1024 experts, 32 chosen ones
- * and 32 groups. */
+ * The choice is that of 64-bit scores or, where nothing is added to a score
+ * (no bias, and no groups that are compared by sums of two), of the logits,
+ * in whose order the scores are: scores that 64 bits round to the same number
+ * do not tie there.  NaN counts as the lowest value in it; a row whose logits
+ * are all -infinity has weights of zero, and a sigmoid below 2^-126 counts as 0
+ * in the weights.  At most 1024 experts, 32 chosen ones and 32 groups. */
 int spmm_route_experts_launch(const void *logits, const float *bias, float *weights, int32_t *experts, int64_t tokens,
                               int64_t num_experts, int64_t top_k, int scoring, int64_t groups, int64_t top_groups,
                               int group_best, int renormalize, double scale, int dtype, void *stream);

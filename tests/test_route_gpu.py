@@ -253,3 +253,21 @@ def test_refusals(lib):  # noqa: F811
     (dx,) = torch.autograd.grad(w.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("options", [{}, {"groups": 8, "top_groups": 3}, {"groups": 8, "top_groups": 3, "group_best": 2}])
+def test_scores_that_saturate(lib, options):  # noqa: F811
+    """Sigmoids that round to 1 (or 0) in 64 bits: without a bias, and with no sums of groups, the logits decide; a bias,
+    of zeros too, or such sums compare the scores, which are equal there."""
+    x = torch.linspace(40, 60, 64, device="cuda").repeat(5, 1)
+    x[1] = 50 + torch.arange(64, device="cuda").flip(0) * 2.0 ** -18
+    x[2:] = torch.stack([x[0, torch.randperm(64, generator=torch.Generator().manual_seed(s))] for s in range(3)])
+    by_score = torch.arange(4, device="cuda", dtype=torch.int32).expand(5, 4)
+    for logits in (x, x - 900):   # scores of 1, and scores of 0
+        _, e = lib.route_experts(logits, 4, scoring="sigmoid", **options)
+        by_logit = ref.route_choice(logits, 4, scoring="sigmoid", **{**options, "group_best": 1})
+        want = by_score.cpu().long() if options.get("group_best") == 2 else by_logit
+        assert torch.equal(e.cpu().long(), want)
+        _, e = lib.route_experts(logits, 4, torch.zeros(64, device="cuda"), "sigmoid", **options)
+        assert torch.equal(e, by_score)
+    assert not torch.equal(by_score.cpu().long(), by_logit)
