@@ -178,3 +178,22 @@ def test_refusals(lib):  # noqa: F811
     (d,) = torch.autograd.grad(lib.embedding(ids, tl).sum(), tl, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         d.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("run", [31, 32, 33, 256, 257, 1024 * 32 - 1, 1024 * 32, 1024 * 32 + 1, 100000])
+@pytest.mark.parametrize("width", [16, 33])
+def test_long_runs_to_the_last_row(lib, run, width, dtype):  # noqa: F811
+    """Whole numbers, whose fp32 sums are exact in any order: a lost, doubled or misplaced row shows."""
+    g = torch.Generator(device="cuda").manual_seed(run)
+    runs = [5, run, 1, run + 40, 3]      # of the ids 2, 9, 3, 0, 7, in shuffled order
+    ids = torch.cat([torch.full((n,), i, device="cuda") for n, i in zip(runs, (2, 9, 3, 0, 7))])
+    ids = ids[torch.randperm(len(ids), generator=g, device="cuda")]
+    dy = torch.randint(-8, 9, (len(ids), width), generator=g, device="cuda")
+    want = torch.zeros(11, width, dtype=torch.int64, device="cuda").index_add_(0, ids, dy)
+    assert int(want.abs().max()) < 1 << 16 and 8 * len(ids) < 1 << 24
+    d = lib.embedding_grad(ids, dy.to(dtype), 11)
+    assert torch.equal(d, want.float().to(dtype))
+    d = lib.embedding_grad(ids, dy.to(dtype), 11, 0.25, 9)
+    want[9] = 0
+    assert torch.equal(d, (want.float() * 0.25).to(dtype))
