@@ -26,9 +26,11 @@ template <typename T> struct Pack16 {
     }
 };
 
-// The 16 bytes at p, which is aligned to its elements: of an array that starts
-// on 16 bytes, the one or two aligned vectors that hold them (each holds one
-// of them at least, so nothing behind the array is read), shifted together.
+// The 16 bytes at p, which is aligned to its elements: the one or two aligned
+// vectors that hold them, shifted together.  Each holds one of these bytes at
+// least: of an array that starts on 16 bytes, what is read besides it lies
+// behind its end and before the next multiple of 16, up to 14 bytes, which are
+// not used (and belong to the array's last vector: no other page, no fault).
 // Called with one alignment by a whole warp, so that the branches are uniform.
 template <bool ALIGNED, typename T> __device__ __forceinline__ Pack16<T> load16(const T *p)
 {

@@ -381,7 +381,9 @@ int spmm_orthogonalize_launch(const void *update, void *out, int64_t batch, int6
 
 /* ---------------------------------------------------------------------- */
 /* Routed experts and learned features.  Their row ranges are              */
-/* spmm_grouped_matmul's groups.                                           */
+/* spmm_grouped_matmul's groups.  Arrays start on 16 bytes; rows are read  */
+/* in 16-byte vectors, so that up to 14 bytes between an array's end and   */
+/* the next multiple of 16 may be read (they are not used).                */
 /* ---------------------------------------------------------------------- */
 
 /* Each row's experts and their weights: with s the softmax or the sigmoid of
