@@ -13,6 +13,8 @@
 //
 // Quantising is bound by memory and, near it, by instructions (14 for an
 // element): 65537 rows of 1024 bf16 41 us, 203 MB, 0.76 of the copy bandwidth.
+// Weights are quantised once, element by element and read twice: 64 x 1024 x 2048
+// bf16 307 us, 1.3 TB/s of their 403 MB.
 #include <cuda_fp8.h>
 
 #include <algorithm>

@@ -15,13 +15,13 @@
 // products, and the blocks are added in fp32 rounded to nearest.
 //
 // What bounds it, 65536 rows of 64 groups, K = 1024, N = 2048, bf16 results:
-// 165 us, 1665 TFLOP/s (the same product in bf16 212 us).  The copies and
+// 160 to 165 us, 1700 TFLOP/s (the same product in bf16 212 us).  The copies and
 // products alone take 105 us, at the pace of shared memory (a pair's slice is
 // written and read at 80 KB a block, 640 cycles for the products' 512).  An
 // accumulator's way from the products to the readers and back is as long as
 // two slices, and TMEM holds two: 25 us.  Reading them takes 14 us; the end of
 // a tile, when the readers store and the products can be two slices ahead
-// only, 30 us (K = 4096: 2100 TFLOP/s).  Measured and slower: eight readers of
+// only, 30 us (K = 4096: 2050 TFLOP/s).  Measured and slower: eight readers of
 // 128 columns (registers spill, and come back from L2, since shared memory
 // leaves no L1: 187 us), 128-column tiles with four accumulators (184 us),
 // stores by the readers' lanes (183 us).

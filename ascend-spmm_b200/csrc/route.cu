@@ -27,8 +27,10 @@
 // What bounds it: instructions (some 1000 a warp for a row of 256 experts in
 // eight groups, eight picks), not the 4 bytes of a logit.  65537 such rows, fp32,
 // sigmoid and bias: 82 us forward (11 us of memory; about 25 are scores, groups and
-// bias, 20 the picks, 6 the 0.5 % of rows that are decided in 64 bits), 26 us
-// backward (21 us of memory); 16411 rows of 64 experts, bf16, six picks: 6.5 and
+// bias, 20 the picks, 6 the 0.5 % of rows that are decided in 64 bits, the others
+// are not told apart), 26 us backward (a sigmoid's reads the sectors of the chosen
+// logits only: some 84 MB, 13 us of memory; a chain of loads, expert and then logit,
+// and issue slots 62 % busy); 16411 rows of 64 experts, bf16, six picks: 6.5 and
 // 6.3 us.  Rows all of whose logits are equal, which 64 bits decide one by one,
 // are the worst: 65537 of 256 experts by softmax 144 us, where random ones take 56.
 #include <algorithm>
