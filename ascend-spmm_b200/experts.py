@@ -64,7 +64,7 @@ class _Router(_KeepsTypes):
         """x [rows, in] -> [rows, out]; ``products(rows, group_ptr)`` are the experts'."""
         with torch.autocast(x.device.type, enabled=False):   # scores are fp32, also in a module that was cast to 16 bits
             logits = x.float() @ self.gate.float()
-        weights, experts = spmm_npu.route_experts(logits, bias=self.bias, **self.options)
+        weights, experts = spmm_npu.route_experts(logits, bias=self.bias.float(), **self.options)
         group_ptr, position, source = spmm_npu.expert_plan(experts, self.gate.size(1))
         self.group_ptr = group_ptr
         rows = spmm_npu.dispatch_rows(x, position, source)

@@ -167,6 +167,21 @@ def test_balance_of_a_layer_cast_to_16_bits(experts):
     assert layer.router.bias.dtype == torch.float32 and layer.half().quantized().bfloat16().router.bias.dtype == torch.float32
 
 
+def test_a_bias_that_was_saved_in_16_bits(experts):
+    """Copied into the fp32 one, or put in its place: the layer answers alike."""
+    torch.manual_seed(10)
+    layer, other = (experts.ExpertLayer(32, 48, 8, 2, scoring="sigmoid").cuda() for _ in range(2))
+    layer.router.bias.copy_(torch.randn(8, device="cuda").bfloat16())
+    state = layer.state_dict()
+    state["router.bias"] = state["router.bias"].bfloat16()
+    x = torch.randn(60, 32, device="cuda")
+    want = layer(x)
+    other.load_state_dict(state)
+    assert other.router.bias.dtype == torch.float32 and torch.equal(other(x), want)
+    other.load_state_dict(state, assign=True)
+    assert other.router.bias.dtype == torch.bfloat16 and torch.equal(other(x), want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_under_autocast(experts, dtype):
     """The scores stay fp32: the same experts, results and gradients as without it."""
