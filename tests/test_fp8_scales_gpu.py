@@ -102,3 +102,31 @@ def test_rows_do_not_depend_on_their_neighbours(lib, sizes, K, N):  # noqa: F811
     assert bool((y[index == 5] == 0).all()) and bool(torch.isnan(y[index == 6]).all())
     assert bool((~torch.isfinite(y[index == 4])).all())
     assert bool((y[index == 3].float().abs() < 2.0 ** -110).all()) and bool((y[index == 3] != 0).any())
+
+
+@pytest.mark.parametrize("sizes,K,N", SHAPES)
+def test_captured_and_on_two_streams(lib, sizes, K, N):  # noqa: F811
+    """One graph replayed with ordinary and far scales; calls with either at once."""
+    (q, near), (wq, ws) = lib.quantize_fp8(normal(sum(sizes), K)), lib.quantize_weight_fp8(normal(len(sizes), K, N, seed=1))
+    far = near.clone()
+    far[::3] = 2.0 ** -140
+    call = lambda s: lib.grouped_matmul_fp8(q, s, wq, ws, ptr, BF16)  # noqa: E731
+    ptr, s = ptr_of(sizes), far.clone()
+    want = [call(far), call(near)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call(s)
+    for i in (0, 1, 0, 1):
+        s.copy_((far, near)[i])
+        graph.replay()
+        assert torch.equal(y, want[i])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append(call((far, near)[i]))
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
